@@ -22,6 +22,7 @@ FIM_ERR_UNSUPPORTED = 99
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
+_f32 = ctypes.c_float
 
 # symbol -> argtypes (all return int)
 SIGNATURES: dict[str, list] = {
@@ -63,6 +64,18 @@ SIGNATURES: dict[str, list] = {
                                               _vp, _vp],
     "fim_depthwise5x5_relu_pointwise_int8": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _vp,
                                              _i32, _vp, _vp],
+    "fim_group_norm_workspace": [_i64, _i64, _i64, _i64, _i32, _vp],
+    "fim_group_norm": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp],
+    "fim_group_norm_backward": [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32,
+                                _vp, _vp, _vp, _vp, _vp, _vp],
+    "fim_gated_linear_workspace": [_i64, _i64, _i64, _i32, _vp],
+    "fim_gated_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _vp, _i64,
+                         _vp],
+    "fim_gated_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _i64,
+                                  _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "fim_grad_norm_workspace": [_i64, _vp, _vp],
+    "fim_grad_norm": [_i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
+    "fim_clip_grad_norm": [_i64, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _vp, _vp, _vp],
 }
 
 # the probe library (csrc/probe.h): test and measurement hooks, not part of the product ABI

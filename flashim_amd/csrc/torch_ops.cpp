@@ -9,11 +9,13 @@
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <array>
+#include <limits>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -430,6 +432,264 @@ Tensor pointwise_bf16(const Tensor& x, const Tensor& weight, const OptTensor& bi
   return out;
 }
 
+// -- training-step operators -------------------------------------------------------------------------------------------
+
+int float_code(const OptTensor& t) { return t ? dtype_code(*t) : 0; }
+
+// x as [B, P, C] with unit channel stride, copied where its strides do not allow that view
+Tensor image_rows(const Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(x.dim() >= 2, what, ": expected [B, ..., C], got shape ", x.sizes());
+  const int64_t b = x.size(0), c = x.size(-1);
+  int64_t p = 1;
+  for (int64_t i = 1; i < x.dim() - 1; ++i) p *= x.size(i);
+  Tensor t = x.reshape({b, p, c});
+  return t.stride(2) == 1 || c == 1 ? t : t.contiguous();
+}
+
+// x as [rows, C] with unit column stride
+Tensor matrix_rows(const Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(x.dim() >= 1, what, ": expected [..., C], got a scalar");
+  const int64_t c = x.size(-1);
+  int64_t m = 1;
+  for (int64_t i = 0; i < x.dim() - 1; ++i) m *= x.size(i);
+  Tensor t = x.reshape({m, c});
+  return t.stride(1) == 1 || c == 1 ? t : t.contiguous();
+}
+
+Tensor dense(const Tensor& t) { return t.contiguous(); }
+OptTensor dense(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : t; }
+
+void check_same(const Tensor& t, at::ScalarType dtype, const Tensor& like, const char* what) {
+  TORCH_CHECK_TYPE(t.scalar_type() == dtype, what, ": expected ", dtype, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == like.device(), what, ": on ", t.device(), ", expected ", like.device());
+}
+
+void check_vector(const OptTensor& t, int64_t n, const Tensor& like, const char* what) {
+  if (!t) return;
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n, what, ": expected ", n, " values, got shape ", t->sizes());
+  TORCH_CHECK_VALUE(t->device() == like.device(), what, ": on ", t->device(), ", expected ", like.device());
+}
+
+Tensor norm_workspace(const Tensor& x3, int64_t groups, int backward) {
+  int64_t floats = 0;
+  check(fim_group_norm_workspace(x3.size(0), x3.size(1), x3.size(2), groups, backward, &floats), "group_norm_act ",
+        x3.sizes(), " in ", groups, " groups");
+  return empty({floats}, x3, at::kFloat);
+}
+
+std::tuple<Tensor, Tensor> group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias,
+                                          double eps, int64_t act) {
+  const c10::DeviceGuard guard(x.device());
+  const Tensor v = image_rows(x, "group_norm_act");
+  const int64_t b = v.size(0), p = v.size(1), c = v.size(2);
+  TORCH_CHECK_VALUE(groups > 0 && c > 0 && c % groups == 0, "group_norm_act: ", c, " channels in ", groups, " groups");
+  check_vector(weight, c, x, "group_norm_act: weight");
+  check_vector(bias, c, x, "group_norm_act: bias");
+  const OptTensor w = dense(weight), bi = dense(bias);
+  Tensor out = empty(x.sizes(), x, x.scalar_type()), stats = empty({b, groups, 2}, x, at::kFloat);
+  const Tensor ws = norm_workspace(v, groups, 0);
+  check(fim_group_norm(v.data_ptr(), dtype_code(x), b, p, c, v.stride(0), v.stride(1), groups, ptr<const void>(w),
+                       float_code(w), ptr<const void>(bi), float_code(bi), (float)eps, (int)act, out.data_ptr(),
+                       ptr<float>(stats), ptr<float>(ws), stream_of(x)),
+        "group_norm_act ", x.sizes(), " in ", groups, " groups");
+  return {out, stats};
+}
+
+// d_weight and d_bias are empty where there is no weight or bias
+std::tuple<Tensor, Tensor, Tensor> group_norm_act_backward(const Tensor& d_out, const Tensor& x, const Tensor& stats,
+                                                           int64_t groups, const OptTensor& weight, const OptTensor& bias,
+                                                           int64_t act) {
+  const c10::DeviceGuard guard(x.device());
+  TORCH_CHECK_VALUE(d_out.sizes() == x.sizes(), "group_norm_act: gradient of shape ", d_out.sizes(), " for ", x.sizes());
+  check_same(d_out, x.scalar_type(), x, "group_norm_act: gradient");
+  const Tensor v = image_rows(x, "group_norm_act"), d = image_rows(d_out, "group_norm_act");
+  const int64_t b = v.size(0), p = v.size(1), c = v.size(2);
+  check_same(stats, at::kFloat, x, "group_norm_act: stats");
+  TORCH_CHECK_VALUE(stats.is_contiguous() && stats.numel() == 2 * b * groups, "group_norm_act: stats of shape ",
+                    stats.sizes());
+  check_vector(weight, c, x, "group_norm_act: weight");
+  check_vector(bias, c, x, "group_norm_act: bias");
+  const OptTensor w = dense(weight), bi = dense(bias);
+  Tensor dx = empty(x.sizes(), x, x.scalar_type());
+  Tensor dw = empty({weight ? c : 0}, x, weight ? weight->scalar_type() : at::kFloat);
+  Tensor db = empty({bias ? c : 0}, x, bias ? bias->scalar_type() : at::kFloat);
+  if (x.numel() == 0) {
+    dw.zero_();
+    db.zero_();
+    return {dx, dw, db};
+  }
+  const Tensor ws = norm_workspace(v, groups, 1);
+  check(fim_group_norm_backward(v.data_ptr(), d.data_ptr(), dtype_code(x), b, p, c, v.stride(0), v.stride(1), d.stride(0),
+                                d.stride(1), groups, ptr<const void>(w), float_code(w), ptr<const void>(bi),
+                                float_code(bi), (int)act, ptr<const float>(stats), dx.data_ptr(),
+                                weight ? dw.data_ptr() : nullptr, bias ? db.data_ptr() : nullptr, ptr<float>(ws),
+                                stream_of(x)),
+        "group_norm_act backward ", x.sizes(), " in ", groups, " groups");
+  return {dx, dw, db};
+}
+
+// The operands of a gated product, checked and as the C ABI reads them
+struct Gated {
+  Tensor x, wg, wu;
+  OptTensor bg, bu;
+  int64_t m, k, h;
+  int bias_dtype;
+  Gated(const Tensor& x_in, const Tensor& w_gate, const Tensor& w_up, const OptTensor& b_gate, const OptTensor& b_up) {
+    x = matrix_rows(x_in, "gated_linear");
+    m = x.size(0);
+    k = x.size(1);
+    check_dims(w_gate, 2, "gated_linear: w_gate");
+    h = w_gate.size(0);
+    TORCH_CHECK_VALUE(w_gate.size(1) == k && w_up.sizes() == w_gate.sizes(), "gated_linear: weights ", w_gate.sizes(),
+                      " and ", w_up.sizes(), " for ", k, " channels");
+    check_same(w_gate, x.scalar_type(), x, "gated_linear: w_gate");
+    check_same(w_up, x.scalar_type(), x, "gated_linear: w_up");
+    check_vector(b_gate, h, x, "gated_linear: b_gate");
+    check_vector(b_up, h, x, "gated_linear: b_up");
+    const auto& any = b_gate ? b_gate : b_up;
+    TORCH_CHECK_TYPE(!any || any->scalar_type() == at::kFloat || any->scalar_type() == x.scalar_type(),
+                     "gated_linear: biases of ", any->scalar_type(), " beside ", x.scalar_type());
+    TORCH_CHECK_TYPE(!b_gate || !b_up || b_gate->scalar_type() == b_up->scalar_type(),
+                     "gated_linear: biases of two types");
+    wg = matrix_rows(w_gate, "gated_linear");
+    wu = matrix_rows(w_up, "gated_linear");
+    bg = dense(b_gate);
+    bu = dense(b_up);
+    bias_dtype = float_code(any);
+  }
+};
+
+Tensor gated_workspace(const Gated& g, int backward) {
+  int64_t bytes = 0;
+  check(fim_gated_linear_workspace(g.m, g.k, g.h, backward, &bytes), "gated_linear ", g.m, "x", g.k, " -> ", g.h);
+  return empty({bytes}, g.x, at::kByte);
+}
+
+std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = last;
+  return sizes;
+}
+
+Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const OptTensor& b_gate,
+                    const OptTensor& b_up, int64_t act) {
+  const c10::DeviceGuard guard(x.device());
+  const Gated g(x, w_gate, w_up, b_gate, b_up);
+  Tensor out = empty(with_last(x, g.h), x, x.scalar_type());
+  const Tensor ws = gated_workspace(g, 0);
+  check(fim_gated_linear(g.x.data_ptr(), dtype_code(x), g.m, g.k, g.x.stride(0), g.wg.data_ptr(), g.wg.stride(0),
+                         g.wu.data_ptr(), g.wu.stride(0), g.h, ptr<const void>(g.bg), ptr<const void>(g.bu),
+                         g.bias_dtype, (int)act, out.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(x)),
+        "gated_linear ", g.m, "x", g.k, " -> ", g.h);
+  return out;
+}
+
+// Gradients that are not wanted come back empty.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward(
+    const Tensor& d_out, const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const OptTensor& b_gate,
+    const OptTensor& b_up, int64_t act, bool want_x, bool want_weights, bool want_biases) {
+  const c10::DeviceGuard guard(x.device());
+  const Gated g(x, w_gate, w_up, b_gate, b_up);
+  TORCH_CHECK_VALUE(d_out.sizes() == at::IntArrayRef(with_last(x, g.h)), "gated_linear: gradient of shape ",
+                    d_out.sizes(), " for ", x.sizes(), " -> ", g.h);
+  check_same(d_out, x.scalar_type(), x, "gated_linear: gradient");
+  const Tensor d = matrix_rows(d_out, "gated_linear");
+  auto weight_grad = [&](bool want) { return want ? empty({g.h, g.k}, x, x.scalar_type()) : empty({0}, x, x.scalar_type()); };
+  auto bias_grad = [&](const OptTensor& b) {
+    return empty({want_biases && b ? g.h : 0}, x, b ? b->scalar_type() : at::kFloat);
+  };
+  Tensor dx = want_x ? empty(x.sizes(), x, x.scalar_type()) : empty({0}, x, x.scalar_type());
+  Tensor dwg = weight_grad(want_weights), dwu = weight_grad(want_weights), dbg = bias_grad(b_gate), dbu = bias_grad(b_up);
+  if (g.m == 0) {
+    for (Tensor* t : {&dwg, &dwu, &dbg, &dbu}) t->zero_();
+    return {dx, dwg, dwu, dbg, dbu};
+  }
+  auto out = [](const Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; };
+  const Tensor ws = gated_workspace(g, 1);
+  check(fim_gated_linear_backward(g.x.data_ptr(), dtype_code(x), g.m, g.k, g.x.stride(0), g.wg.data_ptr(),
+                                  g.wg.stride(0), g.wu.data_ptr(), g.wu.stride(0), g.h, ptr<const void>(g.bg),
+                                  ptr<const void>(g.bu), g.bias_dtype, (int)act, d.data_ptr(), d.stride(0), out(dx),
+                                  out(dwg), out(dwu), out(dbg), out(dbu), ws.data_ptr(), ws.numel(), stream_of(x)),
+        "gated_linear backward ", g.m, "x", g.k, " -> ", g.h);
+  return {dx, dwg, dwu, dbg, dbu};
+}
+
+// The gradients of a list as the C ABI takes them: dense, each in the order of its memory
+struct GradList {
+  std::vector<Tensor> hold;
+  std::vector<const void*> ptrs;
+  std::vector<int> dtypes;
+  std::vector<int64_t> numel;
+  explicit GradList(at::TensorList grads) {
+    for (const Tensor& t : grads) {
+      TORCH_CHECK_VALUE(t.device() == grads[0].device(), "gradients on ", grads[0].device(), " and ", t.device());
+      hold.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+      ptrs.push_back(hold.back().data_ptr());
+      dtypes.push_back(dtype_code(t));
+      numel.push_back(t.numel());
+    }
+  }
+  int64_t count() const { return (int64_t)hold.size(); }
+};
+
+int norm_code(double norm_type) {
+  TORCH_CHECK_VALUE(norm_type == 2.0 || norm_type == std::numeric_limits<double>::infinity(),
+                    "the norm is 2 or infinity, got ", norm_type);
+  return norm_type == 2.0 ? 2 : 0;
+}
+
+Tensor grad_workspace(const GradList& g) {
+  int64_t doubles = 0;
+  check(fim_grad_norm_workspace(g.count(), g.numel.data(), &doubles), "grad_norm");
+  return empty({doubles}, g.hold[0], at::kDouble);
+}
+
+Tensor grad_norm(at::TensorList grads, double norm_type) {
+  TORCH_CHECK_VALUE(!grads.empty(), "grad_norm: no gradients");
+  const c10::DeviceGuard guard(grads[0].device());
+  const GradList g(grads);
+  Tensor total = empty({}, grads[0], at::kFloat);
+  const Tensor ws = grad_workspace(g);
+  check(fim_grad_norm(g.count(), g.ptrs.data(), g.dtypes.data(), g.numel.data(), norm_code(norm_type), ptr<float>(total),
+                      ptr<double>(ws), stream_of(grads[0])),
+        "grad_norm");
+  return total;
+}
+
+Tensor clip_grad_norm_out(at::TensorList grads, at::TensorList out, double max_norm, double norm_type) {
+  TORCH_CHECK_VALUE(!grads.empty(), "clip_grad_norm_: no gradients");
+  TORCH_CHECK_VALUE(grads.size() == out.size(), "clip_grad_norm_: ", out.size(), " outputs for ", grads.size(),
+                    " gradients");
+  const c10::DeviceGuard guard(grads[0].device());
+  const GradList g(grads);
+  std::vector<Tensor> to;  // written by the kernel: `out` itself where its memory lies as the gradient's
+  std::vector<void*> ptrs;
+  std::vector<int> dtypes;
+  for (size_t i = 0; i < out.size(); ++i) {
+    const Tensor& t = out[i];
+    TORCH_CHECK_VALUE(t.sizes() == grads[i].sizes() && t.device() == grads[0].device(), "clip_grad_norm_: output of shape ",
+                      t.sizes(), " on ", t.device(), " for a gradient of shape ", grads[i].sizes());
+    const Tensor& from = g.hold[i];
+    const bool same = t.is_non_overlapping_and_dense() && t.strides() == from.strides();
+    to.push_back(same ? t : at::empty_strided(from.sizes(), from.strides(), t.options().requires_grad(false)));
+    ptrs.push_back(to.back().data_ptr());
+    dtypes.push_back(dtype_code(t));
+  }
+  Tensor total = empty({}, grads[0], at::kFloat);
+  const Tensor ws = grad_workspace(g);
+  check(fim_clip_grad_norm(g.count(), g.ptrs.data(), g.dtypes.data(), ptrs.data(), dtypes.data(), g.numel.data(),
+                           (float)max_norm, norm_code(norm_type), ptr<float>(total), ptr<double>(ws),
+                           stream_of(grads[0])),
+        "clip_grad_norm_");
+  for (size_t i = 0; i < out.size(); ++i)
+    if (!to[i].is_same(out[i])) out[i].copy_(to[i]);
+  return total;
+}
+
+Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double norm_type) {
+  return clip_grad_norm_out(grads, grads, max_norm, norm_type);
+}
+
 }  // namespace
 
 #define FIM_GEO_SCHEMA "SymInt kh, SymInt kw, SymInt sh, SymInt sw, SymInt ph, SymInt pw, SymInt dh, SymInt dw"
@@ -468,17 +728,32 @@ Tensor pointwise_bf16(const Tensor& x, const Tensor& weight, const OptTensor& bi
                                       "Tensor pw_wscale, Tensor? pw_bias) -> Tensor")                                  \
   X(conv3x3_small_cin_quantize_int8, "(Tensor x, Tensor packed, Tensor bias, Tensor scale) -> Tensor")                 \
   X(bias_relu_quantize_int8, "(Tensor raw, Tensor bias, Tensor scale) -> Tensor")                                      \
-  X(pointwise_bf16, "(Tensor x, Tensor weight, Tensor? bias) -> Tensor")
+  X(pointwise_bf16, "(Tensor x, Tensor weight, Tensor? bias) -> Tensor")                                               \
+  X(group_norm_act_backward, "(Tensor d_out, Tensor x, Tensor stats, int groups, Tensor? weight, Tensor? bias, "       \
+                             "int act) -> (Tensor, Tensor, Tensor)")                                                   \
+  X(gated_linear_backward, "(Tensor d_out, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "       \
+                           "int act, bool want_x, bool want_weights, bool want_biases) "                               \
+                           "-> (Tensor, Tensor, Tensor, Tensor, Tensor)")                                              \
+  X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")                                                          \
+  X(clip_grad_norm_, "(Tensor(a!)[] grads, float max_norm, float norm_type) -> Tensor")                                \
+  X(clip_grad_norm_out, "(Tensor[] grads, Tensor(a!)[] out, float max_norm, float norm_type) -> Tensor")
+
+// those with derivative formulas (below)
+#define FIM_DIFFERENTIABLE_OPS(X)                                                                                      \
+  X(group_norm_act, "(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act) -> (Tensor, Tensor)")    \
+  X(gated_linear, "(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor")
 
 TORCH_LIBRARY(flashim_amd, m) {
 #define X(name, schema) m.def(#name schema, {at::Tag::pt2_compliant_tag});
   FIM_OPS(X)
+  FIM_DIFFERENTIABLE_OPS(X)
 #undef X
 }
 
 TORCH_LIBRARY_IMPL(flashim_amd, CUDA, m) {
 #define X(name, schema) m.impl(#name, TORCH_FN(name));
   FIM_OPS(X)
+  FIM_DIFFERENTIABLE_OPS(X)
 #undef X
 }
 
@@ -492,12 +767,15 @@ void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torc
   torch::autograd::variable_list inputs;  // that require a gradient
   if (at::GradMode::is_enabled()) {
     bool dual = false;
-    for (const c10::IValue& arg : torch::jit::last(*stack, op.schema().arguments().size()))
-      if (arg.isTensor()) {
-        const Tensor& t = arg.toTensor();
-        if (t.requires_grad()) inputs.push_back(t);
-        dual = dual || torch::autograd::isFwGradDefined(t);
-      }
+    auto look = [&](const Tensor& t) {
+      if (t.requires_grad()) inputs.push_back(t);
+      dual = dual || torch::autograd::isFwGradDefined(t);
+    };
+    for (const c10::IValue& arg : torch::jit::last(*stack, op.schema().arguments().size())) {
+      if (arg.isTensor()) look(arg.toTensor());
+      if (arg.isTensorList())
+        for (const Tensor& t : arg.toTensorVector()) look(t);
+    }
     TORCH_CHECK_NOT_IMPLEMENTED(inputs.empty() || !dual, name,
                                 ": no forward-mode derivative, and an input requires a gradient");
   }
@@ -513,15 +791,93 @@ void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torc
       torch::autograd::set_history(out.toTensor(), node);
 }
 
-// The version counter of the last argument, the tensor that is written, by which autograd finds a saved tensor that was
-// overwritten since (torch's own fallback counts for returned tensors only).
-void count_write_to_last(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
-  const Tensor out = stack->back().toTensor();
+// The version counters of the arguments that are written, by which autograd finds a saved tensor that was overwritten
+// since (torch's own fallback counts for returned tensors only).
+void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const auto& args = op.schema().arguments();
+  std::vector<Tensor> written;
+  for (size_t i = 0; i < args.size(); ++i) {
+    if (args[i].alias_info() == nullptr || !args[i].alias_info()->isWrite()) continue;
+    const c10::IValue& arg = torch::jit::peek(*stack, i, args.size());
+    if (arg.isTensor()) written.push_back(arg.toTensor());
+    if (arg.isTensorList())
+      for (const Tensor& t : arg.toTensorVector()) written.push_back(t);
+  }
   {
     at::AutoDispatchBelowADInplaceOrView guard;
     op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
   }
-  if (!out.is_inference()) torch::autograd::increment_version(out);
+  for (const Tensor& t : written)
+    if (!t.is_inference()) torch::autograd::increment_version(t);
+}
+
+// Derivatives: each a torch operator of its own, so that compiled graphs hold it (and a second derivative raises).
+OptTensor as_optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor as_tensor(const OptTensor& t) { return t ? *t : Tensor(); }
+
+template <typename Signature>
+c10::TypedOperatorHandle<Signature> typed_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+
+struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, int64_t groups,
+                                                const OptTensor& weight, const OptTensor& bias, double eps, int64_t act) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(group_norm_act)>("flashim_amd::group_norm_act");
+    auto [out, stats] = op.call(x, groups, weight, bias, eps, act);
+    ctx->save_for_backward({x, as_tensor(weight), as_tensor(bias), stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->mark_non_differentiable({stats});
+    return {out, stats};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    static const auto op = typed_op<decltype(group_norm_act_backward)>("flashim_amd::group_norm_act_backward");
+    auto [dx, dw, db] = op.call(grads[0], saved[0], saved[3], ctx->saved_data["groups"].toInt(), as_optional(saved[1]),
+                                as_optional(saved[2]), ctx->saved_data["act"].toInt());
+    return {dx, Tensor(), saved[1].defined() ? dw : Tensor(), saved[2].defined() ? db : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> group_norm_act_autograd(const Tensor& x, int64_t groups, const OptTensor& weight,
+                                                   const OptTensor& bias, double eps, int64_t act) {
+  auto out = GroupNormAct::apply(x, groups, weight, bias, eps, act);
+  return {out[0], out[1]};
+}
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                        const OptTensor& b_gate, const OptTensor& b_up, int64_t act) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(gated_linear)>("flashim_amd::gated_linear");
+    ctx->save_for_backward({x, w_gate, w_up, as_tensor(b_gate), as_tensor(b_up)});
+    ctx->saved_data["act"] = act;
+    return op.call(x, w_gate, w_up, b_gate, b_up, act);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const bool want_x = ctx->needs_input_grad(0);
+    const bool want_w = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    const bool bias[2] = {saved[3].defined(), saved[4].defined()};
+    bool want_b = false;  // (the edges count the tensors that are there)
+    for (int i = 3; i < 3 + bias[0] + bias[1]; ++i) want_b = want_b || ctx->needs_input_grad(i);
+    static const auto op = typed_op<decltype(gated_linear_backward)>("flashim_amd::gated_linear_backward");
+    auto [dx, dwg, dwu, dbg, dbu] = op.call(grads[0], saved[0], saved[1], saved[2], as_optional(saved[3]),
+                                            as_optional(saved[4]), ctx->saved_data["act"].toInt(), want_x, want_w, want_b);
+    return {want_x ? dx : Tensor(),  want_w ? dwg : Tensor(),           want_w ? dwu : Tensor(),
+            want_b && bias[0] ? dbg : Tensor(), want_b && bias[1] ? dbu : Tensor(), Tensor()};
+  }
+};
+
+Tensor gated_linear_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const OptTensor& b_gate,
+                             const OptTensor& b_up, int64_t act) {
+  return GatedLinear::apply(x, w_gate, w_up, b_gate, b_up, act);
 }
 
 }  // namespace
@@ -530,8 +886,11 @@ TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
 #define X(name, schema) m.impl(#name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
   FIM_OPS(X)
 #undef X
+  m.impl("group_norm_act", TORCH_FN(group_norm_act_autograd));
+  m.impl("gated_linear", TORCH_FN(gated_linear_autograd));
 }
 
 TORCH_LIBRARY_IMPL(flashim_amd, ADInplaceOrView, m) {
-  m.impl("int8_linear_quantize_", torch::CppFunction::makeFromBoxedFunction<&count_write_to_last>());
+  for (const char* name : {"int8_linear_quantize_", "clip_grad_norm_", "clip_grad_norm_out"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&count_writes>());
 }

@@ -232,6 +232,53 @@ def pointwise_bf16(x, weight, bias):
     return x.new_empty((x.shape[0], weight.shape[0]), dtype=torch.bfloat16)
 
 
+# -- training-step operators -----------------------------------------------------------------------------------------
+
+
+@_fake
+def group_norm_act(x, groups, weight, bias, eps, act):
+    """``x [B, ..., C]`` -> the normalized, activated map and the statistics ``[B, groups, 2]`` (mean, 1 / deviation);
+    differentiable in ``x``, ``weight`` and ``bias``."""
+    return x.new_empty(x.shape), x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)
+
+
+@_fake
+def group_norm_act_backward(d_out, x, stats, groups, weight, bias, act):
+    return (x.new_empty(x.shape),) + tuple(
+        x.new_empty((0,), dtype=torch.float32) if p is None else p.new_empty((x.shape[-1],)) for p in (weight, bias))
+
+
+@_fake
+def gated_linear(x, w_gate, w_up, b_gate, b_up, act):
+    """``act(x Wg^T + bg) * (x Wu^T + bu)`` of ``x [..., K]``; differentiable in every tensor."""
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+
+@_fake
+def gated_linear_backward(d_out, x, w_gate, w_up, b_gate, b_up, act, want_x, want_weights, want_biases):
+    """The gradients of x, both weights and both biases; those not wanted come back empty."""
+    h, k = w_gate.shape
+    return (x.new_empty(x.shape if want_x else (0,)),
+            *(x.new_empty((h, k) if want_weights else (0,)) for _ in range(2)),
+            *(x.new_empty((h if want_biases and b is not None else 0,),
+                          dtype=torch.float32 if b is None else b.dtype) for b in (b_gate, b_up)))
+
+
+@_fake
+def grad_norm(grads, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@_fake
+def clip_grad_norm_(grads, max_norm, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@_fake
+def clip_grad_norm_out(grads, out, max_norm, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
 # ``torch.ops.flashim_amd`` is there on import. A library that is built later is loaded on first use, and so is one that
 # does not load now (built against another torch, a missing HIP runtime): the first op raises the loader's error.
 if TORCH_LIBRARY.is_file():

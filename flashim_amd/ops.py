@@ -12,6 +12,7 @@ from __future__ import annotations
 from flashim_amd.backends.hip import conv as _conv
 from flashim_amd.backends.hip import gemm as _gemm
 from flashim_amd.backends.hip import quantize as _quantize
+from flashim_amd.backends.hip import train as _train
 from flashim_amd.dispatch import (  # noqa: F401  (re-exported API)
     OPS, BoundOp, DeviceSpec, Op, call_counts, configure, reset_call_counts,
 )
@@ -41,6 +42,11 @@ conv2d_small_cin_quantize_int8 = Op("conv2d_small_cin_quantize_int8", weights=2)
 bias_relu_quantize_int8 = Op("bias_relu_quantize_int8")
 # this backend's refiner-block producer (folded BatchNorm + GELU)
 depthwise5x5_gelu = Op("depthwise5x5_gelu")
+# this backend's training-step operators (differentiable, but for the last two)
+group_norm_act = Op("group_norm_act")
+gated_linear = Op("gated_linear")
+grad_norm = Op("grad_norm")
+clip_grad_norm_ = Op("clip_grad_norm_")
 
 ROCM = DeviceSpec("rocm")
 HIP = "hip"
@@ -72,6 +78,10 @@ IMPLS = (
     ("mxfp8_scaled_mm", _gemm.mxfp8_scaled_mm, _MX, _gemm.eligible_mxfp8_scaled_mm),
     ("mxfp8_gelu_mlp", _gemm.mxfp8_gelu_mlp, _MX, _gemm.eligible_mxfp8_gelu_mlp),
     ("bias_relu_quantize_int8", _conv.bias_relu_quantize_int8, (Feature.HIP,), _conv.eligible_bias_relu_quantize),
+    ("group_norm_act", _train.group_norm_act, (Feature.HIP,), _train.eligible_group_norm_act),
+    ("gated_linear", _train.gated_linear, (Feature.HIP,), _train.eligible_gated_linear),
+    ("grad_norm", _train.grad_norm, (Feature.HIP,), _train.eligible_grad_norm),
+    ("clip_grad_norm_", _train.clip_grad_norm_, (Feature.HIP,), _train.eligible_clip_grad_norm),
 )
 
 for _name, _fn, _requires, _when in IMPLS:

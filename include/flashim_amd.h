@@ -227,6 +227,65 @@ int fim_depthwise5x5_relu_pointwise_int8(const uint16_t* x, int64_t B, int64_t H
 int fim_pointwise_bf16(const uint16_t* x, int64_t M, int64_t K, const uint16_t* weight, int64_t N, const void* bias,
                        int bias_dtype, uint16_t* out, hipStream_t stream);
 
+/* ---- training-step operators: group norm with an activation, the gated feed-forward product, gradient clipping --- */
+
+/* Activation codes: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf form), 4 GELU (tanh form). */
+
+/* FP32 words of workspace that fim_group_norm (backward 0) or fim_group_norm_backward (1) needs. */
+int fim_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t groups, int backward, int64_t* floats);
+
+/* Group norm with an activation, channels last: x [B, P, C] (unit channel stride, image and pixel strides in elements),
+ * per (image, group) over P pixels and C / groups channels out = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]),
+ * biased variance, FP32 arithmetic, rounded once to x's type. weight, bias [C] of any float type, or NULL (1, 0).
+ * out packed [B, P, C]; stats FP32 [B, groups, 2]: mean and 1 / sqrt(var + eps), which the backward pass reads.
+ * C <= 8192 (else 99). No counterpart in the reference. */
+int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, int64_t C, int64_t stride_b, int64_t stride_p,
+                   int64_t groups, const void* weight, int weight_dtype, const void* bias, int bias_dtype, float eps,
+                   int act, void* out, float* stats, float* workspace, hipStream_t stream);
+
+/* Its gradients, from x and the forward pass's stats: d_out [B, P, C] (unit channel stride), dx packed [B, P, C], d_weight
+ * and d_bias [C] in the types of weight and bias (either may be NULL). */
+int fim_group_norm_backward(const void* x, const void* d_out, int dtype, int64_t B, int64_t P, int64_t C,
+                            int64_t stride_b, int64_t stride_p, int64_t d_stride_b, int64_t d_stride_p, int64_t groups,
+                            const void* weight, int weight_dtype, const void* bias, int bias_dtype, int act,
+                            const float* stats, void* dx, void* d_weight, void* d_bias, float* workspace,
+                            hipStream_t stream);
+
+/* Bytes of workspace that fim_gated_linear (backward 0) or fim_gated_linear_backward (1) needs (256-byte aligned). */
+int fim_gated_linear_workspace(int64_t M, int64_t K, int64_t H, int backward, int64_t* bytes);
+
+/* The gated feed-forward product out = act(x Wg^T + bg) * (x Wu^T + bu): x [M, K], weights [H, K] (unit column strides, row
+ * strides in elements), biases [H] FP32 or x's type (bias_dtype; either may be NULL), out packed [M, H]; BF16 or FP16
+ * (else 99) with FP32 sums, rounded once. No counterpart in the reference. */
+int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w_gate,
+                     int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int64_t H, const void* b_gate,
+                     const void* b_up, int bias_dtype, int act, void* out, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
+
+/* Its gradients: d_out [M, H] (unit column stride); dx packed [M, K], dw_gate and dw_up packed [H, K], db_gate and db_up
+ * [H] in the bias type; any of them may be NULL. The pre-activations are computed again; their gradients are rounded to
+ * x's type before the products that make dx and the weights' gradients. */
+int fim_gated_linear_backward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w_gate,
+                              int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int64_t H,
+                              const void* b_gate, const void* b_up, int bias_dtype, int act, const void* d_out,
+                              int64_t d_out_stride, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                              void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* 64-bit words of workspace that fim_grad_norm and fim_clip_grad_norm need for tensors of numel[count] elements. */
+int fim_grad_norm_workspace(int64_t count, const int64_t* numel, int64_t* doubles);
+
+/* *total (device, FP32) = the norm over all elements of `count` dense tensors (host arrays of device pointers, dtype codes
+ * and element counts): norm 2 the square root of the sum of squares (summed in 64 bits), norm 0 the largest magnitude. No
+ * counterpart in the reference, as the next. */
+int fim_grad_norm(int64_t count, const void* const* grads, const int* dtypes, const int64_t* numel, int norm,
+                  float* total, double* workspace, hipStream_t stream);
+
+/* The norm as above, and out[i] = grads[i] * min(1, max_norm / (*total + 1e-6)) (a NaN norm makes every element NaN).
+ * out[i] is grads[i] (in place) or does not overlap any gradient; its type may differ. */
+int fim_clip_grad_norm(int64_t count, const void* const* grads, const int* dtypes, void* const* out,
+                       const int* out_dtypes, const int64_t* numel, float max_norm, int norm, float* total,
+                       double* workspace, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
