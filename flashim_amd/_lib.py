@@ -68,7 +68,7 @@ SIGNATURES: dict[str, list] = {
     "fim_group_norm": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _vp],
     "fim_group_norm_backward": [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32,
                                 _vp, _vp, _vp, _vp, _vp, _vp],
-    "fim_gated_linear_workspace": [_i64, _i64, _i64, _i32, _vp],
+    "fim_gated_linear_workspace": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp],
     "fim_gated_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _vp, _i64,
                          _vp],
     "fim_gated_linear_backward": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _i64,

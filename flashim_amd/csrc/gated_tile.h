@@ -1,0 +1,428 @@
+// The matrix products of the gated feed-forward operator on large tiles: BF16 or FP16, FP32 sums.
+//
+// A workgroup of four wavefronts (2 x 2) computes 64 MB x 64 NB products on 32 x 32 x 16 MFMAs, each wavefront MB x NB
+// blocks. The contraction is walked in steps of 64: both operands of a step lie in one of two LDS stages, filled by
+// 16-byte loads straight into LDS. An operand whose rows run along the contraction is staged as rows of 128 bytes and read
+// in 16-byte pieces; one whose rows run across it (the weights for dx, both operands for the weights' gradients) is staged
+// as it lies, 64 rows of the tile's width, and read transposed by the LDS itself (ds_read_tr16_b64: each 16 lanes read a 4 x
+// 16 block and lane i gets its column i; layout measured), so nothing is transposed in memory. Both layouts are swizzled in
+// 16-byte or 64-byte units against bank conflicts.
+//
+// The loop's order: while the MFMAs of one 16-wide sub-step run, the operands of the next are read, one read between two
+// MFMAs; the next step's stage is waited for before the last sub-step, whose MFMAs cover the first reads from it, and from
+// then on the consumed stage is refilled. One barrier per step.
+#pragma once
+
+#include "activation.h"
+
+namespace fim {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <int DT>
+__device__ __forceinline__ v16f mfma16(s16x8 a, s16x8 b, v16f c) {
+  typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  if constexpr (DT == FIM_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint16_t to16(float v) {
+  return DT == FIM_BF16 ? (uint16_t)(pack_bf16x2(v, 0.0f) & 0xffff) : __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t to16x2(float a, float b) {
+  if constexpr (DT == FIM_BF16) return pack_bf16x2(a, b);
+  return (uint32_t)to16<DT>(a) | (uint32_t)to16<DT>(b) << 16;
+}
+template <int DT>
+__device__ __forceinline__ float from16(uint16_t h) {
+  return DT == FIM_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+}
+
+// FORWARD: out = act(g) u.  GRAD: the same products, out dg and du.  DX: dg Wg + du Wu.  DW: dg^T x and du^T x.
+enum { GATED_FORWARD, GATED_GRAD, GATED_DX, GATED_DW };
+
+// What a product's operands are: x supplies the output rows (the MFMA's columns, one per lane), w the output columns (its
+// rows, four neighbours per lane and register group). 16-byte aligned, row strides and widths multiples of 8, row strides
+// not below the width.
+struct TileArgs {
+  const uint16_t* x[2];  // FORWARD, GRAD: x[0]. DX: dg, du. DW: x[0], whose columns are the output rows
+  const uint16_t* w[2];  // FORWARD, GRAD, DX: gate, up. DW: dg, du, whose columns are the output columns
+  int64_t ldx, ldw;
+  int64_t M, N, K;       // output rows, columns (of one half), contraction (DX: of one half)
+  int64_t xw, ww;        // columns of x and w that may be read where they run across the contraction
+  const void* bias[2];
+  int bias_dtype;
+  const uint16_t* dout;
+  int64_t ldd;
+  uint16_t* out[2];
+  int64_t ldo, out_cols;  // columns written: N, or more (GRAD: with zeros)
+  int wide_out, wide_dout;  // rows of out and dout are 16-byte aligned
+  float* col_sums;        // GRAD: [2 m tiles][2][N] sums of dg and du over 32 MB rows, or null
+  float* part;            // DW: [splits][2][N][M]
+  int mt, nt, group;      // tiles; m tiles of a group that share the columns' operands in L2
+  int64_t k_split;        // DW: contraction of one split (a multiple of 64)
+};
+
+constexpr int TILE_K = 64;
+constexpr uint32_t TILE_OOB = 0x80000000u;  // past every buffer: reads as zero
+
+constexpr int tile_wait(int vm) { return (vm & 0xF) | (0x7 << 4) | (((vm >> 4) & 0x3) << 14); }  // and lgkmcnt(0)
+
+// Orders this wavefront's LDS writes before its reads of what other lanes wrote
+__device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// v[i] summed over the 32 lanes of this half wavefront; lane l returns the sum of v[l % 32]
+__device__ __forceinline__ float sum_lanes32(float (&v)[32], int lane) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const bool up = lane & s;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      const float keep = up ? v[i + s] : v[i], send = up ? v[i] : v[i + s];
+      v[i] = keep + __shfl_xor(send, s);
+    }
+  }
+  return v[0];
+}
+
+template <int DT, int MODE, int ACT, int MB, int NB>
+__global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(const TileArgs a) {
+  constexpr bool PAIR = MODE == GATED_FORWARD || MODE == GATED_GRAD;
+  constexpr bool XT = MODE == GATED_DW, WT = MODE == GATED_DX || MODE == GATED_DW;  // rows run across the contraction
+  constexpr int BM = 64 * MB, BN = 64 * NB;
+  constexpr int CX = BM / 32, CW = BN / 32;  // 1 KB loads of a stage per wavefront
+  constexpr int STAGE = (BM + BN) * 2 * TILE_K;
+  static_assert(!PAIR || NB % 2 == 0, "gate and up blocks");
+  __shared__ __attribute__((aligned(16))) uint8_t st0[STAGE];
+  __shared__ __attribute__((aligned(16))) uint8_t st1[STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1, h = lane >> 5;
+
+  // workgroups go round the 8 XCDs: each takes a contiguous run of tiles, group by group of m tiles, n slowest in a group
+  const int tiles = a.mt * a.nt;
+  const int per_xcd = (int)(gridDim.x >> 3);
+  int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+  const int splits = MODE == GATED_DW ? (int)((a.K + a.k_split - 1) / a.k_split) : 1;
+  if (t >= tiles * splits) return;
+  const int split = MODE == GATED_DW ? t / tiles : 0;
+  t -= split * tiles;
+  const int grp = t / (a.group * a.nt), in_grp = t - grp * a.group * a.nt;
+  const int gm = a.mt - grp * a.group < a.group ? a.mt - grp * a.group : a.group;
+  const int tn = in_grp / gm, tm = grp * a.group + in_grp - tn * gm;
+  const int half = MODE == GATED_DW ? tn & 1 : 0;
+  const int64_t m0 = (int64_t)tm * BM;
+  const int64_t n0 = PAIR ? (int64_t)tn * (BN / 2) : MODE == GATED_DW ? (int64_t)(tn >> 1) * BN : (int64_t)tn * BN;
+
+  const int64_t kb = split * a.k_split;
+  const int64_t klen = MODE == GATED_DW ? (a.K - kb < a.k_split ? a.K - kb : a.k_split) : a.K;
+  const int steps1 = (int)((klen + TILE_K - 1) / TILE_K);
+  const int steps = MODE == GATED_DX ? 2 * steps1 : steps1;
+
+  // -- loads into LDS: chunk c (1 KB) of an operand's part of a stage; wavefront w loads chunks w, w + 4, ... of each
+  // along: chunk c is rows 8 c .. 8 c + 7, lane l row l / 8, LDS slot l % 8, which holds K segment slot ^ (row / 2 % 8)
+  const int seg = (lane & 7) ^ (lane >> 4) ^ (4 * (wave & 1));
+  // across: a row of the stage has BM / 8 slots; slot s of row k holds column segment s ^ 4 (k % 4)
+  auto across_off = [&](int slots, int c, int64_t ld, int64_t cols) __attribute__((always_inline)) {
+    const int k = c * (64 / slots) + lane / slots, s = (lane % slots) ^ ((k & 3) << 2);
+    return s * 8 < cols ? (uint32_t)(k * ld + s * 8) * 2u : TILE_OOB;
+  };
+  uint32_t xo[CX], wo[CW];
+  const int64_t xrows = a.M - m0, wrows = a.N - n0;
+#pragma unroll
+  for (int i = 0; i < CX; ++i) {
+    const int c = wave + 4 * i, r = 8 * c + (lane >> 3);
+    if constexpr (XT) xo[i] = across_off(BM / 8, c, a.ldx, a.xw - m0);
+    else xo[i] = r < xrows ? (uint32_t)(r * a.ldx) * 2u + seg * 16 : TILE_OOB;
+  }
+#pragma unroll
+  for (int i = 0; i < CW; ++i) {
+    const int c = wave + 4 * i;
+    int r = 8 * c + (lane >> 3);
+    if (PAIR && i >= CW / 2) r -= BN / 2;
+    if constexpr (WT) wo[i] = across_off(BN / 8, c, a.ldw, a.ww - n0);
+    else wo[i] = r < wrows ? (uint32_t)(r * a.ldw) * 2u + seg * 16 : TILE_OOB;
+  }
+  // buffers of a tile: its first row (or column) to the end of the operand; bytes left of at most 2^31 - 1
+  auto rest = [](int64_t rows, int64_t ld, int64_t cols) __attribute__((always_inline)) {
+    const int64_t n = rows <= 0 ? 0 : ((rows - 1) * ld + cols) * 2;
+    return (int)(n < 0 ? 0 : n > 0x7fffffff ? 0x7fffffff : n);
+  };
+  int step_at = 0;  // the step whose loads are issued next
+  auto load = [](const uint16_t* p, int records, uint8_t* to, uint32_t off) __attribute__((always_inline)) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), (short)0, __builtin_amdgcn_readfirstlane(records),
+                                          0x00020000),
+        (lds_void*)to, 16, off, 0, 0, 0);
+  };
+  const int64_t kw = (a.K + 7) / 8 * 8;  // whole loads: the operand's rows are padded to them
+  const int xrec = XT ? 0 : rest(xrows < BM ? xrows : BM, a.ldx, kw);
+  const int wrec = WT ? 0 : rest(wrows < BN ? wrows : BN, a.ldw, kw);
+  // per step: scalars, and the lane's K offset of an operand along the contraction
+  uint32_t kbyte, kdead;
+  int64_t krow;
+  int part;
+  auto next_step = [&]() __attribute__((always_inline)) {
+    part = MODE == GATED_DX && step_at >= steps1 ? 1 : 0;
+    const int64_t k0 = (int64_t)(step_at - part * steps1) * TILE_K;
+    kbyte = (uint32_t)k0 * 2u;
+    kdead = step_at < steps && k0 + seg * 8 < a.K ? 0u : TILE_OOB;
+    krow = step_at < steps ? k0 : klen;  // past the last step: no rows are left
+    ++step_at;
+  };
+  // load i of the step: x's, then w's
+  auto issue = [&](uint8_t* st, int i) __attribute__((always_inline)) {
+    if (i < CX) {
+      uint8_t* to = st + (wave + 4 * i) * 1024;
+      if constexpr (XT)
+        load(a.x[0] + (kb + krow) * a.ldx + m0, rest(klen - krow, a.ldx, a.xw - m0), to, xo[i]);
+      else
+        load(a.x[MODE == GATED_DX ? part : 0] + m0 * a.ldx, xrec, to, (xo[i] + kbyte) | kdead);
+    } else if (i < CX + CW) {
+      const int k = i - CX;
+      uint8_t* to = st + BM * 2 * TILE_K + (wave + 4 * k) * 1024;
+      if constexpr (WT)
+        load(a.w[MODE == GATED_DX ? part : half] + (kb + krow) * a.ldw + n0, rest(klen - krow, a.ldw, a.ww - n0), to, wo[k]);
+      else
+        load(a.w[k >= CW / 2] + n0 * a.ldw, wrec, to, (wo[k] + kbyte) | kdead);
+    }
+  };
+
+  // -- operand fragments: lane l holds row (or column) l % 32 of a block, contraction 8 h .. 8 h + 7 of a 16-wide sub-step
+  const int frow = lane & 31;
+  const int fsw = (frow >> 1) & 7;
+  const int tq = (lane & 15) >> 2;
+  const int tcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  auto read_along = [&](const uint8_t* base, int row0, int kk) __attribute__((always_inline)) {
+    return *reinterpret_cast<const s16x8*>(base + (row0 + frow) * 2 * TILE_K + (((2 * kk + h) ^ fsw) << 4));
+  };
+  auto read_across = [&](const uint8_t* base, int rowb, int blk, int kk) __attribute__((always_inline)) {
+    const uint8_t* p = base + (kk * 16 + 8 * h + tq) * rowb + ((blk ^ tq) << 6) + tcol;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * rowb));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  s16x8 fx[2][MB], fw[2][NB];
+  // read r of a sub-step's MB + NB into set s
+  auto read = [&](const uint8_t* st, int s, int kk, int r) __attribute__((always_inline)) {
+    if (r < NB) {
+      const uint8_t* base = st + BM * 2 * TILE_K;
+      if constexpr (WT) fw[s][r] = read_across(base, BN * 2, wn * NB + r, kk);
+      else if constexpr (PAIR) fw[s][r] = read_along(base, (r / (NB / 2)) * (BN / 2) + (wn * (NB / 2) + r % (NB / 2)) * 32, kk);
+      else fw[s][r] = read_along(base, (wn * NB + r) * 32, kk);
+    } else if (r < NB + MB) {
+      if constexpr (XT) fx[s][r - NB] = read_across(st, BM * 2, wm * MB + r - NB, kk);
+      else fx[s][r - NB] = read_along(st, (wm * MB + r - NB) * 32, kk);
+    }
+  };
+
+  // accumulators: lane l, register q of block (i, j): row 32 j + l % 32, column 32 i + 8 (q / 4) + 4 h + q % 4
+  v16f acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    v16f first;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) first[q] = 0.0f;
+    if constexpr (PAIR) {  // started at the bias
+      const void* b = a.bias[i / (NB / 2)];
+      if (b != nullptr) {
+        const int64_t c0 = n0 + (wn * (NB / 2) + i % (NB / 2)) * 32 + 4 * h;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int64_t c = c0 + 8 * (q >> 2) + (q & 3);
+          if (c < a.N)
+            first[q] = a.bias_dtype == FIM_F32 ? static_cast<const float*>(b)[c]
+                                               : from16<DT>(static_cast<const uint16_t*>(b)[c]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[i][j] = first;
+  }
+
+  constexpr int T = MB * NB, READS = MB + NB, LOADS = CX + CW;
+  // The MFMAs of sub-step kk from set s, with READS reads of the next one (from stage `rd`, into set 1 - s) and loads
+  // [l0, l1) of the next step spread between them
+  auto sub_step = [&](int s, const uint8_t* rd, int rkk, uint8_t* fill, int l0, int l1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < T; ++m) {
+      const int i = m % NB, j = m / NB;
+      acc[i][j] = mfma16<DT>(fw[s][i], fx[s][j], acc[i][j]);
+#pragma unroll
+      for (int r = 0; r < READS; ++r)
+        if (r * T / READS == m) read(rd, 1 - s, rkk, r);
+#pragma unroll
+      for (int l = 0; l < LOADS; ++l)
+        if (l >= l0 && l < l1 && (l - l0) * T / (l1 - l0) == m) issue(fill, l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr int L1 = (LOADS + 1) / 2;  // loads issued in the sub-step after the barrier; the others in the next
+  // one step from stage cur, whose refill for two steps on begins after the barrier; the rest of nxt's loads first
+  auto step = [&](uint8_t* cur, uint8_t* nxt) __attribute__((always_inline)) {
+    sub_step(0, cur, 1, nxt, L1, LOADS);
+    next_step();
+    sub_step(1, cur, 2, nxt, 0, 0);
+    sub_step(0, cur, 3, nxt, 0, 0);
+    __builtin_amdgcn_s_waitcnt(tile_wait(0));  // nxt has landed, cur has been read
+    asm volatile("s_barrier" ::: "memory");
+    sub_step(1, nxt, 0, cur, 0, L1);
+  };
+
+  next_step();
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) issue(st0, l);
+  next_step();
+#pragma unroll
+  for (int l = 0; l < L1; ++l) issue(st1, l);
+  __builtin_amdgcn_s_waitcnt(tile_wait(L1));
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < READS; ++r) read(st0, 0, 0, r);
+  // pairs of steps: one exit; a step past the last multiplies zeros
+  for (int k = 0; k < steps; k += 2) {
+    step(st0, st1);
+    step(st1, st0);
+  }
+  __builtin_amdgcn_s_waitcnt(tile_wait(0));
+  asm volatile("s_barrier" ::: "memory");
+
+  // -- epilogue
+  const int64_t mw = m0 + wm * MB * 32;
+  if constexpr (MODE == GATED_DW) {  // lanes are neighbouring columns of the weight: 128-byte runs
+    float* to = a.part + (int64_t)(split * 2 + half) * a.N * a.M;
+    const int64_t nw = n0 + wn * NB * 32 + 4 * h;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int64_t n = nw + 32 * i + 8 * (q >> 2) + (q & 3);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+          const int64_t m = mw + 32 * j + frow;
+          if (n < a.N && m < a.M) to[n * a.M + m] = acc[i][j][q];
+        }
+      }
+  } else {
+    // 32 rows at a time through LDS (this wavefront's own part of the consumed stage): whole runs of the output's rows
+    constexpr int NO = PAIR ? NB / 2 : NB, OC = 32 * NO, RB = OC * 2, SLOTS = RB / 16, PER = 64 / SLOTS;
+    constexpr int AREA = 32 * RB, AREAS = MODE == GATED_GRAD ? 2 : 1;
+    static_assert(4 * AREAS * AREA <= STAGE, "the wavefronts' areas lie in the first stage");
+    uint8_t* area = st0 + wave * AREAS * AREA;
+    auto place = [&](int row, int slot) __attribute__((always_inline)) {
+      constexpr int RPL = RB >= 256 ? 1 : 256 / RB;
+      return row * RB + ((slot ^ ((row / RPL) & (SLOTS - 1))) << 4);
+    };
+    const int64_t nw = n0 + wn * OC;
+    const int slot = lane % SLOTS, prow = lane / SLOTS;
+    const int64_t col = nw + slot * 8;
+    float sums[MODE == GATED_GRAD ? NB : 1][16];
+    if constexpr (MODE == GATED_GRAD) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sums[i][q] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      if constexpr (MODE == GATED_GRAD) {  // the incoming gradient's rows into the first area
+#pragma unroll
+        for (int p = 0; p < 32 / PER; ++p) {
+          const int row = p * PER + prow;
+          const int64_t m = mw + 32 * j + row;
+          uint4 v = {0, 0, 0, 0};
+          if (m < a.M && col < a.N) {
+            const uint16_t* from = a.dout + m * a.ldd + col;
+            if (a.wide_dout && col + 8 <= a.N) {
+              v = *reinterpret_cast<const uint4*>(from);
+            } else {
+              uint32_t e[8];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) e[c] = col + c < a.N ? from[c] : 0;
+              v = uint4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+            }
+          }
+          *reinterpret_cast<uint4*>(area + place(row, slot)) = v;
+        }
+        wave_lds_wait();
+      }
+#pragma unroll
+      for (int o = 0; o < NO; ++o)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint8_t* at = area + place(frow, 4 * o + q) + 8 * h;
+          if constexpr (MODE == GATED_FORWARD) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(acc[o][j][4 * q + e]) * acc[o + NO][j][4 * q + e];
+            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
+          } else if constexpr (MODE == GATED_DX) {
+            const v16f& s = acc[o][j];
+            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(s[4 * q], s[4 * q + 1]), to16x2<DT>(s[4 * q + 2], s[4 * q + 3])};
+          } else {
+            const uint2 d2 = *reinterpret_cast<const uint2*>(at);
+            const uint16_t d[4] = {(uint16_t)d2.x, (uint16_t)(d2.x >> 16), (uint16_t)d2.y, (uint16_t)(d2.y >> 16)};
+            float dg[4], du[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float slope;
+              const float act = activate<ACT, true>(acc[o][j][4 * q + e], slope);
+              const float dv = from16<DT>(d[e]);
+              dg[e] = dv * acc[o + NO][j][4 * q + e] * slope;
+              du[e] = dv * act;
+              if (mw + 32 * j + frow >= a.M) dg[e] = du[e] = 0.0f;  // (zeros times what the padding rows gave)
+              sums[o][4 * q + e] += dg[e];
+              sums[o + NO][4 * q + e] += du[e];
+            }
+            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(dg[0], dg[1]), to16x2<DT>(dg[2], dg[3])};
+            *reinterpret_cast<uint2*>(at + AREA) = uint2{to16x2<DT>(du[0], du[1]), to16x2<DT>(du[2], du[3])};
+          }
+        }
+      wave_lds_wait();
+#pragma unroll
+      for (int k = 0; k < AREAS; ++k)
+#pragma unroll
+        for (int p = 0; p < 32 / PER; ++p) {
+          const int row = p * PER + prow;
+          const int64_t m = mw + 32 * j + row;
+          const uint4 v = *reinterpret_cast<const uint4*>(area + k * AREA + place(row, slot));
+          if (m >= a.M || col >= a.out_cols) continue;
+          uint16_t* to = a.out[k] + m * a.ldo + col;
+          if (a.wide_out && col + 8 <= a.out_cols) {
+            *reinterpret_cast<uint4*>(to) = v;
+          } else {
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (col + c < a.out_cols) to[c] = (uint16_t)(e[c / 2] >> (16 * (c & 1)));
+          }
+        }
+      wave_lds_wait();
+    }
+    if constexpr (MODE == GATED_GRAD) {
+      if (a.col_sums == nullptr) return;
+      // lane l: value l % 32 of each 32: block (value / 16), register value % 16
+#pragma unroll
+      for (int i = 0; i < NB; i += 2) {
+        float v[32];
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] = sums[i + (q >> 4)][q & 15];
+        const float s = sum_lanes32(v, lane);
+        const int blk = i + (frow >> 4), q = frow & 15;
+        const int64_t n = nw + 32 * (blk % NO) + 8 * (q >> 2) + 4 * h + (q & 3);
+        if (n < a.N) a.col_sums[((int64_t)(tm * 2 + wm) * 2 + blk / NO) * a.N + n] = s;
+      }
+    }
+  }
+}
+
+}  // namespace fim

@@ -561,7 +561,9 @@ struct Gated {
 
 Tensor gated_workspace(const Gated& g, int backward) {
   int64_t bytes = 0;
-  check(fim_gated_linear_workspace(g.m, g.k, g.h, backward, &bytes), "gated_linear ", g.m, "x", g.k, " -> ", g.h);
+  check(fim_gated_linear_workspace(g.x.data_ptr(), g.m, g.k, g.x.stride(0), g.wg.data_ptr(), g.wg.stride(0),
+                                   g.wu.data_ptr(), g.wu.stride(0), g.h, backward, &bytes),
+        "gated_linear ", g.m, "x", g.k, " -> ", g.h);
   return empty({bytes}, g.x, at::kByte);
 }
 

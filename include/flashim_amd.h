@@ -251,8 +251,11 @@ int fim_group_norm_backward(const void* x, const void* d_out, int dtype, int64_t
                             const float* stats, void* dx, void* d_weight, void* d_bias, float* workspace,
                             hipStream_t stream);
 
-/* Bytes of workspace that fim_gated_linear (backward 0) or fim_gated_linear_backward (1) needs (256-byte aligned). */
-int fim_gated_linear_workspace(int64_t M, int64_t K, int64_t H, int backward, int64_t* bytes);
+/* Bytes of workspace (256-byte aligned) that fim_gated_linear (backward 0) or fim_gated_linear_backward (1) needs with
+ * these operands: those whose rows are not 16-byte aligned, or lie 2^22 elements apart, are copied there first. */
+int fim_gated_linear_workspace(const void* x, int64_t M, int64_t K, int64_t x_stride, const void* w_gate,
+                               int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int64_t H, int backward,
+                               int64_t* bytes);
 
 /* The gated feed-forward product out = act(x Wg^T + bg) * (x Wu^T + bu): x [M, K], weights [H, K] (unit column strides, row
  * strides in elements), biases [H] FP32 or x's type (bias_dtype; either may be NULL), out packed [M, H]; BF16 or FP16
