@@ -100,7 +100,7 @@ struct Gated {
   int64_t M, K, H;
   // workspace, in bytes: copies of the operands; backward: dg and du [M, hp], bias partials, weight partials
   int64_t x_at, wg_at, wu_at, dgu_at, cols_at, part_at, total;
-  int64_t hp, splits, k_split;
+  int64_t hp, ldg, splits, k_split;
   Tile grad, dw;
 };
 
@@ -119,10 +119,11 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.wu_at = g.wg_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
   g.total = g.wu_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
   g.hp = cdiv(g.H, 8) * 8;
+  g.ldg = cdiv(g.H, 64) * 64 + 64;
   if (!backward) return g;
   g.grad = gated_tile(g.M, 2 * g.H, 1);
   g.dgu_at = g.total;
-  g.cols_at = g.dgu_at + align256(2 * g.M * g.hp * 2);
+  g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
   g.part_at = g.cols_at + align256(2 * cdiv(g.M, 64 * g.grad.mb) * 2 * g.H * 4);
   g.dw = gated_tile(g.K, 2 * g.H, cdiv(g.M, 4096));
   const int64_t tiles = cdiv(g.K, 64 * g.dw.mb) * 2 * cdiv(g.H, 64 * g.dw.nb);
@@ -257,7 +258,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   gated_operands(g, ws, stream);
   uint16_t* dg = reinterpret_cast<uint16_t*>(ws + g.dgu_at);
-  uint16_t* du = dg + M * g.hp;
+  uint16_t* du = dg + M * g.ldg;
   const bool biases = db_gate != nullptr || db_up != nullptr;
   TileArgs a = gated_forward_args(g, b_gate, b_up, bias_dtype);
   a.dout = static_cast<const uint16_t*>(d_out);
@@ -265,7 +266,8 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   a.wide_dout = rows_wide(d_out, d_out_stride);
   a.out[0] = dg;
   a.out[1] = du;
-  a.ldo = a.out_cols = g.hp;
+  a.ldo = g.ldg;
+  a.out_cols = g.hp;
   a.wide_out = 1;
   a.col_sums = biases ? reinterpret_cast<float*>(ws + g.cols_at) : nullptr;
   with_type(dtype, [&](auto dt) {
@@ -282,7 +284,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       d.x[1] = du;
       d.w[0] = g.wg.p;
       d.w[1] = g.wu.p;
-      d.ldx = g.hp;
+      d.ldx = g.ldg;
       d.ldw = g.wg.ld;
       d.M = M;
       d.N = K;
@@ -299,7 +301,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       w.w[0] = dg;
       w.w[1] = du;
       w.ldx = g.x.ld;
-      w.ldw = g.hp;
+      w.ldw = g.ldg;
       w.M = K;
       w.N = H;
       w.K = M;

@@ -114,11 +114,13 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
   const int splits = MODE == GATED_DW ? (int)((a.K + a.k_split - 1) / a.k_split) : 1;
   if (t >= tiles * splits) return;
-  const int split = MODE == GATED_DW ? t / tiles : 0;
+  const int split = MODE == GATED_DW ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
   t -= split * tiles;
   const int grp = t / (a.group * a.nt), in_grp = t - grp * a.group * a.nt;
   const int gm = a.mt - grp * a.group < a.group ? a.mt - grp * a.group : a.group;
-  const int tn = in_grp / gm, tm = grp * a.group + in_grp - tn * gm;
+  // (quotients come from the vector unit: back to scalars, or every buffer descriptor becomes a loop over lanes)
+  const int tn = __builtin_amdgcn_readfirstlane(in_grp / gm);
+  const int tm = __builtin_amdgcn_readfirstlane(grp * a.group + in_grp - tn * gm);
   const int half = MODE == GATED_DW ? tn & 1 : 0;
   const int64_t m0 = (int64_t)tm * BM;
   const int64_t n0 = PAIR ? (int64_t)tn * (BN / 2) : MODE == GATED_DW ? (int64_t)(tn >> 1) * BN : (int64_t)tn * BN;
@@ -152,10 +154,9 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
     if constexpr (WT) wo[i] = across_off(BN / 8, c, a.ldw, a.ww - n0);
     else wo[i] = r < wrows ? (uint32_t)(r * a.ldw) * 2u + seg * 16 : TILE_OOB;
   }
-  // buffers of a tile: its first row (or column) to the end of the operand; bytes left of at most 2^31 - 1
+  // bytes from a tile's first element to the end of its operand
   auto rest = [](int64_t rows, int64_t ld, int64_t cols) __attribute__((always_inline)) {
-    const int64_t n = rows <= 0 ? 0 : ((rows - 1) * ld + cols) * 2;
-    return (int)(n < 0 ? 0 : n > 0x7fffffff ? 0x7fffffff : n);
+    return rows <= 0 ? 0 : ((rows - 1) * ld + cols) * 2;
   };
   int step_at = 0;  // the step whose loads are issued next
   auto load = [](const uint16_t* p, int records, uint8_t* to, uint32_t off) __attribute__((always_inline)) {
@@ -165,33 +166,48 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
         (lds_void*)to, 16, off, 0, 0, 0);
   };
   const int64_t kw = (a.K + 7) / 8 * 8;  // whole loads: the operand's rows are padded to them
-  const int xrec = XT ? 0 : rest(xrows < BM ? xrows : BM, a.ldx, kw);
-  const int wrec = WT ? 0 : rest(wrows < BN ? wrows : BN, a.ldw, kw);
-  // per step: scalars, and the lane's K offset of an operand along the contraction
+  const int xrec = XT ? 0 : (int)rest(xrows < BM ? xrows : BM, a.ldx, kw);
+  const int wrec = WT ? 0 : (int)rest(wrows < BN ? wrows : BN, a.ldw, kw);
+  // per step: the lane's K offset of an operand along the contraction; first row and bytes left of one across it
   uint32_t kbyte, kdead;
-  int64_t krow;
-  int part;
-  auto next_step = [&]() __attribute__((always_inline)) {
-    part = MODE == GATED_DX && step_at >= steps1 ? 1 : 0;
-    const int64_t k0 = (int64_t)(step_at - part * steps1) * TILE_K;
-    kbyte = (uint32_t)k0 * 2u;
-    kdead = step_at < steps && k0 + seg * 8 < a.K ? 0u : TILE_OOB;
-    krow = step_at < steps ? k0 : klen;  // past the last step: no rows are left
-    ++step_at;
+  const uint16_t *xp = XT ? a.x[0] + kb * a.ldx + m0 : a.x[0] + m0 * a.ldx;
+  const uint16_t *wp = MODE == GATED_DX ? a.w[0] + n0 : a.w[half] + kb * a.ldw + n0;
+  int64_t xleft = rest(klen, a.ldx, a.xw - m0), wleft = rest(klen, a.ldw, a.ww - n0);
+  auto bytes = [](int64_t left) __attribute__((always_inline)) {
+    return (int)(left <= 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left);
   };
+  int xbytes = XT ? bytes(xleft) : xrec, wbytes = bytes(wleft);
+  auto next_step = [&]() __attribute__((always_inline)) {
+    ++step_at;
+    if constexpr (MODE == GATED_DX) {
+      const bool second = step_at == steps1;  // on to the other half
+      kbyte = second ? 0u : kbyte + 2 * TILE_K;
+      xp = second ? a.x[1] + m0 * a.ldx : xp;
+      wp = second ? a.w[1] + n0 : wp + TILE_K * a.ldw;
+      wleft = second ? rest(klen, a.ldw, a.ww - n0) : wleft - TILE_K * a.ldw * 2;
+    } else {
+      kbyte += 2 * TILE_K;
+      xp += XT ? TILE_K * a.ldx : 0;
+      xleft -= TILE_K * a.ldx * 2;
+      wp += TILE_K * a.ldw;
+      wleft -= TILE_K * a.ldw * 2;
+    }
+    if constexpr (XT) xbytes = bytes(xleft);
+    if constexpr (WT) wbytes = bytes(wleft);
+    kdead = step_at < steps && kbyte + seg * 16 < (uint32_t)a.K * 2u ? 0u : TILE_OOB;
+  };
+  kbyte = 0;
+  kdead = steps > 0 && seg * 8 < a.K ? 0u : TILE_OOB;
   // load i of the step: x's, then w's
   auto issue = [&](uint8_t* st, int i) __attribute__((always_inline)) {
     if (i < CX) {
       uint8_t* to = st + (wave + 4 * i) * 1024;
-      if constexpr (XT)
-        load(a.x[0] + (kb + krow) * a.ldx + m0, rest(klen - krow, a.ldx, a.xw - m0), to, xo[i]);
-      else
-        load(a.x[MODE == GATED_DX ? part : 0] + m0 * a.ldx, xrec, to, (xo[i] + kbyte) | kdead);
+      if constexpr (XT) load(xp, xbytes, to, xo[i]);
+      else load(xp, xbytes, to, (xo[i] + kbyte) | kdead);
     } else if (i < CX + CW) {
       const int k = i - CX;
       uint8_t* to = st + BM * 2 * TILE_K + (wave + 4 * k) * 1024;
-      if constexpr (WT)
-        load(a.w[MODE == GATED_DX ? part : half] + (kb + krow) * a.ldw + n0, rest(klen - krow, a.ldw, a.ww - n0), to, wo[k]);
+      if constexpr (WT) load(wp, wbytes, to, wo[k]);
       else
         load(a.w[k >= CW / 2] + n0 * a.ldw, wrec, to, (wo[k] + kbyte) | kdead);
     }
@@ -202,26 +218,30 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   const int fsw = (frow >> 1) & 7;
   const int tq = (lane & 15) >> 2;
   const int tcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-  auto read_along = [&](const uint8_t* base, int row0, int kk) __attribute__((always_inline)) {
-    return *reinterpret_cast<const s16x8*>(base + (row0 + frow) * 2 * TILE_K + (((2 * kk + h) ^ fsw) << 4));
+  // (one addition to the stage's address: the compiler tells a stage's reads from the loads in flight into the other by the
+  // pointers' origin, which it follows through few steps)
+  auto read_along = [&](const uint8_t* st, int at, int row0, int kk) __attribute__((always_inline)) {
+    const int off = at + (row0 + frow) * 2 * TILE_K + (((2 * kk + h) ^ fsw) << 4);
+    return *reinterpret_cast<const s16x8*>(st + off);
   };
-  auto read_across = [&](const uint8_t* base, int rowb, int blk, int kk) __attribute__((always_inline)) {
-    const uint8_t* p = base + (kk * 16 + 8 * h + tq) * rowb + ((blk ^ tq) << 6) + tcol;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * rowb));
+  auto read_across = [&](const uint8_t* st, int at, int rowb, int blk, int kk) __attribute__((always_inline)) {
+    const int off = at + (kk * 16 + 8 * h + tq) * rowb + ((blk ^ tq) << 6) + tcol;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st + off));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st + (off + 4 * rowb)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   s16x8 fx[2][MB], fw[2][NB];
   // read r of a sub-step's MB + NB into set s
   auto read = [&](const uint8_t* st, int s, int kk, int r) __attribute__((always_inline)) {
+    constexpr int W_AT = BM * 2 * TILE_K;
     if (r < NB) {
-      const uint8_t* base = st + BM * 2 * TILE_K;
-      if constexpr (WT) fw[s][r] = read_across(base, BN * 2, wn * NB + r, kk);
-      else if constexpr (PAIR) fw[s][r] = read_along(base, (r / (NB / 2)) * (BN / 2) + (wn * (NB / 2) + r % (NB / 2)) * 32, kk);
-      else fw[s][r] = read_along(base, (wn * NB + r) * 32, kk);
+      if constexpr (WT) fw[s][r] = read_across(st, W_AT, BN * 2, wn * NB + r, kk);
+      else if constexpr (PAIR)
+        fw[s][r] = read_along(st, W_AT, (r / (NB / 2)) * (BN / 2) + (wn * (NB / 2) + r % (NB / 2)) * 32, kk);
+      else fw[s][r] = read_along(st, W_AT, (wn * NB + r) * 32, kk);
     } else if (r < NB + MB) {
-      if constexpr (XT) fx[s][r - NB] = read_across(st, BM * 2, wm * MB + r - NB, kk);
-      else fx[s][r - NB] = read_along(st, (wm * MB + r - NB) * 32, kk);
+      if constexpr (XT) fx[s][r - NB] = read_across(st, 0, BM * 2, wm * MB + r - NB, kk);
+      else fx[s][r - NB] = read_along(st, 0, (wm * MB + r - NB) * 32, kk);
     }
   };
 
@@ -278,7 +298,6 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
     sub_step(1, nxt, 0, cur, 0, L1);
   };
 
-  next_step();
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) issue(st0, l);
   next_step();
