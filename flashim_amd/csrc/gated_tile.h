@@ -79,18 +79,17 @@ constexpr int tile_wait(int vm) { return (vm & 0xF) | (0x7 << 4) | (((vm >> 4) &
 // Orders this wavefront's LDS writes before its reads of what other lanes wrote
 __device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// v[i] summed over the 32 lanes of this half wavefront; lane l returns the sum of v[l % 32]
-__device__ __forceinline__ float sum_lanes32(float (&v)[32], int lane) {
+// v[i] summed over the 32 lanes of this half wavefront; lane l ends with the sum of v[l % 32] in v[0]. Each step halves the
+// values: a lane keeps one half and adds the other lane's (31 exchanges for 32 sums).
+template <int S>
+__device__ __forceinline__ void sum_lanes(float (&v)[32], int lane) {
+  const bool up = lane & S;
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    const bool up = lane & s;
-#pragma unroll
-    for (int i = 0; i < s; ++i) {
-      const float keep = up ? v[i + s] : v[i], send = up ? v[i] : v[i + s];
-      v[i] = keep + __shfl_xor(send, s);
-    }
+  for (int i = 0; i < S; ++i) {
+    const float keep = up ? v[i + S] : v[i], send = up ? v[i] : v[i + S];
+    v[i] = keep + __shfl_xor(send, S);
   }
-  return v[0];
+  if constexpr (S > 1) sum_lanes<S / 2>(v, lane);
 }
 
 template <int DT, int MODE, int ACT, int MB, int NB>
@@ -435,10 +434,10 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
         float v[32];
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] = sums[i + (q >> 4)][q & 15];
-        const float s = sum_lanes32(v, lane);
+        sum_lanes<16>(v, lane);
         const int blk = i + (frow >> 4), q = frow & 15;
         const int64_t n = nw + 32 * (blk % NO) + 8 * (q >> 2) + 4 * h + (q & 3);
-        if (n < a.N) a.col_sums[((int64_t)(tm * 2 + wm) * 2 + blk / NO) * a.N + n] = s;
+        if (n < a.N) a.col_sums[((int64_t)(tm * 2 + wm) * 2 + blk / NO) * a.N + n] = v[0];
       }
     }
   }
