@@ -10,7 +10,7 @@ them; here they train a channels-last block before it is quantized, and run it u
 from __future__ import annotations
 
 import math
-from collections.abc import Iterable
+from collections.abc import Sequence
 
 import torch
 from torch import Tensor
@@ -40,25 +40,24 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Tensor | None 
     return library.gated_linear(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation])
 
 
-def grad_norm(grads: Iterable[Tensor], *, norm_type: float = 2.0) -> Tensor:
+def grad_norm(grads: Sequence[Tensor], *, norm_type: float = 2.0) -> Tensor:
     """The norm (2 or ``math.inf``) over all elements of ``grads``: an FP32 value on their device, squares summed in 64
     bits. Nothing waits for the GPU."""
-    return library.grad_norm(list(grads), float(norm_type))
+    return library.grad_norm(grads, float(norm_type))
 
 
-def clip_grad_norm_(grads: Iterable[Tensor], max_norm: float, *, norm_type: float = 2.0,
-                    out: Iterable[Tensor] | None = None, error_if_nonfinite: bool = False) -> Tensor:
+def clip_grad_norm_(grads: Sequence[Tensor], max_norm: float, *, norm_type: float = 2.0,
+                    out: Sequence[Tensor] | None = None, error_if_nonfinite: bool = False) -> Tensor:
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` in place, or into ``out`` (tensors of the same shapes that
     do not overlap the gradients, of any float type: BF16 gradients into the FP32 ones an optimizer reads), and returns
     the norm. A NaN norm makes every element NaN, as in ``torch.nn.utils.clip_grad_norm_``; with ``error_if_nonfinite``
     a norm that is not finite raises before anything is written (this waits for the GPU)."""
-    grads = list(grads)
     with torch.no_grad():
         if error_if_nonfinite and not math.isfinite(library.grad_norm(grads, float(norm_type)).item()):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm of type {norm_type} is not finite")
         if out is None:
             return library.clip_grad_norm_(grads, float(max_norm), float(norm_type))
-        return library.clip_grad_norm_out(grads, list(out), float(max_norm), float(norm_type))
+        return library.clip_grad_norm_out(grads, out, float(max_norm), float(norm_type))
 
 
 # -- eligibility -------------------------------------------------------------------------------------------------------
@@ -90,18 +89,17 @@ def eligible_gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, *, activation
 
 
 def _tensors(tensors) -> bool:
-    return (
-        isinstance(tensors, (list, tuple)) and len(tensors) > 0 and all(isinstance(t, Tensor) for t in tensors)
-        and is_gfx950(tensors[0].device)
-        and all(t.device == tensors[0].device and t.dtype in _FLOATS for t in tensors)
-    )
+    return isinstance(tensors, (list, tuple)) and len(tensors) > 0 and all(issubclass(t, Tensor)
+                                                                           for t in set(map(type, tensors)))
+
+
+# The first gradient stands for the others here; the operators themselves look at each tensor's device, type and size, and
+# raise NotImplementedError as a refused predicate does.
 
 
 def eligible_grad_norm(grads, *, norm_type=2.0) -> bool:
-    return _tensors(grads) and norm_type in (2.0, math.inf)
+    return _tensors(grads) and is_gfx950(grads[0].device) and grads[0].dtype in _FLOATS and norm_type in (2.0, math.inf)
 
 
 def eligible_clip_grad_norm(grads, max_norm, *, norm_type=2.0, out=None, error_if_nonfinite=False) -> bool:
-    return eligible_grad_norm(grads, norm_type=norm_type) and (
-        out is None or (_tensors(out) and len(out) == len(grads) and out[0].device == grads[0].device
-                        and all(o.shape == g.shape for o, g in zip(out, grads))))
+    return eligible_grad_norm(grads, norm_type=norm_type) and (out is None or (_tensors(out) and len(out) == len(grads)))

@@ -5,7 +5,7 @@
 // A stream: every gradient is read for the norm, then read again and written, in place or elsewhere (the floor is one read
 // and one write; the second read comes from the Infinity Cache for gradients of up to about its 256 MB). Tensors are
 // handed over in kernel arguments, up to 168 or 248 a launch (no table to upload, capturable); a workgroup finds its
-// tensor by bisection over the tensors' first workgroups and takes one run of its elements.
+// tensor among their first workgroups and takes one run of its elements.
 //
 // Squares are summed in 64 bits: FP32 gradients above 1.8e19 would overflow in 32, and the conversions and FMAs hide behind
 // the loads. Each workgroup writes one partial; every workgroup of the second launch adds them all up in the same order
@@ -35,15 +35,18 @@ typedef ClipTable<248, false> NormTable;
 typedef ClipTable<168, true> ScaleTable;
 static_assert(sizeof(NormTable) <= 4000 && sizeof(ScaleTable) <= 4000 + 56, "kernel arguments");
 
+// The entry whose workgroups hold wg: the entries that start at or before it, counted by the wavefront's lanes (one load
+// latency; a bisection's dependent loads took eight)
 template <typename Table>
 __device__ __forceinline__ int entry_of(const Table& t, uint32_t wg) {
-  uint32_t lo = 0, hi = t.entries;  // first[lo] <= wg < first[hi]
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (t.first[mid] <= wg) lo = mid;
-    else hi = mid;
+  const uint32_t lane = threadIdx.x & 63;
+  int n = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < Table::ENTRIES; i += 64) {
+    const uint32_t at = i + lane < Table::ENTRIES ? i + lane : Table::ENTRIES - 1;
+    n += __popcll(__builtin_amdgcn_ballot_w64(i + lane < t.entries && t.first[at] <= wg));
   }
-  return (int)lo;
+  return n - 1;
 }
 
 template <int DT>
@@ -217,9 +220,9 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
   }
 }
 
-// Elements of a workgroup: about four workgroups per CU over all tensors, in steps of 2048.
+// Elements of a workgroup: about sixteen workgroups per CU over all tensors, in steps of 2048.
 static uint32_t clip_chunk(int64_t elements) {
-  const int64_t c = cdiv(cdiv(elements, 4 * (int64_t)device_cus()), 2048) * 2048;
+  const int64_t c = cdiv(cdiv(elements, 16 * (int64_t)device_cus()), 2048) * 2048;
   return (uint32_t)(c < 2048 ? 2048 : c > CLIP_ENTRY ? CLIP_ENTRY : c);
 }
 

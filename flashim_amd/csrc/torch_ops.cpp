@@ -616,6 +616,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward(
   return {dx, dwg, dwu, dbg, dbu};
 }
 
+// Refusals that the ops' predicates leave to these operators: in Python, looking at hundreds of tensors costs more than the
+// kernels take
+void check_grad(const Tensor& t, const Tensor& first) {
+  const auto type = t.scalar_type();
+  TORCH_CHECK_NOT_IMPLEMENTED(t.device() == first.device() && t.is_cuda(),
+                              "no HIP impl applies: gradients on ", first.device(), " and ", t.device());
+  TORCH_CHECK_NOT_IMPLEMENTED(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf,
+                              "no HIP impl applies: a gradient of ", type);
+}
+
 // The gradients of a list as the C ABI takes them: dense, each in the order of its memory
 struct GradList {
   std::vector<Tensor> hold;
@@ -623,8 +633,12 @@ struct GradList {
   std::vector<int> dtypes;
   std::vector<int64_t> numel;
   explicit GradList(at::TensorList grads) {
+    hold.reserve(grads.size());
+    ptrs.reserve(grads.size());
+    dtypes.reserve(grads.size());
+    numel.reserve(grads.size());
     for (const Tensor& t : grads) {
-      TORCH_CHECK_VALUE(t.device() == grads[0].device(), "gradients on ", grads[0].device(), " and ", t.device());
+      check_grad(t, grads[0]);
       hold.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
       ptrs.push_back(hold.back().data_ptr());
       dtypes.push_back(dtype_code(t));
@@ -667,10 +681,14 @@ Tensor clip_grad_norm_out(at::TensorList grads, at::TensorList out, double max_n
   std::vector<Tensor> to;  // written by the kernel: `out` itself where its memory lies as the gradient's
   std::vector<void*> ptrs;
   std::vector<int> dtypes;
+  to.reserve(out.size());
+  ptrs.reserve(out.size());
+  dtypes.reserve(out.size());
   for (size_t i = 0; i < out.size(); ++i) {
     const Tensor& t = out[i];
-    TORCH_CHECK_VALUE(t.sizes() == grads[i].sizes() && t.device() == grads[0].device(), "clip_grad_norm_: output of shape ",
-                      t.sizes(), " on ", t.device(), " for a gradient of shape ", grads[i].sizes());
+    check_grad(t, grads[0]);
+    TORCH_CHECK_NOT_IMPLEMENTED(t.sizes() == grads[i].sizes(), "no HIP impl applies: an output of shape ", t.sizes(),
+                                " for a gradient of shape ", grads[i].sizes());
     const Tensor& from = g.hold[i];
     const bool same = t.is_non_overlapping_and_dense() && t.strides() == from.strides();
     to.push_back(same ? t : at::empty_strided(from.sizes(), from.strides(), t.options().requires_grad(false)));
@@ -736,26 +754,26 @@ Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double norm_type) 
   X(gated_linear_backward, "(Tensor d_out, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "       \
                            "int act, bool want_x, bool want_weights, bool want_biases) "                               \
                            "-> (Tensor, Tensor, Tensor, Tensor, Tensor)")                                              \
-  X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")                                                          \
-  X(clip_grad_norm_, "(Tensor(a!)[] grads, float max_norm, float norm_type) -> Tensor")                                \
-  X(clip_grad_norm_out, "(Tensor[] grads, Tensor(a!)[] out, float max_norm, float norm_type) -> Tensor")
+  X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")
 
-// those with derivative formulas (below)
-#define FIM_DIFFERENTIABLE_OPS(X)                                                                                      \
+// those with an autograd kernel of their own (below)
+#define FIM_AUTOGRAD_OPS(X)                                                                                            \
+  X(clip_grad_norm_, "(Tensor(a!)[] grads, float max_norm, float norm_type) -> Tensor")                                \
+  X(clip_grad_norm_out, "(Tensor[] grads, Tensor(a!)[] out, float max_norm, float norm_type) -> Tensor")               \
   X(group_norm_act, "(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act) -> (Tensor, Tensor)")    \
   X(gated_linear, "(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor")
 
 TORCH_LIBRARY(flashim_amd, m) {
 #define X(name, schema) m.def(#name schema, {at::Tag::pt2_compliant_tag});
   FIM_OPS(X)
-  FIM_DIFFERENTIABLE_OPS(X)
+  FIM_AUTOGRAD_OPS(X)
 #undef X
 }
 
 TORCH_LIBRARY_IMPL(flashim_amd, CUDA, m) {
 #define X(name, schema) m.impl(#name, TORCH_FN(name));
   FIM_OPS(X)
-  FIM_DIFFERENTIABLE_OPS(X)
+  FIM_AUTOGRAD_OPS(X)
 #undef X
 }
 
@@ -813,6 +831,19 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch
     if (!t.is_inference()) torch::autograd::increment_version(t);
 }
 
+// Clipping below autograd, the versions of what it wrote counted: as no_derivative and count_writes do for any operator, but
+// without boxing hundreds of tensors.
+void refuse_gradients(at::TensorList tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");
+}
+
+void count_writes_to(at::TensorList tensors) {
+  for (const Tensor& t : tensors)
+    if (!t.is_inference()) torch::autograd::increment_version(t);
+}
+
 // Derivatives: each a torch operator of its own, so that compiled graphs hold it (and a second derivative raises).
 OptTensor as_optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor as_tensor(const OptTensor& t) { return t ? *t : Tensor(); }
@@ -820,6 +851,25 @@ Tensor as_tensor(const OptTensor& t) { return t ? *t : Tensor(); }
 template <typename Signature>
 c10::TypedOperatorHandle<Signature> typed_op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+
+Tensor clip_grad_norm_out_autograd(at::TensorList grads, at::TensorList out, double max_norm, double norm_type) {
+  refuse_gradients(grads);
+  refuse_gradients(out);
+  static const auto op = typed_op<decltype(clip_grad_norm_out)>("flashim_amd::clip_grad_norm_out");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor total = op.call(grads, out, max_norm, norm_type);
+  count_writes_to(out);
+  return total;
+}
+
+Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double norm_type) {
+  refuse_gradients(grads);
+  static const auto op = typed_op<decltype(clip_grad_norm_)>("flashim_amd::clip_grad_norm_");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor total = op.call(grads, max_norm, norm_type);
+  count_writes_to(grads);
+  return total;
 }
 
 struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
@@ -890,6 +940,8 @@ TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
 #undef X
   m.impl("group_norm_act", TORCH_FN(group_norm_act_autograd));
   m.impl("gated_linear", TORCH_FN(gated_linear_autograd));
+  m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_autograd_));
+  m.impl("clip_grad_norm_out", TORCH_FN(clip_grad_norm_out_autograd));
 }
 
 TORCH_LIBRARY_IMPL(flashim_amd, ADInplaceOrView, m) {
