@@ -12,34 +12,40 @@
 //
 // A workgroup of 512 threads takes a run of pixels ("chunk") of one image and all channels: thread t keeps the V channels
 // of column t % (C / V) and every (512 / (C / V))th pixel, so a wavefront reads whole contiguous runs and the per-channel
-// parameters and sums stay in registers. Forward sums are kept per thread and channel about the thread's first pixel (no
-// cancellation where the mean is large), merged as (count, mean, squared deviations); nothing is summed by atomics, so
-// results do not depend on the order of workgroups.
+// parameters and sums stay in registers, and loads a batch of pixels ahead. The first pass writes one partial per
+// (chunk, group), the second adds up its image's partials before it starts, while its first loads are on their way (a
+// launch between the two for groups so many that every workgroup would read them for long). Nothing is summed by atomics:
+// results do not depend on the order of workgroups. Forward sums are kept about the mean of a thread's first pixels (no
+// cancellation where the mean is large) and merged as means and squared deviations.
 #include "activation.h"
 
 namespace fim {
 
 constexpr int NORM_T = 512;           // threads of a workgroup
+// Pixels of a batch of loads (the next batch is loaded while one is worked on), with registers for four wavefronts per SIMD:
+// backward, with two tensors and the activation's slope, 4 took 180 to 230 registers and ran half as many wavefronts
+constexpr int NORM_U = 4, NORM_GRAD_U = 2;
 constexpr int NORM_MAX_C = 8192;      // per-channel partials of a workgroup lie in LDS
-constexpr int NORM_UNROLL = 4;        // pixels in flight per thread
+constexpr int NORM_MERGE_G = 512;     // groups, and partials, that the workgroups of the second pass add up themselves
+constexpr int64_t NORM_MERGE = 2 << 20;  // (over all workgroups)
 
 struct NormArgs {
-  const void* x;
-  const void* dy;
-  void* out;            // y, or dx
+  const uint8_t* x;
+  const uint8_t* dy;
+  uint8_t* out;         // y, or dx
   const void* weight;   // null: 1
   const void* bias;     // null: 0
   int wdt, bdt;         // their types
   float* stats;         // [B, G, 2]: mean, rstd
-  float* part;          // [B, chunks, G, 2] forward; [B, chunks, C, 2] backward
-  float* csum;          // backward: [B, C, 2] sums over pixels of dz, dz * xhat
-  float* coef;          // backward: [B, G, 2]: s1, s2
+  float* gpart;         // [B, chunks, G, 2]: mean and squared deviations; backward sums of dz * weight, dz * weight * xhat
+  float* cpart;         // backward: [B, chunks, C, 2]: sums of dz, dz * xhat
+  float* coef;          // backward, merged between the passes: [B, G, 2]: s1, s2
   void* dweight;
   void* dbias;
   int64_t P, sb, sp, db, dp;  // image and pixel strides of x and of dy, in elements
   int B, C, G, D;
-  int chunks;
-  int64_t chunk;        // pixels of a chunk
+  int chunks, chunk;    // chunks of an image, and their pixels
+  int merged;           // stats (coef) were merged by a launch between the passes
   float eps;
 };
 
@@ -47,6 +53,38 @@ __device__ __forceinline__ float param(const void* p, int dt, int i, float missi
   if (p == nullptr) return missing;
   return dt == FIM_F32 ? static_cast<const float*>(p)[i]
                        : dt == FIM_BF16 ? load_elem<FIM_BF16>(p, i) : load_elem<FIM_F16>(p, i);
+}
+
+// V neighbouring parameters: all loads on one side of the branch on their type, so their latencies overlap
+template <int V>
+__device__ __forceinline__ void params(const void* p, int dt, int i, float missing, float (&f)[V]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = missing;
+  } else if (dt == FIM_F32) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = static_cast<const float*>(p)[i + k];
+  } else {
+    uint16_t h[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) h[k] = static_cast<const uint16_t*>(p)[i + k];
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      f[k] = dt == FIM_BF16 ? bf16_to_f32(h[k]) : (float)__builtin_bit_cast(_Float16, h[k]);
+  }
+}
+
+// g[k]: the group of channel c0 + k
+template <int V>
+__device__ __forceinline__ void groups_of(int c0, int D, int (&g)[V]) {
+  int at = c0 / D, r = c0 - at * D;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    g[k] = at;
+    ++r;
+    at += r == D;
+    r = r == D ? 0 : r;
+  }
 }
 
 __device__ __forceinline__ void store_param(void* p, int dt, int i, float v) {
@@ -58,11 +96,9 @@ __device__ __forceinline__ void store_param(void* p, int dt, int i, float v) {
 // V elements as they lie in memory, and as floats
 template <int DT, int V>
 struct Pack {
-  static constexpr int BYTES = V * (DT == FIM_F32 ? 4 : 2);
+  static constexpr int ES = DT == FIM_F32 ? 4 : 2, BYTES = V * ES;
   struct alignas(BYTES < 16 ? BYTES : 16) Raw { uint8_t b[BYTES]; };
-  static __device__ __forceinline__ Raw load(const void* p, int64_t i) {
-    return *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(p) + i * (BYTES / V));
-  }
+  static __device__ __forceinline__ Raw load(const uint8_t* p) { return *reinterpret_cast<const Raw*>(p); }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[V]) {
     if constexpr (DT == FIM_F32) {
       __builtin_memcpy(f, &r, BYTES);
@@ -73,7 +109,7 @@ struct Pack {
       for (int i = 0; i < V; ++i) f[i] = DT == FIM_BF16 ? bf16_to_f32(h[i]) : (float)__builtin_bit_cast(_Float16, h[i]);
     }
   }
-  static __device__ __forceinline__ void store(void* p, int64_t i, const float (&f)[V]) {
+  static __device__ __forceinline__ void store(uint8_t* p, const float (&f)[V]) {
     Raw r;
     if constexpr (DT == FIM_F32) {
       __builtin_memcpy(&r, f, BYTES);
@@ -89,371 +125,537 @@ struct Pack {
         h[k] = DT == FIM_BF16 ? (uint16_t)(pack_bf16x2(f[k], 0.0f) & 0xffff) : __builtin_bit_cast(uint16_t, (_Float16)f[k]);
       __builtin_memcpy(&r, h, BYTES);
     }
-    *reinterpret_cast<Raw*>(static_cast<uint8_t*>(p) + i * (BYTES / V)) = r;
+    *reinterpret_cast<Raw*>(p) = r;
   }
 };
 
-// This thread's share of a workgroup: column `col` (V channels) of pixels row, row + rows, ... of [begin, end)
+// This thread's share of a chunk: V channels from `c0`, pixels row, row + rows, ...: `n` of them
 struct Share {
-  int col, row, rows;
+  int c0, row, rows, n;
   bool live;
 };
 
-__device__ __forceinline__ Share share_of(int cols, int pass) {
+template <int V>
+__device__ __forceinline__ Share share_of(const NormArgs& a, int pass, int pixels) {
+  const int cols = a.C / V;
   Share s;
+  int col;
   if (cols >= NORM_T) {
-    s.col = pass * NORM_T + threadIdx.x;
+    col = pass * NORM_T + threadIdx.x;
     s.row = 0;
     s.rows = 1;
-    s.live = s.col < cols;
+    s.live = col < cols;
   } else {
     s.rows = NORM_T / cols;
     s.row = threadIdx.x / cols;
-    s.col = threadIdx.x - s.row * cols;
+    col = threadIdx.x - s.row * cols;
     s.live = s.row < s.rows;
   }
+  s.c0 = col * V;
+  s.n = s.row < pixels ? (pixels - s.row + s.rows - 1) / s.rows : 0;
   return s;
 }
+template <int V>
+__device__ __forceinline__ int passes_of(const NormArgs& a) {
+  return a.C / V >= NORM_T ? (a.C / V + NORM_T - 1) / NORM_T : 1;
+}
 
-__device__ __forceinline__ int passes_of(int cols) { return cols >= NORM_T ? (cols + NORM_T - 1) / NORM_T : 1; }
+// The workgroup's image, chunk and pixels
+struct Chunk {
+  int b, i, pixels;
+  int64_t begin;
+};
+__device__ __forceinline__ Chunk chunk_of(const NormArgs& a) {
+  Chunk c;
+  c.b = blockIdx.x / a.chunks;
+  c.i = blockIdx.x - c.b * a.chunks;
+  c.begin = (int64_t)c.i * a.chunk;
+  c.pixels = c.begin + a.chunk < a.P ? a.chunk : (int)(a.P - c.begin);
+  return c;
+}
+__device__ __forceinline__ int pixels_of(const NormArgs& a, int chunk) {
+  const int64_t begin = (int64_t)chunk * a.chunk;
+  return begin + a.chunk < a.P ? a.chunk : (int)(a.P - begin);
+}
 
-// f(pixel, unpacked...) over this thread's pixels of [begin, end), NORM_UNROLL loads in flight
-template <int DT, int V, typename F>
-__device__ __forceinline__ void for_pixels(const void* p, int64_t base, int64_t stride, int64_t begin, int64_t end,
-                                           const Share& s, F&& f) {
+// A thread's pixels of one tensor, U at a time; batch k's loads past the end repeat the last pixel
+template <int DT, int V, int U>
+struct Rows {
   typedef Pack<DT, V> Pk;
-  int64_t i = begin + s.row;
-  const int64_t step = s.rows;
-  for (; i + (NORM_UNROLL - 1) * step < end; i += NORM_UNROLL * step) {
-    typename Pk::Raw r[NORM_UNROLL];
+  const uint8_t* p;
+  int64_t step;
+  int n;
+  __device__ __forceinline__ Rows(const uint8_t* base, int64_t image, int64_t sp, const Chunk& c, const Share& s) {
+    p = base + (c.b * image + (c.begin + s.row) * sp + s.c0) * Pk::ES;
+    step = s.rows * sp * Pk::ES;
+    n = s.n;
+  }
+  __device__ __forceinline__ void load(int k, typename Pk::Raw (&r)[U]) const {
+    const uint8_t* at = p + k * step;
 #pragma unroll
-    for (int u = 0; u < NORM_UNROLL; ++u) r[u] = Pk::load(p, base + (i + u * step) * stride);
-#pragma unroll
-    for (int u = 0; u < NORM_UNROLL; ++u) {
-      float v[V];
-      Pk::unpack(r[u], v);
-      f(i + u * step, v);
+    for (int u = 0; u < U; ++u) r[u] = Pk::load(at + (k + u < n ? u : n - 1 - k) * step);
+  }
+  // f(first pixel's index, batch) over all pixels; r[0] holds the first batch
+  template <typename F>
+  __device__ __forceinline__ void batches(typename Pk::Raw (&r)[2][U], F&& f) const {
+    for (int i = 0;;) {
+      if (i + U < n) load(i + U, r[1]);
+      f(i, r[0]);
+      i += U;
+      if (i >= n) break;
+      if (i + U < n) load(i + U, r[0]);
+      f(i, r[1]);
+      i += U;
+      if (i >= n) break;
     }
   }
-  for (; i < end; i += step) {
-    float v[V];
-    Pk::unpack(Pk::load(p, base + i * stride), v);
-    f(i, v);
+};
+
+// the same over the rows of two tensors
+template <int DT, int V, int U, typename F>
+__device__ __forceinline__ void batches2(const Rows<DT, V, U>& x, const Rows<DT, V, U>& d,
+                                         typename Pack<DT, V>::Raw (&rx)[2][U], typename Pack<DT, V>::Raw (&rd)[2][U],
+                                         F&& f) {
+  auto next = [&](int i, int k) __attribute__((always_inline)) {
+    if (i >= x.n) return;
+    x.load(i, rx[k]);
+    d.load(i, rd[k]);
+  };
+  for (int i = 0;;) {
+    next(i + U, 1);
+    f(i, rx[0], rd[0]);
+    i += U;
+    if (i >= x.n) break;
+    next(i + U, 0);
+    f(i, rx[1], rd[1]);
+    i += U;
+    if (i >= x.n) break;
   }
 }
 
-template <int DT, int V, typename F>
-__device__ __forceinline__ void for_pixels2(const NormArgs& a, int64_t xbase, int64_t dbase, int64_t begin, int64_t end,
-                                            const Share& s, F&& f) {
-  typedef Pack<DT, V> Pk;
-  int64_t i = begin + s.row;
-  const int64_t step = s.rows;
-  for (; i + (NORM_UNROLL - 1) * step < end; i += NORM_UNROLL * step) {
-    typename Pk::Raw r[NORM_UNROLL], q[NORM_UNROLL];
-#pragma unroll
-    for (int u = 0; u < NORM_UNROLL; ++u) {
-      r[u] = Pk::load(a.x, xbase + (i + u * step) * a.sp);
-      q[u] = Pk::load(a.dy, dbase + (i + u * step) * a.dp);
-    }
-#pragma unroll
-    for (int u = 0; u < NORM_UNROLL; ++u) {
-      float v[V], d[V];
-      Pk::unpack(r[u], v);
-      Pk::unpack(q[u], d);
-      f(i + u * step, v, d);
-    }
-  }
-  for (; i < end; i += step) {
-    float v[V], d[V];
-    Pk::unpack(Pk::load(a.x, xbase + i * a.sp), v);
-    Pk::unpack(Pk::load(a.dy, dbase + i * a.dp), d);
-    f(i, v, d);
-  }
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
-}
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// pixels of [begin, end) that row `row` of `rows` takes
-__device__ __forceinline__ int64_t row_count(int64_t begin, int64_t end, int row, int rows) {
-  const int64_t n = end - begin - row;
-  return n <= 0 ? 0 : (n + rows - 1) / rows;
 }
 
 // Forward, first pass: per (chunk, group) the mean and the sum of squared deviations.
 template <int DT, int V>
-__global__ __launch_bounds__(NORM_T) void norm_stats_kernel(const NormArgs a) {
-  extern __shared__ float lds[];  // [rows][C] means, then [rows][C] squared deviations
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const int64_t begin = chunk * a.chunk, end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
-  const int cols = a.C / V;
+__global__ __launch_bounds__(NORM_T, 4) void norm_stats_kernel(const NormArgs a) {
+  extern __shared__ float2 lds2[];  // [rows][C]: mean and squared deviations of a thread's pixels
+  const Chunk ch = chunk_of(a);
   int rows = 1;
-  const int passes = passes_of(cols);
-  for (int pass = 0; pass < passes; ++pass) {
-    const Share s = share_of(cols, pass);
+  for (int pass = 0; pass < passes_of<V>(a); ++pass) {
+    const Share s = share_of<V>(a, pass, ch.pixels);
     rows = s.rows;
     if (!s.live) continue;
-    const int c0 = s.col * V;
-    const int64_t base = b * a.sb + c0;
-    const int64_t n = row_count(begin, end, s.row, s.rows);
-    float shift[V], s1[V], s2[V];
+    float s1[V], s2[V], shift[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) shift[k] = s1[k] = s2[k] = 0.0f;
-    if (n > 0) Pack<DT, V>::unpack(Pack<DT, V>::load(a.x, base + (begin + s.row) * a.sp), shift);
-    for_pixels<DT, V>(a.x, base, a.sp, begin, end, s, [&](int64_t, const float(&v)[V]) __attribute__((always_inline)) {
+    for (int k = 0; k < V; ++k) s1[k] = s2[k] = shift[k] = 0.0f;
+    if (s.n > 0) {
+      const Rows<DT, V, NORM_U> x(a.x, a.sb, a.sp, ch, s);
+      typename Pack<DT, V>::Raw r[2][NORM_U];
+      x.load(0, r[0]);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float d = v[k] - shift[k];
-        s1[k] += d;
-        s2[k] = fmaf(d, d, s2[k]);
+      for (int u = 0; u < NORM_U; ++u) {  // the first pixels' mean (repeats weigh in: any value near will do)
+        float v[V];
+        Pack<DT, V>::unpack(r[0][u], v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) shift[k] = fmaf(v[k], 1.0f / NORM_U, shift[k]);
       }
-    });
-    const float inv = n > 0 ? 1.0f / (float)n : 0.0f;
+      x.batches(r, [&](int i, const typename Pack<DT, V>::Raw(&now)[NORM_U]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NORM_U; ++u) {
+          if (i + u >= s.n) break;
+          float v[V];
+          Pack<DT, V>::unpack(now[u], v);
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float d = v[k] - shift[k];
+            s1[k] += d;
+            s2[k] = fmaf(d, d, s2[k]);
+          }
+        }
+      });
+    }
+    const float inv = s.n > 0 ? 1.0f / (float)s.n : 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const float m = s1[k] * inv;
-      lds[s.row * a.C + c0 + k] = shift[k] + m;
-      lds[(s.rows + s.row) * a.C + c0 + k] = fmaf(-m, s1[k], s2[k]);
+      lds2[s.row * a.C + s.c0 + k] = float2{shift[k] + m, fmaf(-m, s1[k], s2[k])};
     }
   }
   __syncthreads();
-  const float* m2 = lds + rows * a.C;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const float total = (float)(end - begin) * (float)a.D;
-  for (int g = wave; g < a.G; g += NORM_T / 64) {
-    float sum = 0.0f;
-    for (int i = lane; i < rows * a.D; i += 64) {
-      const int r = i / a.D, at = r * a.C + g * a.D + (i - r * a.D);
-      sum += (float)row_count(begin, end, r, rows) * lds[at];
+  // the threads' means and deviations about the group's first: rows of a channel by several threads, then a wavefront per
+  // group over its channels' parts
+  __shared__ float2 sums[NORM_T];
+  const int q = ch.pixels / rows, more = ch.pixels - q * rows;  // row r has q + (r < more) pixels
+  const int parts = a.C < NORM_T ? NORM_T / a.C : 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  auto add = [&](int part, int c, float& s1, float& s2) __attribute__((always_inline)) {
+    const float centre = lds2[c - c % a.D].x;
+    for (int r = part; r < rows; r += parts) {
+      const float n = (float)(q + (r < more));
+      const float2 v = lds2[r * a.C + c];
+      const float d = v.x - centre;
+      s1 = fmaf(n, d, s1);
+      s2 += fmaf(n * d, d, v.y);
     }
-    const float mean = wave_sum(sum) / total;
-    float dev = 0.0f;
-    for (int i = lane; i < rows * a.D; i += 64) {
-      const int r = i / a.D, at = r * a.C + g * a.D + (i - r * a.D);
-      const float n = (float)row_count(begin, end, r, rows), d = lds[at] - mean;
-      if (n > 0) dev += fmaf(n * d, d, m2[at]);
+  };
+  auto put = [&](int g, float s1, float s2) __attribute__((always_inline)) {
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    const float m = s1 / ((float)ch.pixels * (float)a.D);
+    if (lane == 0)
+      reinterpret_cast<float2*>(a.gpart)[(int64_t)blockIdx.x * a.G + g] = float2{lds2[g * a.D].x + m, fmaf(-m, s1, s2)};
+  };
+  if (parts > 1) {
+    const int part = threadIdx.x / a.C, c = threadIdx.x - part * a.C;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (part < parts) add(part, c, s1, s2);
+    sums[threadIdx.x] = float2{s1, s2};
+    __syncthreads();
+    for (int g = wave; g < a.G; g += NORM_T / 64) {
+      s1 = s2 = 0.0f;
+      for (int i = lane; i < parts * a.D; i += 64) {
+        const int p = i / a.D;
+        const float2 v = sums[p * a.C + g * a.D + (i - p * a.D)];
+        s1 += v.x;
+        s2 += v.y;
+      }
+      put(g, s1, s2);
     }
-    dev = wave_sum(dev);
-    if (lane == 0) {
-      float* p = a.part + ((int64_t)blockIdx.x * a.G + g) * 2;
-      p[0] = mean;
-      p[1] = dev;
+  } else {
+    for (int g = wave; g < a.G; g += NORM_T / 64) {
+      float s1 = 0.0f, s2 = 0.0f;
+      for (int d = lane; d < a.D; d += 64) add(0, g * a.D + d, s1, s2);
+      put(g, s1, s2);
     }
   }
 }
 
-// One wavefront per (image, group): the chunks' means and deviations merged.
+// A workgroup adds up its image's partials: thread t takes group t % G of every (threads / G)th chunk, all loads at once,
+// about the first chunk's mean; then the threads of a group through LDS. to[g]: mean and 1 / deviation, or, BACKWARD, the
+// group's means of dz * weight and dz * weight * xhat.
+template <bool BACKWARD>
+__device__ __forceinline__ void merge_groups(const NormArgs& a, int b, float2* to) {
+  __shared__ double2 part[NORM_T];
+  const float2* p = reinterpret_cast<const float2*>(a.gpart) + (int64_t)b * a.chunks * a.G;
+  const int slices = NORM_T / a.G, slice = threadIdx.x / a.G, g = threadIdx.x - slice * a.G;
+  const double total = (double)a.P * a.D;
+  double s1 = 0.0, s2 = 0.0;
+  const float centre = BACKWARD ? 0.0f : p[g].x;
+  if (slice < slices) {
+    for (int i = slice; i < a.chunks; i += slices) {
+      const float2 v = p[(int64_t)i * a.G + g];
+      if constexpr (BACKWARD) {
+        s1 += v.x;
+        s2 += v.y;
+      } else {
+        const double n = (double)pixels_of(a, i) * a.D, d = (double)v.x - centre;
+        s1 += n * d;
+        s2 += n * d * d + v.y;
+      }
+    }
+  }
+  part[threadIdx.x] = double2{s1, s2};
+  __syncthreads();
+  if ((int)threadIdx.x < a.G) {
+    s1 = s2 = 0.0;
+    for (int k = 0; k < slices; ++k) {
+      const double2 v = part[k * a.G + g];
+      s1 += v.x;
+      s2 += v.y;
+    }
+    s1 /= total;
+    s2 /= total;
+    to[g] = BACKWARD ? float2{(float)s1, (float)s2}
+                     : float2{(float)(centre + s1), (float)(1.0 / sqrt(fmax(s2 - s1 * s1, 0.0) + (double)a.eps))};
+  }
+  __syncthreads();
+}
+
+// Between the passes, where an image's partials are many: one wavefront per (image, group), a row of partials a lane
+template <bool BACKWARD>
 __global__ __launch_bounds__(256) void norm_merge_kernel(const NormArgs a) {
   const int64_t bg = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (bg >= (int64_t)a.B * a.G) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t b = bg / a.G, g = bg - b * a.G;
-  const float* p = a.part + (b * a.chunks * a.G + g) * 2;
+  const int64_t b = bg / a.G;
+  const float2* p = reinterpret_cast<const float2*>(a.gpart) + b * a.chunks * a.G + (bg - b * a.G);
   const double total = (double)a.P * a.D;
-  double sum = 0.0;
-  for (int i = lane; i < a.chunks; i += 64) {
-    const int64_t begin = i * a.chunk, n = (begin + a.chunk < a.P ? begin + a.chunk : a.P) - begin;
-    sum += (double)(n * a.D) * p[(int64_t)i * a.G * 2];
+  const float centre = BACKWARD ? 0.0f : p[0].x;
+  double s1 = 0.0, s2 = 0.0;
+  for (int i = threadIdx.x & 63; i < a.chunks; i += 64) {
+    const float2 v = p[(int64_t)i * a.G];
+    if constexpr (BACKWARD) {
+      s1 += v.x;
+      s2 += v.y;
+    } else {
+      const double n = (double)pixels_of(a, i) * a.D, d = (double)v.x - centre;
+      s1 += n * d;
+      s2 += n * d * d + v.y;
+    }
   }
-  const double mean = wave_sum(sum) / total;
-  double dev = 0.0;
-  for (int i = lane; i < a.chunks; i += 64) {
-    const int64_t begin = i * a.chunk, n = (begin + a.chunk < a.P ? begin + a.chunk : a.P) - begin;
-    const double d = p[(int64_t)i * a.G * 2] - mean;
-    dev += (double)(n * a.D) * d * d + p[(int64_t)i * a.G * 2 + 1];
-  }
-  dev = wave_sum(dev);
-  if (lane == 0) {
-    a.stats[2 * bg] = (float)mean;
-    a.stats[2 * bg + 1] = (float)(1.0 / sqrt(dev / total + (double)a.eps));
-  }
+  s1 = wave_sum(s1) / total;
+  s2 = wave_sum(s2) / total;
+  if ((threadIdx.x & 63) == 0)
+    reinterpret_cast<float2*>(BACKWARD ? a.coef : a.stats)[bg] =
+        BACKWARD ? float2{(float)s1, (float)s2}
+                 : float2{(float)(centre + s1), (float)(1.0 / sqrt(fmax(s2 - s1 * s1, 0.0) + (double)a.eps))};
 }
 
+// Forward, second pass.
 template <int DT, int V, int ACT>
-__global__ __launch_bounds__(NORM_T) void norm_apply_kernel(const NormArgs a) {
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const int64_t begin = chunk * a.chunk, end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
-  const int cols = a.C / V, passes = passes_of(cols);
-  for (int pass = 0; pass < passes; ++pass) {
-    const Share s = share_of(cols, pass);
-    if (!s.live) continue;
-    const int c0 = s.col * V;
+__global__ __launch_bounds__(NORM_T, 4) void norm_apply_kernel(const NormArgs a) {
+  typedef Pack<DT, V> Pk;
+  __shared__ float2 stat[NORM_MERGE_G];
+  const Chunk ch = chunk_of(a);
+  for (int pass = 0; pass < passes_of<V>(a); ++pass) {
+    const Share s = share_of<V>(a, pass, ch.pixels);
+    const bool any = s.live && s.n > 0;
+    const Rows<DT, V, NORM_U> x(a.x, a.sb, a.sp, ch, s);
+    typename Pk::Raw r[2][NORM_U];
     float mean[V], mul[V], add[V];
+    if (any) {
+      x.load(0, r[0]);
+      params<V>(a.weight, a.wdt, s.c0, 1.0f, mul);
+      params<V>(a.bias, a.bdt, s.c0, 0.0f, add);
+    }
+    if (pass == 0 && !a.merged) {
+      merge_groups<false>(a, ch.b, stat);
+      if (ch.i == 0 && (int)threadIdx.x < a.G)
+        reinterpret_cast<float2*>(a.stats)[(int64_t)ch.b * a.G + threadIdx.x] = stat[threadIdx.x];
+    }
+    if (!any) continue;
+    int g[V];
+    groups_of<V>(s.c0, a.D, g);
+    float2 st[V];
+    if (a.merged) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) st[k] = reinterpret_cast<const float2*>(a.stats)[(int64_t)ch.b * a.G + g[k]];
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) st[k] = stat[g[k]];
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float* st = a.stats + ((int64_t)b * a.G + (c0 + k) / a.D) * 2;
-      mean[k] = st[0];
-      mul[k] = st[1] * param(a.weight, a.wdt, c0 + k, 1.0f);
-      add[k] = param(a.bias, a.bdt, c0 + k, 0.0f);
+      mean[k] = st[k].x;
+      mul[k] *= st[k].y;
     }
-    const int64_t out = (int64_t)b * a.P * a.C + c0;
-    for_pixels<DT, V>(a.x, b * a.sb + c0, a.sp, begin, end, s,
-                      [&](int64_t i, const float(&v)[V]) __attribute__((always_inline)) {
-                        float y[V];
+    uint8_t* out = a.out + (((int64_t)ch.b * a.P + ch.begin + s.row) * a.C + s.c0) * Pk::ES;
+    const int64_t step = (int64_t)s.rows * a.C * Pk::ES;
+    x.batches(r, [&](int i, const typename Pk::Raw(&now)[NORM_U]) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int k = 0; k < V; ++k) y[k] = activate<ACT>(fmaf(v[k] - mean[k], mul[k], add[k]));
-                        Pack<DT, V>::store(a.out, out + i * a.C, y);
-                      });
+      for (int u = 0; u < NORM_U; ++u) {
+        if (i + u >= s.n) break;
+        float v[V];
+        Pk::unpack(now[u], v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = activate<ACT>(fmaf(v[k] - mean[k], mul[k], add[k]));
+        Pk::store(out + (i + u) * step, v);
+      }
+    });
   }
 }
 
-// Backward, first pass: per (chunk, channel) the sums of dz and dz * xhat.
+// The per-channel values of a backward pass in registers: z = (x - mean) * mul + add, mul = rstd * weight
+template <int V>
+struct GradParams {
+  float mean[V], mul[V], add[V];
+  __device__ __forceinline__ GradParams(const NormArgs& a, int b, int c0) {
+    int g[V];
+    groups_of<V>(c0, a.D, g);
+    float2 st[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) st[k] = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + g[k]];
+    params<V>(a.weight, a.wdt, c0, 1.0f, mul);
+    params<V>(a.bias, a.bdt, c0, 0.0f, add);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      mean[k] = st[k].x;
+      mul[k] *= st[k].y;
+    }
+  }
+};
+
+// Backward, first pass: per (chunk, channel) the sums of dz and dz * xhat, per (chunk, group) those times the weight.
 template <int DT, int V, int ACT>
-__global__ __launch_bounds__(NORM_T) void norm_grad_sums_kernel(const NormArgs a) {
-  extern __shared__ float lds[];  // [rows][C][2]
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const int64_t begin = chunk * a.chunk, end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
-  const int cols = a.C / V, passes = passes_of(cols);
+__global__ __launch_bounds__(NORM_T, 4) void norm_grad_sums_kernel(const NormArgs a) {
+  typedef Pack<DT, V> Pk;
+  extern __shared__ float2 lds2[];  // [rows][C]
+  const Chunk ch = chunk_of(a);
   int rows = 1;
-  for (int pass = 0; pass < passes; ++pass) {
-    const Share s = share_of(cols, pass);
+  for (int pass = 0; pass < passes_of<V>(a); ++pass) {
+    const Share s = share_of<V>(a, pass, ch.pixels);
     rows = s.rows;
     if (!s.live) continue;
-    const int c0 = s.col * V;
-    float mean[V], rstd[V], w[V], add[V], s1[V], s2[V];
+    float s1[V], s2[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float* st = a.stats + ((int64_t)b * a.G + (c0 + k) / a.D) * 2;
-      mean[k] = st[0];
-      rstd[k] = st[1];
-      w[k] = param(a.weight, a.wdt, c0 + k, 1.0f);
-      add[k] = param(a.bias, a.bdt, c0 + k, 0.0f);
-      s1[k] = s2[k] = 0.0f;
+    for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.0f;
+    if (s.n > 0) {
+      const Rows<DT, V, NORM_GRAD_U> x(a.x, a.sb, a.sp, ch, s), d(a.dy, a.db, a.dp, ch, s);
+      typename Pk::Raw rx[2][NORM_GRAD_U], rd[2][NORM_GRAD_U];
+      x.load(0, rx[0]);
+      d.load(0, rd[0]);
+      const GradParams<V> p(a, ch.b, s.c0);
+      batches2<DT, V, NORM_GRAD_U>(x, d, rx, rd, [&](int i, const typename Pk::Raw(&nx)[NORM_GRAD_U], const typename Pk::Raw(&nd)[NORM_GRAD_U])
+                      __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NORM_GRAD_U; ++u) {
+          if (i + u >= s.n) break;
+          float v[V], e[V];
+          Pk::unpack(nx[u], v);
+          Pk::unpack(nd[u], e);
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float c = v[k] - p.mean[k];
+            float slope;
+            activate<ACT, true>(fmaf(c, p.mul[k], p.add[k]), slope);
+            const float dz = e[k] * slope;
+            s1[k] += dz;
+            s2[k] = fmaf(dz, c, s2[k]);  // (times rstd at the end)
+          }
+        }
+      });
     }
-    for_pixels2<DT, V>(a, b * a.sb + c0, b * a.db + c0, begin, end, s,
-                       [&](int64_t, const float(&v)[V], const float(&d)[V]) __attribute__((always_inline)) {
 #pragma unroll
-                         for (int k = 0; k < V; ++k) {
-                           const float xhat = (v[k] - mean[k]) * rstd[k];
-                           float slope;
-                           activate<ACT, true>(fmaf(xhat, w[k], add[k]), slope);
-                           const float dz = d[k] * slope;
-                           s1[k] += dz;
-                           s2[k] = fmaf(dz, xhat, s2[k]);
-                         }
-                       });
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      lds[(s.row * a.C + c0 + k) * 2] = s1[k];
-      lds[(s.row * a.C + c0 + k) * 2 + 1] = s2[k];
-    }
+    for (int k = 0; k < V; ++k) lds2[s.row * a.C + s.c0 + k] = float2{s1[k], s2[k]};
   }
   __syncthreads();
-  float* p = a.part + (int64_t)blockIdx.x * a.C * 2;
-  for (int i = threadIdx.x; i < 2 * a.C; i += NORM_T) {
-    float sum = 0.0f;
-    for (int r = 0; r < rows; ++r) sum += lds[r * a.C * 2 + i];
-    p[i] = sum;
+  __shared__ float2 sums[NORM_T];
+  const int parts = a.C < NORM_T ? NORM_T / a.C : 1;
+  if (parts > 1) {  // rows of a channel by several threads
+    const int part = threadIdx.x / a.C, c = threadIdx.x - part * a.C;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (part < parts) {
+      for (int r = part; r < rows; r += parts) {
+        s1 += lds2[r * a.C + c].x;
+        s2 += lds2[r * a.C + c].y;
+      }
+    }
+    sums[threadIdx.x] = float2{s1, s2};
+    __syncthreads();
   }
-}
-
-// One workgroup per (image, group): the chunks' sums per channel, and the group's two means.
-__global__ __launch_bounds__(256) void norm_grad_merge_kernel(const NormArgs a) {
-  __shared__ float red[4][2];
-  const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float g1 = 0.0f, g2 = 0.0f;
-  for (int d = wave; d < a.D; d += 4) {
-    const int c = g * a.D + d;
-    double s1 = 0.0, s2 = 0.0;
-    for (int i = lane; i < a.chunks; i += 64) {
-      const float* p = a.part + (((int64_t)b * a.chunks + i) * a.C + c) * 2;
-      s1 += p[0];
-      s2 += p[1];
+  for (int c = threadIdx.x; c < a.C; c += NORM_T) {
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int p = 0; p < parts; ++p) {
+      const float2 v = parts > 1 ? sums[p * a.C + c] : lds2[c];  // (one row where there is one part)
+      s1 += v.x;
+      s2 += v.y;
     }
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
-    if (lane == 0) {
-      a.csum[((int64_t)b * a.C + c) * 2] = (float)s1;
-      a.csum[((int64_t)b * a.C + c) * 2 + 1] = (float)s2;
+    for (int r = 1; parts == 1 && r < rows; ++r) {
+      s1 += lds2[r * a.C + c].x;
+      s2 += lds2[r * a.C + c].y;
     }
+    s2 *= a.stats[2 * ((int64_t)ch.b * a.G + c / a.D) + 1];
+    reinterpret_cast<float2*>(a.cpart)[(int64_t)blockIdx.x * a.C + c] = float2{s1, s2};
     const float w = param(a.weight, a.wdt, c, 1.0f);
-    g1 = fmaf((float)s1, w, g1);
-    g2 = fmaf((float)s2, w, g2);
-  }
-  if (lane == 0) {
-    red[wave][0] = g1;
-    red[wave][1] = g2;
+    lds2[c] = float2{s1 * w, s2 * w};
   }
   __syncthreads();
-  if (threadIdx.x < 2) {
-    const int k = threadIdx.x;
-    a.coef[2 * (int64_t)blockIdx.x + k] = (red[0][k] + red[1][k] + red[2][k] + red[3][k]) / ((float)a.P * (float)a.D);
+  const int lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < a.G; g += NORM_T / 64) {
+    float t1 = 0.0f, t2 = 0.0f;
+    for (int d = lane; d < a.D; d += 64) {
+      t1 += lds2[g * a.D + d].x;
+      t2 += lds2[g * a.D + d].y;
+    }
+    t1 = wave_sum(t1);
+    t2 = wave_sum(t2);
+    if (lane == 0) reinterpret_cast<float2*>(a.gpart)[(int64_t)blockIdx.x * a.G + g] = float2{t1, t2};
   }
 }
 
-// Parameter gradients: the images' per-channel sums, in the order of the images. One wavefront per channel.
-__global__ __launch_bounds__(256) void norm_grad_params_kernel(const NormArgs a) {
-  const int c = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (c >= a.C) return;
+// Parameter gradients: 8 channels a workgroup, all chunks of all images in order
+__device__ __forceinline__ void norm_grad_params(const NormArgs& a, int block) {
+  __shared__ double red[NORM_T / 8][8][2];
+  const int c = block * 8 + (threadIdx.x & 7), row = threadIdx.x >> 3;
   double s1 = 0.0, s2 = 0.0;
-  for (int b = lane; b < a.B; b += 64) {
-    s1 += a.csum[((int64_t)b * a.C + c) * 2];
-    s2 += a.csum[((int64_t)b * a.C + c) * 2 + 1];
+  if (c < a.C) {
+    for (int64_t i = row; i < (int64_t)a.B * a.chunks; i += NORM_T / 8) {
+      const float2 v = reinterpret_cast<const float2*>(a.cpart)[i * a.C + c];
+      s1 += v.x;
+      s2 += v.y;
+    }
   }
-  s1 = wave_sum(s1);
-  s2 = wave_sum(s2);
-  if (lane == 0) {
-    if (a.dbias != nullptr) store_param(a.dbias, a.bdt, c, (float)s1);
-    if (a.dweight != nullptr) store_param(a.dweight, a.wdt, c, (float)s2);
+  red[row][threadIdx.x & 7][0] = s1;
+  red[row][threadIdx.x & 7][1] = s2;
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    const int k = threadIdx.x & 1, ch = threadIdx.x >> 1;
+    double sum = 0.0;
+    for (int r = 0; r < NORM_T / 8; ++r) sum += red[r][ch][k];
+    if (block * 8 + ch < a.C) {
+      if (k == 0 && a.dbias != nullptr) store_param(a.dbias, a.bdt, block * 8 + ch, (float)sum);
+      if (k == 1 && a.dweight != nullptr) store_param(a.dweight, a.wdt, block * 8 + ch, (float)sum);
+    }
   }
 }
 
+// Backward, second pass: dx; the workgroups past the chunks', the parameters' gradients.
 template <int DT, int V, int ACT>
-__global__ __launch_bounds__(NORM_T) void norm_grad_apply_kernel(const NormArgs a) {
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const int64_t begin = chunk * a.chunk, end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
-  const int cols = a.C / V, passes = passes_of(cols);
-  for (int pass = 0; pass < passes; ++pass) {
-    const Share s = share_of(cols, pass);
-    if (!s.live) continue;
-    const int c0 = s.col * V;
-    float mean[V], rstd[V], w[V], add[V], m1[V], m2[V];
+__global__ __launch_bounds__(NORM_T, 4) void norm_grad_apply_kernel(const NormArgs a) {
+  typedef Pack<DT, V> Pk;
+  __shared__ float2 coef[NORM_MERGE_G];
+  if ((int)blockIdx.x >= a.B * a.chunks) {
+    norm_grad_params(a, blockIdx.x - a.B * a.chunks);
+    return;
+  }
+  const Chunk ch = chunk_of(a);
+  for (int pass = 0; pass < passes_of<V>(a); ++pass) {
+    const Share s = share_of<V>(a, pass, ch.pixels);
+    const bool any = s.live && s.n > 0;
+    const Rows<DT, V, NORM_GRAD_U> x(a.x, a.sb, a.sp, ch, s), d(a.dy, a.db, a.dp, ch, s);
+    if (pass == 0 && !a.merged) merge_groups<true>(a, ch.b, coef);
+    if (!any) continue;
+    typename Pk::Raw rx[2][NORM_GRAD_U], rd[2][NORM_GRAD_U];
+    x.load(0, rx[0]);
+    d.load(0, rd[0]);
+    const GradParams<V> p(a, ch.b, s.c0);
+    float k1[V], k2[V];  // dx = mul dz - ((x - mean) rstd^2 s2 + rstd s1)
+    int g[V];
+    groups_of<V>(s.c0, a.D, g);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int64_t bg = (int64_t)b * a.G + (c0 + k) / a.D;
-      mean[k] = a.stats[2 * bg];
-      rstd[k] = a.stats[2 * bg + 1];
-      m1[k] = a.coef[2 * bg];
-      m2[k] = a.coef[2 * bg + 1];
-      w[k] = param(a.weight, a.wdt, c0 + k, 1.0f);
-      add[k] = param(a.bias, a.bdt, c0 + k, 0.0f);
+      const float rstd = a.stats[2 * ((int64_t)ch.b * a.G + g[k]) + 1];
+      const float2 v = a.merged ? reinterpret_cast<const float2*>(a.coef)[(int64_t)ch.b * a.G + g[k]] : coef[g[k]];
+      k1[k] = rstd * v.x;
+      k2[k] = rstd * rstd * v.y;
     }
-    const int64_t out = (int64_t)b * a.P * a.C + c0;
-    for_pixels2<DT, V>(a, b * a.sb + c0, b * a.db + c0, begin, end, s,
-                       [&](int64_t i, const float(&v)[V], const float(&d)[V]) __attribute__((always_inline)) {
-                         float dx[V];
+    uint8_t* out = a.out + (((int64_t)ch.b * a.P + ch.begin + s.row) * a.C + s.c0) * Pk::ES;
+    const int64_t step = (int64_t)s.rows * a.C * Pk::ES;
+    batches2<DT, V, NORM_GRAD_U>(x, d, rx, rd, [&](int i, const typename Pk::Raw(&nx)[NORM_GRAD_U], const typename Pk::Raw(&nd)[NORM_GRAD_U])
+                    __attribute__((always_inline)) {
 #pragma unroll
-                         for (int k = 0; k < V; ++k) {
-                           const float xhat = (v[k] - mean[k]) * rstd[k];
-                           float slope;
-                           activate<ACT, true>(fmaf(xhat, w[k], add[k]), slope);
-                           dx[k] = rstd[k] * (fmaf(d[k] * slope, w[k], -m1[k]) - xhat * m2[k]);
-                         }
-                         Pack<DT, V>::store(a.out, out + i * a.C, dx);
-                       });
+      for (int u = 0; u < NORM_GRAD_U; ++u) {
+        if (i + u >= s.n) break;
+        float v[V], e[V];
+        Pk::unpack(nx[u], v);
+        Pk::unpack(nd[u], e);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float c = v[k] - p.mean[k];
+          float slope;
+          activate<ACT, true>(fmaf(c, p.mul[k], p.add[k]), slope);
+          v[k] = e[k] * slope * p.mul[k] - fmaf(c, k2[k], k1[k]);  // (equal products of a single value cancel)
+        }
+        Pk::store(out + (i + u) * step, v);
+      }
+    });
   }
 }
 
 // -- launches ----------------------------------------------------------------------------------------------------------
 
-// Chunks of an image: about two workgroups per CU over all images (each keeps 512 x 4 loads in flight), but at least
-// 8 pixels per thread row of a workgroup.
-static void norm_split(int64_t B, int64_t P, int64_t C, int64_t& chunk, int& chunks) {
+// Chunks of an image: about two workgroups per CU over all images, each thread at least two pixels (8 channels a load)
+static void norm_split(int64_t B, int64_t P, int64_t C, int& chunk, int& chunks) {
   const int64_t want = cdiv(2 * (int64_t)device_cus(), B > 0 ? B : 1);
-  int64_t least = cdiv(8 * NORM_T * 8, C);
-  if (least < 1) least = 1;
-  chunk = cdiv(P, want > 0 ? want : 1);
-  if (chunk < least) chunk = least;
-  if (chunk > P) chunk = P > 0 ? P : 1;
+  const int64_t rows = C >= 8 * NORM_T ? 1 : 8 * NORM_T / C;
+  int64_t size = cdiv(P, want);
+  if (size < rows * 2) size = rows * 2;
+  if (size > P) size = P;
+  if (size < 1) size = 1;
+  chunk = (int)(size > INT32_MAX ? INT32_MAX : size);
   chunks = (int)cdiv(P > 0 ? P : 1, chunk);
 }
 
@@ -504,6 +706,18 @@ static size_t norm_lds(int64_t C, int v) {
   return (size_t)(rows * C * 2 * 4);
 }
 
+// Sizes and chunks; false: too many
+static bool norm_shape(NormArgs& a, int64_t B, int64_t P, int64_t C, int64_t groups) {
+  a.P = P;
+  a.B = (int)B;
+  a.C = (int)C;
+  a.G = (int)groups;
+  a.D = (int)(C / groups);
+  norm_split(B, P, C, a.chunk, a.chunks);
+  a.merged = a.G > NORM_MERGE_G || B * a.chunks * a.chunks * a.G > NORM_MERGE;
+  return B * a.chunks + C <= INT32_MAX;
+}
+
 }  // namespace fim
 
 using namespace fim;
@@ -512,10 +726,9 @@ extern "C" int fim_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t
   if (floats == nullptr) return FIM_ERR_INVALID;
   const int rc = norm_check(FIM_F32, B, P, C, groups, FIM_F32, FIM_F32, 0);
   if (rc != FIM_OK) return rc;
-  int64_t chunk;
-  int chunks;
+  int chunk, chunks;
   norm_split(B, P, C, chunk, chunks);
-  *floats = 2 * B * (backward ? (int64_t)chunks * C + C + groups : (int64_t)chunks * groups);
+  *floats = 2 * B * ((int64_t)chunks * groups + (backward ? chunks * C + groups : 0));
   return FIM_OK;
 }
 
@@ -528,30 +741,24 @@ extern "C" int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, in
   if (B * P == 0) return FIM_OK;
   if (x == nullptr || out == nullptr || stats == nullptr || workspace == nullptr) return FIM_ERR_INVALID;
   NormArgs a{};
-  a.x = x;
-  a.out = out;
+  a.x = static_cast<const uint8_t*>(x);
+  a.out = static_cast<uint8_t*>(out);
   a.weight = weight;
   a.bias = bias;
   a.wdt = weight_dtype;
   a.bdt = bias_dtype;
   a.stats = stats;
-  a.part = workspace;
-  a.P = P;
+  a.gpart = workspace;
   a.sb = stride_b;
   a.sp = stride_p;
-  a.B = (int)B;
-  a.C = (int)C;
-  a.G = (int)groups;
-  a.D = (int)(C / groups);
   a.eps = eps;
-  norm_split(B, P, C, a.chunk, a.chunks);
-  if (B * a.chunks > INT32_MAX) return FIM_ERR_UNSUPPORTED;
+  if (!norm_shape(a, B, P, C, groups)) return FIM_ERR_UNSUPPORTED;
   const int v = norm_vector(dtype, C, {stride_b, stride_p}, {x, out});
   const dim3 grid((unsigned)(B * a.chunks));
   with_vector(dtype, v, [&](auto dt, auto vec) {
     constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
     norm_stats_kernel<DT, V><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(a);
-    norm_merge_kernel<<<dim3((unsigned)cdiv(B * groups, 4)), dim3(256), 0, stream>>>(a);
+    if (a.merged) norm_merge_kernel<false><<<dim3((unsigned)cdiv(B * groups, 4)), dim3(256), 0, stream>>>(a);
     with_activation(act, [&](auto act_c) {
       norm_apply_kernel<DT, V, decltype(act_c)::value><<<grid, dim3(NORM_T), 0, stream>>>(a);
     });
@@ -569,9 +776,9 @@ extern "C" int fim_group_norm_backward(const void* x, const void* d_out, int dty
   if (B * P == 0) return FIM_OK;
   if (x == nullptr || d_out == nullptr || dx == nullptr || stats == nullptr || workspace == nullptr) return FIM_ERR_INVALID;
   NormArgs a{};
-  a.x = x;
-  a.dy = d_out;
-  a.out = dx;
+  a.x = static_cast<const uint8_t*>(x);
+  a.dy = static_cast<const uint8_t*>(d_out);
+  a.out = static_cast<uint8_t*>(dx);
   a.weight = weight;
   a.bias = bias;
   a.wdt = weight_dtype;
@@ -579,32 +786,24 @@ extern "C" int fim_group_norm_backward(const void* x, const void* d_out, int dty
   a.stats = const_cast<float*>(stats);
   a.dweight = d_weight;
   a.dbias = d_bias;
-  a.P = P;
   a.sb = stride_b;
   a.sp = stride_p;
   a.db = d_stride_b;
   a.dp = d_stride_p;
-  a.B = (int)B;
-  a.C = (int)C;
-  a.G = (int)groups;
-  a.D = (int)(C / groups);
-  norm_split(B, P, C, a.chunk, a.chunks);
-  if (B * a.chunks > INT32_MAX) return FIM_ERR_UNSUPPORTED;
-  a.part = workspace;
-  a.csum = workspace + 2 * B * (int64_t)a.chunks * C;
-  a.coef = a.csum + 2 * B * C;
+  if (!norm_shape(a, B, P, C, groups)) return FIM_ERR_UNSUPPORTED;
+  a.gpart = workspace;
+  a.cpart = a.gpart + 2 * B * a.chunks * groups;
+  a.coef = a.cpart + 2 * B * a.chunks * C;
   const int v = norm_vector(dtype, C, {stride_b, stride_p, d_stride_b, d_stride_p}, {x, d_out, dx});
-  const dim3 grid((unsigned)(B * a.chunks));
+  const int64_t chunks = B * a.chunks, params = d_weight != nullptr || d_bias != nullptr ? cdiv(C, 8) : 0;
   with_vector(dtype, v, [&](auto dt, auto vec) {
     constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
     with_activation(act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
-      norm_grad_sums_kernel<DT, V, ACT><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(a);
-      norm_grad_merge_kernel<<<dim3((unsigned)(B * groups)), dim3(256), 0, stream>>>(a);
-      norm_grad_apply_kernel<DT, V, ACT><<<grid, dim3(NORM_T), 0, stream>>>(a);
+      norm_grad_sums_kernel<DT, V, ACT><<<dim3((unsigned)chunks), dim3(NORM_T), norm_lds(C, V), stream>>>(a);
+      if (a.merged) norm_merge_kernel<true><<<dim3((unsigned)cdiv(B * groups, 4)), dim3(256), 0, stream>>>(a);
+      norm_grad_apply_kernel<DT, V, ACT><<<dim3((unsigned)(chunks + params)), dim3(NORM_T), 0, stream>>>(a);
     });
-    if (d_weight != nullptr || d_bias != nullptr)
-      norm_grad_params_kernel<<<dim3((unsigned)cdiv(C, 4)), dim3(256), 0, stream>>>(a);
   });
   return launch_status();
 }
