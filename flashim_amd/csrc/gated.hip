@@ -26,33 +26,70 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(const uint16_t* from, i
   }
 }
 
-// out[i] = sum over s of part[s][i], in order
+// out[i] = sum over s of part[s][i], in order. Few splits: four values a thread where n and the outputs' addresses allow
 template <int DT>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* part, int64_t n, int64_t splits, uint16_t* out0,
-                                                         uint16_t* out1) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int64_t s = 0; s < splits; ++s) v += part[s * 2 * n + i];
-    uint16_t* out = i < n ? out0 : out1;
-    if (out != nullptr) out[i < n ? i : i - n] = to16<DT>(v);
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* part, int64_t n, int splits, uint16_t* out0,
+                                                         uint16_t* out1, int wide) {
+  if (wide) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < 2 * n; i += (int64_t)gridDim.x * 1024) {
+      v4f v = *reinterpret_cast<const v4f*>(part + i);
+      for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(part + s * 2 * n + i);
+      uint16_t* out = i < n ? out0 : out1;
+      if (out == nullptr) continue;
+      *reinterpret_cast<uint2*>(out + (i < n ? i : i - n)) = uint2{to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
+    }
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * 256) {
+      float v = part[i];
+      for (int s = 1; s < splits; ++s) v += part[s * 2 * n + i];
+      uint16_t* out = i < n ? out0 : out1;
+      if (out != nullptr) out[i < n ? i : i - n] = to16<DT>(v);
+    }
   }
 }
 
-// db[i][c] = sum over tiles of col_sums[tile][i][c]: one wavefront per value
+// Many splits: 64 values a workgroup, the splits dealt to its four wavefronts, whose sums are added in their order
 template <int DT>
-__global__ __launch_bounds__(256) void gated_bias_kernel(const float* col_sums, int64_t n, int64_t tiles, void* db0,
-                                                         void* db1, int bdt) {
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= 2 * n) return;
+__global__ __launch_bounds__(256) void gated_join_many_kernel(const float* part, int64_t n, int splits, uint16_t* out0,
+                                                              uint16_t* out1) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  float v = 0.0f;
+  if (i < 2 * n) {
+#pragma unroll 8
+    for (int s = wave; s < splits; s += 4) v += part[s * 2 * n + i];
+  }
+  sums[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0 || i >= 2 * n) return;
+  uint16_t* out = i < n ? out0 : out1;
+  if (out != nullptr) out[i < n ? i : i - n] = to16<DT>(sums[0][lane] + sums[1][lane] + (sums[2][lane] + sums[3][lane]));
+}
+
+// db[i][c] = sum over tiles of col_sums[tile][i][c]: 16 values a workgroup, the tiles dealt to 64 rows of threads
+template <int DT>
+__global__ __launch_bounds__(1024) void gated_bias_kernel(const float* col_sums, int64_t n, int64_t tiles, void* db0,
+                                                          void* db1, int bdt) {
+  __shared__ double sums[64][16];
+  const int c = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t at = (int64_t)blockIdx.x * 16 + c;
   double v = 0.0;
-  for (int64_t t = threadIdx.x & 63; t < tiles; t += 64) v += col_sums[t * 2 * n + at];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if (at < 2 * n) {
+#pragma unroll 8
+    for (int64_t t = row; t < tiles; t += 64) v += col_sums[t * 2 * n + at];
+  }
+  sums[row][c] = v;
+  __syncthreads();
+  for (int half = 32; half > 0; half /= 2) {
+    if (row < half) sums[row][c] += sums[row + half][c];
+    __syncthreads();
+  }
   void* db = at < n ? db0 : db1;
-  if ((threadIdx.x & 63) != 0 || db == nullptr) return;
-  const int64_t c = at < n ? at : at - n;
-  if (bdt == FIM_F32) static_cast<float*>(db)[c] = (float)v;
-  else static_cast<uint16_t*>(db)[c] = to16<DT>((float)v);
+  if (row != 0 || at >= 2 * n || db == nullptr) return;
+  const int64_t to = at < n ? at : at - n;
+  if (bdt == FIM_F32) static_cast<float*>(db)[to] = (float)sums[0][c];
+  else static_cast<uint16_t*>(db)[to] = to16<DT>((float)sums[0][c]);
 }
 
 // -- launches ----------------------------------------------------------------------------------------------------------
@@ -121,7 +158,7 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.hp = cdiv(g.H, 8) * 8;
   g.ldg = cdiv(g.H, 64) * 64 + 64;
   if (!backward) return g;
-  g.grad = gated_tile(g.M, 2 * g.H, 1);
+  g.grad = {2, 2};  // (its epilogue has no registers left beside 256 x 256 accumulators)
   g.dgu_at = g.total;
   g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
   g.part_at = g.cols_at + align256(2 * cdiv(g.M, 64 * g.grad.mb) * 2 * g.H * 4);
@@ -166,8 +203,10 @@ static void launch_tile(TileArgs a, int64_t splits, hipStream_t stream) {
 
 template <int DT, int MODE, int ACT>
 static void launch_product(const TileArgs& a, Tile t, int64_t splits, hipStream_t stream) {
-  if (t.mb == 4) launch_tile<DT, MODE, ACT, 4, 4>(a, splits, stream);
-  else launch_tile<DT, MODE, ACT, 2, 2>(a, splits, stream);
+  if constexpr (MODE != GATED_GRAD) {
+    if (t.mb == 4) return launch_tile<DT, MODE, ACT, 4, 4>(a, splits, stream);
+  }
+  launch_tile<DT, MODE, ACT, 2, 2>(a, splits, stream);
 }
 
 static int gated_check(int dtype, int64_t M, int64_t K, int64_t H, int bias_dtype, int act) {
@@ -255,6 +294,8 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || d_out == nullptr) return FIM_ERR_INVALID;
   Gated g = gated_plan(matrix(x, x_stride, M, K), matrix(w_gate, w_gate_stride, H, K), matrix(w_up, w_up_stride, H, K), true);
   if (workspace == nullptr || workspace_bytes < g.total) return FIM_ERR_INVALID;
+  if (M == 1) d_out_stride = H;
+  if (d_out_stride >= (1 << 22)) return FIM_ERR_UNSUPPORTED;  // 32-bit offsets inside a tile
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   gated_operands(g, ws, stream);
   uint16_t* dg = reinterpret_cast<uint16_t*>(ws + g.dgu_at);
@@ -263,7 +304,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   TileArgs a = gated_forward_args(g, b_gate, b_up, bias_dtype);
   a.dout = static_cast<const uint16_t*>(d_out);
   a.ldd = d_out_stride;
-  a.wide_dout = rows_wide(d_out, d_out_stride);
+  a.wide_dout = rows_wide(d_out, d_out_stride) && H % 8 == 0;
   a.out[0] = dg;
   a.out[1] = du;
   a.ldo = g.ldg;
@@ -276,7 +317,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       launch_product<DT, GATED_GRAD, decltype(act_c)::value>(a, g.grad, 1, stream);
     });
     if (biases)
-      gated_bias_kernel<DT><<<dim3((unsigned)cdiv(2 * H, 4)), dim3(256), 0, stream>>>(
+      gated_bias_kernel<DT><<<dim3((unsigned)cdiv(2 * H, 16)), dim3(1024), 0, stream>>>(
           a.col_sums, H, 2 * cdiv(M, 64 * g.grad.mb), db_gate, db_up, bias_dtype);
     if (dx != nullptr) {
       TileArgs d{};
@@ -310,9 +351,16 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       w.part = reinterpret_cast<float*>(ws + g.part_at);
       w.k_split = g.k_split;
       launch_product<DT, GATED_DW, ACT_NONE>(w, g.dw, g.splits, stream);
-      const int64_t blocks = cdiv(2 * H * K, 256);
-      gated_join_kernel<DT><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream>>>(
-          w.part, H * K, g.splits, static_cast<uint16_t*>(dw_gate), static_cast<uint16_t*>(dw_up));
+      uint16_t *g16 = static_cast<uint16_t*>(dw_gate), *u16 = static_cast<uint16_t*>(dw_up);
+      if (g.splits <= 4) {
+        const int wide = H * K % 4 == 0 && (reinterpret_cast<uintptr_t>(g16) | reinterpret_cast<uintptr_t>(u16)) % 8 == 0;
+        const int64_t blocks = cdiv(2 * H * K, wide ? 1024 : 256);
+        gated_join_kernel<DT><<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream>>>(
+            w.part, H * K, (int)g.splits, g16, u16, wide);
+      } else {
+        gated_join_many_kernel<DT><<<dim3((unsigned)cdiv(2 * H * K, 64)), dim3(256), 0, stream>>>(w.part, H * K,
+                                                                                                  (int)g.splits, g16, u16);
+      }
     }
   });
   return launch_status();

@@ -331,18 +331,31 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
         }
       }
   } else {
-    // 32 rows at a time through LDS (this wavefront's own part of the consumed stage): whole runs of the output's rows
+    // 32 rows at a time through LDS (this wavefront's own part of the consumed stage): whole runs of the output's rows, by
+    // buffer stores whose rows and columns past the end go out of range, without branches
     constexpr int NO = PAIR ? NB / 2 : NB, OC = 32 * NO, RB = OC * 2, SLOTS = RB / 16, PER = 64 / SLOTS;
-    constexpr int AREA = 32 * RB, AREAS = MODE == GATED_GRAD ? 2 : 1;
+    constexpr int AREA = 32 * RB, AREAS = MODE == GATED_GRAD ? 2 : 1, RUNS = 32 / PER;
     static_assert(4 * AREAS * AREA <= STAGE, "the wavefronts' areas lie in the first stage");
     uint8_t* area = st0 + wave * AREAS * AREA;
     auto place = [&](int row, int slot) __attribute__((always_inline)) {
       constexpr int RPL = RB >= 256 ? 1 : 256 / RB;
       return row * RB + ((slot ^ ((row / RPL) & (SLOTS - 1))) << 4);
     };
-    const int64_t nw = n0 + wn * OC;
+    const int64_t nw = n0 + wn * OC, rows_left = a.M - mw;
     const int slot = lane % SLOTS, prow = lane / SLOTS;
-    const int64_t col = nw + slot * 8;
+    const int cols_out = (int)(a.out_cols - nw < OC ? a.out_cols - nw : OC);
+    const int cols_in = (int)(a.N - nw < OC ? a.N - nw : OC);
+    auto buffer_bytes = [&](int64_t ld, int64_t cols) __attribute__((always_inline)) {
+      const int64_t n = cols <= 0 ? 0 : rest(rows_left < 32 * MB ? rows_left : 32 * MB, ld, cols);
+      return __builtin_amdgcn_readfirstlane((int)(n > 0x7fffffff ? 0x7fffffff : n));
+    };
+    const __amdgpu_buffer_rsrc_t o0 =
+        __builtin_amdgcn_make_buffer_rsrc(a.out[0] + mw * a.ldo + nw, (short)0, buffer_bytes(a.ldo, cols_out), 0x00020000);
+    const __amdgpu_buffer_rsrc_t o1 = __builtin_amdgcn_make_buffer_rsrc(
+        (MODE == GATED_GRAD ? a.out[1] : a.out[0]) + mw * a.ldo + nw, (short)0, buffer_bytes(a.ldo, cols_out), 0x00020000);
+    const __amdgpu_buffer_rsrc_t din = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(a.dout) + (MODE == GATED_GRAD ? mw * a.ldd + nw : 0), (short)0,
+        MODE == GATED_GRAD ? buffer_bytes(a.ldd, cols_in) : 0, 0x00020000);
     float sums[MODE == GATED_GRAD ? NB : 1][16];
     if constexpr (MODE == GATED_GRAD) {
 #pragma unroll
@@ -350,82 +363,102 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
 #pragma unroll
         for (int q = 0; q < 16; ++q) sums[i][q] = 0.0f;
     }
+    auto epilogue = [&](auto wide_c) __attribute__((always_inline)) {
+      constexpr bool WIDE = decltype(wide_c)::value;  // 16-byte rows of out (GRAD: of dout)
+      v4i grad[2][MODE == GATED_GRAD ? RUNS : 1];  // rows of the incoming gradient, 32 ahead
+      auto load_grad = [&](int j) __attribute__((always_inline)) {
+        if constexpr (MODE == GATED_GRAD) {
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      if constexpr (MODE == GATED_GRAD) {  // the incoming gradient's rows into the first area
-#pragma unroll
-        for (int p = 0; p < 32 / PER; ++p) {
-          const int row = p * PER + prow;
-          const int64_t m = mw + 32 * j + row;
-          uint4 v = {0, 0, 0, 0};
-          if (m < a.M && col < a.N) {
-            const uint16_t* from = a.dout + m * a.ldd + col;
-            if (a.wide_dout && col + 8 <= a.N) {
-              v = *reinterpret_cast<const uint4*>(from);
+          for (int p = 0; p < RUNS; ++p) {
+            const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldd + slot * 8) * 2u;
+            if constexpr (WIDE) {
+              grad[j & 1][p] = __builtin_bit_cast(
+                  v4i, __builtin_amdgcn_raw_buffer_load_b128(din, (int)(slot * 8 < cols_in ? at : TILE_OOB), 0, 0));
             } else {
               uint32_t e[8];
 #pragma unroll
-              for (int c = 0; c < 8; ++c) e[c] = col + c < a.N ? from[c] : 0;
-              v = uint4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+              for (int c = 0; c < 8; ++c)
+                e[c] = __builtin_amdgcn_raw_buffer_load_b16(din, (int)(slot * 8 + c < cols_in ? at + 2 * c : TILE_OOB), 0, 0);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) grad[j & 1][p][c] = (int)(e[2 * c] | e[2 * c + 1] << 16);
             }
           }
-          *reinterpret_cast<uint4*>(area + place(row, slot)) = v;
         }
+      };
+      load_grad(0);
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+        if constexpr (MODE == GATED_GRAD) {
+          if (j + 1 < MB) load_grad(j + 1);
+#pragma unroll
+          for (int p = 0; p < RUNS; ++p) *reinterpret_cast<v4i*>(area + place(p * PER + prow, slot)) = grad[j & 1][p];
+          wave_lds_wait();
+          if (rows_left < 32 * (j + 1)) {  // rows past the end: zero times anything
+            const bool past = 32 * j + frow >= rows_left;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+              for (int q = 0; q < 16; ++q) acc[i][j][q] = past ? 0.0f : acc[i][j][q];
+          }
+        }
+#pragma unroll
+        for (int o = 0; o < NO; ++o)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint8_t* at = area + place(frow, 4 * o + q) + 8 * h;
+            typedef int v2i __attribute__((ext_vector_type(2)));
+            if constexpr (MODE == GATED_FORWARD) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(acc[o][j][4 * q + e]) * acc[o + NO][j][4 * q + e];
+              *reinterpret_cast<v2i*>(at) = v2i{(int)to16x2<DT>(v[0], v[1]), (int)to16x2<DT>(v[2], v[3])};
+            } else if constexpr (MODE == GATED_DX) {
+              const v16f& s = acc[o][j];
+              *reinterpret_cast<v2i*>(at) =
+                  v2i{(int)to16x2<DT>(s[4 * q], s[4 * q + 1]), (int)to16x2<DT>(s[4 * q + 2], s[4 * q + 3])};
+            } else {
+              const v2i d2 = *reinterpret_cast<const v2i*>(at);
+              const uint16_t d[4] = {(uint16_t)d2[0], (uint16_t)((uint32_t)d2[0] >> 16), (uint16_t)d2[1],
+                                     (uint16_t)((uint32_t)d2[1] >> 16)};
+              float dg[4], du[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float slope;
+                const float act = activate<ACT, true>(acc[o][j][4 * q + e], slope);
+                const float dv = from16<DT>(d[e]);
+                dg[e] = dv * acc[o + NO][j][4 * q + e] * slope;
+                du[e] = dv * act;
+                sums[o][4 * q + e] += dg[e];
+                sums[o + NO][4 * q + e] += du[e];
+              }
+              *reinterpret_cast<v2i*>(at) = v2i{(int)to16x2<DT>(dg[0], dg[1]), (int)to16x2<DT>(dg[2], dg[3])};
+              *reinterpret_cast<v2i*>(at + AREA) = v2i{(int)to16x2<DT>(du[0], du[1]), (int)to16x2<DT>(du[2], du[3])};
+            }
+          }
+        wave_lds_wait();
+#pragma unroll
+        for (int k = 0; k < AREAS; ++k)
+#pragma unroll
+          for (int p = 0; p < RUNS; ++p) {
+            const int row = p * PER + prow;
+            const v4i v = *reinterpret_cast<const v4i*>(area + k * AREA + place(row, slot));
+            const uint32_t at = (uint32_t)((32 * j + row) * a.ldo + slot * 8) * 2u;
+            if constexpr (WIDE || MODE == GATED_GRAD) {
+              typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), k ? o1 : o0,
+                                                     (int)(slot * 8 < cols_out ? at : TILE_OOB), 0, 0);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                __builtin_amdgcn_raw_buffer_store_b16((uint16_t)((uint32_t)v[c / 2] >> (16 * (c & 1))), o0,
+                                                      (int)(slot * 8 + c < cols_out ? at + 2 * c : TILE_OOB), 0, 0);
+            }
+          }
         wave_lds_wait();
       }
-#pragma unroll
-      for (int o = 0; o < NO; ++o)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint8_t* at = area + place(frow, 4 * o + q) + 8 * h;
-          if constexpr (MODE == GATED_FORWARD) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(acc[o][j][4 * q + e]) * acc[o + NO][j][4 * q + e];
-            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
-          } else if constexpr (MODE == GATED_DX) {
-            const v16f& s = acc[o][j];
-            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(s[4 * q], s[4 * q + 1]), to16x2<DT>(s[4 * q + 2], s[4 * q + 3])};
-          } else {
-            const uint2 d2 = *reinterpret_cast<const uint2*>(at);
-            const uint16_t d[4] = {(uint16_t)d2.x, (uint16_t)(d2.x >> 16), (uint16_t)d2.y, (uint16_t)(d2.y >> 16)};
-            float dg[4], du[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float slope;
-              const float act = activate<ACT, true>(acc[o][j][4 * q + e], slope);
-              const float dv = from16<DT>(d[e]);
-              dg[e] = dv * acc[o + NO][j][4 * q + e] * slope;
-              du[e] = dv * act;
-              if (mw + 32 * j + frow >= a.M) dg[e] = du[e] = 0.0f;  // (zeros times what the padding rows gave)
-              sums[o][4 * q + e] += dg[e];
-              sums[o + NO][4 * q + e] += du[e];
-            }
-            *reinterpret_cast<uint2*>(at) = uint2{to16x2<DT>(dg[0], dg[1]), to16x2<DT>(dg[2], dg[3])};
-            *reinterpret_cast<uint2*>(at + AREA) = uint2{to16x2<DT>(du[0], du[1]), to16x2<DT>(du[2], du[3])};
-          }
-        }
-      wave_lds_wait();
-#pragma unroll
-      for (int k = 0; k < AREAS; ++k)
-#pragma unroll
-        for (int p = 0; p < 32 / PER; ++p) {
-          const int row = p * PER + prow;
-          const int64_t m = mw + 32 * j + row;
-          const uint4 v = *reinterpret_cast<const uint4*>(area + k * AREA + place(row, slot));
-          if (m >= a.M || col >= a.out_cols) continue;
-          uint16_t* to = a.out[k] + m * a.ldo + col;
-          if (a.wide_out && col + 8 <= a.out_cols) {
-            *reinterpret_cast<uint4*>(to) = v;
-          } else {
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (col + c < a.out_cols) to[c] = (uint16_t)(e[c / 2] >> (16 * (c & 1)));
-          }
-        }
-      wave_lds_wait();
-    }
+    };
+    if (MODE == GATED_GRAD ? a.wide_dout : a.wide_out) epilogue(std::integral_constant<bool, true>{});
+    else epilogue(std::integral_constant<bool, false>{});
     if constexpr (MODE == GATED_GRAD) {
       if (a.col_sums == nullptr) return;
       // lane l: value l % 32 of each 32: block (value / 16), register value % 16

@@ -595,7 +595,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward(
   TORCH_CHECK_VALUE(d_out.sizes() == at::IntArrayRef(with_last(x, g.h)), "gated_linear: gradient of shape ",
                     d_out.sizes(), " for ", x.sizes(), " -> ", g.h);
   check_same(d_out, x.scalar_type(), x, "gated_linear: gradient");
-  const Tensor d = matrix_rows(d_out, "gated_linear");
+  Tensor d = matrix_rows(d_out, "gated_linear");
+  if (d.stride(0) >= (1 << 22)) d = d.contiguous();  // (the kernels' limit)
   auto weight_grad = [&](bool want) { return want ? empty({g.h, g.k}, x, x.scalar_type()) : empty({0}, x, x.scalar_type()); };
   auto bias_grad = [&](const OptTensor& b) {
     return empty({want_biases && b ? g.h : 0}, x, b ? b->scalar_type() : at::kFloat);

@@ -265,7 +265,7 @@ int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t x_s
                      const void* b_up, int bias_dtype, int act, void* out, void* workspace, int64_t workspace_bytes,
                      hipStream_t stream);
 
-/* Its gradients: d_out [M, H] (unit column stride); dx packed [M, K], dw_gate and dw_up packed [H, K], db_gate and db_up
+/* Its gradients: d_out [M, H] (unit column stride, rows less than 2^22 elements apart, else 99); dx packed [M, K], dw_gate and dw_up packed [H, K], db_gate and db_up
  * [H] in the bias type; any of them may be NULL. The pre-activations are computed again; their gradients are rounded to
  * x's type before the products that make dx and the weights' gradients. */
 int fim_gated_linear_backward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w_gate,
