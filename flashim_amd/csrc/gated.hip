@@ -9,6 +9,7 @@
 // forward pass: with K below about 1000 their two writes and reads cost more than the products), which writes dg and du in
 // x's type (they are operands of 16-bit matrix products next; FP32 sums for the bias gradients are taken before that
 // rounding); then one product for dx over both halves and one for the weights, split over rows where its tiles are few.
+#include "gated_rows.h"
 #include "gated_tile.h"
 
 namespace fim {
@@ -132,13 +133,29 @@ static int64_t gated_splits(int64_t tiles, int64_t k) {
   return s < 1 ? 1 : s;
 }
 
+// Whether a launch is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half the
+// CUs. Backward also needs all weights in one workgroup's LDS.
+static bool gated_rows(int64_t M, int64_t K, int64_t H, bool backward) {
+  if (K > 128 || M < 32 * ROWS_WAVES * (int64_t)device_cus() / 2) return false;
+  return !backward || (K <= 64 && H <= rows_hidden(64));
+}
+
+static int64_t rows_blocks(int64_t K, int64_t H) { return cdiv(H, rows_hidden(K <= 64 ? 64 : 128)); }
+
+// Workgroups per hidden block: one per CU over all blocks
+static int64_t rows_groups(int64_t M, int64_t K, int64_t H) {
+  const int64_t most = cdiv(M, 32 * ROWS_WAVES), n = device_cus() / rows_blocks(K, H);
+  return n < 1 ? 1 : n < most ? n : most;
+}
+
 struct Gated {
   Matrix x, wg, wu;
   int64_t M, K, H;
   // workspace, in bytes: copies of the operands; backward: dg and du [M, hp], bias partials, weight partials
   int64_t x_at, wg_at, wu_at, dgu_at, cols_at, part_at, total;
-  int64_t hp, ldg, splits, k_split;
+  int64_t hp, ldg, splits, k_split, sum_rows;
   Tile grad, dw;
+  bool rows;  // backward: dg, du and dx by rows
 };
 
 static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, bool backward) {
@@ -161,7 +178,9 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.grad = {2, 2};  // (its epilogue has no registers left beside 256 x 256 accumulators)
   g.dgu_at = g.total;
   g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
-  g.part_at = g.cols_at + align256(2 * cdiv(g.M, 64 * g.grad.mb) * 2 * g.H * 4);
+  g.rows = gated_rows(g.M, g.K, g.H, true);
+  g.sum_rows = g.rows ? rows_groups(g.M, g.K, g.H) * ROWS_WAVES : 2 * cdiv(g.M, 64 * g.grad.mb);
+  g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
   g.dw = gated_tile(g.K, 2 * g.H, cdiv(g.M, 4096));
   const int64_t tiles = cdiv(g.K, 64 * g.dw.mb) * 2 * cdiv(g.H, 64 * g.dw.nb);
   g.k_split = cdiv(cdiv(g.M, gated_splits(tiles, g.M)), TILE_K) * TILE_K;
@@ -207,6 +226,38 @@ static void launch_product(const TileArgs& a, Tile t, int64_t splits, hipStream_
     if (t.mb == 4) return launch_tile<DT, MODE, ACT, 4, 4>(a, splits, stream);
   }
   launch_tile<DT, MODE, ACT, 2, 2>(a, splits, stream);
+}
+
+template <int DT, int MODE, int ACT, int KP>
+static void launch_rows(const RowsArgs& a, bool wide, hipStream_t stream) {
+  const dim3 grid((unsigned)(rows_groups(a.M, a.K, a.H) * a.blocks));
+  if (wide) gated_rows_kernel<DT, MODE, ACT, KP, true><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+  else gated_rows_kernel<DT, MODE, ACT, KP, false><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+}
+
+// The same launch by rows, from the tiles' arguments
+static RowsArgs rows_args(const TileArgs& a, int64_t K) {
+  RowsArgs r{};
+  r.x = a.x[0];
+  r.ldx = a.ldx;
+  r.ldw = a.ldw;
+  r.M = a.M;
+  r.K = (int)K;
+  r.kw = (int)(cdiv(a.K, 8) * 8);
+  r.H = (int)a.N;
+  for (int i = 0; i < 2; ++i) {
+    r.w[i] = a.w[i];
+    r.bias[i] = a.bias[i];
+    r.out[i] = a.out[i];
+  }
+  r.bias_dtype = a.bias_dtype;
+  r.dout = a.dout;
+  r.ldd = a.ldd;
+  r.ldo = a.ldo;
+  r.out_cols = (int)a.out_cols;
+  r.col_sums = a.col_sums;
+  r.blocks = (int)rows_blocks(K, a.N);
+  return r;
 }
 
 static int gated_check(int dtype, int64_t M, int64_t K, int64_t H, int bias_dtype, int act) {
@@ -275,8 +326,12 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.wide_out = rows_wide(out, H);
   const Tile tile = gated_tile(M, 2 * H, 1);
   with_type(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
     with_activation(act, [&](auto act_c) {
-      launch_product<decltype(dt)::value, GATED_FORWARD, decltype(act_c)::value>(a, tile, 1, stream);
+      constexpr int ACT = decltype(act_c)::value;
+      if (!gated_rows(M, K, H, false)) launch_product<DT, GATED_FORWARD, ACT>(a, tile, 1, stream);
+      else if (K <= 64) launch_rows<DT, GATED_FORWARD, ACT, 64>(rows_args(a, K), a.wide_out, stream);
+      else launch_rows<DT, GATED_FORWARD, ACT, 128>(rows_args(a, K), a.wide_out, stream);
     });
   });
   return launch_status();
@@ -314,12 +369,20 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   with_type(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     with_activation(act, [&](auto act_c) {
-      launch_product<DT, GATED_GRAD, decltype(act_c)::value>(a, g.grad, 1, stream);
+      constexpr int ACT = decltype(act_c)::value;
+      if (g.rows) {
+        RowsArgs r = rows_args(a, K);
+        r.dx = static_cast<uint16_t*>(dx);
+        r.wide_dx = rows_wide(dx, K);
+        launch_rows<DT, GATED_GRAD, ACT, 64>(r, a.wide_dout, stream);
+      } else {
+        launch_product<DT, GATED_GRAD, ACT>(a, g.grad, 1, stream);
+      }
     });
     if (biases)
       gated_bias_kernel<DT><<<dim3((unsigned)cdiv(2 * H, 16)), dim3(1024), 0, stream>>>(
-          a.col_sums, H, 2 * cdiv(M, 64 * g.grad.mb), db_gate, db_up, bias_dtype);
-    if (dx != nullptr) {
+          a.col_sums, H, g.sum_rows, db_gate, db_up, bias_dtype);
+    if (dx != nullptr && !g.rows) {
       TileArgs d{};
       d.x[0] = dg;
       d.x[1] = du;

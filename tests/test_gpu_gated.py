@@ -84,6 +84,21 @@ def test_forward_and_gradients(m, k, h, dtype):
     _backward(x, wg, wu, bg, bu, act, d_out)
 
 
+LONG = [  # many rows of few channels: a last block of one row, odd widths, several hidden blocks, channels up to 128
+    (32800, 64, 256), (32769, 33, 77), (33333, 8, 256), (40001, 40, 104), (36000, 64, 264), (33000, 100, 300),
+    (32768, 128, 136), (35001, 127, 131),
+]
+
+
+@pytest.mark.parametrize("m,k,h", LONG)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_rows_of_few_channels(m, k, h, dtype):
+    act = ("silu", "gelu", "gelu_tanh")[(m + k + h) % 3]
+    x, wg, wu, bg, bu, d_out = _inputs(m, k, h, dtype, bias=(None, F32, dtype)[(m + h) % 3], seed=m + k + h)
+    _forward(x, wg, wu, bg, bu, act)
+    _backward(x, wg, wu, bg, bu, act, d_out)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("bias", [None, "gate", "up", BF16, F32])
 @pytest.mark.parametrize("m", [5, 200])
