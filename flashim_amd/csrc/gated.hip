@@ -115,22 +115,38 @@ static Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t cols) {
 
 struct Tile { int mb, nb; };
 
-// The tile of a product of `rows` x `cols` outputs: 256 x 256 with one workgroup per CU reads half of the operand bytes of
-// 128 x 128 with two per CU, which fill the last round better and cover each other's prologue and epilogue. Costs in
-// rounds of the large tile.
-static Tile gated_tile(int64_t rows, int64_t cols, int64_t splits) {
-  const int64_t cus = device_cus();
-  const double large = (double)cdiv(cdiv(rows, 256) * cdiv(cols, 256) * splits, cus);
-  const double small = 0.65 * (double)cdiv(cdiv(rows, 128) * cdiv(cols, 128) * splits, 2 * cus);
-  return large < small ? Tile{4, 4} : Tile{2, 2};
+// The time of a product of `rows` x `cols` outputs over `k` on a tile, in steps of a 128 x 128 tile (0.9 us). A round of 256
+// x 256 tiles, one per CU, measured 1.4 us a step and 9 us beside (prologue, epilogue); of 128 x 128 tiles, two per CU, which
+// read the operands twice as often but cover each other's prologue and epilogue, 0.9 us and 3 us. (16384 x 1024 x 8192
+// outputs: 256 against 273 us; 20000 x 512 x 4096: 104 against 98; 16384 x 8192 x 1024: 227 against 310.)
+static double tile_time(Tile t, int64_t rows, int64_t cols, int64_t splits, int64_t k) {
+  const int64_t cus = device_cus(), size = 64 * t.mb;
+  const int64_t rounds = cdiv(cdiv(rows, size) * cdiv(cols, size) * splits, cus);
+  const double steps = (double)cdiv(k, TILE_K);
+  // (a last small tile alone on its CU takes more than half the time of two)
+  return t.mb == 4 ? rounds * (1.6 * steps + 10.0) : (0.5 * rounds + 0.1 * (rounds & 1)) * (steps + 3.0);
 }
 
-// Splits of a contraction over `k` rows for `tiles` tiles: enough to fill the CUs about twice, each at least 512 rows
-static int64_t gated_splits(int64_t tiles, int64_t k) {
-  int64_t s = cdiv(2 * (int64_t)device_cus(), tiles);
-  const int64_t most = cdiv(k, 512);
-  if (s > most) s = most;
-  return s < 1 ? 1 : s;
+static Tile gated_tile(int64_t rows, int64_t cols, int64_t k) {
+  const Tile large{4, 4}, small{2, 2};
+  return tile_time(large, rows, cols, 1, k) < tile_time(small, rows, cols, 1, k) ? large : small;
+}
+
+// The weights' gradients: tile, and splits of the rows (their FP32 partials are written once and read once, at 4.5 TB/s)
+static void weights_plan(int64_t M, int64_t K, int64_t H, Tile& tile, int64_t& splits) {
+  double best = 0.0;
+  splits = 0;
+  for (const Tile t : {Tile{4, 4}, Tile{2, 2}}) {
+    for (int64_t s = 1; s <= 256 && (s == 1 || M / s >= 256); s += s < 8 ? 1 : s / 4) {
+      const int64_t size = 64 * t.mb, cols = 2 * cdiv(H, size) * size;
+      const double join = (double)(s + 1) * 2.0 * H * K * 4.0 / 4.5e6;  // us
+      const double time = 0.9 * tile_time(t, K, cols, s, cdiv(M, s)) + join;
+      if (splits != 0 && time >= best) continue;
+      best = time;
+      tile = t;
+      splits = s;
+    }
+  }
 }
 
 // Whether a launch is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half the
@@ -181,9 +197,8 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.rows = gated_rows(g.M, g.K, g.H, true);
   g.sum_rows = g.rows ? rows_groups(g.M, g.K, g.H) * ROWS_WAVES : 2 * cdiv(g.M, 64 * g.grad.mb);
   g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
-  g.dw = gated_tile(g.K, 2 * g.H, cdiv(g.M, 4096));
-  const int64_t tiles = cdiv(g.K, 64 * g.dw.mb) * 2 * cdiv(g.H, 64 * g.dw.nb);
-  g.k_split = cdiv(cdiv(g.M, gated_splits(tiles, g.M)), TILE_K) * TILE_K;
+  weights_plan(g.M, g.K, g.H, g.dw, g.splits);
+  g.k_split = cdiv(cdiv(g.M, g.splits), TILE_K) * TILE_K;
   g.splits = cdiv(g.M, g.k_split);
   g.total = g.part_at + align256(g.splits * 2 * g.H * g.K * 4);
   return g;
@@ -324,7 +339,7 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.out[0] = static_cast<uint16_t*>(out);
   a.ldo = a.out_cols = H;
   a.wide_out = rows_wide(out, H);
-  const Tile tile = gated_tile(M, 2 * H, 1);
+  const Tile tile = gated_tile(M, 2 * H, K);
   with_type(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     with_activation(act, [&](auto act_c) {
@@ -397,7 +412,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       d.out[0] = static_cast<uint16_t*>(dx);
       d.ldo = d.out_cols = K;
       d.wide_out = rows_wide(dx, K);
-      launch_product<DT, GATED_DX, ACT_NONE>(d, gated_tile(M, K, 1), 1, stream);
+      launch_product<DT, GATED_DX, ACT_NONE>(d, gated_tile(M, K, 2 * H), 1, stream);
     }
     if (dw_gate != nullptr || dw_up != nullptr) {
       TileArgs w{};

@@ -244,24 +244,30 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
     }
   };
 
-  // accumulators: lane l, register q of block (i, j): row 32 j + l % 32, column 32 i + 8 (q / 4) + 4 h + q % 4
+  // accumulators: lane l, register q of block (i, j): row 32 j + l % 32, column 32 i + 8 (q / 4) + 4 h + q % 4; started at
+  // the bias (all its loads on one side of the branch on its type: one latency; columns past the end repeat the last)
   v16f acc[NB][MB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     v16f first;
 #pragma unroll
     for (int q = 0; q < 16; ++q) first[q] = 0.0f;
-    if constexpr (PAIR) {  // started at the bias
+    if constexpr (PAIR) {
       const void* b = a.bias[i / (NB / 2)];
-      if (b != nullptr) {
-        const int64_t c0 = n0 + (wn * (NB / 2) + i % (NB / 2)) * 32 + 4 * h;
+      const int64_t c0 = n0 + (wn * (NB / 2) + i % (NB / 2)) * 32 + 4 * h;
+      auto column = [&](int q) __attribute__((always_inline)) {
+        const int64_t c = c0 + 8 * (q >> 2) + (q & 3);
+        return c < a.N ? c : a.N - 1;
+      };
+      if (b != nullptr && a.bias_dtype == FIM_F32) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int64_t c = c0 + 8 * (q >> 2) + (q & 3);
-          if (c < a.N)
-            first[q] = a.bias_dtype == FIM_F32 ? static_cast<const float*>(b)[c]
-                                               : from16<DT>(static_cast<const uint16_t*>(b)[c]);
-        }
+        for (int q = 0; q < 16; ++q) first[q] = static_cast<const float*>(b)[column(q)];
+      } else if (b != nullptr) {
+        uint16_t e[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) e[q] = static_cast<const uint16_t*>(b)[column(q)];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) first[q] = from16<DT>(e[q]);
       }
     }
 #pragma unroll

@@ -436,28 +436,43 @@ Tensor pointwise_bf16(const Tensor& x, const Tensor& weight, const OptTensor& bi
 
 int float_code(const OptTensor& t) { return t ? dtype_code(*t) : 0; }
 
-// x as [B, P, C] with unit channel stride, copied where its strides do not allow that view
-Tensor image_rows(const Tensor& x, const char* what) {
-  TORCH_CHECK_VALUE(x.dim() >= 2, what, ": expected [B, ..., C], got shape ", x.sizes());
-  const int64_t b = x.size(0), c = x.size(-1);
-  int64_t p = 1;
-  for (int64_t i = 1; i < x.dim() - 1; ++i) p *= x.size(i);
-  Tensor t = x.reshape({b, p, c});
-  return t.stride(2) == 1 || c == 1 ? t : t.contiguous();
-}
+// x as [B, P, C] with unit channel stride: its own memory where its strides allow that view, else a copy's
+struct ImageRows {
+  Tensor hold;
+  int64_t b, p = 1, c, sb, sp;
+  ImageRows(const Tensor& x, const char* what) : hold(x) {
+    TORCH_CHECK_VALUE(x.dim() >= 2, what, ": expected [B, ..., C], got shape ", x.sizes());
+    b = x.size(0);
+    c = x.size(-1);
+    bool view = x.stride(-1) == 1 || c == 1;
+    sp = c;
+    for (int64_t i = x.dim() - 2; i > 0; --i) {
+      if (x.size(i) != 1) {
+        if (p == 1) sp = x.stride(i);
+        else view = view && x.stride(i) == sp * p;
+      }
+      p *= x.size(i);
+    }
+    sb = x.stride(0);
+    if (view) return;
+    hold = x.contiguous();
+    sp = c;
+    sb = c * p;
+  }
+};
 
 // x as [rows, C] with unit column stride
 Tensor matrix_rows(const Tensor& x, const char* what) {
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": expected [..., C], got a scalar");
   const int64_t c = x.size(-1);
+  if (x.dim() == 2 && (x.stride(1) == 1 || c == 1)) return x;
   int64_t m = 1;
   for (int64_t i = 0; i < x.dim() - 1; ++i) m *= x.size(i);
   Tensor t = x.reshape({m, c});
   return t.stride(1) == 1 || c == 1 ? t : t.contiguous();
 }
 
-Tensor dense(const Tensor& t) { return t.contiguous(); }
-OptTensor dense(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : t; }
+OptTensor dense(const OptTensor& t) { return t && !t->is_contiguous() ? OptTensor(t->contiguous()) : t; }
 
 void check_same(const Tensor& t, at::ScalarType dtype, const Tensor& like, const char* what) {
   TORCH_CHECK_TYPE(t.scalar_type() == dtype, what, ": expected ", dtype, ", got ", t.scalar_type());
@@ -470,25 +485,25 @@ void check_vector(const OptTensor& t, int64_t n, const Tensor& like, const char*
   TORCH_CHECK_VALUE(t->device() == like.device(), what, ": on ", t->device(), ", expected ", like.device());
 }
 
-Tensor norm_workspace(const Tensor& x3, int64_t groups, int backward) {
+Tensor norm_workspace(const ImageRows& v, int64_t groups, int backward) {
   int64_t floats = 0;
-  check(fim_group_norm_workspace(x3.size(0), x3.size(1), x3.size(2), groups, backward, &floats), "group_norm_act ",
-        x3.sizes(), " in ", groups, " groups");
-  return empty({floats}, x3, at::kFloat);
+  check(fim_group_norm_workspace(v.b, v.p, v.c, groups, backward, &floats), "group_norm_act ", v.hold.sizes(), " in ",
+        groups, " groups");
+  return empty({floats}, v.hold, at::kFloat);
 }
 
 std::tuple<Tensor, Tensor> group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias,
                                           double eps, int64_t act) {
   const c10::DeviceGuard guard(x.device());
-  const Tensor v = image_rows(x, "group_norm_act");
-  const int64_t b = v.size(0), p = v.size(1), c = v.size(2);
+  const ImageRows v(x, "group_norm_act");
+  const int64_t b = v.b, p = v.p, c = v.c;
   TORCH_CHECK_VALUE(groups > 0 && c > 0 && c % groups == 0, "group_norm_act: ", c, " channels in ", groups, " groups");
   check_vector(weight, c, x, "group_norm_act: weight");
   check_vector(bias, c, x, "group_norm_act: bias");
   const OptTensor w = dense(weight), bi = dense(bias);
   Tensor out = empty(x.sizes(), x, x.scalar_type()), stats = empty({b, groups, 2}, x, at::kFloat);
   const Tensor ws = norm_workspace(v, groups, 0);
-  check(fim_group_norm(v.data_ptr(), dtype_code(x), b, p, c, v.stride(0), v.stride(1), groups, ptr<const void>(w),
+  check(fim_group_norm(v.hold.data_ptr(), dtype_code(x), b, p, c, v.sb, v.sp, groups, ptr<const void>(w),
                        float_code(w), ptr<const void>(bi), float_code(bi), (float)eps, (int)act, out.data_ptr(),
                        ptr<float>(stats), ptr<float>(ws), stream_of(x)),
         "group_norm_act ", x.sizes(), " in ", groups, " groups");
@@ -502,8 +517,8 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_act_backward(const Tensor& d_out, 
   const c10::DeviceGuard guard(x.device());
   TORCH_CHECK_VALUE(d_out.sizes() == x.sizes(), "group_norm_act: gradient of shape ", d_out.sizes(), " for ", x.sizes());
   check_same(d_out, x.scalar_type(), x, "group_norm_act: gradient");
-  const Tensor v = image_rows(x, "group_norm_act"), d = image_rows(d_out, "group_norm_act");
-  const int64_t b = v.size(0), p = v.size(1), c = v.size(2);
+  const ImageRows v(x, "group_norm_act"), d(d_out, "group_norm_act");
+  const int64_t b = v.b, p = v.p, c = v.c;
   check_same(stats, at::kFloat, x, "group_norm_act: stats");
   TORCH_CHECK_VALUE(stats.is_contiguous() && stats.numel() == 2 * b * groups, "group_norm_act: stats of shape ",
                     stats.sizes());
@@ -519,8 +534,8 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_act_backward(const Tensor& d_out, 
     return {dx, dw, db};
   }
   const Tensor ws = norm_workspace(v, groups, 1);
-  check(fim_group_norm_backward(v.data_ptr(), d.data_ptr(), dtype_code(x), b, p, c, v.stride(0), v.stride(1), d.stride(0),
-                                d.stride(1), groups, ptr<const void>(w), float_code(w), ptr<const void>(bi),
+  check(fim_group_norm_backward(v.hold.data_ptr(), d.hold.data_ptr(), dtype_code(x), b, p, c, v.sb, v.sp, d.sb, d.sp,
+                                groups, ptr<const void>(w), float_code(w), ptr<const void>(bi),
                                 float_code(bi), (int)act, ptr<const float>(stats), dx.data_ptr(),
                                 weight ? dw.data_ptr() : nullptr, bias ? db.data_ptr() : nullptr, ptr<float>(ws),
                                 stream_of(x)),
@@ -564,7 +579,7 @@ Tensor gated_workspace(const Gated& g, int backward) {
   check(fim_gated_linear_workspace(g.x.data_ptr(), g.m, g.k, g.x.stride(0), g.wg.data_ptr(), g.wg.stride(0),
                                    g.wu.data_ptr(), g.wu.stride(0), g.h, backward, &bytes),
         "gated_linear ", g.m, "x", g.k, " -> ", g.h);
-  return empty({bytes}, g.x, at::kByte);
+  return bytes > 0 ? empty({bytes}, g.x, at::kByte) : Tensor();
 }
 
 std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
@@ -578,10 +593,11 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
   const c10::DeviceGuard guard(x.device());
   const Gated g(x, w_gate, w_up, b_gate, b_up);
   Tensor out = empty(with_last(x, g.h), x, x.scalar_type());
-  const Tensor ws = gated_workspace(g, 0);
+  const Tensor ws = gated_workspace(g, 0);  // undefined: none is needed
   check(fim_gated_linear(g.x.data_ptr(), dtype_code(x), g.m, g.k, g.x.stride(0), g.wg.data_ptr(), g.wg.stride(0),
                          g.wu.data_ptr(), g.wu.stride(0), g.h, ptr<const void>(g.bg), ptr<const void>(g.bu),
-                         g.bias_dtype, (int)act, out.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(x)),
+                         g.bias_dtype, (int)act, out.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
+                         ws.defined() ? ws.numel() : 0, stream_of(x)),
         "gated_linear ", g.m, "x", g.k, " -> ", g.h);
   return out;
 }
