@@ -9,6 +9,7 @@
 // forward pass: with K below about 1000 their two writes and reads cost more than the products), which writes dg and du in
 // x's type (they are operands of 16-bit matrix products next; FP32 sums for the bias gradients are taken before that
 // rounding); then one product for dx over both halves and one for the weights, split over rows where its tiles are few.
+#include "gated_few.h"
 #include "gated_rows.h"
 #include "gated_tile.h"
 
@@ -185,6 +186,7 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   // both weights are read with one stride
   const bool copy_w = !wg.as_is() || !wu.as_is() || wg.ld != wu.ld;
   g.x_at = 0;
+  if (!backward && g.M <= FEW_ROWS) return g;  // any rows are read in place
   g.wg_at = g.x_at + x.copy_bytes();
   g.wu_at = g.wg_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
   g.total = g.wu_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
@@ -275,6 +277,26 @@ static RowsArgs rows_args(const TileArgs& a, int64_t K) {
   return r;
 }
 
+template <int DT, int ACT, int V>
+static void launch_few(const FewArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(a.H, 16)), block(64 * FEW_WAVES);
+  if (a.M <= 16) gated_few_kernel<DT, ACT, 1, V><<<grid, block, 0, stream>>>(a);
+  else if (a.M <= 32) gated_few_kernel<DT, ACT, 2, V><<<grid, block, 0, stream>>>(a);
+  else gated_few_kernel<DT, ACT, 4, V><<<grid, block, 0, stream>>>(a);
+}
+
+// Elements per load that every row of the three operands allows: 8, 2 or 1
+static int few_vector(const Matrix& x, const Matrix& wg, const Matrix& wu) {
+  int v = 8;
+  for (const Matrix* m : {&x, &wg, &wu}) {
+    auto fits = [&](int w) {
+      return reinterpret_cast<uintptr_t>(m->p) % (2 * w) == 0 && m->ld % w == 0 && m->cols % w == 0;
+    };
+    while (v > 1 && !fits(v)) v = v == 8 ? 2 : 1;
+  }
+  return v;
+}
+
 static int gated_check(int dtype, int64_t M, int64_t K, int64_t H, int bias_dtype, int act) {
   if (M < 0 || K <= 0 || H <= 0 || act < 0 || act >= ACT_COUNT) return FIM_ERR_INVALID;
   if (dtype != FIM_BF16 && dtype != FIM_F16) return FIM_ERR_UNSUPPORTED;
@@ -334,6 +356,33 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || out == nullptr) return FIM_ERR_INVALID;
   Gated g = gated_plan(matrix(x, x_stride, M, K), matrix(w_gate, w_gate_stride, H, K), matrix(w_up, w_up_stride, H, K), false);
   if (g.total > 0 && (workspace == nullptr || workspace_bytes < g.total)) return FIM_ERR_INVALID;
+  if (M <= FEW_ROWS) {
+    FewArgs f{};
+    f.x = g.x.p;
+    f.w[0] = g.wg.p;
+    f.w[1] = g.wu.p;
+    f.ldx = g.x.ld;
+    f.ldw[0] = g.wg.ld;
+    f.ldw[1] = g.wu.ld;
+    f.M = (int)M;
+    f.K = (int)K;
+    f.H = (int)H;
+    f.bias[0] = b_gate;
+    f.bias[1] = b_up;
+    f.bias_dtype = bias_dtype;
+    f.out = static_cast<uint16_t*>(out);
+    f.wide_out = H % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
+    const int v = few_vector(g.x, g.wg, g.wu);
+    with_type(dtype, [&](auto dt) {
+      with_activation(act, [&](auto act_c) {
+        constexpr int DT = decltype(dt)::value, ACT = decltype(act_c)::value;
+        if (v == 8) launch_few<DT, ACT, 8>(f, stream);
+        else if (v == 2) launch_few<DT, ACT, 2>(f, stream);
+        else launch_few<DT, ACT, 1>(f, stream);
+      });
+    });
+    return launch_status();
+  }
   gated_operands(g, static_cast<uint8_t*>(workspace), stream);
   TileArgs a = gated_forward_args(g, b_gate, b_up, bias_dtype);
   a.out[0] = static_cast<uint16_t*>(out);
