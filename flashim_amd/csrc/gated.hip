@@ -28,45 +28,46 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(const uint16_t* from, i
   }
 }
 
-// out[i] = sum over s of part[s][i], in order. Few splits: four values a thread where n and the outputs' addresses allow
+// The sums of `splits` parts of n values, in order: the first n0 to out0, the others to out1 (either may be null). Few
+// splits: four values a thread where n, n0 and the outputs' addresses allow (wide)
 template <int DT>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* part, int64_t n, int splits, uint16_t* out0,
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* part, int64_t n, int64_t n0, int splits, uint16_t* out0,
                                                          uint16_t* out1, int wide) {
   if (wide) {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < 2 * n; i += (int64_t)gridDim.x * 1024) {
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
       v4f v = *reinterpret_cast<const v4f*>(part + i);
-      for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(part + s * 2 * n + i);
-      uint16_t* out = i < n ? out0 : out1;
+      for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const v4f*>(part + s * n + i);
+      uint16_t* out = i < n0 ? out0 : out1;
       if (out == nullptr) continue;
-      *reinterpret_cast<uint2*>(out + (i < n ? i : i - n)) = uint2{to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
+      *reinterpret_cast<uint2*>(out + (i < n0 ? i : i - n0)) = uint2{to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
     }
   } else {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
       float v = part[i];
-      for (int s = 1; s < splits; ++s) v += part[s * 2 * n + i];
-      uint16_t* out = i < n ? out0 : out1;
-      if (out != nullptr) out[i < n ? i : i - n] = to16<DT>(v);
+      for (int s = 1; s < splits; ++s) v += part[s * n + i];
+      uint16_t* out = i < n0 ? out0 : out1;
+      if (out != nullptr) out[i < n0 ? i : i - n0] = to16<DT>(v);
     }
   }
 }
 
 // Many splits: 64 values a workgroup, the splits dealt to its four wavefronts, whose sums are added in their order
 template <int DT>
-__global__ __launch_bounds__(256) void gated_join_many_kernel(const float* part, int64_t n, int splits, uint16_t* out0,
-                                                              uint16_t* out1) {
+__global__ __launch_bounds__(256) void gated_join_many_kernel(const float* part, int64_t n, int64_t n0, int splits,
+                                                              uint16_t* out0, uint16_t* out1) {
   __shared__ float sums[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i = (int64_t)blockIdx.x * 64 + lane;
   float v = 0.0f;
-  if (i < 2 * n) {
+  if (i < n) {
 #pragma unroll 8
-    for (int s = wave; s < splits; s += 4) v += part[s * 2 * n + i];
+    for (int s = wave; s < splits; s += 4) v += part[s * n + i];
   }
   sums[wave][lane] = v;
   __syncthreads();
-  if (wave != 0 || i >= 2 * n) return;
-  uint16_t* out = i < n ? out0 : out1;
-  if (out != nullptr) out[i < n ? i : i - n] = to16<DT>(sums[0][lane] + sums[1][lane] + (sums[2][lane] + sums[3][lane]));
+  if (wave != 0 || i >= n) return;
+  uint16_t* out = i < n0 ? out0 : out1;
+  if (out != nullptr) out[i < n0 ? i : i - n0] = to16<DT>(sums[0][lane] + sums[1][lane] + (sums[2][lane] + sums[3][lane]));
 }
 
 // db[i][c] = sum over tiles of col_sums[tile][i][c]: 16 values a workgroup, the tiles dealt to 64 rows of threads
@@ -133,21 +134,26 @@ static Tile gated_tile(int64_t rows, int64_t cols, int64_t k) {
   return tile_time(large, rows, cols, 1, k) < tile_time(small, rows, cols, 1, k) ? large : small;
 }
 
-// The weights' gradients: tile, and splits of the rows (their FP32 partials are written once and read once, at 4.5 TB/s)
-static void weights_plan(int64_t M, int64_t K, int64_t H, Tile& tile, int64_t& splits) {
-  double best = 0.0;
-  splits = 0;
+struct Splits {
+  Tile tile;
+  int64_t n;
+};
+
+// Tile and splits of the contraction of `cols` x `rows` outputs over k, where splits are joined (their FP32 partials written
+// and read once, at 4.5 TB/s, and a launch); `alone`: one split needs no join
+static Splits split_plan(int64_t rows, int64_t cols, int64_t k, bool alone) {
+  Splits best{{2, 2}, 0};
+  double best_time = 0.0;
   for (const Tile t : {Tile{4, 4}, Tile{2, 2}}) {
-    for (int64_t s = 1; s <= 256 && (s == 1 || M / s >= 256); s += s < 8 ? 1 : s / 4) {
-      const int64_t size = 64 * t.mb, cols = 2 * cdiv(H, size) * size;
-      const double join = (double)(s + 1) * 2.0 * H * K * 4.0 / 4.5e6;  // us
-      const double time = 0.9 * tile_time(t, K, cols, s, cdiv(M, s)) + join;
-      if (splits != 0 && time >= best) continue;
-      best = time;
-      tile = t;
-      splits = s;
+    for (int64_t s = 1; s <= 256 && (s == 1 || k / s >= 256); s += s < 8 ? 1 : s / 4) {
+      const double join = s == 1 && alone ? 0.0 : (double)(s + 1) * rows * cols * 4.0 / 4.5e6 + 3.0;  // us
+      const double time = 0.9 * tile_time(t, rows, cols, s, cdiv(k, s)) + join;
+      if (best.n != 0 && time >= best_time) continue;
+      best_time = time;
+      best = {t, s};
     }
   }
+  return best;
 }
 
 // Whether a launch is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half the
@@ -170,8 +176,9 @@ struct Gated {
   int64_t M, K, H;
   // workspace, in bytes: copies of the operands; backward: dg and du [M, hp], bias partials, weight partials
   int64_t x_at, wg_at, wu_at, dgu_at, cols_at, part_at, total;
-  int64_t hp, ldg, splits, k_split, sum_rows;
-  Tile grad, dw;
+  int64_t hp, ldg, sum_rows;
+  int64_t dw_splits, dw_rows, dx_splits, dx_steps;  // splits, and what each contracts over
+  Tile grad, dw, dx;
   bool rows;  // backward: dg, du and dx by rows
 };
 
@@ -199,10 +206,20 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.rows = gated_rows(g.M, g.K, g.H, true);
   g.sum_rows = g.rows ? rows_groups(g.M, g.K, g.H) * ROWS_WAVES : 2 * cdiv(g.M, 64 * g.grad.mb);
   g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
-  weights_plan(g.M, g.K, g.H, g.dw, g.splits);
-  g.k_split = cdiv(cdiv(g.M, g.splits), TILE_K) * TILE_K;
-  g.splits = cdiv(g.M, g.k_split);
-  g.total = g.part_at + align256(g.splits * 2 * g.H * g.K * 4);
+  // (the weights' gradients have both halves' tiles)
+  const Splits dw = split_plan(g.K, 2 * cdiv(g.H, 128) * 128, g.M, false);
+  g.dw = dw.tile;
+  g.dw_rows = cdiv(cdiv(g.M, dw.n), TILE_K) * TILE_K;
+  g.dw_splits = cdiv(g.M, g.dw_rows);
+  const int64_t steps = 2 * cdiv(g.H, TILE_K);
+  const Splits dx = split_plan(g.M, g.K, steps * TILE_K, true);
+  g.dx = dx.tile;
+  g.dx_steps = cdiv(steps, dx.n);
+  g.dx_splits = cdiv(steps, g.dx_steps);
+  // one area for both products' partials, one after the other
+  const int64_t dw_bytes = g.dw_splits * 2 * g.H * g.K * 4;
+  const int64_t dx_bytes = g.rows || g.dx_splits == 1 ? 0 : g.dx_splits * g.M * g.K * 4;
+  g.total = g.part_at + align256(dw_bytes > dx_bytes ? dw_bytes : dx_bytes);
   return g;
 }
 
@@ -243,6 +260,21 @@ static void launch_product(const TileArgs& a, Tile t, int64_t splits, hipStream_
     if (t.mb == 4) return launch_tile<DT, MODE, ACT, 4, 4>(a, splits, stream);
   }
   launch_tile<DT, MODE, ACT, 2, 2>(a, splits, stream);
+}
+
+template <int DT>
+static void launch_join(const float* part, int64_t n, int64_t n0, int64_t splits, void* out0, void* out1,
+                        hipStream_t stream) {
+  uint16_t *o0 = static_cast<uint16_t*>(out0), *o1 = static_cast<uint16_t*>(out1);
+  if (splits <= 4) {
+    const int wide = n % 4 == 0 && n0 % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(o0) | reinterpret_cast<uintptr_t>(o1)) % 8 == 0;
+    const int64_t blocks = cdiv(n, wide ? 1024 : 256);
+    gated_join_kernel<DT><<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream>>>(part, n, n0, (int)splits,
+                                                                                                    o0, o1, wide);
+  } else {
+    gated_join_many_kernel<DT><<<dim3((unsigned)cdiv(n, 64)), dim3(256), 0, stream>>>(part, n, n0, (int)splits, o0, o1);
+  }
 }
 
 template <int DT, int MODE, int ACT, int KP>
@@ -461,7 +493,10 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       d.out[0] = static_cast<uint16_t*>(dx);
       d.ldo = d.out_cols = K;
       d.wide_out = rows_wide(dx, K);
-      launch_product<DT, GATED_DX, ACT_NONE>(d, gated_tile(M, K, 2 * H), 1, stream);
+      d.k_split = g.dx_steps;
+      d.part = g.dx_splits > 1 ? reinterpret_cast<float*>(ws + g.part_at) : nullptr;
+      launch_product<DT, GATED_DX, ACT_NONE>(d, g.dx, g.dx_splits, stream);
+      if (g.dx_splits > 1) launch_join<DT>(d.part, M * K, M * K, g.dx_splits, dx, nullptr, stream);
     }
     if (dw_gate != nullptr || dw_up != nullptr) {
       TileArgs w{};
@@ -476,18 +511,9 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       w.xw = g.x.padded();
       w.ww = g.hp;
       w.part = reinterpret_cast<float*>(ws + g.part_at);
-      w.k_split = g.k_split;
-      launch_product<DT, GATED_DW, ACT_NONE>(w, g.dw, g.splits, stream);
-      uint16_t *g16 = static_cast<uint16_t*>(dw_gate), *u16 = static_cast<uint16_t*>(dw_up);
-      if (g.splits <= 4) {
-        const int wide = H * K % 4 == 0 && (reinterpret_cast<uintptr_t>(g16) | reinterpret_cast<uintptr_t>(u16)) % 8 == 0;
-        const int64_t blocks = cdiv(2 * H * K, wide ? 1024 : 256);
-        gated_join_kernel<DT><<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream>>>(
-            w.part, H * K, (int)g.splits, g16, u16, wide);
-      } else {
-        gated_join_many_kernel<DT><<<dim3((unsigned)cdiv(2 * H * K, 64)), dim3(256), 0, stream>>>(w.part, H * K,
-                                                                                                  (int)g.splits, g16, u16);
-      }
+      w.k_split = g.dw_rows;
+      launch_product<DT, GATED_DW, ACT_NONE>(w, g.dw, g.dw_splits, stream);
+      launch_join<DT>(w.part, 2 * H * K, H * K, g.dw_splits, dw_gate, dw_up, stream);
     }
   });
   return launch_status();

@@ -66,9 +66,9 @@ struct TileArgs {
   int64_t ldo, out_cols;  // columns written: N, or more (GRAD: with zeros)
   int wide_out, wide_dout;  // rows of out and dout are 16-byte aligned
   float* col_sums;        // GRAD: [2 m tiles][2][N] sums of dg and du over 32 MB rows, or null
-  float* part;            // DW: [splits][2][N][M]
+  float* part;            // DW: [splits][2][N][M]; DX: [splits][M][N], or null
   int mt, nt, group;      // tiles; m tiles of a group that share the columns' operands in L2
-  int64_t k_split;        // DW: contraction of one split (a multiple of 64)
+  int64_t k_split;        // contraction of one split: DW rows (a multiple of 64), DX steps over both halves
 };
 
 constexpr int TILE_K = 64;
@@ -111,9 +111,12 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   const int tiles = a.mt * a.nt;
   const int per_xcd = (int)(gridDim.x >> 3);
   int t = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  const int splits = MODE == GATED_DW ? (int)((a.K + a.k_split - 1) / a.k_split) : 1;
+  const int half_steps = (int)((a.K + TILE_K - 1) / TILE_K);
+  const int splits = MODE == GATED_DW   ? (int)((a.K + a.k_split - 1) / a.k_split)
+                     : MODE == GATED_DX ? (int)((2 * half_steps + a.k_split - 1) / a.k_split)
+                                        : 1;
   if (t >= tiles * splits) return;
-  const int split = MODE == GATED_DW ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
+  const int split = WT ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
   t -= split * tiles;
   const int grp = t / (a.group * a.nt), in_grp = t - grp * a.group * a.nt;
   const int gm = a.mt - grp * a.group < a.group ? a.mt - grp * a.group : a.group;
@@ -124,10 +127,12 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   const int64_t m0 = (int64_t)tm * BM;
   const int64_t n0 = PAIR ? (int64_t)tn * (BN / 2) : MODE == GATED_DW ? (int64_t)(tn >> 1) * BN : (int64_t)tn * BN;
 
-  const int64_t kb = split * a.k_split;
+  const int64_t kb = MODE == GATED_DW ? split * a.k_split : 0;
   const int64_t klen = MODE == GATED_DW ? (a.K - kb < a.k_split ? a.K - kb : a.k_split) : a.K;
-  const int steps1 = (int)((klen + TILE_K - 1) / TILE_K);
-  const int steps = MODE == GATED_DX ? 2 * steps1 : steps1;
+  // steps [first, last): of both halves for dx
+  const int first = MODE == GATED_DX ? (int)(split * a.k_split) : 0;
+  int last = MODE == GATED_DX ? 2 * half_steps : (int)((klen + TILE_K - 1) / TILE_K);
+  if (MODE == GATED_DX && first + a.k_split < last) last = (int)(first + a.k_split);
 
   // -- loads into LDS: chunk c (1 KB) of an operand's part of a stage; wavefront w loads chunks w, w + 4, ... of each
   // along: chunk c is rows 8 c .. 8 c + 7, lane l row l / 8, LDS slot l % 8, which holds K segment slot ^ (row / 2 % 8)
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   auto rest = [](int64_t rows, int64_t ld, int64_t cols) __attribute__((always_inline)) {
     return rows <= 0 ? 0 : ((rows - 1) * ld + cols) * 2;
   };
-  int step_at = 0;  // the step whose loads are issued next
+  int step_at = first;  // the step whose loads are issued next
   auto load = [](const uint16_t* p, int records, uint8_t* to, uint32_t off) __attribute__((always_inline)) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), (short)0, __builtin_amdgcn_readfirstlane(records),
@@ -168,35 +173,37 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   const int xrec = XT ? 0 : (int)rest(xrows < BM ? xrows : BM, a.ldx, kw);
   const int wrec = WT ? 0 : (int)rest(wrows < BN ? wrows : BN, a.ldw, kw);
   // per step: the lane's K offset of an operand along the contraction; first row and bytes left of one across it
-  uint32_t kbyte, kdead;
-  const uint16_t *xp = XT ? a.x[0] + kb * a.ldx + m0 : a.x[0] + m0 * a.ldx;
-  const uint16_t *wp = MODE == GATED_DX ? a.w[0] + n0 : a.w[half] + kb * a.ldw + n0;
-  int64_t xleft = rest(klen, a.ldx, a.xw - m0), wleft = rest(klen, a.ldw, a.ww - n0);
+  const bool second = MODE == GATED_DX && first >= half_steps;
+  const int64_t skip = MODE == GATED_DX ? (int64_t)(first - (second ? half_steps : 0)) * TILE_K : 0;
+  uint32_t kbyte = (uint32_t)skip * 2u, kdead;
+  const uint16_t *xp = XT ? a.x[0] + kb * a.ldx + m0 : a.x[second] + m0 * a.ldx;
+  const uint16_t *wp = a.w[MODE == GATED_DX ? second : half] + (kb + skip) * a.ldw + n0;
+  int64_t xleft = rest(klen, a.ldx, a.xw - m0), wleft = rest(klen - skip, a.ldw, a.ww - n0);
   auto bytes = [](int64_t left) __attribute__((always_inline)) {
     return (int)(left <= 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left);
   };
   int xbytes = XT ? bytes(xleft) : xrec, wbytes = bytes(wleft);
   auto next_step = [&]() __attribute__((always_inline)) {
     ++step_at;
-    if constexpr (MODE == GATED_DX) {
-      const bool second = step_at == steps1;  // on to the other half
-      kbyte = second ? 0u : kbyte + 2 * TILE_K;
-      xp = second ? a.x[1] + m0 * a.ldx : xp;
-      wp = second ? a.w[1] + n0 : wp + TILE_K * a.ldw;
-      wleft = second ? rest(klen, a.ldw, a.ww - n0) : wleft - TILE_K * a.ldw * 2;
-    } else {
-      kbyte += 2 * TILE_K;
-      xp += XT ? TILE_K * a.ldx : 0;
-      xleft -= TILE_K * a.ldx * 2;
-      wp += TILE_K * a.ldw;
-      wleft -= TILE_K * a.ldw * 2;
+    kbyte += 2 * TILE_K;
+    wp += TILE_K * a.ldw;
+    wleft -= TILE_K * a.ldw * 2;
+    if (MODE == GATED_DX && step_at == half_steps) {  // on to the other half
+      kbyte = 0u;
+      xp = a.x[1] + m0 * a.ldx;
+      wp = a.w[1] + n0;
+      wleft = rest(klen, a.ldw, a.ww - n0);
     }
-    if constexpr (XT) xbytes = bytes(xleft);
-    if constexpr (WT) wbytes = bytes(wleft);
-    kdead = step_at < steps && kbyte + seg * 16 < (uint32_t)a.K * 2u ? 0u : TILE_OOB;
+    if constexpr (XT) {
+      xp += TILE_K * a.ldx;
+      xleft -= TILE_K * a.ldx * 2;
+      xbytes = bytes(xleft);
+    }
+    // (past the last step nothing is read: zeros of one operand would meet infinities of the other)
+    if constexpr (WT) wbytes = step_at < last ? bytes(wleft) : 0;
+    kdead = step_at < last && kbyte + seg * 16 < (uint32_t)a.K * 2u ? 0u : TILE_OOB;
   };
-  kbyte = 0;
-  kdead = steps > 0 && seg * 8 < a.K ? 0u : TILE_OOB;
+  kdead = first < last && kbyte + seg * 16 < (uint32_t)a.K * 2u ? 0u : TILE_OOB;
   // load i of the step: x's, then w's
   auto issue = [&](uint8_t* st, int i) __attribute__((always_inline)) {
     if (i < CX) {
@@ -313,7 +320,7 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(st0, 0, 0, r);
   // pairs of steps: one exit; a step past the last multiplies zeros
-  for (int k = 0; k < steps; k += 2) {
+  for (int k = first; k < last; k += 2) {
     step(st0, st1);
     step(st1, st0);
   }
@@ -336,7 +343,25 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
           if (n < a.N && m < a.M) to[n * a.M + m] = acc[i][j][q];
         }
       }
-  } else {
+    return;
+  }
+  if (MODE == GATED_DX && a.part != nullptr) {
+    float* to = a.part + (int64_t)split * a.M * a.N;
+    const int64_t nw = n0 + wn * NB * 32 + 4 * h;
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const int64_t m = mw + 32 * j + frow;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int64_t n = nw + 32 * i + 8 * (q >> 2) + (q & 3);
+          if (n < a.N && m < a.M) to[m * a.N + n] = acc[i][j][q];
+        }
+    }
+    return;
+  }
+  if constexpr (MODE != GATED_DW) {
     // 32 rows at a time through LDS (this wavefront's own part of the consumed stage): whole runs of the output's rows, by
     // buffer stores whose rows and columns past the end go out of range, without branches
     constexpr int NO = PAIR ? NB / 2 : NB, OC = 32 * NO, RB = OC * 2, SLOTS = RB / 16, PER = 64 / SLOTS;
