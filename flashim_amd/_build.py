@@ -63,8 +63,8 @@ def build_torch_ops() -> Path:
                 for flag in ("-isystem", path)]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes, str(CSRC / "torch_ops.cpp"),
-          "-o", str(temporary), f"-L{PACKAGE}", "-lflashim_amd", f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-lc10_hip",
-          "-Wl,-rpath,$ORIGIN"])
+          "-o", str(temporary), f"-L{PACKAGE}", "-lflashim_amd", f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-ltorch_python",
+          "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
     temporary.replace(TORCH_LIBRARY)
     return TORCH_LIBRARY
 

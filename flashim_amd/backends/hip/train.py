@@ -55,9 +55,7 @@ def clip_grad_norm_(grads: Sequence[Tensor], max_norm: float, *, norm_type: floa
     with torch.no_grad():
         if error_if_nonfinite and not math.isfinite(library.grad_norm(grads, float(norm_type)).item()):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm of type {norm_type} is not finite")
-        if out is None:
-            return library.clip_grad_norm_(grads, float(max_norm), float(norm_type))
-        return library.clip_grad_norm_out(grads, out, float(max_norm), float(norm_type))
+        return library.clip_lists(grads, out, float(max_norm), float(norm_type))
 
 
 # -- eligibility -------------------------------------------------------------------------------------------------------

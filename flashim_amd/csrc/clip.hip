@@ -49,13 +49,14 @@ __device__ __forceinline__ int entry_of(const Table& t, uint32_t wg) {
   return n - 1;
 }
 
-template <int DT>
-struct Vec16 {
-  static constexpr int N = DT == FIM_F32 ? 4 : 8;
-  static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[N]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// A load of 16 bytes, or of the 8 bytes that become 16 as FP32
+template <int DT, bool HALF = false>
+struct Vec {
+  static constexpr int WORDS = HALF ? 2 : 4, N = DT == FIM_F32 ? WORDS : 2 * WORDS;
+  typedef uint32_t T __attribute__((ext_vector_type(WORDS)));
+  static __device__ __forceinline__ void unpack(const T& w, float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < WORDS; ++i) {
       if constexpr (DT == FIM_F32) {
         f[i] = u2f(w[i]);
       } else if constexpr (DT == FIM_BF16) {
@@ -101,7 +102,8 @@ __device__ __forceinline__ double join_workgroup(double v) {
 
 template <int DT, typename R>
 __global__ __launch_bounds__(CLIP_T) void grad_norm_kernel(const NormTable t, double* __restrict__ part) {
-  constexpr int ES = DT == FIM_F32 ? 4 : 2, N = Vec16<DT>::N, U = 4;
+  constexpr int ES = DT == FIM_F32 ? 4 : 2, N = Vec<DT>::N, U = 4;
+  typedef typename Vec<DT>::T V;
   const int e = entry_of(t, blockIdx.x);
   const uint32_t begin = (blockIdx.x - t.first[e]) * t.chunk;
   const uint32_t n = t.n[e] - begin < t.chunk ? t.n[e] - begin : t.chunk;
@@ -110,26 +112,26 @@ __global__ __launch_bounds__(CLIP_T) void grad_norm_kernel(const NormTable t, do
   uint32_t head = (uint32_t)(-(intptr_t)p & 15) / ES;
   if (head > n) head = n;
   const uint32_t vecs = (n - head) / N;
-  const uint4* v = reinterpret_cast<const uint4*>(p + head * ES);
+  const V* v = reinterpret_cast<const V*>(p + head * ES);
   double acc[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) acc[u] = R::zero();
   uint32_t i = threadIdx.x;
   for (; i + (U - 1) * CLIP_T < vecs; i += U * CLIP_T) {
-    uint4 r[U];
+    V r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) r[u] = v[i + u * CLIP_T];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float f[N];
-      Vec16<DT>::unpack(r[u], f);
+      Vec<DT>::unpack(r[u], f);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[u] = R::add(acc[u], f[k]);
     }
   }
   for (; i < vecs; i += CLIP_T) {
     float f[N];
-    Vec16<DT>::unpack(v[i], f);
+    Vec<DT>::unpack(v[i], f);
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[0] = R::add(acc[0], f[k]);
   }
@@ -163,7 +165,10 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float v, int dt) 
 template <int DT, int DO, typename R>
 __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, const double* __restrict__ part, int parts,
                                                             float* total, float max_norm, int writes_total) {
-  constexpr int ES = DT == FIM_F32 ? 4 : 2, N = Vec16<DT>::N, EO = DO == FIM_F32 ? 4 : 2, U = 4;
+  constexpr bool HALF = DT != FIM_F32 && DO == FIM_F32;
+  typedef Vec<DT, HALF> In;
+  typedef typename In::T V;
+  constexpr int ES = DT == FIM_F32 ? 4 : 2, N = In::N, EO = DO == FIM_F32 ? 4 : 2, U = HALF ? 8 : 4;
   const float sum = parts > 0 ? total_of<R>(part, parts) : *total;
   if (parts > 0 && writes_total && blockIdx.x == 0 && threadIdx.x == 0) *total = sum;
   const float quotient = max_norm / (sum + 1e-6f);
@@ -174,15 +179,15 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
   const uint32_t n = t.n[e] - begin < t.chunk ? t.n[e] - begin : t.chunk;
   const uint8_t* p = static_cast<const uint8_t*>(t.in[e]) + (int64_t)begin * ES;
   uint8_t* q = static_cast<uint8_t*>(t.out[e]) + (int64_t)begin * EO;
-  uint32_t head = (uint32_t)(-(intptr_t)p & 15) / ES;
+  uint32_t head = (uint32_t)(-(intptr_t)p & (sizeof(V) - 1)) / ES;
   if (head > n) head = n;
   uint32_t vecs = (n - head) / N;
-  constexpr int WB = N * EO < 16 ? N * EO : 16;  // bytes of a store
+  constexpr int WB = N * EO;  // bytes of a store: 16, or 8 of FP32 into 16 bits
   if ((reinterpret_cast<uintptr_t>(q) + head * EO) % WB) head = vecs = 0;  // unlike alignments: element by element
-  const uint4* v = reinterpret_cast<const uint4*>(p + head * ES);
-  auto put = [&](uint32_t at, const uint4& r) __attribute__((always_inline)) {
+  const V* v = reinterpret_cast<const V*>(p + head * ES);
+  auto put = [&](uint32_t at, const V& r) __attribute__((always_inline)) {
     float f[N];
-    Vec16<DT>::unpack(r, f);
+    In::unpack(r, f);
 #pragma unroll
     for (int k = 0; k < N; ++k) f[k] *= scale;
     uint32_t w[N * EO / 4];
@@ -197,17 +202,12 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
                                     (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * k + 1]) << 16;
     }
     uint8_t* to = q + (int64_t)(head + at * N) * EO;
-    if constexpr (N * EO == 8) {
-      *reinterpret_cast<uint2*>(to) = uint2{w[0], w[1]};
-    } else {
-#pragma unroll
-      for (int k = 0; k < N * EO / 16; ++k)
-        reinterpret_cast<uint4*>(to)[k] = uint4{w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]};
-    }
+    if constexpr (N * EO == 8) *reinterpret_cast<uint2*>(to) = uint2{w[0], w[1]};
+    else *reinterpret_cast<uint4*>(to) = uint4{w[0], w[1], w[2], w[3]};
   };
   uint32_t i = threadIdx.x;
   for (; i + (U - 1) * CLIP_T < vecs; i += U * CLIP_T) {
-    uint4 r[U];
+    V r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) r[u] = v[i + u * CLIP_T];
 #pragma unroll

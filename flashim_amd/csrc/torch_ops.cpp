@@ -8,10 +8,12 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <array>
@@ -964,4 +966,34 @@ TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
 TORCH_LIBRARY_IMPL(flashim_amd, ADInplaceOrView, m) {
   for (const char* name : {"int8_linear_quantize_", "clip_grad_norm_", "clip_grad_norm_out"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&count_writes>());
+}
+
+// clip_grad_norm_ (out None) and clip_grad_norm_out of Python lists or tuples, through the same dispatcher: torch's binding
+// of operators converts a list of tensors three times over, 0.12 us a tensor, which for hundreds of gradients is more than
+// the kernels take. None where an element is not a plain tensor (a subclass has its own say in operators): the caller then
+// goes through torch.ops. Called with the GIL held.
+extern "C" PyObject* flashim_amd_clip_lists(PyObject* grads, PyObject* out, double max_norm, double norm_type) {
+  HANDLE_TH_ERRORS
+  const auto unpack = [](PyObject* list, std::vector<Tensor>& to) {
+    if (!PyList_Check(list) && !PyTuple_Check(list)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+    to.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* item = PySequence_Fast_GET_ITEM(list, i);
+      if (!THPVariable_CheckExact(item)) return false;
+      to.push_back(THPVariable_Unpack(item));
+    }
+    return true;
+  };
+  std::vector<Tensor> from, to;
+  if (!unpack(grads, from) || (out != Py_None && !unpack(out, to))) Py_RETURN_NONE;
+  static const auto in_place = typed_op<decltype(clip_grad_norm_)>("flashim_amd::clip_grad_norm_");
+  static const auto into = typed_op<decltype(clip_grad_norm_out)>("flashim_amd::clip_grad_norm_out");
+  Tensor total;
+  {
+    pybind11::gil_scoped_release release;
+    total = out == Py_None ? in_place.call(from, max_norm, norm_type) : into.call(from, to, max_norm, norm_type);
+  }
+  return THPVariable_Wrap(total);
+  END_HANDLE_TH_ERRORS
 }
