@@ -11,6 +11,7 @@
 // rounding); then one product for dx over both halves and one for the weights, split over rows where its tiles are few.
 #include "gated_few.h"
 #include "gated_rows.h"
+#include "gated_rows_grad.h"
 #include "gated_tile.h"
 
 namespace fim {
@@ -160,7 +161,7 @@ static Splits split_plan(int64_t rows, int64_t cols, int64_t k, bool alone) {
 // CUs. Backward also needs all weights in one workgroup's LDS.
 static bool gated_rows(int64_t M, int64_t K, int64_t H, bool backward) {
   if (K > 128 || M < 32 * ROWS_WAVES * (int64_t)device_cus() / 2) return false;
-  return !backward || (K <= 64 && H <= rows_hidden(64));
+  return !backward || (K <= 64 && H <= GRAD_HIDDEN);
 }
 
 static int64_t rows_blocks(int64_t K, int64_t H) { return cdiv(H, rows_hidden(K <= 64 ? 64 : 128)); }
@@ -171,6 +172,12 @@ static int64_t rows_groups(int64_t M, int64_t K, int64_t H) {
   return n < 1 ? 1 : n < most ? n : most;
 }
 
+// The same of a backward pass by rows
+static int64_t rows_grad_groups(int64_t M, int64_t H) {
+  const int64_t most = cdiv(M, 32 * rows_grad_sub(H));
+  return device_cus() < most ? device_cus() : most;
+}
+
 struct Gated {
   Matrix x, wg, wu;
   int64_t M, K, H;
@@ -179,7 +186,7 @@ struct Gated {
   int64_t hp, ldg, sum_rows;
   int64_t dw_splits, dw_rows, dx_splits, dx_steps;  // splits, and what each contracts over
   Tile grad, dw, dx;
-  bool rows;  // backward: dg, du and dx by rows
+  bool rows;  // backward by rows: no dg, du in memory
 };
 
 static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, bool backward) {
@@ -200,11 +207,18 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.hp = cdiv(g.H, 8) * 8;
   g.ldg = cdiv(g.H, 64) * 64 + 64;
   if (!backward) return g;
-  g.grad = {2, 2};  // (its epilogue has no registers left beside 256 x 256 accumulators)
   g.dgu_at = g.total;
-  g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
   g.rows = gated_rows(g.M, g.K, g.H, true);
-  g.sum_rows = g.rows ? rows_groups(g.M, g.K, g.H) * ROWS_WAVES : 2 * cdiv(g.M, 64 * g.grad.mb);
+  if (g.rows) {
+    g.sum_rows = g.dw_splits = rows_grad_groups(g.M, g.H) * rows_grad_sub(g.H);
+    g.cols_at = g.dgu_at;
+    g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
+    g.total = g.part_at + align256(g.dw_splits * 2 * g.H * g.K * 4);
+    return g;
+  }
+  g.grad = {2, 2};  // (its epilogue has no registers left beside 256 x 256 accumulators)
+  g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
+  g.sum_rows = 2 * cdiv(g.M, 64 * g.grad.mb);
   g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
   // (the weights' gradients have both halves' tiles)
   const Splits dw = split_plan(g.K, 2 * cdiv(g.H, 128) * 128, g.M, false);
@@ -218,7 +232,7 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.dx_splits = cdiv(steps, g.dx_steps);
   // one area for both products' partials, one after the other
   const int64_t dw_bytes = g.dw_splits * 2 * g.H * g.K * 4;
-  const int64_t dx_bytes = g.rows || g.dx_splits == 1 ? 0 : g.dx_splits * g.M * g.K * 4;
+  const int64_t dx_bytes = g.dx_splits == 1 ? 0 : g.dx_splits * g.M * g.K * 4;
   g.total = g.part_at + align256(dw_bytes > dx_bytes ? dw_bytes : dx_bytes);
   return g;
 }
@@ -277,11 +291,18 @@ static void launch_join(const float* part, int64_t n, int64_t n0, int64_t splits
   }
 }
 
-template <int DT, int MODE, int ACT, int KP>
+template <int DT, int ACT, int KP>
 static void launch_rows(const RowsArgs& a, bool wide, hipStream_t stream) {
   const dim3 grid((unsigned)(rows_groups(a.M, a.K, a.H) * a.blocks));
-  if (wide) gated_rows_kernel<DT, MODE, ACT, KP, true><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
-  else gated_rows_kernel<DT, MODE, ACT, KP, false><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+  if (wide) gated_rows_kernel<DT, ACT, KP, true><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+  else gated_rows_kernel<DT, ACT, KP, false><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+}
+
+template <int DT, int ACT>
+static void launch_rows_grad(const RowsArgs& a, bool wide, hipStream_t stream) {
+  const dim3 grid((unsigned)rows_grad_groups(a.M, a.H));
+  if (wide) gated_rows_grad_kernel<DT, ACT, true><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
+  else gated_rows_grad_kernel<DT, ACT, false><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
 }
 
 // The same launch by rows, from the tiles' arguments
@@ -297,15 +318,14 @@ static RowsArgs rows_args(const TileArgs& a, int64_t K) {
   for (int i = 0; i < 2; ++i) {
     r.w[i] = a.w[i];
     r.bias[i] = a.bias[i];
-    r.out[i] = a.out[i];
   }
   r.bias_dtype = a.bias_dtype;
   r.dout = a.dout;
   r.ldd = a.ldd;
-  r.ldo = a.ldo;
-  r.out_cols = (int)a.out_cols;
+  r.out = a.out[0];
   r.col_sums = a.col_sums;
   r.blocks = (int)rows_blocks(K, a.N);
+  r.sub = rows_grad_sub(a.N);
   return r;
 }
 
@@ -426,8 +446,8 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
     with_activation(act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
       if (!gated_rows(M, K, H, false)) launch_product<DT, GATED_FORWARD, ACT>(a, tile, 1, stream);
-      else if (K <= 64) launch_rows<DT, GATED_FORWARD, ACT, 64>(rows_args(a, K), a.wide_out, stream);
-      else launch_rows<DT, GATED_FORWARD, ACT, 128>(rows_args(a, K), a.wide_out, stream);
+      else if (K <= 64) launch_rows<DT, ACT, 64>(rows_args(a, K), a.wide_out, stream);
+      else launch_rows<DT, ACT, 128>(rows_args(a, K), a.wide_out, stream);
     });
   });
   return launch_status();
@@ -469,8 +489,9 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       if (g.rows) {
         RowsArgs r = rows_args(a, K);
         r.dx = static_cast<uint16_t*>(dx);
-        r.wide_dx = rows_wide(dx, K);
-        launch_rows<DT, GATED_GRAD, ACT, 64>(r, a.wide_dout, stream);
+        r.wide_dx = K % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 8 == 0;
+        if (dw_gate != nullptr || dw_up != nullptr) r.dw_part = reinterpret_cast<float*>(ws + g.part_at);
+        launch_rows_grad<DT, ACT>(r, a.wide_dout, stream);
       } else {
         launch_product<DT, GATED_GRAD, ACT>(a, g.grad, 1, stream);
       }
@@ -512,7 +533,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
       w.ww = g.hp;
       w.part = reinterpret_cast<float*>(ws + g.part_at);
       w.k_split = g.dw_rows;
-      launch_product<DT, GATED_DW, ACT_NONE>(w, g.dw, g.dw_splits, stream);
+      if (!g.rows) launch_product<DT, GATED_DW, ACT_NONE>(w, g.dw, g.dw_splits, stream);
       launch_join<DT>(w.part, 2 * H * K, H * K, g.dw_splits, dw_gate, dw_up, stream);
     }
   });

@@ -5,10 +5,6 @@
 // eight wavefronts works alone on 32 rows at a time: it loads them straight into MFMA operand registers, the next 32 while it
 // works, multiplies them by 32 hidden columns at a time, and writes whole 128-byte lines through its own LDS area. No barrier
 // after the weights are in; the wavefronts of a SIMD drift apart, one's vector work covers another's loads.
-//
-// GRAD computes dx as well, without a trip through memory: an accumulator register block of dg (lane: row, registers: 4 h + 8
-// q + e) is, packed to 16 bits, the MFMA operand of a product that contracts over those columns in the order (h, q, e); the
-// weights' operand is read from LDS, transposed, in the same order.
 #pragma once
 
 #include "gated_tile.h"
@@ -22,15 +18,16 @@ struct RowsArgs {
   int K, kw, H;           // kw: K rounded up to 8
   const void* bias[2];
   int bias_dtype;
+  uint16_t* out;          // [M, H] packed
+  int blocks;             // hidden blocks; workgroup i takes block i % blocks
+  // backward (gated_rows_grad.h)
   const uint16_t* dout;
   int64_t ldd;
-  uint16_t* out[2];
-  int64_t ldo;
-  int out_cols;
-  uint16_t* dx;           // GRAD: [M, K] packed, or null
-  float* col_sums;        // GRAD: [wavefronts][2][H], or null
-  int wide_out, wide_dout, wide_dx;
-  int blocks;             // hidden blocks; workgroup i takes block i % blocks
+  uint16_t* dx;           // [M, K] packed, or null
+  float* dw_part;         // [workgroups * sub][2][H][K], or null
+  float* col_sums;        // [workgroups * sub][2][H], or null
+  int wide_dx;            // 8-byte stores of dx
+  int sub;                // 32-row blocks of a step
 };
 
 constexpr int ROWS_WAVES = 8;
@@ -60,15 +57,13 @@ __device__ __forceinline__ void store_rows64(const uint8_t* area, const __amdgpu
   }
 }
 
-template <int DT, int MODE, int ACT, int KP, bool WIDE>
+template <int DT, int ACT, int KP, bool WIDE>
 __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const RowsArgs a) {
   constexpr int HB = rows_hidden(KP), KS = KP / 16, KB = KP / 32;
   constexpr int REGION = 2 * HB * 128;  // 64 channels of all weight rows
-  constexpr bool GRAD = MODE == GATED_GRAD;
   __shared__ __attribute__((aligned(16))) uint8_t wl[KP / 64 * REGION];
   __shared__ __attribute__((aligned(16))) float bias[2 * HB];
-  __shared__ __attribute__((aligned(16))) uint8_t areas[ROWS_WAVES * (GRAD ? 2 : 1) * 4096];
-  __shared__ float sums[GRAD ? ROWS_WAVES * 2 * HB : 1];
+  __shared__ __attribute__((aligned(16))) uint8_t areas[ROWS_WAVES * 4096];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, row = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = __builtin_amdgcn_readfirstlane((int)blockIdx.x % a.blocks);
@@ -91,11 +86,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const Ro
               : a.bias_dtype == FIM_F32   ? static_cast<const float*>(b)[n0 + n]
                                           : from16<DT>(static_cast<const uint16_t*>(b)[n0 + n]);
   }
-  if constexpr (GRAD)
-    for (int i = tid; i < ROWS_WAVES * 2 * HB; i += 64 * ROWS_WAVES) sums[i] = 0.0f;
   __syncthreads();
 
-  uint8_t* area = areas + wave * (GRAD ? 2 : 1) * 4096;
+  uint8_t* area = areas + wave * 4096;
   const int64_t row_blocks = (a.M + 31) / 32, step = (int64_t)groups * ROWS_WAVES;
   const int fsw = (row >> 1) & 7;
   auto left_bytes = [&](int64_t r0, int64_t ld, int64_t cols) __attribute__((always_inline)) {
@@ -116,45 +109,10 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const Ro
           s16x8, __builtin_amdgcn_raw_buffer_load_b128(src, (int)(k < a.kw ? at : TILE_OOB), 0, 0));
     }
   };
-  // the incoming gradient of 32 hidden columns as an accumulator block lies: lane h loads 8 columns 16 p + 8 h, then the
-  // wavefront's halves exchange the 4 that are the other's
-  auto load_d = [&](const __amdgpu_buffer_rsrc_t src, int hb, v4i (&d)[2]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int col = hb * 32 + 16 * p + 8 * h;
-      const uint32_t at = (uint32_t)(row * a.ldd + col) * 2u;
-      if constexpr (WIDE) {
-        d[p] = __builtin_bit_cast(
-            v4i, __builtin_amdgcn_raw_buffer_load_b128(src, (int)(col < hidden ? at : TILE_OOB), 0, 0));
-      } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          e[c] = __builtin_amdgcn_raw_buffer_load_b16(src, (int)(col + c < hidden ? at + 2 * c : TILE_OOB), 0, 0);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) d[p][c] = (int)(e[2 * c] | e[2 * c + 1] << 16);
-      }
-    }
-  };
 
   auto work = [&](int64_t rb, const s16x8 (&x)[KS]) __attribute__((always_inline)) {
     const int64_t r0 = rb * 32;
-    const bool past = r0 + row >= a.M;
-    const auto o0 = __builtin_amdgcn_make_buffer_rsrc(a.out[0] + r0 * a.ldo + n0, (short)0,
-                                                      left_bytes(r0, a.ldo, a.out_cols - n0), 0x00020000);
-    const auto o1 = __builtin_amdgcn_make_buffer_rsrc(a.out[GRAD] + r0 * a.ldo + n0, (short)0,
-                                                      left_bytes(r0, a.ldo, a.out_cols - n0), 0x00020000);
-    const auto din = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.dout) + (GRAD ? r0 * a.ldd + n0 : 0), (short)0,
-                                                       GRAD ? left_bytes(r0, a.ldd, hidden) : 0, 0x00020000);
-    v16f dxa[GRAD ? KB : 1];
-    v4i d[2][GRAD ? 2 : 1];
-    if constexpr (GRAD) {
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) dxa[b][q] = 0.0f;
-      load_d(din, 0, d[0]);
-    }
+    const auto to = __builtin_amdgcn_make_buffer_rsrc(a.out + r0 * a.H + n0, (short)0, left_bytes(r0, a.H, hidden), 0x00020000);
     const int hbs = (hidden + 31) / 32;
     // 32 hidden columns; odd: the second half of a 64-column line
     auto part = [&](int hb, auto odd_c) __attribute__((always_inline)) {
@@ -178,102 +136,21 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const Ro
         u = mfma16<DT>(*reinterpret_cast<const s16x8*>(wrow + HB * 128 + off), x[kk], u);
       }
       typedef int v2i __attribute__((ext_vector_type(2)));
-      auto at = [&](int q) __attribute__((always_inline)) {
-        return area + row * 128 + (((ODD * 4 + q) ^ fsw) << 4) + 8 * h;
-      };
-      if constexpr (!GRAD) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(g[4 * q + e]) * u[4 * q + e];
-          *reinterpret_cast<v2i*>(at(q)) = v2i{(int)to16x2<DT>(v[0], v[1]), (int)to16x2<DT>(v[2], v[3])};
-        }
-      } else {
-        if (hb + 1 < hbs) load_d(din, hb + 1, d[1 - ODD]);
-        v2i dv[4];
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)d[ODD][p][c], (uint32_t)d[ODD][p][c + 2], false, false);
-            dv[2 * p][c] = (int)r[0];
-            dv[2 * p + 1][c] = (int)r[1];
-          }
-        float v[32];
-        v4i dgp[2], dup[2];  // packed: operand of sub-step s
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t w = (uint32_t)dv[q][e >> 1];
-            const float dd = from16<DT>((uint16_t)(e & 1 ? w >> 16 : w));
-            float slope;
-            const float act = activate<ACT, true>(g[4 * q + e], slope);
-            v[4 * q + e] = past ? 0.0f : dd * u[4 * q + e] * slope;
-            v[16 + 4 * q + e] = past ? 0.0f : dd * act;
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            dgp[q >> 1][2 * (q & 1) + c] = (int)to16x2<DT>(v[4 * q + 2 * c], v[4 * q + 2 * c + 1]);
-            dup[q >> 1][2 * (q & 1) + c] = (int)to16x2<DT>(v[16 + 4 * q + 2 * c], v[16 + 4 * q + 2 * c + 1]);
-          }
-          *reinterpret_cast<v2i*>(at(q)) = v2i{dgp[q >> 1][2 * (q & 1)], dgp[q >> 1][2 * (q & 1) + 1]};
-          *reinterpret_cast<v2i*>(at(q) + 4096) = v2i{dup[q >> 1][2 * (q & 1)], dup[q >> 1][2 * (q & 1) + 1]};
-        }
-        if (a.dx != nullptr) {
-          const int i = lane & 15, col = ((lane >> 4) & 1) * 16 + 4 * (i & 3);
-#pragma unroll
-          for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int up = 0; up < 2; ++up) {
-                s16x4 t[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int r = up * HB + hb * 32 + 16 * s + 8 * k + 4 * h + (i >> 2), c = (b & 1) * 32 + col;
-                  t[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                      (lds_s16x4*)(wl + ((b >> 1) * REGION + r * 128 + (((c >> 3) ^ ((r >> 1) & 7)) << 4) + (c & 7) * 2)));
-                }
-                dxa[b] = mfma16<DT>(__builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                    __builtin_bit_cast(s16x8, up ? dup[s] : dgp[s]), dxa[b]);
-              }
-        }
-        if (a.col_sums != nullptr) {  // lane l: the sum of value l % 32 (gate: 0..15, up) of its half's columns
-          sum_lanes<16>(v, lane);
-          const int q = row & 15;
-          sums[(wave * 2 + (row >> 4)) * HB + hb * 32 + 8 * (q >> 2) + 4 * h + (q & 3)] += v[0];
-        }
+        for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(g[4 * q + e]) * u[4 * q + e];
+        *reinterpret_cast<v2i*>(area + row * 128 + (((ODD * 4 + q) ^ fsw) << 4) + 8 * h) =
+            v2i{(int)to16x2<DT>(v[0], v[1]), (int)to16x2<DT>(v[2], v[3])};
       }
     };
     for (int hb = 0; hb < hbs; hb += 2) {
       part(hb, std::integral_constant<int, 0>{});
       if (hb + 1 < hbs) part(hb + 1, std::integral_constant<int, 1>{});
       wave_lds_wait();
-      store_rows64<WIDE || GRAD>(area, o0, a.ldo, hb * 32, a.out_cols - n0 < HB ? a.out_cols - n0 : HB, lane);
-      if constexpr (GRAD)
-        store_rows64<true>(area + 4096, o1, a.ldo, hb * 32, a.out_cols - n0 < HB ? a.out_cols - n0 : HB, lane);
+      store_rows64<WIDE>(area, to, a.H, hb * 32, hidden, lane);
       wave_lds_wait();
-    }
-    if constexpr (GRAD) {
-      if (a.dx != nullptr) {
-        const auto to = __builtin_amdgcn_make_buffer_rsrc(a.dx + r0 * a.K, (short)0, left_bytes(r0, a.K, a.K), 0x00020000);
-        typedef int v2i __attribute__((ext_vector_type(2)));
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<v2i*>(area + row * 128 + ((((b & 1) * 4 + q) ^ fsw) << 4) + 8 * h) =
-                v2i{(int)to16x2<DT>(dxa[b][4 * q], dxa[b][4 * q + 1]), (int)to16x2<DT>(dxa[b][4 * q + 2], dxa[b][4 * q + 3])};
-          if (b & 1) {
-            wave_lds_wait();
-            if (a.wide_dx) store_rows64<true>(area, to, a.K, (b >> 1) * 64, a.K, lane);
-            else store_rows64<false>(area, to, a.K, (b >> 1) * 64, a.K, lane);
-            wave_lds_wait();
-          }
-        }
-      }
     }
   };
 
@@ -285,12 +162,6 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const Ro
     if (rb + step >= row_blocks) break;
     load_x(rb + 2 * step, xf[0]);
     work(rb + step, xf[1]);
-  }
-  if constexpr (GRAD) {
-    if (a.col_sums == nullptr) return;
-    float* to = a.col_sums + ((int64_t)group * ROWS_WAVES + wave) * 2 * a.H;
-    for (int i = lane; i < 2 * HB; i += 64)
-      if (i % HB < hidden) to[(i / HB) * a.H + n0 + i % HB] = sums[wave * 2 * HB + i];
   }
 }
 
