@@ -6,8 +6,8 @@
 // rows at a time (64 where H is at most 128). Each of its eight wavefronts owns 32 hidden columns: it multiplies them,
 // applies the epilogue, adds its dg^T x and du^T x to accumulators that stay in registers for the whole launch, and its
 // column sums too. dg and du go to LDS in 16 bits (operands of 16-bit products, as everywhere in this operator); after one
-// barrier each wavefront takes a 16 x 16 tile of dx, contracted over all of them. The two LDS copies of dg, du and x make
-// that barrier the only one of a step: a wavefront writes the next step's while others still read this one's.
+// barrier each wavefront takes a 16 x 16 tile of dx, contracted over all of them. With two LDS copies of dg, du and x that is
+// the only barrier of a step: a wavefront writes the next step's while others still read this one's.
 #pragma once
 
 #include "gated_few.h"
@@ -47,6 +47,8 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
               : a.bias_dtype == FIM_F32 ? static_cast<const float*>(b)[n]
                                         : from16<DT>(static_cast<const uint16_t*>(b)[n]);
   }
+  // (hidden blocks past the end stay zero: dx's contraction runs over them)
+  for (int i = tid; i < 2 * DT_BYTES / 16; i += 64 * ROWS_WAVES) *reinterpret_cast<v4i*>(dl + i * 16) = v4i{0, 0, 0, 0};
 
   const int rows_step = 32 * a.sub;
   const int64_t steps = (a.M + rows_step - 1) / rows_step;
@@ -105,15 +107,10 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
 #pragma unroll
   for (int i = 0; i < 32; ++i) sums[i] = 0.0f;
 
-  int64_t step = blockIdx.x;
-  int cur = 0;
-  v4i xr = load_x(step), d[2];
-  load_d(step, d);
-  if (loads_x) *reinterpret_cast<v4i*>(xl + xat) = xr;
-  xr = load_x(step + gridDim.x);
-  __syncthreads();
+  v4i xr, d[2];
 
-  for (; step < steps; step += gridDim.x, cur ^= 1) {
+  // A step's dg, du and their part of the weights' gradients; x and dout of the next ones are on their way meanwhile
+  auto gradients = [&](int64_t step, int cur) __attribute__((always_inline)) {
     const uint8_t* xt = xl + cur * XT + rs * 4096;
     uint8_t* dt = dl + cur * DT_BYTES;
     if (active) {
@@ -147,27 +144,36 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
         g = mfma16<DT>(*reinterpret_cast<const s16x8*>(wrow + off), x, g);
         u = mfma16<DT>(*reinterpret_cast<const s16x8*>(wrow + HB * 128 + off), x, u);
       }
-      const bool past = step * rows_step + 32 * rs + row >= a.M;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w = (uint32_t)dv[i >> 2][(i >> 1) & 1];
+        const float dd = from16<DT>((uint16_t)(i & 1 ? w >> 16 : w));
+        float slope;
+        const float act = activate<ACT, true>(g[i], slope);
+        g[i] = dd * u[i] * slope;
+        u[i] = dd * act;
+      }
+      const int64_t left = a.M - step * rows_step - 32 * rs;
+      if (left < 32) {  // rows past the end: zero times anything
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          g[i] = row < left ? g[i] : 0.0f;
+          u[i] = row < left ? u[i] : 0.0f;
+        }
+      }
       const int drow = 32 * rs + row;
       uint8_t* drow_at = dt + drow * stride + 8 * h;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float vg[4], vu[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t w = (uint32_t)dv[q][e >> 1];
-          const float dd = from16<DT>((uint16_t)(e & 1 ? w >> 16 : w));
-          float slope;
-          const float act = activate<ACT, true>(g[4 * q + e], slope);
-          vg[e] = past ? 0.0f : dd * u[4 * q + e] * slope;  // (a row past the end: zero times anything)
-          vu[e] = past ? 0.0f : dd * act;
-          sums[4 * q + e] += vg[e];
-          sums[16 + 4 * q + e] += vu[e];
+          sums[4 * q + e] += g[4 * q + e];
+          sums[16 + 4 * q + e] += u[4 * q + e];
         }
         *reinterpret_cast<v2i*>(drow_at + (((hb * 4 + q) ^ (drow & 15)) << 4)) =
-            v2i{(int)to16x2<DT>(vg[0], vg[1]), (int)to16x2<DT>(vg[2], vg[3])};
+            v2i{(int)to16x2<DT>(g[4 * q], g[4 * q + 1]), (int)to16x2<DT>(g[4 * q + 2], g[4 * q + 3])};
         *reinterpret_cast<v2i*>(drow_at + (((nb * 4 + hb * 4 + q) ^ (drow & 15)) << 4)) =
-            v2i{(int)to16x2<DT>(vu[0], vu[1]), (int)to16x2<DT>(vu[2], vu[3])};
+            v2i{(int)to16x2<DT>(u[4 * q], u[4 * q + 1]), (int)to16x2<DT>(u[4 * q + 2], u[4 * q + 3])};
       }
     }
     if (loads_x) *reinterpret_cast<v4i*>(xl + (cur ^ 1) * XT + xat) = xr;
@@ -195,46 +201,66 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
           for (int b = 0; b < 2; ++b) dw[up][b] = mfma16<DT>(df[up], xf[b], dw[up][b]);
       }
     }
-    __syncthreads();
-    if (a.dx != nullptr) {
-      const int64_t r0 = step * rows_step;
-      const auto to = __builtin_amdgcn_make_buffer_rsrc(a.dx + r0 * a.K, (short)0, left_bytes(r0, rows_step, a.K, a.K),
-                                                        0x00020000);
-      const int kg = lane >> 4, ct = wave & 3, c = ct * 16 + 4 * (i16 & 3);
-      for (int rt = wave >> 2; rt < 2 * a.sub; rt += 2) {
-        const int r = rt * 16 + i16;
-        const uint8_t* drow_at = dt + r * stride;
-        v4f acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll 2
-        for (int st = 0; st < hbs; ++st) {
+  };
+
+  // This wavefront's tiles of a step's dx
+  const int kg = lane >> 4, ct = wave & 3, col = ct * 16 + 4 * kg;
+  auto products = [&](int64_t step, int cur) __attribute__((always_inline)) {
+    const uint8_t* dt = dl + cur * DT_BYTES;
+    const int64_t r0 = step * rows_step;
+    const auto to = __builtin_amdgcn_make_buffer_rsrc(a.dx + r0 * a.K, (short)0, left_bytes(r0, rows_step, a.K, a.K),
+                                                      0x00020000);
+    const int c = ct * 16 + 4 * (i16 & 3), wr = 8 * kg + (i16 >> 2);
+    const uint8_t* w_at[2];  // + 4 k rows; a swizzle that is the same 32 rows on
 #pragma unroll
-          for (int up = 0; up < 2; ++up) {
-            const int slot = up * nb * 4 + 4 * st + kg;
-            const s16x8 df = *reinterpret_cast<const s16x8*>(drow_at + ((slot ^ i16) << 4));
-            s16x4 t[2];
+    for (int k = 0; k < 2; ++k)
+      w_at[k] = wl + (wr + 4 * k) * 128 + (((c >> 3) ^ (((wr + 4 * k) >> 1) & 7)) << 4) + (c & 7) * 2;
+    for (int rt = wave >> 2; rt < 2 * a.sub; rt += 2) {
+      const int r = rt * 16 + i16;
+      v4f acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll 1
+      for (int st = 0; st < 2 * nb; st += 4) {  // four hidden blocks, of the gate's first: 256 bytes of a row
+        const int on = (st < nb ? 32 * st : HB + 32 * (st - nb)) * 128;
+        s16x8 df[4], wf[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int wr = up * HB + 32 * st + 8 * kg + 4 * k + (i16 >> 2);
-              t[k] = transposed(wl + wr * 128 + (((c >> 3) ^ ((wr >> 1) & 7)) << 4) + (c & 7) * 2);
-            }
-            acc[up] = mfma16x16<DT>(__builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7), df, acc[up]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          df[j] = *reinterpret_cast<const s16x8*>(dt + r * stride + st * 64 + (((4 * j + kg) ^ i16) << 4));
+          wf[j] = __builtin_shufflevector(transposed(w_at[0] + on + j * 4096), transposed(w_at[1] + on + j * 4096), 0, 1, 2, 3,
+                                          4, 5, 6, 7);
         }
-        const v4f v = acc[0] + acc[1];  // lane: row, registers: channels 4 kg ..
-        const uint32_t w[2] = {to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
-        const int col = ct * 16 + 4 * kg;
-        const uint32_t at = (uint32_t)(r * a.K + col) * 2u;
-        if (a.wide_dx) {
-          typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2{w[0], w[1]}, to, (int)(col < a.K ? at : TILE_OOB), 0, 0);
-        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(w[e >> 1] >> (16 * (e & 1))), to,
-                                                  (int)(col + e < a.K ? at + 2 * e : TILE_OOB), 0, 0);
-        }
+        for (int j = 0; j < 4; ++j) acc[j & 1] = mfma16x16<DT>(wf[j], df[j], acc[j & 1]);
+      }
+      const v4f v = acc[0] + acc[1];  // lane: row, registers: channels 4 kg ..
+      const uint32_t w[2] = {to16x2<DT>(v[0], v[1]), to16x2<DT>(v[2], v[3])};
+      const uint32_t at = (uint32_t)(r * a.K + col) * 2u;
+      if (a.wide_dx) {
+        typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{w[0], w[1]}, to, (int)(col < a.K ? at : TILE_OOB), 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(w[e >> 1] >> (16 * (e & 1))), to,
+                                                (int)(col + e < a.K ? at + 2 * e : TILE_OOB), 0, 0);
       }
     }
+  };
+
+  // Between two barriers: dx of one step and the gradients of the next, in either order. The two wavefronts of a SIMD take
+  // them in opposite orders, so one's matrix and LDS work runs beside the other's vector work.
+  const int64_t first = blockIdx.x;
+  xr = load_x(first);
+  load_d(first, d);
+  if (loads_x) *reinterpret_cast<v4i*>(xl + xat) = xr;
+  xr = load_x(first + gridDim.x);
+  const bool late = wave >= 4;
+  int cur = 1;
+  for (int64_t next = first; next < steps + gridDim.x; next += gridDim.x, cur ^= 1) {  // (first: nothing to contract yet)
+    __syncthreads();
+    const bool contracts = a.dx != nullptr && next != first;
+    if (contracts && !late) products(next - gridDim.x, cur);
+    if (next < steps) gradients(next, cur ^ 1);
+    if (contracts && late) products(next - gridDim.x, cur);
   }
 
   if (!active) return;
