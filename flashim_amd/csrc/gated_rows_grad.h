@@ -20,6 +20,11 @@ constexpr int GRAD_HIDDEN = 256;  // hidden columns whose weights fit: 64 KB wit
 // 32-row blocks of a step: as many as wavefronts per hidden block allow
 inline int rows_grad_sub(int64_t H) { return H <= GRAD_HIDDEN / 2 ? 2 : 1; }
 
+// Where a row's 16-byte slots go, by XOR: rows of 128 bytes (x, weights), and of 256 or more (dg, du). Sixteen rows read at
+// one slot spread over all banks either way; and so do the four rows by 64 bytes, or eight by 32, of a transposed read.
+__device__ __forceinline__ int swizzle8(int r) { return ((r << 1) & 4) | ((r >> 2) & 2) | ((r >> 2) & 1); }
+__device__ __forceinline__ int swizzle16(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+
 template <int DT, int ACT, bool WIDE>
 __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(const RowsArgs a) {
   constexpr int HB = GRAD_HIDDEN, XT = 2 * 4096, DT_BYTES = 32 * 2 * HB * 2;
@@ -33,12 +38,12 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
   const int hbs = (a.H + 31) / 32, stride = nb * 128;                 // bytes of a row of dg and du in LDS
   const bool active = hb < hbs;
 
-  // weights as gated_rows_kernel keeps them: 128 bytes a row, 16-byte slots swizzled by the row
+  // weights: 128 bytes a row
   for (int i = tid; i < 2 * HB * 8; i += 64 * ROWS_WAVES) {
     const int r = i >> 3, seg = i & 7, n = r % HB;
     v4i v = {0, 0, 0, 0};
     if (n < a.H && seg * 8 < a.kw) v = *reinterpret_cast<const v4i*>(a.w[r / HB] + (int64_t)n * a.ldw + seg * 8);
-    *reinterpret_cast<v4i*>(wl + r * 128 + ((seg ^ ((r >> 1) & 7)) << 4)) = v;
+    *reinterpret_cast<v4i*>(wl + r * 128 + ((seg ^ swizzle8(r)) << 4)) = v;
   }
   for (int i = tid; i < 2 * HB; i += 64 * ROWS_WAVES) {
     const void* b = a.bias[i / HB];
@@ -52,7 +57,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
 
   const int rows_step = 32 * a.sub;
   const int64_t steps = (a.M + rows_step - 1) / rows_step;
-  const int fsw = (row >> 1) & 7;
+  const int fsw = swizzle8(row);
   auto left_bytes = [&](int64_t r0, int most, int64_t ld, int64_t cols) __attribute__((always_inline)) {
     const int64_t rows = a.M - r0 < most ? a.M - r0 : most;
     return __builtin_amdgcn_readfirstlane(rows <= 0 ? 0 : (int)(((rows - 1) * ld + cols) * 2));
@@ -60,7 +65,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
   // 16 bytes of x a thread, and where they lie in LDS
   const int xrow = tid >> 3, xseg = tid & 7;
   const bool loads_x = xrow < rows_step;
-  const int xat = xrow * 128 + ((xseg ^ ((xrow >> 1) & 7)) << 4);
+  const int xat = xrow * 128 + ((xseg ^ swizzle8(xrow)) << 4);
   auto load_x = [&](int64_t step) __attribute__((always_inline)) {
     const int64_t r0 = step < steps ? step * rows_step : a.M;
     const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.x) + r0 * a.ldx, (short)0,
@@ -161,8 +166,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
           u[i] = row < left ? u[i] : 0.0f;
         }
       }
-      const int drow = 32 * rs + row;
-      uint8_t* drow_at = dt + drow * stride + 8 * h;
+      uint8_t* drow_at = dt + (32 * rs + row) * stride + 8 * h;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
 #pragma unroll
@@ -170,9 +174,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
           sums[4 * q + e] += g[4 * q + e];
           sums[16 + 4 * q + e] += u[4 * q + e];
         }
-        *reinterpret_cast<v2i*>(drow_at + (((hb * 4 + q) ^ (drow & 15)) << 4)) =
+        *reinterpret_cast<v2i*>(drow_at + (((hb * 4 + q) ^ swizzle16(row)) << 4)) =
             v2i{(int)to16x2<DT>(g[4 * q], g[4 * q + 1]), (int)to16x2<DT>(g[4 * q + 2], g[4 * q + 3])};
-        *reinterpret_cast<v2i*>(drow_at + (((nb * 4 + hb * 4 + q) ^ (drow & 15)) << 4)) =
+        *reinterpret_cast<v2i*>(drow_at + (((nb * 4 + hb * 4 + q) ^ swizzle16(row)) << 4)) =
             v2i{(int)to16x2<DT>(u[4 * q], u[4 * q + 1]), (int)to16x2<DT>(u[4 * q + 2], u[4 * q + 3])};
       }
     }
@@ -188,9 +192,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
           s16x4 t[2], td[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int r = 16 * s + 4 * k + trow, c = b * 32 + tcol, dr = 32 * rs + r;
-            t[k] = transposed(xt + r * 128 + (((c >> 3) ^ ((r >> 1) & 7)) << 4) + (c & 7) * 2);
-            td[k] = transposed(dt + dr * stride + (((b * nb * 4 + hb * 4 + (tcol >> 3)) ^ (dr & 15)) << 4) + (tcol & 7) * 2);
+            const int r = 16 * s + 4 * k + trow, c = b * 32 + tcol;
+            t[k] = transposed(xt + r * 128 + (((c >> 3) ^ swizzle8(r)) << 4) + (c & 7) * 2);
+            td[k] = transposed(dt + (32 * rs + r) * stride + (((b * nb * 4 + hb * 4 + (tcol >> 3)) ^ swizzle16(r)) << 4) + (tcol & 7) * 2);
           }
           xf[b] = __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7);
           df[b] = __builtin_shufflevector(td[0], td[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -214,7 +218,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
     const uint8_t* w_at[2];  // + 4 k rows; a swizzle that is the same 32 rows on
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-      w_at[k] = wl + (wr + 4 * k) * 128 + (((c >> 3) ^ (((wr + 4 * k) >> 1) & 7)) << 4) + (c & 7) * 2;
+      w_at[k] = wl + (wr + 4 * k) * 128 + (((c >> 3) ^ swizzle8(wr + 4 * k)) << 4) + (c & 7) * 2;
     for (int rt = wave >> 2; rt < 2 * a.sub; rt += 2) {
       const int r = rt * 16 + i16;
       v4f acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
         s16x8 df[4], wf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          df[j] = *reinterpret_cast<const s16x8*>(dt + r * stride + st * 64 + (((4 * j + kg) ^ i16) << 4));
+          df[j] = *reinterpret_cast<const s16x8*>(dt + r * stride + st * 64 + (((4 * j + kg) ^ swizzle16(i16)) << 4));
           wf[j] = __builtin_shufflevector(transposed(w_at[0] + on + j * 4096), transposed(w_at[1] + on + j * 4096), 0, 1, 2, 3,
                                           4, 5, 6, 7);
         }
