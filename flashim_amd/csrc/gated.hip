@@ -157,12 +157,14 @@ static Splits split_plan(int64_t rows, int64_t cols, int64_t k, bool alone) {
   return best;
 }
 
-// Whether a launch is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half the
-// CUs. Backward also needs all weights in one workgroup's LDS.
-static bool gated_rows(int64_t M, int64_t K, int64_t H, bool backward) {
-  if (K > 128 || M < 32 * ROWS_WAVES * (int64_t)device_cus() / 2) return false;
-  return !backward || (K <= 64 && H <= GRAD_HIDDEN);
-}
+// Whether the forward pass is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half
+// the CUs. (On rows and on tiles: 24000 x 64 -> 256, 13.3 and 12.0 us; 40000: 15.6 and 14.4; 80000: 23.5 and 30.1; 32768 x 128
+// -> 512: 22.1 and 22.3; 160000: 61.6 and 97.7.)
+static bool gated_rows(int64_t M, int64_t K) { return K <= 128 && M >= 32 * ROWS_WAVES * (int64_t)device_cus() / 2; }
+
+// Whether the backward pass is (gated_rows_grad.h): all weights fit one workgroup's LDS, any number of rows. (1000 x 64 -> 256:
+// 15 us, 24 on tiles; 24000: 32 and 37; 320000: 158 and 241.)
+static bool gated_rows_grad(int64_t K, int64_t H) { return K <= 64 && H <= GRAD_HIDDEN; }
 
 static int64_t rows_blocks(int64_t K, int64_t H) { return cdiv(H, rows_hidden(K <= 64 ? 64 : 128)); }
 
@@ -172,10 +174,21 @@ static int64_t rows_groups(int64_t M, int64_t K, int64_t H) {
   return n < 1 ? 1 : n < most ? n : most;
 }
 
-// The same of a backward pass by rows
-static int64_t rows_grad_groups(int64_t M, int64_t H) {
-  const int64_t most = cdiv(M, 32 * rows_grad_sub(H));
-  return device_cus() < most ? device_cus() : most;
+// Workgroups of a backward pass by rows: one per CU at most, fewer where the steps saved (3.7 us each) would cost less than the
+// partial weight gradients they leave (written, then joined, at 5 TB/s)
+static int64_t rows_grad_groups(int64_t M, int64_t K, int64_t H) {
+  const int64_t steps = cdiv(M, 32 * rows_grad_sub(H));
+  const double part = rows_grad_sub(H) * 2.0 * H * K * 4 * 2 / 5e6;  // us
+  int64_t best = 0;
+  double best_time = 0.0;
+  for (int64_t rounds = cdiv(steps, device_cus()), i = 0; i < 16; ++rounds, ++i) {
+    const int64_t groups = cdiv(steps, rounds);
+    const double time = 3.7 * rounds + part * groups;
+    if (best != 0 && time >= best_time) continue;
+    best_time = time;
+    best = groups;
+  }
+  return best;
 }
 
 struct Gated {
@@ -208,9 +221,9 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.ldg = cdiv(g.H, 64) * 64 + 64;
   if (!backward) return g;
   g.dgu_at = g.total;
-  g.rows = gated_rows(g.M, g.K, g.H, true);
+  g.rows = gated_rows_grad(g.K, g.H);
   if (g.rows) {
-    g.sum_rows = g.dw_splits = rows_grad_groups(g.M, g.H) * rows_grad_sub(g.H);
+    g.sum_rows = g.dw_splits = rows_grad_groups(g.M, g.K, g.H) * rows_grad_sub(g.H);
     g.cols_at = g.dgu_at;
     g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
     g.total = g.part_at + align256(g.dw_splits * 2 * g.H * g.K * 4);
@@ -300,7 +313,7 @@ static void launch_rows(const RowsArgs& a, bool wide, hipStream_t stream) {
 
 template <int DT, int ACT>
 static void launch_rows_grad(const RowsArgs& a, bool wide, hipStream_t stream) {
-  const dim3 grid((unsigned)rows_grad_groups(a.M, a.H));
+  const dim3 grid((unsigned)rows_grad_groups(a.M, a.K, a.H));
   if (wide) gated_rows_grad_kernel<DT, ACT, true><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
   else gated_rows_grad_kernel<DT, ACT, false><<<grid, dim3(64 * ROWS_WAVES), 0, stream>>>(a);
 }
@@ -445,7 +458,7 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
     constexpr int DT = decltype(dt)::value;
     with_activation(act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
-      if (!gated_rows(M, K, H, false)) launch_product<DT, GATED_FORWARD, ACT>(a, tile, 1, stream);
+      if (!gated_rows(M, K)) launch_product<DT, GATED_FORWARD, ACT>(a, tile, 1, stream);
       else if (K <= 64) launch_rows<DT, ACT, 64>(rows_args(a, K), a.wide_out, stream);
       else launch_rows<DT, ACT, 128>(rows_args(a, K), a.wide_out, stream);
     });
