@@ -16,16 +16,43 @@
 
 namespace fim {
 
-// An operand copied to packed rows of `to_cols` elements, zeros past its own: 16-byte stores
-__global__ __launch_bounds__(256) void gated_pack_kernel(const uint16_t* from, int64_t ld, int64_t rows, int64_t cols,
-                                                         uint16_t* to, int64_t to_cols) {
-  const int64_t per_row = to_cols / 8;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per_row; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-    uint32_t e[8];
+// Operands copied to packed rows of `to_cols` elements, zeros past their own: 16-byte stores, up to three operands a launch
+struct PackArgs {
+  struct {
+    const uint16_t* from;
+    uint16_t* to;
+    int64_t ld, rows;
+    int cols, per_row;    // per_row: 16-byte runs of a packed row
+    int64_t first_block;  // the operand's first workgroup
+  } m[3];
+  int count;
+};
+
+__global__ __launch_bounds__(256) void gated_pack_kernel(const PackArgs a) {
+  int o = 0;
+  while (o + 1 < a.count && (int64_t)blockIdx.x >= a.m[o + 1].first_block) ++o;
+  const auto& m = a.m[o];
+  // (one 64-bit division a workgroup)
+  const int64_t run0 = ((int64_t)blockIdx.x - m.first_block) * 1024, row0 = run0 / m.per_row;
+  const uint32_t rest = (uint32_t)(run0 - row0 * m.per_row);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = c + k < cols ? from[r * ld + c + k] : 0;
-    reinterpret_cast<uint4*>(to)[i] = uint4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t at = rest + k * 256 + threadIdx.x, down = at / (uint32_t)m.per_row;
+    const int64_t r = row0 + down;
+    const int c = (int)(at - down * m.per_row) * 8;
+    if (r >= m.rows) return;
+    const uint16_t* from = m.from + r * m.ld + c;
+    v4i v;
+    if (c + 8 <= m.cols) {
+      v = *reinterpret_cast<const v4i_any*>(from);
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < m.cols ? from[i] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (int)(e[2 * i] | e[2 * i + 1] << 16);
+    }
+    reinterpret_cast<v4i*>(m.to)[r * m.per_row + (c >> 3)] = v;
   }
 }
 
@@ -250,17 +277,14 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   return g;
 }
 
-static void gated_pack(const Matrix& m, uint16_t* to, hipStream_t stream) {
-  const int64_t blocks = cdiv(m.rows * m.padded() / 8, 256);
-  gated_pack_kernel<<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream>>>(m.p, m.ld, m.rows, m.cols, to,
-                                                                                              m.padded());
-}
-
 // Copies what has to be copied; g.x, g.wg and g.wu are readable by the tiles afterwards
 static void gated_operands(Gated& g, uint8_t* ws, hipStream_t stream) {
+  PackArgs a{};
+  int64_t blocks = 0;
   auto copy = [&](Matrix& m, int64_t at) {
     uint16_t* to = reinterpret_cast<uint16_t*>(ws + at);
-    gated_pack(m, to, stream);
+    a.m[a.count++] = {m.p, to, m.ld, m.rows, (int)m.cols, (int)(m.padded() / 8), blocks};
+    blocks += cdiv(m.rows * m.padded() / 8, 1024);
     m = {to, m.padded(), m.rows, m.padded()};
   };
   const bool copy_w = g.wu_at != g.wg_at;
@@ -269,6 +293,7 @@ static void gated_operands(Gated& g, uint8_t* ws, hipStream_t stream) {
     copy(g.wg, g.wg_at);
     copy(g.wu, g.wu_at);
   }
+  if (a.count > 0) gated_pack_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
 }
 
 template <int DT, int MODE, int ACT, int MB, int NB>

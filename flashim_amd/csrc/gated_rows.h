@@ -33,27 +33,35 @@ struct RowsArgs {
 constexpr int ROWS_WAVES = 8;
 constexpr int rows_hidden(int kp) { return 16384 / kp; }  // hidden columns of a block: 64 KB of weights
 
-// A wavefront's [32 rows, 64 columns] in its LDS area to rows of 128 bytes at `to` (rows `ld` apart): bytes and columns
-// past the end go out of range
+// A wavefront's [32 rows, 64 columns] in its LDS area to rows of 128 bytes at `out` (rows `ld` apart, `rows` of them; `to`: the
+// same as a buffer, where bytes and columns past the end go out of range)
 template <bool WIDE>
-__device__ __forceinline__ void store_rows64(const uint8_t* area, const __amdgpu_buffer_rsrc_t to, int64_t ld, int col0,
-                                             int cols, int lane) {
+__device__ __forceinline__ void store_rows64(const uint8_t* area, uint16_t* out, const __amdgpu_buffer_rsrc_t to, int64_t ld,
+                                             int64_t rows, int col0, int cols, int lane) {
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-  const int slot = lane & 7;
+  const int slot = lane & 7, row0 = lane >> 3, col = col0 + slot * 8;
+  v4i v[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const int row = p * 8 + (lane >> 3);
-    const u32x4 v = *reinterpret_cast<const u32x4*>(area + row * 128 + ((slot ^ ((row >> 1) & 7)) << 4));
-    const int col = col0 + slot * 8;
-    const uint32_t at = (uint32_t)(row * ld + col) * 2u;
-    if constexpr (WIDE) {
-      __builtin_amdgcn_raw_buffer_store_b128(v, to, (int)(col < cols ? at : TILE_OOB), 0, 0);
-    } else {
+    const int row = p * 8 + row0;
+    v[p] = *reinterpret_cast<const v4i*>(area + row * 128 + ((slot ^ ((row >> 1) & 7)) << 4));
+  }
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[p]), to,
+                                             (int)(col < cols ? (uint32_t)((p * 8 + row0) * ld + col) * 2u : TILE_OOB), 0, 0);
+  } else if (rows >= 32 && col + 8 <= cols) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) *reinterpret_cast<v4i_any*>(out + (p * 8 + row0) * ld + col) = v[p];
+  } else {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(v[c / 2] >> (16 * (c & 1))), to,
-                                              (int)(col + c < cols ? at + 2 * c : TILE_OOB), 0, 0);
-    }
+        __builtin_amdgcn_raw_buffer_store_b16(
+            (uint16_t)((uint32_t)v[p][c / 2] >> (16 * (c & 1))), to,
+            (int)(col + c < cols ? (uint32_t)((p * 8 + row0) * ld + col + c) * 2u : TILE_OOB), 0, 0);
   }
 }
 
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_kernel(const Ro
       part(hb, std::integral_constant<int, 0>{});
       if (hb + 1 < hbs) part(hb + 1, std::integral_constant<int, 1>{});
       wave_lds_wait();
-      store_rows64<WIDE>(area, to, a.H, hb * 32, hidden, lane);
+      store_rows64<WIDE>(area, a.out + r0 * a.H + n0, to, a.H, a.M - r0, hb * 32, hidden, lane);
       wave_lds_wait();
     }
   };

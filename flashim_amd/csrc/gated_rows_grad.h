@@ -79,14 +79,22 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void gated_rows_grad_kernel(con
     const int64_t at0 = step * rows_step + 32 * rs, r0 = step < steps && at0 < a.M ? at0 : a.M;
     const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.dout) + r0 * a.ldd, (short)0,
                                                        left_bytes(r0, 32, a.ldd, a.H), 0x00020000);
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int col = hb * 32 + 16 * p + 8 * h;
-      const uint32_t at = (uint32_t)(row * a.ldd + col) * 2u;
-      if constexpr (WIDE) {
-        d[p] = __builtin_bit_cast(
-            v4i, __builtin_amdgcn_raw_buffer_load_b128(src, (int)(col < a.H ? at : TILE_OOB), 0, 0));
-      } else {
+      for (int p = 0; p < 2; ++p) {
+        const int col = hb * 32 + 16 * p + 8 * h;
+        d[p] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(
+                                           src, (int)(col < a.H ? (uint32_t)(row * a.ldd + col) * 2u : TILE_OOB), 0, 0));
+      }
+    } else if (a.M - r0 >= 32 && hb * 32 + 32 <= a.H) {
+      const uint16_t* from = a.dout + (r0 + row) * a.ldd + hb * 32 + 8 * h;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) d[p] = *reinterpret_cast<const v4i_any*>(from + 16 * p);
+    } else {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int col = hb * 32 + 16 * p + 8 * h;
+        const uint32_t at = (uint32_t)(row * a.ldd + col) * 2u;
         uint32_t e[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c)

@@ -92,6 +92,10 @@ __device__ __forceinline__ void sum_lanes(float (&v)[32], int lane) {
   if constexpr (S > 1) sum_lanes<S / 2>(v, lane);
 }
 
+// Sixteen bytes of a row whose width or address is not a multiple of 16 bytes: global loads and stores take any alignment of
+// the element.
+typedef v4i v4i_any __attribute__((aligned(2)));
+
 template <int DT, int MODE, int ACT, int MB, int NB>
 __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(const TileArgs a) {
   constexpr bool PAIR = MODE == GATED_FORWARD || MODE == GATED_GRAD;
@@ -396,22 +400,35 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
     }
     auto epilogue = [&](auto wide_c) __attribute__((always_inline)) {
       constexpr bool WIDE = decltype(wide_c)::value;  // 16-byte rows of out (GRAD: of dout)
+      const bool whole = rows_left >= 32 * MB;
       v4i grad[2][MODE == GATED_GRAD ? RUNS : 1];  // rows of the incoming gradient, 32 ahead
       auto load_grad = [&](int j) __attribute__((always_inline)) {
         if constexpr (MODE == GATED_GRAD) {
 #pragma unroll
           for (int p = 0; p < RUNS; ++p) {
-            const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldd + slot * 8) * 2u;
             if constexpr (WIDE) {
+              const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldd + slot * 8) * 2u;
               grad[j & 1][p] = __builtin_bit_cast(
                   v4i, __builtin_amdgcn_raw_buffer_load_b128(din, (int)(slot * 8 < cols_in ? at : TILE_OOB), 0, 0));
+            }
+          }
+          if constexpr (!WIDE) {
+            if (whole && slot * 8 + 8 <= cols_in) {
+              const uint16_t* from = a.dout + (mw + 32 * j + prow) * a.ldd + nw + slot * 8;
+#pragma unroll
+              for (int p = 0; p < RUNS; ++p)
+                grad[j & 1][p] = *reinterpret_cast<const v4i_any*>(from + (int64_t)p * PER * a.ldd);
             } else {
-              uint32_t e[8];
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                e[c] = __builtin_amdgcn_raw_buffer_load_b16(din, (int)(slot * 8 + c < cols_in ? at + 2 * c : TILE_OOB), 0, 0);
+              for (int p = 0; p < RUNS; ++p) {
+                const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldd + slot * 8) * 2u;
+                uint32_t e[8];
 #pragma unroll
-              for (int c = 0; c < 4; ++c) grad[j & 1][p][c] = (int)(e[2 * c] | e[2 * c + 1] << 16);
+                for (int c = 0; c < 8; ++c)
+                  e[c] = __builtin_amdgcn_raw_buffer_load_b16(din, (int)(slot * 8 + c < cols_in ? at + 2 * c : TILE_OOB), 0, 0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) grad[j & 1][p][c] = (int)(e[2 * c] | e[2 * c + 1] << 16);
+              }
             }
           }
         }
@@ -468,23 +485,34 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
           }
         wave_lds_wait();
 #pragma unroll
-        for (int k = 0; k < AREAS; ++k)
+        for (int k = 0; k < AREAS; ++k) {
+          auto run = [&](int p) __attribute__((always_inline)) {
+            return *reinterpret_cast<const v4i*>(area + k * AREA + place(p * PER + prow, slot));
+          };
+          if constexpr (WIDE || MODE == GATED_GRAD) {
 #pragma unroll
-          for (int p = 0; p < RUNS; ++p) {
-            const int row = p * PER + prow;
-            const v4i v = *reinterpret_cast<const v4i*>(area + k * AREA + place(row, slot));
-            const uint32_t at = (uint32_t)((32 * j + row) * a.ldo + slot * 8) * 2u;
-            if constexpr (WIDE || MODE == GATED_GRAD) {
+            for (int p = 0; p < RUNS; ++p) {
               typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), k ? o1 : o0,
+              const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldo + slot * 8) * 2u;
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, run(p)), k ? o1 : o0,
                                                      (int)(slot * 8 < cols_out ? at : TILE_OOB), 0, 0);
-            } else {
+            }
+          } else if (whole && slot * 8 + 8 <= cols_out) {
+            uint16_t* to = a.out[0] + (mw + 32 * j + prow) * a.ldo + nw + slot * 8;
+#pragma unroll 2  // (whole, its addresses spill)
+            for (int p = 0; p < RUNS; ++p) *reinterpret_cast<v4i_any*>(to + (int64_t)p * PER * a.ldo) = run(p);
+          } else {
+#pragma unroll
+            for (int p = 0; p < RUNS; ++p) {
+              const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldo + slot * 8) * 2u;
+              const v4i v = run(p);
 #pragma unroll
               for (int c = 0; c < 8; ++c)
                 __builtin_amdgcn_raw_buffer_store_b16((uint16_t)((uint32_t)v[c / 2] >> (16 * (c & 1))), o0,
                                                       (int)(slot * 8 + c < cols_out ? at + 2 * c : TILE_OOB), 0, 0);
             }
           }
+        }
         wave_lds_wait();
       }
     };
