@@ -48,9 +48,9 @@ def grad_norm(grads: Sequence[Tensor], *, norm_type: float = 2.0) -> Tensor:
 
 def clip_grad_norm_(grads: Sequence[Tensor], max_norm: float, *, norm_type: float = 2.0,
                     out: Sequence[Tensor] | None = None, error_if_nonfinite: bool = False) -> Tensor:
-    """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` in place, or into ``out`` (tensors of the same shapes that
-    do not overlap the gradients, of any float type: BF16 gradients into the FP32 ones an optimizer reads), and returns
-    the norm. A NaN norm makes every element NaN, as in ``torch.nn.utils.clip_grad_norm_``; with ``error_if_nonfinite``
+    """Scales ``grads`` (no two of which overlap) by ``min(1, max_norm / (norm + 1e-6))`` in place, or into ``out`` (tensors
+    of the same shapes that do not overlap the gradients, of any float type: BF16 gradients into the FP32 ones an optimizer
+    reads), and returns the norm. A NaN norm makes every element NaN, as in ``torch.nn.utils.clip_grad_norm_``; with ``error_if_nonfinite``
     a norm that is not finite raises before anything is written (this waits for the GPU)."""
     with torch.no_grad():
         if error_if_nonfinite and not math.isfinite(library.grad_norm(grads, float(norm_type)).item()):

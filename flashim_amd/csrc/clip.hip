@@ -11,6 +11,11 @@
 // the loads. Each workgroup writes one partial; every workgroup of the second launch adds them all up in the same order
 // (at most 2048 of them: a few kilobytes from the L2, less than another launch; beyond that a launch of its own does), so
 // results do not depend on the order of workgroups.
+//
+// Measured (MI355X): 200 million BF16 gradients into FP32 ones, norm 119 us (3.4 TB/s: the lines that the pass before has
+// written leave the Infinity Cache meanwhile; 69 us without them) and scaling 231 us (5.2 TB/s, a copy's rate; 310 us where a
+// lane wrote 32 bytes in two stores instead of 16 in one). 320 FP32 tensors of 22.6 million elements: 19 + 4 us, 6 us for the
+// total, 6 + 27 us, less than the host takes for 640 tensors (65 us). Ten tensors of 35000 elements: 4 + 4 us.
 #include <type_traits>
 
 #include "common.h"

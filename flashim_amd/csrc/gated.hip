@@ -9,6 +9,9 @@
 // forward pass: with K below about 1000 their two writes and reads cost more than the products), which writes dg and du in
 // x's type (they are operands of 16-bit matrix products next; FP32 sums for the bias gradients are taken before that
 // rounding); then one product for dx over both halves and one for the weights, split over rows where its tiles are few.
+//
+// Four forms, chosen by sizes: up to 64 rows forward (gated_few.h), many rows of at most 128 channels forward (gated_rows.h),
+// backward of at most 64 channels and 256 hidden columns (gated_rows_grad.h), and tiles (gated_tile.h).
 #include "gated_few.h"
 #include "gated_rows.h"
 #include "gated_rows_grad.h"
@@ -245,6 +248,7 @@ static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, boo
   g.wu_at = g.wg_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
   g.total = g.wu_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
   g.hp = cdiv(g.H, 8) * 8;
+  // whole 128-byte lines, one more than fit: rows of a power of two apart would meet in the same cache sets and channels
   g.ldg = cdiv(g.H, 64) * 64 + 64;
   if (!backward) return g;
   g.dgu_at = g.total;

@@ -5,6 +5,9 @@
 // eight wavefronts works alone on 32 rows at a time: it loads them straight into MFMA operand registers, the next 32 while it
 // works, multiplies them by 32 hidden columns at a time, and writes whole 128-byte lines through its own LDS area. No barrier
 // after the weights are in; the wavefronts of a SIMD drift apart, one's vector work covers another's loads.
+//
+// A stream: x read once, the output written once. Measured (MI355X, BF16, SiLU): 320000 x 64 -> 256, 58 us (205 MB, 3.5 TB/s;
+// the vector work of the activation and the stores' way through LDS are 55% of it); 160000 x 128 -> 512, 62 us (98 on tiles).
 #pragma once
 
 #include "gated_tile.h"

@@ -8,6 +8,9 @@
 // column sums too. dg and du go to LDS in 16 bits (operands of 16-bit products, as everywhere in this operator); after one
 // barrier each wavefront takes a 16 x 16 tile of dx, contracted over all of them. With two LDS copies of dg, du and x that is
 // the only barrier of a step: a wavefront writes the next step's while others still read this one's.
+//
+// Measured (MI355X, BF16, SiLU): 320000 x 64 -> 256, 144 us (246 MB are 48 us): vector work 50% of the cycles, matrix products
+// 20%, LDS 42%, with two wavefronts per SIMD to overlap them.
 #pragma once
 
 #include "gated_few.h"

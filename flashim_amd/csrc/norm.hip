@@ -17,6 +17,11 @@
 // launch between the two for groups so many that every workgroup would read them for long). Nothing is summed by atomics:
 // results do not depend on the order of workgroups. Forward sums are kept about the mean of a thread's first pixels (no
 // cancellation where the mean is large) and merged as means and squared deviations.
+//
+// Measured (device time, MI355X; a large copy reaches 5.1 TB/s): 160000 x 64 BF16 with GELU, 15 us for the statistics and 25
+// us for the apply forward, 27 us and 32 us backward, where a map's read or write is 4 us: the activation with its slope is
+// 20 to 40 vector operations a value (8 to 16 us), and each pass starts with a launch, the partials of the pass before and
+// its first round of loads (5 us). 40000 x 128: 13 + 4 (merge) + 15 us. 1024 x 64: 6 + 8 us, latencies alone.
 #include "activation.h"
 
 namespace fim {

@@ -284,7 +284,7 @@ int fim_grad_norm(int64_t count, const void* const* grads, const int* dtypes, co
                   float* total, double* workspace, hipStream_t stream);
 
 /* The norm as above, and out[i] = grads[i] * min(1, max_norm / (*total + 1e-6)) (a NaN norm makes every element NaN).
- * out[i] is grads[i] (in place) or does not overlap any gradient; its type may differ. */
+ * out[i] is grads[i] (in place) or does not overlap any gradient; its type may differ. No two outputs overlap. */
 int fim_clip_grad_norm(int64_t count, const void* const* grads, const int* dtypes, void* const* out,
                        const int* out_dtypes, const int64_t* numel, float max_norm, int norm, float* total,
                        double* workspace, hipStream_t stream);
