@@ -16,12 +16,13 @@
 // (chunk, group), the second adds up its image's partials before it starts, while its first loads are on their way (a
 // launch between the two for groups so many that every workgroup would read them for long). Nothing is summed by atomics:
 // results do not depend on the order of workgroups. Forward sums are kept about the mean of a thread's first pixels (no
-// cancellation where the mean is large) and merged as means and squared deviations.
+// cancellation where the mean is large) and merged as means and squared deviations. Small maps take one launch forward
+// (norm_group_kernel).
 //
 // Measured (device time, MI355X; a large copy reaches 5.1 TB/s): 160000 x 64 BF16 with GELU, 15 us for the statistics and 25
 // us for the apply forward, 27 us and 32 us backward, where a map's read or write is 4 us: the activation with its slope is
 // 20 to 40 vector operations a value (8 to 16 us), and each pass starts with a launch, the partials of the pass before and
-// its first round of loads (5 us). 40000 x 128: 13 + 4 (merge) + 15 us. 1024 x 64: 6 + 8 us, latencies alone.
+// its first round of loads (5 us). 40000 x 128: 13 + 4 (merge) + 15 us. 1024 x 64: 6.7 us in one launch (12 in two), latencies alone.
 #include "activation.h"
 
 namespace fim {
@@ -30,9 +31,14 @@ constexpr int NORM_T = 512;           // threads of a workgroup
 // Pixels of a batch of loads (the next batch is loaded while one is worked on), with registers for four wavefronts per SIMD:
 // backward, with two tensors and the activation's slope, 4 took 180 to 230 registers and ran half as many wavefronts
 constexpr int NORM_U = 4, NORM_GRAD_U = 2;
+constexpr int NORM_OWN = 8;           // loads of a thread that owns its values (small maps)
 constexpr int NORM_MAX_C = 8192;      // per-channel partials of a workgroup lie in LDS
 constexpr int NORM_MERGE_G = 512;     // groups, and partials, that the workgroups of the second pass add up themselves
 constexpr int64_t NORM_MERGE = 2 << 20;  // (over all workgroups)
+// Bytes of a map that is small. One workgroup per (image, group) reads D channels of each pixel, as little as 16 bytes of a line:
+// against two launches 1024 x 64, 6.7 and 12.1 us; 16 images of it (2 MB), 8.9 and 12.8; 16 x 256 x 512 (4 MB), 11 and 14; 16 x
+// 900 x 196 (5.6 MB), 13.3 and 13.2; 64 x 1024 x 64 (8 MB), 23 and 18 us
+constexpr int64_t NORM_SMALL = 5 << 20;
 
 struct NormArgs {
   const uint8_t* x;
@@ -463,6 +469,78 @@ __global__ __launch_bounds__(NORM_T, 4) void norm_apply_kernel(const NormArgs a)
   }
 }
 
+// Small maps, forward: one workgroup per (image, group), whose values all stay in registers between the statistics and the
+// output, up to NORM_OWN loads a thread. The mean first, then the deviations about it (and their sum, which takes out what the
+// mean's rounding left).
+template <int DT, int V, int ACT>
+__global__ __launch_bounds__(NORM_T) void norm_group_kernel(const NormArgs a) {
+  typedef Pack<DT, V> Pk;
+  __shared__ float red[3][NORM_T / 64];
+  const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
+  const int cols = a.D / V, rows = NORM_T / cols, row = threadIdx.x / cols, col = threadIdx.x - row * cols;
+  const int P = (int)a.P, c0 = g * a.D + col * V;
+  const int n = row < rows && row < P ? (P - row + rows - 1) / rows : 0;
+  typename Pk::Raw r[NORM_OWN];
+  const uint8_t* x = a.x + (b * a.sb + (n > 0 ? row : 0) * a.sp + (n > 0 ? c0 : 0)) * Pk::ES;
+  const int64_t step = rows * a.sp * Pk::ES;
+#pragma unroll
+  for (int i = 0; i < NORM_OWN; ++i) r[i] = Pk::load(x + (i < n ? i : 0) * step);
+  float mul[V], add[V];
+  params<V>(a.weight, a.wdt, n > 0 ? c0 : 0, 1.0f, mul);
+  params<V>(a.bias, a.bdt, n > 0 ? c0 : 0, 0.0f, add);
+  auto all = [&](float v, float (&to)[NORM_T / 64]) __attribute__((always_inline)) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) to[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NORM_T / 64; ++i) sum += to[i];
+    return sum;
+  };
+  const float count = (float)((int64_t)P * a.D);
+  float s0 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NORM_OWN; ++i) {
+    float v[V], t = 0.0f;
+    Pk::unpack(r[i], v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) t += v[k];
+    s0 += i < n ? t : 0.0f;
+  }
+  const float shift = all(s0, red[0]) / count;
+  float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NORM_OWN; ++i) {
+    float v[V], t = 0.0f, q = 0.0f;
+    Pk::unpack(r[i], v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float d = v[k] - shift;
+      t += d;
+      q = fmaf(d, d, q);
+    }
+    s1 += i < n ? t : 0.0f;
+    s2 += i < n ? q : 0.0f;
+  }
+  s2 = all(s2, red[1]);
+  const float off = all(s1, red[2]) / count, mean = shift + off;
+  const float var = s2 / count - off * off, rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(a.stats)[blockIdx.x] = float2{mean, rstd};
+#pragma unroll
+  for (int k = 0; k < V; ++k) mul[k] *= rstd;
+  uint8_t* out = a.out + (((int64_t)b * P + row) * a.C + c0) * Pk::ES;
+  const int64_t out_step = (int64_t)rows * a.C * Pk::ES;
+#pragma unroll
+  for (int i = 0; i < NORM_OWN; ++i) {
+    if (i >= n) break;
+    float v[V];
+    Pk::unpack(r[i], v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = activate<ACT>(fmaf(v[k] - mean, mul[k], add[k]));
+    Pk::store(out + i * out_step, v);
+  }
+}
+
 // The per-channel values of a backward pass in registers: z = (x - mean) * mul + add, mul = rstd * weight
 template <int V>
 struct GradParams {
@@ -711,6 +789,15 @@ static size_t norm_lds(int64_t C, int v) {
   return (size_t)(rows * C * 2 * 4);
 }
 
+// Elements per load of a workgroup per (image, group), or 0: not a small map, or more than a workgroup's
+// registers hold
+static int norm_own_vector(const NormArgs& a, int v, int es) {
+  while (a.D % v) v /= 2;
+  const int64_t cols = a.D / v;
+  if (cols > NORM_T || cdiv(a.P, NORM_T / cols) > NORM_OWN) return 0;
+  return (int64_t)a.B * a.P * a.C * es <= NORM_SMALL ? v : 0;
+}
+
 // Sizes and chunks; false: too many
 static bool norm_shape(NormArgs& a, int64_t B, int64_t P, int64_t C, int64_t groups) {
   a.P = P;
@@ -760,6 +847,15 @@ extern "C" int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, in
   if (!norm_shape(a, B, P, C, groups)) return FIM_ERR_UNSUPPORTED;
   const int v = norm_vector(dtype, C, {stride_b, stride_p}, {x, out});
   const dim3 grid((unsigned)(B * a.chunks));
+  if (const int own = norm_own_vector(a, v, elem_size(dtype))) {
+    with_vector(dtype, own, [&](auto dt, auto vec) {
+      with_activation(act, [&](auto act_c) {
+        norm_group_kernel<decltype(dt)::value, decltype(vec)::value, decltype(act_c)::value>
+            <<<dim3((unsigned)(B * groups)), dim3(NORM_T), 0, stream>>>(a);
+      });
+    });
+    return launch_status();
+  }
   with_vector(dtype, v, [&](auto dt, auto vec) {
     constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
     norm_stats_kernel<DT, V><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(a);

@@ -907,6 +907,8 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
                                                  torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
+    std::optional<at::AutoDispatchBelowAutograd> below;  // (nothing is recorded: past the refusal of second derivatives)
+    if (!at::GradMode::is_enabled()) below.emplace();
     static const auto op = typed_op<decltype(group_norm_act_backward)>("flashim_amd::group_norm_act_backward");
     auto [dx, dw, db] = op.call(grads[0], saved[0], saved[3], ctx->saved_data["groups"].toInt(), as_optional(saved[1]),
                                 as_optional(saved[2]), ctx->saved_data["act"].toInt());
@@ -914,8 +916,20 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   }
 };
 
+// Whether an operator has anything to record: a node costs 2 us of host time
+template <typename... Tensors>
+bool records(const Tensors&... tensors) {
+  const auto one = [](const OptTensor& t) { return t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined()); };
+  return at::GradMode::is_enabled() && (one(tensors) || ...);
+}
+
 std::tuple<Tensor, Tensor> group_norm_act_autograd(const Tensor& x, int64_t groups, const OptTensor& weight,
                                                    const OptTensor& bias, double eps, int64_t act) {
+  if (!records(x, weight, bias)) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(group_norm_act)>("flashim_amd::group_norm_act");
+    return op.call(x, groups, weight, bias, eps, act);
+  }
   auto out = GroupNormAct::apply(x, groups, weight, bias, eps, act);
   return {out[0], out[1]};
 }
@@ -933,6 +947,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                                                  torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
+    std::optional<at::AutoDispatchBelowAutograd> below;  // (nothing is recorded: past the refusal of second derivatives)
+    if (!at::GradMode::is_enabled()) below.emplace();
     const bool want_x = ctx->needs_input_grad(0);
     const bool want_w = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const bool bias[2] = {saved[3].defined(), saved[4].defined()};
@@ -948,6 +964,11 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const OptTensor& b_gate,
                              const OptTensor& b_up, int64_t act) {
+  if (!records(x, w_gate, w_up, b_gate, b_up)) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(gated_linear)>("flashim_amd::gated_linear");
+    return op.call(x, w_gate, w_up, b_gate, b_up, act);
+  }
   return GatedLinear::apply(x, w_gate, w_up, b_gate, b_up, act);
 }
 
