@@ -84,6 +84,36 @@ def test_forward_and_gradients(m, k, h, dtype):
     _backward(x, wg, wu, bg, bu, act, d_out)
 
 
+NARROW = [  # backward in one pass: channels up to 64, hidden up to 256; one or two row blocks a step, steps past the last row
+    (1, 64, 256), (31, 64, 256), (32, 63, 255), (33, 64, 128), (63, 8, 129), (64, 64, 160), (65, 57, 31), (127, 64, 256),
+    (1000, 64, 96), (4097, 24, 200), (9000, 40, 128), (20011, 64, 256), (8191, 64, 64), (8300, 5, 33),
+]
+
+
+@pytest.mark.parametrize("m,k,h", NARROW)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_narrow_layers(m, k, h, dtype):
+    act = ("silu", "gelu", "gelu_tanh")[(m + k + h) % 3]
+    x, wg, wu, bg, bu, d_out = _inputs(m, k, h, dtype, bias=(None, F32, dtype)[(m + h) % 3], seed=m + k + h)
+    _forward(x, wg, wu, bg, bu, act)
+    _backward(x, wg, wu, bg, bu, act, d_out)
+
+
+@pytest.mark.parametrize("m,k,h", [(500, 64, 256), (500, 40, 100), (500, 72, 300)])
+@pytest.mark.parametrize("wanted", [(0,), (1, 2), (3, 4), (0, 3), (2,)])
+def test_wanted_gradients_alone_are_those_of_all(m, k, h, wanted):
+    tensors = [t.to(DEV) for t in _inputs(m, k, h, BF16, bias=F32, seed=9)]
+    d_out = tensors.pop()
+
+    def grads(which):
+        leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate(tensors)]
+        return torch.autograd.grad(ops.gated_linear(*leaves), [leaves[i] for i in which], d_out)
+
+    every = grads(range(5))
+    for i, got in zip(wanted, grads(wanted)):
+        assert torch.equal(got, every[i])
+
+
 LONG = [  # many rows of few channels: a last block of one row, odd widths, several hidden blocks, channels up to 128
     (32800, 64, 256), (32769, 33, 77), (33333, 8, 256), (40001, 40, 104), (36000, 64, 264), (33000, 100, 300),
     (32768, 128, 136), (35001, 127, 131),

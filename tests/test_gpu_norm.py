@@ -97,6 +97,44 @@ def test_forward_and_gradients(shape, groups, dtype):
     _backward(x, groups, w, b, 1e-5, act, d_out)
 
 
+SPLIT = [  # more than a workgroup's registers hold: groups of odd widths, one group, wide maps, a group that crosses loads
+    ((2, 70, 71, 12), 3), ((1, 9000, 5), 5), ((1, 5000, 3), 1), ((1, 1300, 999), 9), ((1, 900, 4099), 1), ((1, 330, 8192), 16),
+    ((3, 2100, 196), 14), ((1, 130, 131, 64), 32), ((17, 1023, 196), 14),
+]
+
+
+@pytest.mark.parametrize("shape,groups", SPLIT)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_split_maps(shape, groups, dtype):
+    x, w, b, d_out = _inputs(shape, dtype, seed=len(shape) + groups)
+    act = ("silu", "gelu", "gelu_tanh", "none")[shape[-1] % 4]
+    _forward(x, groups, w, b, 1e-5, act)
+    _backward(x, groups, w, b, 1e-5, act, d_out)
+
+
+@pytest.mark.parametrize("param", [BF16, F16, F32])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_activations_and_parameter_types_of_split_maps(act, param):
+    x, w, b, _ = _inputs((2, 5003, 48), BF16, param=param, seed=3)
+    _forward(x, 6, w, b, 1e-3, act)
+    _forward(x, 6, None, b, 1e-3, act)
+
+
+def test_split_maps_of_a_large_mean_and_of_single_nonfinite_values():
+    g = torch.Generator().manual_seed(10)
+    x = 100.0 + 0.1 * torch.randn(2, 20000, 32, generator=g)
+    _, w, b, _ = _inputs((1, 1, 32), F32)
+    _forward(x, 4, w, b, 1e-5, "none")
+    x = torch.randn(2, 20000, 32, generator=g)
+    clean = ops.group_norm_act(x.to(DEV), 4)
+    for bad in (math.nan, math.inf):
+        x[1, 19999, 9] = bad  # the second of four groups
+        got = ops.group_norm_act(x.to(DEV), 4)
+        assert got[1, :, 8:16].isnan().all()
+        got[1, :, 8:16] = clean[1, :, 8:16]
+        assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("params", ["both", "weight", "bias", "neither"])
 def test_activations_and_missing_parameters(act, params):
