@@ -12,10 +12,15 @@
 // (at most 2048 of them: a few kilobytes from the L2, less than another launch; beyond that a launch of its own does), so
 // results do not depend on the order of workgroups.
 //
-// Measured (MI355X): 200 million BF16 gradients into FP32 ones, norm 119 us (3.4 TB/s: the lines that the pass before has
-// written leave the Infinity Cache meanwhile; 69 us without them) and scaling 231 us (5.2 TB/s, a copy's rate; 310 us where a
-// lane wrote 32 bytes in two stores instead of 16 in one). 320 FP32 tensors of 22.6 million elements: 19 + 4 us, 6 us for the
-// total, 6 + 27 us, less than the host takes for 640 tensors (65 us). Ten tensors of 35000 elements: 4 + 4 us.
+// Scaling takes the gradients from the last one back, whose lines the norm's pass left in the Infinity Cache, and from 128 MB
+// marks its loads and stores as streams, which leave those lines there: 200 million BF16 gradients into FP32 ones, both launches,
+// 355 us forward and plain, 345 with the marked stores alone, 355 backward alone, 320 with both, 316 with marked loads too (and
+// with an optimizer's read of the outputs after it 799 -> 741 us); 320 FP32 tensors (181 MB) 69 -> 61 us. Smaller gradients fit
+// the cache and gain nothing; marked stores to unaligned lines cost them (4 million BF16: 5.8 -> 9.5 us).
+//
+// Measured (MI355X): 200 million BF16 gradients into FP32 ones, norm 69 us and scaling 235 us (5.1 TB/s, a copy's rate; 310 us
+// where a lane wrote 32 bytes in two stores instead of 16 in one). 320 FP32 tensors of 22.6 million elements: 19 + 4 us, 6 us
+// for the total, 6 + 27 us, as long as the host takes for 640 tensors. Ten tensors of 35000 elements: 4 + 4 us.
 #include <type_traits>
 
 #include "common.h"
@@ -24,6 +29,7 @@ namespace fim {
 
 constexpr int CLIP_T = 256;
 constexpr int CLIP_PARTIALS = 2048;   // partials that every workgroup of the scaling launch adds up itself
+constexpr int64_t CLIP_STREAM = 128 << 20;  // bytes of gradients and outputs from which scaling streams: half the Infinity Cache
 constexpr int64_t CLIP_ENTRY = 1 << 30;  // elements of one table entry: 32-bit indexing inside it
 
 template <int N, bool OUT>
@@ -166,8 +172,9 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float v, int dt) 
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
-// DO: the outputs' type. parts > 0: the total is added up here, and workgroup `writer` writes it; else it is read.
-template <int DT, int DO, typename R>
+// DO: the outputs' type. STREAM: loads and stores marked as not read again soon.
+// parts > 0: the total is added up here, and workgroup 0 writes it; else it is read.
+template <int DT, int DO, typename R, bool STREAM>
 __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, const double* __restrict__ part, int parts,
                                                             float* total, float max_norm, int writes_total) {
   constexpr bool HALF = DT != FIM_F32 && DO == FIM_F32;
@@ -180,7 +187,9 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
   const float scale = __builtin_elementwise_minimum(quotient, 1.0f);  // NaN stays NaN
   const int e = entry_of(t, blockIdx.x);
   if (scale == 1.0f && t.out[e] == t.in[e] && DT == DO) return;  // in place, unclipped: nothing changes
-  const uint32_t begin = (blockIdx.x - t.first[e]) * t.chunk;
+  // runs from the last one: what the norm's pass read last is still in the Infinity Cache
+  const uint32_t last = (e + 1 < (int)t.entries ? t.first[e + 1] : gridDim.x) - 1;
+  const uint32_t begin = (last - blockIdx.x) * t.chunk;
   const uint32_t n = t.n[e] - begin < t.chunk ? t.n[e] - begin : t.chunk;
   const uint8_t* p = static_cast<const uint8_t*>(t.in[e]) + (int64_t)begin * ES;
   uint8_t* q = static_cast<uint8_t*>(t.out[e]) + (int64_t)begin * EO;
@@ -195,7 +204,8 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
     In::unpack(r, f);
 #pragma unroll
     for (int k = 0; k < N; ++k) f[k] *= scale;
-    uint32_t w[N * EO / 4];
+    typedef uint32_t Out __attribute__((ext_vector_type(N * EO / 4)));
+    Out w;
     if constexpr (DO == FIM_F32) {
 #pragma unroll
       for (int k = 0; k < N; ++k) w[k] = f2u(f[k]);
@@ -206,15 +216,15 @@ __global__ __launch_bounds__(CLIP_T) void grad_scale_kernel(const ScaleTable t, 
                               : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * k]) |
                                     (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * k + 1]) << 16;
     }
-    uint8_t* to = q + (int64_t)(head + at * N) * EO;
-    if constexpr (N * EO == 8) *reinterpret_cast<uint2*>(to) = uint2{w[0], w[1]};
-    else *reinterpret_cast<uint4*>(to) = uint4{w[0], w[1], w[2], w[3]};
+    Out* to = reinterpret_cast<Out*>(q + (int64_t)(head + at * N) * EO);
+    if constexpr (STREAM) __builtin_nontemporal_store(w, to);
+    else *to = w;
   };
   uint32_t i = threadIdx.x;
   for (; i + (U - 1) * CLIP_T < vecs; i += U * CLIP_T) {
     V r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = v[i + u * CLIP_T];
+    for (int u = 0; u < U; ++u) r[u] = STREAM ? __builtin_nontemporal_load(v + i + u * CLIP_T) : v[i + u * CLIP_T];
 #pragma unroll
     for (int u = 0; u < U; ++u) put(i + u * CLIP_T, r[u]);
   }
@@ -274,7 +284,7 @@ static int64_t clip_parts(const Grads& g, uint32_t chunk) {
   return parts;
 }
 
-// launch(table, workgroups) over the tensors of types (in, out), a table at a time
+// launch(table, workgroups) over the tensors of types (in, out), a table at a time; those with outputs from the last one
 template <typename Table, typename Launch>
 static void for_tables(const Grads& g, int in_dtype, int out_dtype, uint32_t chunk, Launch&& launch) {
   Table t;
@@ -286,7 +296,8 @@ static void for_tables(const Grads& g, int in_dtype, int out_dtype, uint32_t chu
     t.entries = 0;
     wgs = 0;
   };
-  for (int64_t i = 0; i < g.count; ++i) {
+  for (int64_t j = 0; j < g.count; ++j) {
+    const int64_t i = Table::OUTPUTS ? g.count - 1 - j : j;
     if (g.in_dtype[i] != in_dtype || (Table::OUTPUTS && g.out_dtype[i] != out_dtype)) continue;
     for (int64_t at = 0; at < g.numel[i]; at += CLIP_ENTRY) {
       const uint32_t n = (uint32_t)(g.numel[i] - at < CLIP_ENTRY ? g.numel[i] - at : CLIP_ENTRY);
@@ -319,10 +330,14 @@ template <typename R>
 static void launch_scale(const Grads& g, uint32_t chunk, const double* part, int parts, float* total, float max_norm,
                          hipStream_t stream) {
   int writes = 1;
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < g.count; ++i) bytes += g.numel[i] * (clip_size(g.in_dtype[i]) + clip_size(g.out_dtype[i]));
+  const bool streams = bytes >= CLIP_STREAM;
   auto of_types = [&](auto dt, auto dout) {
     constexpr int DT = decltype(dt)::value, DO = decltype(dout)::value;
     for_tables<ScaleTable>(g, DT, DO, chunk, [&](const ScaleTable& t, uint32_t wgs) {
-      grad_scale_kernel<DT, DO, R><<<dim3(wgs), dim3(CLIP_T), 0, stream>>>(t, part, parts, total, max_norm, writes);
+      const auto kernel = streams ? grad_scale_kernel<DT, DO, R, true> : grad_scale_kernel<DT, DO, R, false>;
+      kernel<<<dim3(wgs), dim3(CLIP_T), 0, stream>>>(t, part, parts, total, max_norm, writes);
       writes = 0;
     });
   };

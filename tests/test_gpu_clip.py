@@ -78,6 +78,26 @@ def test_packed_views_at_odd_offsets(dtype, out_dtype):
     _check(list(before.split(sizes)), 0.5, 2.0, total, grads)
 
 
+@pytest.mark.parametrize("dtype, out_dtype", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F32), (F32, BF16)])
+def test_more_than_the_caches_hold(dtype, out_dtype):
+    """134 million bytes of gradients and outputs and more, in two launches' tables, packed at odd offsets."""
+    sizes = [1 + 2 * i for i in range(170)] + [9_000_001, 31, 5_500_007] + [17] * 40 + [8_000_003]
+    sizes += [13_000_009] if dtype != F32 or out_dtype != F32 else []
+    if dtype != F32 and out_dtype != F32:
+        sizes.append(9_000_013)
+    assert sum(sizes) * (dtype.itemsize + out_dtype.itemsize) > 1 << 27
+    bucket = torch.cat(_grads(sizes, (dtype,), seed=9)).to(DEV)
+    grads, cpu = list(bucket.split(sizes)), list(bucket.cpu().split(sizes))
+    memory = torch.full((sum(sizes) + 16,), 9.0, dtype=out_dtype, device=DEV)
+    out = list(memory[3:3 + sum(sizes)].split(sizes))
+    _check(cpu, 0.5, 2.0, ops.clip_grad_norm_(grads, 0.5, out=out), out)
+    assert (memory[:3] == 9).all() and (memory[3 + sum(sizes):] == 9).all()
+    assert torch.equal(bucket.cpu(), torch.cat(cpu))
+    aligned = list(memory[:sum(sizes)].split(sizes))
+    _check(cpu, 0.5, 2.0, ops.clip_grad_norm_(grads, 0.5, out=aligned), aligned)
+    _check(cpu, 0.5, 2.0, ops.clip_grad_norm_(grads, 0.5), grads)
+
+
 def test_layouts():
     """Dense tensors of any order are scaled in place; gaps of strided ones stay as they are."""
     g = torch.Generator().manual_seed(2)
