@@ -8,6 +8,7 @@
 //
 // A stream: x read once, the output written once. Measured (MI355X, BF16, SiLU): 320000 x 64 -> 256, 58 us (205 MB, 3.5 TB/s;
 // the vector work of the activation and the stores' way through LDS are 55% of it); 160000 x 128 -> 512, 62 us (98 on tiles).
+// Outputs are stored plainly: marked as streams, the product that read them next took 104 us in place of 97 with this one.
 #pragma once
 
 #include "gated_tile.h"

@@ -52,6 +52,11 @@ __device__ __forceinline__ float from16(uint16_t h) {
   return DT == FIM_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
+// A buffer access's bit for lines that are not read again soon (non-temporal): out and dx, written past the operands that the
+// other tiles still read (16384 x 1024 -> 2 x 4096 with its backward 1012 -> 1000 us, a product that reads `out` next takes as
+// long as before). dg and du are read next.
+constexpr int STREAM_BIT = 2;
+
 // FORWARD: out = act(g) u.  GRAD: the same products, out dg and du.  DX: dg Wg + du Wu.  DW: dg^T x and du^T x.
 enum { GATED_FORWARD, GATED_GRAD, GATED_DX, GATED_DW };
 
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
               typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
               const uint32_t at = (uint32_t)((32 * j + p * PER + prow) * a.ldo + slot * 8) * 2u;
               __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, run(p)), k ? o1 : o0,
-                                                     (int)(slot * 8 < cols_out ? at : TILE_OOB), 0, 0);
+                                                     (int)(slot * 8 < cols_out ? at : TILE_OOB), 0, MODE == GATED_GRAD ? 0 : STREAM_BIT);
             }
           } else if (whole && slot * 8 + 8 <= cols_out) {
             uint16_t* to = a.out[0] + (mw + 32 * j + prow) * a.ldo + nw + slot * 8;
