@@ -916,11 +916,15 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   }
 };
 
-// Whether an operator has anything to record: a node costs 2 us of host time
+// Whether an operator has anything to record, or a tangent to refuse (no_grad ends the recording, not forward mode): a node
+// costs 2 us of host time
 template <typename... Tensors>
 bool records(const Tensors&... tensors) {
-  const auto one = [](const OptTensor& t) { return t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined()); };
-  return at::GradMode::is_enabled() && (one(tensors) || ...);
+  const bool grads = at::GradMode::is_enabled();
+  const auto one = [grads](const OptTensor& t) {
+    return t && t->defined() && ((grads && t->requires_grad()) || torch::autograd::isFwGradDefined(*t));
+  };
+  return (one(tensors) || ...);
 }
 
 std::tuple<Tensor, Tensor> group_norm_act_autograd(const Tensor& x, int64_t groups, const OptTensor& weight,

@@ -8,6 +8,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 
 from flashim_amd import _lib, library, ops
 from flashim_amd.backends.hip import train as ht
@@ -123,6 +124,22 @@ def test_clip_counts_its_writes():
         y.sum().backward()
     with pytest.raises(NotImplementedError):  # no derivative through the clip
         torch.ops.flashim_amd.clip_grad_norm_([x], 1.0, 2.0)
+
+
+@pytest.mark.parametrize("grads", [True, False])
+def test_forward_mode_is_refused(grads):
+    """A tangent raises, under ``no_grad`` too: that ends the recording of gradients, not forward mode."""
+    x, w = torch.empty(3, 16, device="meta", dtype=torch.bfloat16), torch.empty(8, 16, device="meta", dtype=torch.bfloat16)
+    b = torch.empty(16, device="meta")
+    calls = [(lambda t: ht.group_norm_act(t, 4), x), (lambda t: ht.group_norm_act(x, 4, None, t), b),
+             (lambda t: ht.gated_linear(t, w, w), x), (lambda t: ht.gated_linear(x, w, t), w)]
+    with torch.set_grad_enabled(grads):
+        for call, t in calls:
+            with pytest.raises(RuntimeError):
+                torch.func.jvp(call, (t,), (torch.empty_like(t),))
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp is not implemented"):
+                call(forward_ad.make_dual(t, torch.empty_like(t)))
+            assert not call(t).requires_grad
 
 
 # -- refusals ------------------------------------------------------------------------------------------------------------
