@@ -851,11 +851,14 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch
 }
 
 // Clipping below autograd, the versions of what it wrote counted: as no_derivative and count_writes do for any operator, but
-// without boxing hundreds of tensors.
-void refuse_gradients(at::TensorList tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor& t : tensors)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");
+// without boxing hundreds of tensors. A tangent is refused whatever the mode: the tensor's values would change and its tangent
+// stay, or an output keep the tangent of what it held.
+void refuse_derivatives(at::TensorList tensors) {
+  const bool grads = at::GradMode::is_enabled();
+  for (const Tensor& t : tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!grads || !t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "clip_grad_norm_: no derivative, and a tensor has a tangent");
+  }
 }
 
 void count_writes_to(at::TensorList tensors) {
@@ -873,8 +876,8 @@ c10::TypedOperatorHandle<Signature> typed_op(const char* name) {
 }
 
 Tensor clip_grad_norm_out_autograd(at::TensorList grads, at::TensorList out, double max_norm, double norm_type) {
-  refuse_gradients(grads);
-  refuse_gradients(out);
+  refuse_derivatives(grads);
+  refuse_derivatives(out);
   static const auto op = typed_op<decltype(clip_grad_norm_out)>("flashim_amd::clip_grad_norm_out");
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor total = op.call(grads, out, max_norm, norm_type);
@@ -883,7 +886,7 @@ Tensor clip_grad_norm_out_autograd(at::TensorList grads, at::TensorList out, dou
 }
 
 Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double norm_type) {
-  refuse_gradients(grads);
+  refuse_derivatives(grads);
   static const auto op = typed_op<decltype(clip_grad_norm_)>("flashim_amd::clip_grad_norm_");
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor total = op.call(grads, max_norm, norm_type);

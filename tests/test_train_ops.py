@@ -142,6 +142,18 @@ def test_forward_mode_is_refused(grads):
             assert not call(t).requires_grad
 
 
+def test_clip_refuses_tangents():
+    """In place, a clipped gradient would keep its unclipped tangent."""
+    with forward_ad.dual_level():
+        plain = torch.empty(5, device="meta")
+        dual = forward_ad.make_dual(torch.empty(5, device="meta"), torch.empty(5, device="meta"))
+        for grads, out in (([plain, dual], None), ([dual], [torch.empty(5, device="meta")]), ([plain], [dual])):
+            for mode in (True, False):
+                with torch.set_grad_enabled(mode), pytest.raises(NotImplementedError, match="has a tangent"):
+                    ht.clip_grad_norm_(grads, 1.0, out=out)
+        assert plain._version == 0 and dual._version == 0
+
+
 # -- refusals ------------------------------------------------------------------------------------------------------------
 
 
