@@ -52,11 +52,12 @@ class GatedBlock(nn.Module):
 def train_step(module: nn.Module, optimizer: torch.optim.Optimizer, loss: Callable[[], Tensor],
                max_norm: float) -> tuple[Tensor, Tensor]:
     """One step: ``loss()`` and its gradients, clipped in place to a global norm of ``max_norm``. Returns the loss and the
-    norm before clipping, both on the GPU (nothing waits for it)."""
+    norm before clipping (0 where no parameter of ``module`` has a gradient), both on the GPU (nothing waits for it)."""
     optimizer.zero_grad(set_to_none=True)
     value = loss()
     value.backward()
-    norm = ops.clip_grad_norm_([p.grad for p in module.parameters() if p.grad is not None], max_norm)
+    grads = [p.grad for p in module.parameters() if p.grad is not None]
+    norm = ops.clip_grad_norm_(grads, max_norm) if grads else torch.zeros((), device=value.device)
     optimizer.step()
     return value.detach(), norm
 

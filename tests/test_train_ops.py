@@ -10,7 +10,7 @@ import torch.nn.functional as F
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
-from flashim_amd import _lib, library, ops
+from flashim_amd import _lib, gated, library, ops
 from flashim_amd.backends.hip import train as ht
 from oracle import train as ref
 
@@ -152,6 +152,14 @@ def test_clip_refuses_tangents():
                 with torch.set_grad_enabled(mode), pytest.raises(NotImplementedError, match="has a tangent"):
                     ht.clip_grad_norm_(grads, 1.0, out=out)
         assert plain._version == 0 and dual._version == 0
+
+
+def test_train_step_of_a_module_without_gradients():
+    """Frozen, beside a parameter that the loss also has: nothing to clip, and the other one still steps."""
+    module, other = torch.nn.Linear(3, 2).requires_grad_(False), torch.nn.Parameter(torch.ones(2))
+    loss, norm = gated.train_step(module, torch.optim.SGD([other], lr=0.5), lambda: (module(torch.ones(3)) * 0 + other).sum(), 1.0)
+    assert loss.item() == 2.0 and norm.shape == () and norm.dtype == torch.float32 and norm.item() == 0.0
+    assert torch.equal(other.detach(), torch.full((2,), 0.5))
 
 
 # -- refusals ------------------------------------------------------------------------------------------------------------
