@@ -355,6 +355,13 @@ __global__ __launch_bounds__(NORM_T, 4) void norm_stats_kernel(const NormArgs a)
   }
 }
 
+// 1 / deviation from the means of a group's deviations and of their squares. A NaN variance, as infinite values leave, stays NaN
+// (fmax would make it 0, and the group's finite values the activation of an infinity).
+__device__ __forceinline__ float deviation_inverse(double s1, double s2, float eps) {
+  const double var = s2 - s1 * s1;
+  return (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)eps));
+}
+
 // A workgroup adds up its image's partials: thread t takes group t % G of every (threads / G)th chunk, all loads at once,
 // about the first chunk's mean; then the threads of a group through LDS. to[g]: mean and 1 / deviation, or, BACKWARD, the
 // group's means of dz * weight and dz * weight * xhat.
@@ -391,7 +398,7 @@ __device__ __forceinline__ void merge_groups(const NormArgs& a, int b, float2* t
     s1 /= total;
     s2 /= total;
     to[g] = BACKWARD ? float2{(float)s1, (float)s2}
-                     : float2{(float)(centre + s1), (float)(1.0 / sqrt(fmax(s2 - s1 * s1, 0.0) + (double)a.eps))};
+                     : float2{(float)(centre + s1), deviation_inverse(s1, s2, a.eps)};
   }
   __syncthreads();
 }
@@ -422,7 +429,7 @@ __global__ __launch_bounds__(256) void norm_merge_kernel(const NormArgs a) {
   if ((threadIdx.x & 63) == 0)
     reinterpret_cast<float2*>(BACKWARD ? a.coef : a.stats)[bg] =
         BACKWARD ? float2{(float)s1, (float)s2}
-                 : float2{(float)(centre + s1), (float)(1.0 / sqrt(fmax(s2 - s1 * s1, 0.0) + (double)a.eps))};
+                 : float2{(float)(centre + s1), deviation_inverse(s1, s2, a.eps)};
 }
 
 // Forward, second pass.

@@ -135,6 +135,40 @@ def test_split_maps_of_a_large_mean_and_of_single_nonfinite_values():
         assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("groups", [8, 32])  # the second pass adds up the partials, and a launch of its own does
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+def test_nonfinite_values_anywhere_in_a_thread_s_pixels(act, bad, groups):
+    """Ten pixels a thread, of which the first four give the shift: a first one, one past the fourth, in the first, the last
+    but one and the last chunk. An infinity leaves no variance, whatever the mean: NaN in the whole group."""
+    g = torch.Generator(device=DEV).manual_seed(17)
+    x = torch.randn(2, 160000, 64, generator=g, device=DEV).to(BF16)
+    w, b = (t.to(DEV) for t in _inputs((1, 1, 64), F32)[1:3])
+    d = 64 // groups
+    clean = ops.group_norm_act(x, groups, w, b, activation=act)
+    for pixel in (0, 3 + 5 * 64, 254 * 625 + 1 + 7 * 64, 159999):
+        broken = x.clone()
+        broken[1, pixel, 2 * d + 1] = bad
+        got = ops.group_norm_act(broken, groups, w, b, activation=act)
+        assert got[1, :, 2 * d:3 * d].isnan().all(), pixel
+        got[1, :, 2 * d:3 * d] = clean[1, :, 2 * d:3 * d]
+        assert torch.equal(got, clean), pixel
+
+
+@pytest.mark.parametrize("pixels", [40, 20000])  # one launch, two
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_a_variance_past_fp32_is_infinite(act, pixels):
+    """Deviations of 1e25, whose squares FP32 does not hold: the normalized values are 0 at every map size."""
+    x, w, b, _ = (t.to(DEV) for t in _inputs((2, pixels, 32), F32, seed=18))
+    clean = ops.group_norm_act(x, 4, w, b, activation=act)
+    x[1, :, 8:16] *= 1e25
+    got = ops.group_norm_act(x, 4, w, b, activation=act)
+    flat = ops.group_norm_act(torch.zeros(1, 1, 32, device=DEV), 4, w, b, activation=act)  # a constant map: act(bias)
+    assert torch.equal(got[1, :, 8:16], flat[0, :, 8:16].expand(pixels, 8))
+    got[1, :, 8:16] = clean[1, :, 8:16]
+    assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("params", ["both", "weight", "bias", "neither"])
 def test_activations_and_missing_parameters(act, params):
