@@ -31,7 +31,7 @@ __device__ __forceinline__ float logistic(float z) {
 constexpr float kTanhA = 0.79788456080286535588f;  // sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
 
-// act(z), and act'(z) in `slope` where WITH_SLOPE. ReLU's slope at 0 is 0, as autograd has it.
+// act(z), and act'(z) in `slope` where WITH_SLOPE, as autograd has them: ReLU's slope is 0 at 0 and 1 at NaN, the others' NaN.
 //   SiLU: z s, s (1 + z (1 - s)) with s = logistic(z)
 //   GELU: z Phi(z) = max(z, 0) - |z| E, Phi(z) + z phi(z)
 //   GELU, tanh form: z s with s = logistic(2 y), y = a (z + b z^3) (0.5 (1 + tanh y) = s); s + z s (1 - s) 2 y'
@@ -41,7 +41,7 @@ __device__ __forceinline__ float activate(float z, float& slope) {
     if constexpr (WITH_SLOPE) slope = 1.0f;
     return z;
   } else if constexpr (ACT == ACT_RELU) {
-    if constexpr (WITH_SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (WITH_SLOPE) slope = z <= 0.0f ? 0.0f : 1.0f;
     return __builtin_elementwise_maximum(z, 0.0f);  // NaN stays NaN
   } else if constexpr (ACT == ACT_SILU) {
     const float s = logistic(z);
@@ -55,7 +55,8 @@ __device__ __forceinline__ float activate(float z, float& slope) {
     }
     return fmaf(-__builtin_elementwise_minimum(az, 3e38f), e, __builtin_elementwise_maximum(z, -0.0f));
   } else {
-    const float zc = __builtin_amdgcn_fmed3f(z, -1e4f, 1e4f), z2 = zc * zc;  // s is 0 or 1 long before: no inf times 0
+    // s is 0 or 1 long before the bounds: no inf times 0 (minimum and maximum keep a NaN, the median would not)
+    const float zc = __builtin_elementwise_minimum(__builtin_elementwise_maximum(z, -1e4f), 1e4f), z2 = zc * zc;
     const float s = logistic(2.0f * kTanhA * zc * fmaf(kTanhB, z2, 1.0f));
     if constexpr (WITH_SLOPE) slope = s * fmaf(zc * (1.0f - s), 2.0f * kTanhA * fmaf(3.0f * kTanhB, z2, 1.0f), 1.0f);
     return z * s;

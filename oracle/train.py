@@ -14,7 +14,7 @@ def activation(z: Tensor, act: str) -> tuple[Tensor, Tensor]:
     if act == "none":
         return z, torch.ones_like(z)
     if act == "relu":
-        return torch.maximum(z, torch.zeros_like(z)), (z > 0).to(z.dtype)
+        return torch.maximum(z, torch.zeros_like(z)), (~(z <= 0)).to(z.dtype)  # (1 at NaN, as autograd has it)
     if act == "silu":
         s = 1 / (1 + torch.exp(-z))
         return z * s, s * (1 + z * (1 - s))

@@ -11,6 +11,7 @@ import math
 
 import pytest
 import torch
+import torch.nn.functional as F
 
 from flashim_amd import ops
 from oracle import train as ref
@@ -18,6 +19,7 @@ from oracle import train as ref
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+ACTS = {"none": lambda z: z, "relu": F.relu, "silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh")}
 U = {BF16: 2.0**-8, F16: 2.0**-11, F32: 2.0**-24}
 TINY = {BF16: 1e-38, F16: 2.0**-25, F32: 1e-38}
 SUM = 2.0**-18
@@ -234,6 +236,23 @@ def test_nonfinite_rows_stay_in_their_row(m):
     assert torch.equal(out[keep], clean[keep]) and torch.isnan(out[5]).all()
     (dx,) = torch.autograd.grad(out, leaf, d_out)
     assert torch.isfinite(dx[keep]).all() and torch.isnan(dx[5]).all()
+
+
+@pytest.mark.parametrize("k,h", [(64, 96), (72, 87)])  # backward in one pass, on tiles
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_nan_biases_reach_their_gradients(act, k, h):
+    """A NaN in one gate's bias: NaN where autograd of the same formulas has it, ReLU's slope of 1 there included."""
+    x, wg, wu, bg, bu, d_out = _inputs(70, k, h, F16, bias=F32, seed=15)
+    bg[11] = math.nan
+    leaves = [t.double().requires_grad_() for t in (x, wg, wu, bg, bu)]
+    want = torch.autograd.grad(ACTS[act](F.linear(leaves[0], leaves[1], leaves[3])) * F.linear(leaves[0], leaves[2], leaves[4]),
+                               leaves, d_out.double())
+    leaves = [t.requires_grad_() for t in _dev(x, wg, wu, bg, bu)]
+    got = torch.autograd.grad(ops.gated_linear(*leaves, activation=act), leaves, d_out.to(DEV))
+    for name, t, v in zip(("x", "w_gate", "w_up", "b_gate", "b_up"), got, want):
+        assert torch.equal(t.isnan().cpu(), v.isnan()), name
+    # sums of 70 terms of about 0.25, each good to 2^-13 (the bound of _backward)
+    torch.testing.assert_close(got[3].double().cpu(), want[3], rtol=2e-3, atol=1e-2, equal_nan=True)
 
 
 def test_nonfinite_values_beside_a_view_are_not_read_into_it():

@@ -10,6 +10,7 @@ import math
 
 import pytest
 import torch
+import torch.nn.functional as F
 
 from flashim_amd import ops
 from oracle import train as ref
@@ -19,6 +20,7 @@ DEV = "cuda"
 U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
 TINY = {torch.bfloat16: 1e-38, torch.float16: 2.0**-25, torch.float32: 1e-38}  # half the smallest step of all
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+ACTS = {"none": lambda z: z, "relu": F.relu, "silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh")}
 
 
 def _inputs(shape, dtype, param=F32, seed=0, mean=0.5):
@@ -287,6 +289,22 @@ def test_nonfinite_values_stay_in_their_group(bad):
     assert torch.equal(out[~hit], clean[~hit]) and not torch.isfinite(out[hit]).any()
     (dx,) = torch.autograd.grad(out, leaf, d_out.to(DEV))
     assert torch.isfinite(dx[~hit]).all() and torch.isnan(dx[hit]).all()
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_nan_parameters_reach_their_gradients(act):
+    """A NaN in one channel's bias: NaN where autograd of the same formulas has it, ReLU's slope of 1 there included."""
+    x, w, b, d_out = _inputs((2, 40, 32), F32, seed=19)
+    b[9] = math.nan
+    leaves = [t.double().requires_grad_() for t in (x, w, b)]
+    rows = torch.group_norm(leaves[0].transpose(1, 2), 4, leaves[1], leaves[2]).transpose(1, 2)
+    want = torch.autograd.grad(ACTS[act](rows), leaves, d_out.double())
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(ops.group_norm_act(leaves[0], 4, leaves[1], leaves[2], activation=act), leaves, d_out.to(DEV))
+    assert act in ("none", "relu") or want[2].isnan().any()
+    for name, t, v in zip(("x", "weight", "bias"), got, want):
+        assert torch.equal(t.isnan().cpu(), v.isnan()), name
+        torch.testing.assert_close(t.double().cpu(), v, rtol=1e-4, atol=1e-4, equal_nan=True)
 
 
 def test_offsets_past_32_bits():
