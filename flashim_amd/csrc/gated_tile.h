@@ -267,7 +267,8 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
   };
 
   // accumulators: lane l, register q of block (i, j): row 32 j + l % 32, column 32 i + 8 (q / 4) + 4 h + q % 4; started at
-  // the bias (all its loads on one side of the branch on its type: one latency; columns past the end repeat the last)
+  // the bias (all its loads on one side of the branch on its type: one latency). Columns past the end read the last bias and
+  // start at 0: GRAD writes zeros there, and zero times an infinite bias is none
   v16f acc[NB][MB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
@@ -290,6 +291,10 @@ __global__ __launch_bounds__(256, MB * NB > 8 ? 1 : 2) void gated_tile_kernel(co
         for (int q = 0; q < 16; ++q) e[q] = static_cast<const uint16_t*>(b)[column(q)];
 #pragma unroll
         for (int q = 0; q < 16; ++q) first[q] = from16<DT>(e[q]);
+      }
+      if constexpr (MODE == GATED_GRAD) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) first[q] = c0 + 8 * (q >> 2) + (q & 3) < a.N ? first[q] : 0.0f;
       }
     }
 #pragma unroll

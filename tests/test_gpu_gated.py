@@ -255,6 +255,19 @@ def test_nan_biases_reach_their_gradients(act, k, h):
     torch.testing.assert_close(got[3].double().cpu(), want[3], rtol=2e-3, atol=1e-2, equal_nan=True)
 
 
+@pytest.mark.parametrize("k,h", [(64, 129), (72, 87), (200, 523)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_an_infinite_bias_of_the_last_column(k, h, dtype):
+    """dx is infinite with its sign, as the definition has it: the columns that pad the hidden width have no bias."""
+    x, wg, wu, bg, bu, d_out = _inputs(70, k, h, dtype, bias=F32, seed=16)
+    bu[-1] = math.inf
+    want = ref.gated_linear_gradients(d_out, x, wg, wu, bg, bu, "silu")["x"]
+    leaves = [t.requires_grad_() for t in _dev(x, wg, wu, bg, bu)]
+    (dx,) = torch.autograd.grad(ops.gated_linear(*leaves), leaves[:1], d_out.to(DEV))
+    sure = want.isinf()
+    assert sure.float().mean() > 0.9 and torch.equal(dx.double().cpu()[sure], want[sure])
+
+
 def test_nonfinite_values_beside_a_view_are_not_read_into_it():
     """The memory between a view's rows, and past its last one, holds NaN."""
     for k, h in ((72, 88), (71, 87)):
