@@ -58,6 +58,7 @@ struct NormArgs {
   int B, C, G, D;
   int chunks, chunk;    // chunks of an image, and their pixels
   int merged;           // stats (coef) were merged by a launch between the passes
+  int first;            // of the workgroups of a pass, the launch's first (launch_pass)
   float eps;
 };
 
@@ -186,10 +187,11 @@ struct Chunk {
   int b, i, pixels;
   int64_t begin;
 };
+__device__ __forceinline__ int block_of(const NormArgs& a) { return a.first + (int)blockIdx.x; }  // (below 2^31)
 __device__ __forceinline__ Chunk chunk_of(const NormArgs& a) {
   Chunk c;
-  c.b = blockIdx.x / a.chunks;
-  c.i = blockIdx.x - c.b * a.chunks;
+  c.b = (int)((uint32_t)block_of(a) / (uint32_t)a.chunks);
+  c.i = block_of(a) - c.b * a.chunks;
   c.begin = (int64_t)c.i * a.chunk;
   c.pixels = c.begin + a.chunk < a.P ? a.chunk : (int)(a.P - c.begin);
   return c;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(NORM_T, 4) void norm_stats_kernel(const NormArgs a)
     s2 = wave_sum(s2);
     const float m = s1 / ((float)ch.pixels * (float)a.D);
     if (lane == 0)
-      reinterpret_cast<float2*>(a.gpart)[(int64_t)blockIdx.x * a.G + g] = float2{lds2[g * a.D].x + m, fmaf(-m, s1, s2)};
+      reinterpret_cast<float2*>(a.gpart)[(int64_t)block_of(a) * a.G + g] = float2{lds2[g * a.D].x + m, fmaf(-m, s1, s2)};
   };
   if (parts > 1) {
     const int part = threadIdx.x / a.C, c = threadIdx.x - part * a.C;
@@ -406,7 +408,7 @@ __device__ __forceinline__ void merge_groups(const NormArgs& a, int b, float2* t
 // Between the passes, where an image's partials are many: one wavefront per (image, group), a row of partials a lane
 template <bool BACKWARD>
 __global__ __launch_bounds__(256) void norm_merge_kernel(const NormArgs a) {
-  const int64_t bg = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t bg = (int64_t)block_of(a) * 4 + (threadIdx.x >> 6);
   if (bg >= (int64_t)a.B * a.G) return;
   const int64_t b = bg / a.G;
   const float2* p = reinterpret_cast<const float2*>(a.gpart) + b * a.chunks * a.G + (bg - b * a.G);
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(NORM_T, 4) void norm_grad_sums_kernel(const NormArg
       s2 += lds2[r * a.C + c].y;
     }
     s2 *= a.stats[2 * ((int64_t)ch.b * a.G + c / a.D) + 1];
-    reinterpret_cast<float2*>(a.cpart)[(int64_t)blockIdx.x * a.C + c] = float2{s1, s2};
+    reinterpret_cast<float2*>(a.cpart)[(int64_t)block_of(a) * a.C + c] = float2{s1, s2};
     const float w = param(a.weight, a.wdt, c, 1.0f);
     lds2[c] = float2{s1 * w, s2 * w};
   }
@@ -662,7 +664,7 @@ __global__ __launch_bounds__(NORM_T, 4) void norm_grad_sums_kernel(const NormArg
     }
     t1 = wave_sum(t1);
     t2 = wave_sum(t2);
-    if (lane == 0) reinterpret_cast<float2*>(a.gpart)[(int64_t)blockIdx.x * a.G + g] = float2{t1, t2};
+    if (lane == 0) reinterpret_cast<float2*>(a.gpart)[(int64_t)block_of(a) * a.G + g] = float2{t1, t2};
   }
 }
 
@@ -697,8 +699,8 @@ template <int DT, int V, int ACT>
 __global__ __launch_bounds__(NORM_T, 4) void norm_grad_apply_kernel(const NormArgs a) {
   typedef Pack<DT, V> Pk;
   __shared__ float2 coef[NORM_MERGE_G];
-  if ((int)blockIdx.x >= a.B * a.chunks) {
-    norm_grad_params(a, blockIdx.x - a.B * a.chunks);
+  if (block_of(a) >= a.B * a.chunks) {
+    norm_grad_params(a, block_of(a) - a.B * a.chunks);
     return;
   }
   const Chunk ch = chunk_of(a);
@@ -815,6 +817,24 @@ static int norm_own_vector(const NormArgs& a, int v, int es) {
   return (int64_t)a.B * a.P * a.C * es <= NORM_SMALL ? v : 0;
 }
 
+// One pass of `blocks` workgroups: launch(arguments, grid), several times where there are more than a launch takes (2^32
+// threads; every image of a map has a workgroup at least)
+template <typename F>
+static void launch_pass(NormArgs a, int64_t blocks, F&& launch) {
+  constexpr int64_t MOST = 1 << 22;
+  for (int64_t first = 0; first < blocks; first += MOST) {
+    a.first = (int)first;
+    launch(a, dim3((unsigned)(blocks - first < MOST ? blocks - first : MOST)));
+  }
+}
+
+template <bool BACKWARD>
+static void launch_merge(const NormArgs& a, hipStream_t stream) {
+  launch_pass(a, cdiv((int64_t)a.B * a.G, 4), [&](const NormArgs& p, dim3 grid) {
+    norm_merge_kernel<BACKWARD><<<grid, dim3(256), 0, stream>>>(p);
+  });
+}
+
 // Sizes and chunks; false: too many
 static bool norm_shape(NormArgs& a, int64_t B, int64_t P, int64_t C, int64_t groups) {
   a.P = P;
@@ -863,7 +883,6 @@ extern "C" int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, in
   a.eps = eps;
   if (!norm_shape(a, B, P, C, groups)) return FIM_ERR_UNSUPPORTED;
   const int v = norm_vector(dtype, C, {stride_b, stride_p}, {x, out});
-  const dim3 grid((unsigned)(B * a.chunks));
   if (const int own = norm_own_vector(a, v, elem_size(dtype))) {
     with_vector(dtype, own, [&](auto dt, auto vec) {
       with_activation(act, [&](auto act_c) {
@@ -875,10 +894,14 @@ extern "C" int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, in
   }
   with_vector(dtype, v, [&](auto dt, auto vec) {
     constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
-    norm_stats_kernel<DT, V><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(a);
-    if (a.merged) norm_merge_kernel<false><<<dim3((unsigned)cdiv(B * groups, 4)), dim3(256), 0, stream>>>(a);
+    launch_pass(a, B * a.chunks, [&](const NormArgs& p, dim3 grid) {
+      norm_stats_kernel<DT, V><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(p);
+    });
+    if (a.merged) launch_merge<false>(a, stream);
     with_activation(act, [&](auto act_c) {
-      norm_apply_kernel<DT, V, decltype(act_c)::value><<<grid, dim3(NORM_T), 0, stream>>>(a);
+      launch_pass(a, B * a.chunks, [&](const NormArgs& p, dim3 grid) {
+        norm_apply_kernel<DT, V, decltype(act_c)::value><<<grid, dim3(NORM_T), 0, stream>>>(p);
+      });
     });
   });
   return launch_status();
@@ -918,9 +941,13 @@ extern "C" int fim_group_norm_backward(const void* x, const void* d_out, int dty
     constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
     with_activation(act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
-      norm_grad_sums_kernel<DT, V, ACT><<<dim3((unsigned)chunks), dim3(NORM_T), norm_lds(C, V), stream>>>(a);
-      if (a.merged) norm_merge_kernel<true><<<dim3((unsigned)cdiv(B * groups, 4)), dim3(256), 0, stream>>>(a);
-      norm_grad_apply_kernel<DT, V, ACT><<<dim3((unsigned)(chunks + params)), dim3(NORM_T), 0, stream>>>(a);
+      launch_pass(a, chunks, [&](const NormArgs& p, dim3 grid) {
+        norm_grad_sums_kernel<DT, V, ACT><<<grid, dim3(NORM_T), norm_lds(C, V), stream>>>(p);
+      });
+      if (a.merged) launch_merge<true>(a, stream);
+      launch_pass(a, chunks + params, [&](const NormArgs& p, dim3 grid) {
+        norm_grad_apply_kernel<DT, V, ACT><<<grid, dim3(NORM_T), 0, stream>>>(p);
+      });
     });
   });
   return launch_status();

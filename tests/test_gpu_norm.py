@@ -324,6 +324,29 @@ def test_offsets_past_32_bits():
     assert torch.equal(torch.autograd.grad(out, leaf, d)[0], torch.autograd.grad(want, dense, d_out.to(DEV))[0])
 
 
+def test_more_images_than_a_launch_has_workgroups():
+    """2^23 images and some: a workgroup each, and their partials' merge, take several launches. Spot images; the parameters'
+    gradients over all of them."""
+    n, w, b = 2**23 + 5, *_inputs((1, 1, 8), F32, seed=20)[1:3]
+    g = torch.Generator(device=DEV).manual_seed(21)
+    x, d_out = (torch.randn(n, 2, 8, generator=g, device=DEV, dtype=BF16) for _ in range(2))
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    out = ops.group_norm_act(leaves[0], 4, leaves[1], leaves[2], eps=0.01)
+    dx, dw, db = torch.autograd.grad(out, leaves, d_out)
+    at = torch.tensor([0, 1, 2**22 - 1, 2**22, 2**22 + 1, 2**23 - 1, 2**23, n - 1])
+    xs, ds = x[at.to(DEV)].cpu(), d_out[at.to(DEV)].cpu()
+    want = ref.group_norm_act(xs, 4, w, b, 0.01, "none")
+    _check(out[at.to(DEV)], want, _forward_bound(xs, 4, w, b, 0.01, want))
+    _check_gradients({"x": dx[at.to(DEV)]}, xs, 4, w, b, 0.01, "none", ds)
+    v = x.view(n, 2, 4, 2).double()
+    mean = v.mean(dim=(1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(((v - mean) ** 2).mean(dim=(1, 3), keepdim=True) + 0.01)
+    hat, d = ((v - mean) * rstd).view(-1, 8), d_out.view(-1, 8).double()
+    off = 2.0**-20 * ((v.abs() + mean.abs()) * rstd).view(-1, 8)  # of xhat
+    for got, terms, moved in ((dw, d * hat, d.abs() * off), (db, d, 0 * d)):
+        _check(got, terms.sum(0).cpu(), (moved.sum(0) + 2.0**-19 * terms.abs().sum(0)).cpu())
+
+
 def test_same_bits_every_time_and_on_another_stream():
     x, w, b, d_out = (t.to(DEV) for t in _inputs((2, 100, 90, 64), BF16, seed=13))
     leaf = x.requires_grad_()
