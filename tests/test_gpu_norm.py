@@ -347,6 +347,15 @@ def test_more_images_than_a_launch_has_workgroups():
         _check(got, terms.sum(0).cpu(), (moved.sum(0) + 2.0**-19 * terms.abs().sum(0)).cpu())
 
 
+@pytest.mark.parametrize("shape,groups", [((2, 700, 1024), 1024), ((3, 130, 1040), 520), ((1, 9000, 640), 640)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_than_512_groups(shape, groups, dtype):
+    """Their partials are merged by a launch of their own, in either direction."""
+    x, w, b, d_out = _inputs(shape, dtype, seed=groups)
+    _forward(x, groups, w, b, 1e-5, "silu")
+    _backward(x, groups, w, b, 1e-5, "silu", d_out)
+
+
 def test_same_bits_every_time_and_on_another_stream():
     x, w, b, d_out = (t.to(DEV) for t in _inputs((2, 100, 90, 64), BF16, seed=13))
     leaf = x.requires_grad_()
