@@ -86,6 +86,7 @@ PROBE_SIGNATURES: dict[str, list] = {
     "fim_test_bf16": [_vp, _i64, _vp, _vp],
     "fim_test_gelu": [_vp, _i64, _vp, _vp],
     "fim_test_deep_plan": [_i32] + [_i64] * 5 + [_i32] * 10 + [_vp],
+    "fim_test_gated_plan": [_i64] * 3 + [_vp],
 }
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -10,12 +10,9 @@
 // x's type (they are operands of 16-bit matrix products next; FP32 sums for the bias gradients are taken before that
 // rounding); then one product for dx over both halves and one for the weights, split over rows where its tiles are few.
 //
-// Four forms, chosen by sizes: up to 64 rows forward (gated_few.h), many rows of at most 128 channels forward (gated_rows.h),
-// backward of at most 64 channels and 256 hidden columns (gated_rows_grad.h), and tiles (gated_tile.h).
-#include "gated_few.h"
-#include "gated_rows.h"
-#include "gated_rows_grad.h"
-#include "gated_tile.h"
+// Four forms, chosen by sizes (gated_plan.h): up to 64 rows forward (gated_few.h), many rows of at most 128 channels forward
+// (gated_rows.h), backward of at most 64 channels and 256 hidden columns (gated_rows_grad.h), and tiles (gated_tile.h).
+#include "gated_plan.h"
 
 namespace fim {
 
@@ -127,159 +124,6 @@ __global__ __launch_bounds__(1024) void gated_bias_kernel(const float* col_sums,
 }
 
 // -- launches ----------------------------------------------------------------------------------------------------------
-
-static int64_t align256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-
-// A [rows, cols] operand as the caller has it
-struct Matrix {
-  const uint16_t* p;
-  int64_t ld, rows, cols;
-  // The tile kernels read 16-byte runs at 32-bit offsets inside a tile; other operands are copied first
-  bool as_is() const {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld >= cols && ld < (1 << 22);
-  }
-  int64_t padded() const { return cdiv(cols, 8) * 8; }
-  int64_t copy_bytes() const { return as_is() ? 0 : align256(rows * padded() * 2); }
-};
-
-static Matrix matrix(const void* p, int64_t ld, int64_t rows, int64_t cols) {
-  return {static_cast<const uint16_t*>(p), rows == 1 ? cols : ld, rows, cols};
-}
-
-struct Tile { int mb, nb; };
-
-// The time of a product of `rows` x `cols` outputs over `k` on a tile, in steps of a 128 x 128 tile (0.9 us). A round of 256
-// x 256 tiles, one per CU, measured 1.4 us a step and 9 us beside (prologue, epilogue); of 128 x 128 tiles, two per CU, which
-// read the operands twice as often but cover each other's prologue and epilogue, 0.9 us and 3 us. (16384 x 1024 x 8192
-// outputs: 256 against 273 us; 20000 x 512 x 4096: 104 against 98; 16384 x 8192 x 1024: 227 against 310.)
-static double tile_time(Tile t, int64_t rows, int64_t cols, int64_t splits, int64_t k) {
-  const int64_t cus = device_cus(), size = 64 * t.mb;
-  const int64_t rounds = cdiv(cdiv(rows, size) * cdiv(cols, size) * splits, cus);
-  const double steps = (double)cdiv(k, TILE_K);
-  // (a last small tile alone on its CU takes more than half the time of two)
-  return t.mb == 4 ? rounds * (1.6 * steps + 10.0) : (0.5 * rounds + 0.1 * (rounds & 1)) * (steps + 3.0);
-}
-
-static Tile gated_tile(int64_t rows, int64_t cols, int64_t k) {
-  const Tile large{4, 4}, small{2, 2};
-  return tile_time(large, rows, cols, 1, k) < tile_time(small, rows, cols, 1, k) ? large : small;
-}
-
-struct Splits {
-  Tile tile;
-  int64_t n;
-};
-
-// Tile and splits of the contraction of `cols` x `rows` outputs over k, where splits are joined (their FP32 partials written
-// and read once, at 4.5 TB/s, and a launch); `alone`: one split needs no join
-static Splits split_plan(int64_t rows, int64_t cols, int64_t k, bool alone) {
-  Splits best{{2, 2}, 0};
-  double best_time = 0.0;
-  for (const Tile t : {Tile{4, 4}, Tile{2, 2}}) {
-    for (int64_t s = 1; s <= 256 && (s == 1 || k / s >= 256); s += s < 8 ? 1 : s / 4) {
-      const double join = s == 1 && alone ? 0.0 : (double)(s + 1) * rows * cols * 4.0 / 4.5e6 + 3.0;  // us
-      const double time = 0.9 * tile_time(t, rows, cols, s, cdiv(k, s)) + join;
-      if (best.n != 0 && time >= best_time) continue;
-      best_time = time;
-      best = {t, s};
-    }
-  }
-  return best;
-}
-
-// Whether the forward pass is a stream of rows (gated_rows.h): a short contraction and enough rows for the wavefronts of half
-// the CUs. (On rows and on tiles: 24000 x 64 -> 256, 13.3 and 12.0 us; 40000: 15.6 and 14.4; 80000: 23.5 and 30.1; 32768 x 128
-// -> 512: 22.1 and 22.3; 160000: 61.6 and 97.7.)
-static bool gated_rows(int64_t M, int64_t K) { return K <= 128 && M >= 32 * ROWS_WAVES * (int64_t)device_cus() / 2; }
-
-// Whether the backward pass is (gated_rows_grad.h): all weights fit one workgroup's LDS, any number of rows. (1000 x 64 -> 256:
-// 15 us, 24 on tiles; 24000: 32 and 37; 320000: 158 and 241.)
-static bool gated_rows_grad(int64_t K, int64_t H) { return K <= 64 && H <= GRAD_HIDDEN; }
-
-static int64_t rows_blocks(int64_t K, int64_t H) { return cdiv(H, rows_hidden(K <= 64 ? 64 : 128)); }
-
-// Workgroups per hidden block: one per CU over all blocks
-static int64_t rows_groups(int64_t M, int64_t K, int64_t H) {
-  const int64_t most = cdiv(M, 32 * ROWS_WAVES), n = device_cus() / rows_blocks(K, H);
-  return n < 1 ? 1 : n < most ? n : most;
-}
-
-// Workgroups of a backward pass by rows: one per CU at most, fewer where the steps saved (3.7 us each) would cost less than the
-// partial weight gradients they leave (written, then joined, at 5 TB/s)
-static int64_t rows_grad_groups(int64_t M, int64_t K, int64_t H) {
-  const int64_t steps = cdiv(M, 32 * rows_grad_sub(H));
-  const double part = rows_grad_sub(H) * 2.0 * H * K * 4 * 2 / 5e6;  // us
-  int64_t best = 0;
-  double best_time = 0.0;
-  for (int64_t rounds = cdiv(steps, device_cus()), i = 0; i < 16; ++rounds, ++i) {
-    const int64_t groups = cdiv(steps, rounds);
-    const double time = 3.7 * rounds + part * groups;
-    if (best != 0 && time >= best_time) continue;
-    best_time = time;
-    best = groups;
-  }
-  return best;
-}
-
-struct Gated {
-  Matrix x, wg, wu;
-  int64_t M, K, H;
-  // workspace, in bytes: copies of the operands; backward: dg and du [M, hp], bias partials, weight partials
-  int64_t x_at, wg_at, wu_at, dgu_at, cols_at, part_at, total;
-  int64_t hp, ldg, sum_rows;
-  int64_t dw_splits, dw_rows, dx_splits, dx_steps;  // splits, and what each contracts over
-  Tile grad, dw, dx;
-  bool rows;  // backward by rows: no dg, du in memory
-};
-
-static Gated gated_plan(const Matrix& x, const Matrix& wg, const Matrix& wu, bool backward) {
-  Gated g{};
-  g.x = x;
-  g.wg = wg;
-  g.wu = wu;
-  g.M = x.rows;
-  g.K = x.cols;
-  g.H = wg.rows;
-  // both weights are read with one stride
-  const bool copy_w = !wg.as_is() || !wu.as_is() || wg.ld != wu.ld;
-  g.x_at = 0;
-  if (!backward && g.M <= FEW_ROWS) return g;  // any rows are read in place
-  g.wg_at = g.x_at + x.copy_bytes();
-  g.wu_at = g.wg_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
-  g.total = g.wu_at + (copy_w ? align256(g.H * wg.padded() * 2) : 0);
-  g.hp = cdiv(g.H, 8) * 8;
-  // whole 128-byte lines, one more than fit: rows of a power of two apart would meet in the same cache sets and channels
-  g.ldg = cdiv(g.H, 64) * 64 + 64;
-  if (!backward) return g;
-  g.dgu_at = g.total;
-  g.rows = gated_rows_grad(g.K, g.H);
-  if (g.rows) {
-    g.sum_rows = g.dw_splits = rows_grad_groups(g.M, g.K, g.H) * rows_grad_sub(g.H);
-    g.cols_at = g.dgu_at;
-    g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
-    g.total = g.part_at + align256(g.dw_splits * 2 * g.H * g.K * 4);
-    return g;
-  }
-  g.grad = {2, 2};  // (its epilogue has no registers left beside 256 x 256 accumulators)
-  g.cols_at = g.dgu_at + align256(2 * g.M * g.ldg * 2);
-  g.sum_rows = 2 * cdiv(g.M, 64 * g.grad.mb);
-  g.part_at = g.cols_at + align256(g.sum_rows * 2 * g.H * 4);
-  // (the weights' gradients have both halves' tiles)
-  const Splits dw = split_plan(g.K, 2 * cdiv(g.H, 128) * 128, g.M, false);
-  g.dw = dw.tile;
-  g.dw_rows = cdiv(cdiv(g.M, dw.n), TILE_K) * TILE_K;
-  g.dw_splits = cdiv(g.M, g.dw_rows);
-  const int64_t steps = 2 * cdiv(g.H, TILE_K);
-  const Splits dx = split_plan(g.M, g.K, steps * TILE_K, true);
-  g.dx = dx.tile;
-  g.dx_steps = cdiv(steps, dx.n);
-  g.dx_splits = cdiv(steps, g.dx_steps);
-  // one area for both products' partials, one after the other
-  const int64_t dw_bytes = g.dw_splits * 2 * g.H * g.K * 4;
-  const int64_t dx_bytes = g.dx_splits == 1 ? 0 : g.dx_splits * g.M * g.K * 4;
-  g.total = g.part_at + align256(dw_bytes > dx_bytes ? dw_bytes : dx_bytes);
-  return g;
-}
 
 // Copies what has to be copied; g.x, g.wg and g.wu are readable by the tiles afterwards
 static void gated_operands(Gated& g, uint8_t* ws, hipStream_t stream) {
@@ -450,7 +294,7 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || out == nullptr) return FIM_ERR_INVALID;
   Gated g = gated_plan(matrix(x, x_stride, M, K), matrix(w_gate, w_gate_stride, H, K), matrix(w_up, w_up_stride, H, K), false);
   if (g.total > 0 && (workspace == nullptr || workspace_bytes < g.total)) return FIM_ERR_INVALID;
-  if (M <= FEW_ROWS) {
+  if (g.form == FORM_FEW) {
     FewArgs f{};
     f.x = g.x.p;
     f.w[0] = g.wg.p;
@@ -482,12 +326,11 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   a.out[0] = static_cast<uint16_t*>(out);
   a.ldo = a.out_cols = H;
   a.wide_out = rows_wide(out, H);
-  const Tile tile = gated_tile(M, 2 * H, K);
   with_type(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     with_activation(act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
-      if (!gated_rows(M, K)) launch_product<DT, GATED_FORWARD, ACT>(a, tile, 1, stream);
+      if (g.form == FORM_TILES) launch_product<DT, GATED_FORWARD, ACT>(a, g.forward, 1, stream);
       else if (K <= 64) launch_rows<DT, ACT, 64>(rows_args(a, K), a.wide_out, stream);
       else launch_rows<DT, ACT, 128>(rows_args(a, K), a.wide_out, stream);
     });

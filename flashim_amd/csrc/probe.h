@@ -36,6 +36,11 @@ int fim_test_mfma_peak(int kind, int64_t blocks, int iters, float* out, hipStrea
 int fim_test_deep_plan(int kind, int64_t B, int64_t H, int64_t W, int64_t Cin, int64_t Cout, int kh, int kw, int sh, int sw,
                        int ph, int pw, int dh, int dw, int out_mode, int residual, int* plan);
 
+/* The gated product's plan for packed operands (gated_plan.h): plan = {form of the forward pass (0: few rows, 1: rows, 2:
+ * tiles), 64-row blocks of its tile, backward in one pass by rows, blocks of dx's tile, its splits, blocks of the weights'
+ * gradients' tile, its splits}. Runs on the host only. */
+int fim_test_gated_plan(int64_t M, int64_t K, int64_t H, int* plan);
+
 #ifdef __cplusplus
 }
 #endif

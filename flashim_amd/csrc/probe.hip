@@ -4,6 +4,7 @@
 // quoted against). Declarations: probe.h.
 #include "common.h"
 #include "deep_plan.h"
+#include "gated_plan.h"
 #include "probe.h"
 
 namespace fim {
@@ -145,6 +146,16 @@ int fim_test_deep_plan(int kind, int64_t B, int64_t H, int64_t W, int64_t Cin, i
   }
   const DeepPlan p = deep_plan(a, kind);
   plan[0] = p.wn; plan[1] = p.mbw; plan[2] = p.rag; plan[3] = p.two;
+  return FIM_OK;
+}
+
+int fim_test_gated_plan(int64_t M, int64_t K, int64_t H, int* plan) {
+  if (plan == nullptr || M <= 0 || K <= 0 || H <= 0) return FIM_ERR_INVALID;
+  const void* at = reinterpret_cast<const void*>(4096);  // only the alignment is looked at
+  const Matrix x = matrix(at, K, M, K), w = matrix(at, K, H, K);
+  const Gated f = gated_plan(x, w, w, false), b = gated_plan(x, w, w, true);
+  plan[0] = f.form; plan[1] = f.forward.mb; plan[2] = b.rows;
+  plan[3] = b.dx.mb; plan[4] = (int)b.dx_splits; plan[5] = b.dw.mb; plan[6] = (int)b.dw_splits;
   return FIM_OK;
 }
 

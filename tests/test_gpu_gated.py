@@ -7,13 +7,14 @@ next product: independent errors of at most u of a term, so a sum of them stays 
 terms' squares (six standard deviations), beside the FP32 sum and the final rounding. Bias gradients are sums of unrounded
 values."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 import torch.nn.functional as F
 
-from flashim_amd import ops
+from flashim_amd import _lib, ops
 from oracle import train as ref
 
 pytestmark = pytest.mark.gpu
@@ -68,6 +69,17 @@ def _backward(x, wg, wu, bg, bu, act, d_out):
             n = x.shape[0] if name != "x" else 2 * wg.shape[0]
             bound = bound + 6 / math.sqrt(3) * (u * want[name + "_squares"] + TINY[x.dtype] * scale * n**0.5)
         _check(name, got, want[name], bound)
+
+
+FEW, ROWS, TILES = range(3)  # forms of the forward pass
+
+
+def plan(m, k, h):
+    """Form of the forward pass, blocks of its tile, backward in one pass, blocks of dx's tile, its splits, blocks of the
+    weights' tile, its splits."""
+    out = (ctypes.c_int * 7)()
+    _lib.probe_call("fim_test_gated_plan", m, k, h, ctypes.addressof(out))
+    return tuple(out)
 
 
 SHAPES = [  # rows, channels, hidden: single values, one row, odd and prime sizes, tile edges, several tiles each way
@@ -129,6 +141,20 @@ def test_many_rows_of_few_channels(m, k, h, dtype):
     x, wg, wu, bg, bu, d_out = _inputs(m, k, h, dtype, bias=(None, F32, dtype)[(m + h) % 3], seed=m + k + h)
     _forward(x, wg, wu, bg, bu, act)
     _backward(x, wg, wu, bg, bu, act, d_out)
+
+
+ROWS_SHAPES = [  # the forward pass by rows: a last block of one row, odd widths, hidden blocks that end inside, few rows of many
+    (40001, 64, 256), (40003, 33, 77), (41000, 8, 255), (20100, 40, 520), (8300, 64, 1240), (160001, 100, 60), (80100, 128, 264),
+    (9100, 127, 2300),
+]
+
+
+@pytest.mark.parametrize("m,k,h", ROWS_SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_forward_by_rows(m, k, h, dtype):
+    assert plan(m, k, h)[0] == ROWS
+    x, wg, wu, bg, bu, _ = _inputs(m, k, h, dtype, bias=(None, F32, dtype)[(m + h) % 3], seed=m + k + h)
+    _forward(x, wg, wu, bg, bu, ("silu", "gelu", "gelu_tanh")[(m + k + h) % 3])
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
