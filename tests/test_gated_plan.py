@@ -3,7 +3,7 @@ measured, and the forms and tiles that the GPU tests' shapes are there for."""
 
 import pytest
 
-from tests.test_gpu_gated import FEW, ROWS, ROWS_SHAPES, TILES, plan
+from tests.test_gpu_gated import FEW, LARGE_TILES, ROWS, ROWS_SHAPES, TILES, plan
 
 # rows x channels -> hidden columns, on either side of the rule where the two forms were measured 3% and more apart
 FASTER = {
@@ -24,3 +24,5 @@ def test_forward_form(form):
 def test_shapes_of_the_gpu_tests():
     for shape in ROWS_SHAPES:
         assert plan(*shape)[0] == ROWS, shape
+    for shape, fields in LARGE_TILES.items():
+        assert all(plan(*shape)[i] == v for i, v in fields.items()), shape

@@ -157,6 +157,34 @@ def test_forward_by_rows(m, k, h, dtype):
     _forward(x, wg, wu, bg, bu, ("silu", "gelu", "gelu_tanh")[(m + k + h) % 3])
 
 
+LARGE_TILES = {  # 256 x 256 tiles, by what takes them (the plan's fields): odd sizes and sizes of whole 16-byte rows
+    (3001, 1031, 2053): {1: 4, 5: 4, 6: 3},        # forward; weights in three splits
+    (3000, 776, 2056): {1: 4},
+    (4101, 1031, 2051): {3: 4, 4: 3, 5: 4, 6: 3},  # dx and weights in three splits
+    (4100, 1032, 2056): {3: 4, 4: 3, 5: 4, 6: 3},
+    (8201, 1541, 523): {3: 4, 4: 1},               # dx whole
+    (8200, 1544, 520): {3: 4, 4: 1},
+}
+
+
+@pytest.mark.parametrize("m,k,h", LARGE_TILES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_tiles(m, k, h, dtype):
+    chosen = plan(m, k, h)
+    assert chosen[0] == TILES and all(chosen[i] == v for i, v in LARGE_TILES[m, k, h].items())
+    act = ("silu", "gelu", "gelu_tanh")[(m + k + h) % 3]
+    x, wg, wu, bg, bu, d_out = _inputs(m, k, h, dtype, bias=(None, F32, dtype)[(m + h) % 3], seed=m + k + h)
+    _forward(x, wg, wu, bg, bu, act)
+    _backward(x, wg, wu, bg, bu, act, d_out)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_large_tiles_of_every_activation(act):
+    x, wg, wu, bg, bu, _ = _inputs(3001, 777, 2053, BF16, bias=BF16, seed=17)
+    assert plan(3001, 777, 2053)[1] == 4
+    _forward(x, wg, wu, bg, bu, act)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("bias", [None, "gate", "up", BF16, F32])
 @pytest.mark.parametrize("m", [5, 200])
