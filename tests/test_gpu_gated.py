@@ -377,6 +377,40 @@ def test_many_rows():
            + 6 / math.sqrt(3) * U[BF16] * grads["x_squares"])
 
 
+def test_many_rows_on_tiles():
+    """Backward on tiles with dg and du of more than 4 GB each: spot rows of dx, and the gradients over all rows against
+    float64 on the GPU, in parts."""
+    m, k, h, part = 5_700_001, 72, 264, 300_000
+    assert not plan(m, k, h)[2] and 2 * m * h > 2**31
+    g = torch.Generator(device=DEV).manual_seed(18)
+    x = torch.randn(m, k, generator=g, device=DEV, dtype=BF16)
+    wg, wu = ((torch.randn(h, k, generator=g, device=DEV) * k**-0.5).to(BF16) for _ in range(2))
+    bg, bu = (0.5 * torch.randn(h, generator=g, device=DEV) for _ in range(2))
+    d_out = torch.randn(m, h, generator=g, device=DEV, dtype=BF16)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    names = ("x", "w_gate", "w_up", "b_gate", "b_up")
+    got = dict(zip(names, torch.autograd.grad(ops.gated_linear(*leaves), leaves, d_out)))
+    tensors = [t.detach() for t in leaves]
+    pre = SUM * (4 * k**0.5 + 4)
+    at = torch.tensor([0, 127, 128, 2**21 + 5, 2**22 - 1, 2**22, 5_592_405, 5_592_406, m - 2, m - 1], device=DEV)
+    want = ref.gated_linear_gradients(d_out[at].cpu(), x.detach()[at].cpu(), *(t.cpu() for t in tensors[1:]), "silu")
+    _check("dx", got["x"][at], want["x"], U[BF16] * want["x"].abs() + (SUM + pre) * want["x_terms"]
+           + 6 / math.sqrt(3) * U[BF16] * want["x_squares"])
+    sums = {}
+    for i in range(0, m, part):
+        r = ref.gated_linear_gradients(d_out[i:i + part], tensors[0][i:i + part], *tensors[1:], "silu")
+        for name, v in r.items():
+            if name[0] != "x":
+                v = v.square() if name.endswith("squares") else v
+                sums[name] = v if i == 0 else sums[name] + v
+    for name in names[1:]:
+        want, terms = sums[name].cpu(), sums[name + "_terms"].cpu()
+        bound = U[got[name].dtype] * want.abs() + (SUM + pre) * terms
+        if name[0] == "w":
+            bound = bound + 6 / math.sqrt(3) * U[BF16] * sums[name + "_squares"].sqrt().cpu()
+        _check(name, got[name], want, bound)
+
+
 def test_same_bits_every_time_and_on_another_stream():
     x, wg, wu, bg, bu, d_out = _dev(*_inputs(3000, 200, 264, BF16, bias=F32, seed=11))
     leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
