@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -855,9 +856,12 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch
 // stay, or an output keep the tangent of what it held.
 void refuse_derivatives(at::TensorList tensors) {
   const bool grads = at::GradMode::is_enabled();
+  const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // (no level, no tangents: one look, not one a tensor)
+  if (!grads && !tangents) return;
   for (const Tensor& t : tensors) {
     TORCH_CHECK_NOT_IMPLEMENTED(!grads || !t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "clip_grad_norm_: no derivative, and a tensor has a tangent");
+    TORCH_CHECK_NOT_IMPLEMENTED(!tangents || !torch::autograd::isFwGradDefined(t),
+                                "clip_grad_norm_: no derivative, and a tensor has a tangent");
   }
 }
 
