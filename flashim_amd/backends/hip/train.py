@@ -28,7 +28,8 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Tensor | None = None, bia
                    eps: float = 1e-5, activation: str = "none") -> Tensor:
     """``act((x - mean) / sqrt(var + eps) * weight + bias)`` of a channels-last ``x`` ``[B, ..., C]``, mean and biased
     variance over the pixels and the ``C / num_groups`` channels of each (image, group). ``weight`` and ``bias`` ``[C]``
-    in any float type; FP32 arithmetic, rounded once to ``x``'s type. Differentiable in ``x``, ``weight`` and ``bias``."""
+    in any float type; FP32 arithmetic, rounded once to ``x``'s type. A group with an infinity is NaN. Differentiable in
+    ``x``, ``weight`` and ``bias``; second and forward-mode derivatives raise, here and in ``gated_linear``."""
     return library.group_norm_act(x, num_groups, weight, bias, eps, ACTIVATIONS[activation])[0]
 
 

@@ -31,8 +31,9 @@ struct Tile { int mb, nb; };
 
 // The time of a product of `rows` x `cols` outputs over `k` on a tile, in steps of a 128 x 128 tile (0.9 us). A round of 256
 // x 256 tiles, one per CU, measured 1.4 us a step and 9 us beside (prologue, epilogue); of 128 x 128 tiles, two per CU, which
-// read the operands twice as often but cover each other's prologue and epilogue, 0.9 us and 3 us. (16384 x 1024 x 8192
-// outputs: 256 against 273 us; 20000 x 512 x 4096: 104 against 98; 16384 x 8192 x 1024: 227 against 310.)
+// read the operands twice as often but cover each other's prologue and epilogue, 0.9 us and 3 us. (Large and small, 16384 x
+// 1024 x 8192 outputs: 255 and 280 us; 20000 x 512 x 4096, which the estimate gives to the small ones: 99 and 101 with GELU, 90 and
+// 94 with SiLU; 16384 x 8192 x 1024: 208 and 287, in FP16 237 and 292.)
 inline double tile_time(Tile t, int64_t rows, int64_t cols, int64_t splits, int64_t k) {
   const int64_t cus = device_cus(), size = 64 * t.mb;
   const int64_t rounds = cdiv(cdiv(rows, size) * cdiv(cols, size) * splits, cus);
@@ -68,8 +69,8 @@ inline Splits split_plan(int64_t rows, int64_t cols, int64_t k, bool alone) {
   return best;
 }
 
-// Whether the backward pass is (gated_rows_grad.h): all weights fit one workgroup's LDS, any number of rows. (1000 x 64 -> 256:
-// 15 us, 24 on tiles; 24000: 32 and 37; 320000: 158 and 241.)
+// Whether the backward pass is (gated_rows_grad.h): all weights fit one workgroup's LDS, any number of rows. (Kernels of a call,
+// 1000 x 64 -> 256: 20 us, 29 on tiles; 24000: 38 and 45; 320000: 156 and 337.)
 inline bool gated_rows_grad(int64_t K, int64_t H) { return K <= 64 && H <= GRAD_HIDDEN; }
 
 // Hidden columns of a block of the forward pass by rows

@@ -6,8 +6,9 @@
 // works, multiplies them by 32 hidden columns at a time, and writes whole 128-byte lines through its own LDS area. No barrier
 // after the weights are in; the wavefronts of a SIMD drift apart, one's vector work covers another's loads.
 //
-// A stream: x read once, the output written once. Measured (MI355X, BF16, SiLU): 320000 x 64 -> 256, 58 us (205 MB, 3.5 TB/s;
-// the vector work of the activation and the stores' way through LDS are 55% of it); 160000 x 128 -> 512, 62 us (98 on tiles).
+// A stream: x read once, the output written once. Measured (device time, MI355X, BF16, SiLU): 320000 x 64 -> 256, 48 us (77 on
+// tiles; 205 MB, 4.3 TB/s; 58 us in the first calls after a pause; the vector work of the activation and the stores' way through
+// LDS are 55% of it); 160000 x 128 -> 512, 64 us (82 on tiles).
 // Outputs are stored plainly: marked as streams, the product that read them next took 104 us in place of 97 with this one.
 #pragma once
 

@@ -1,16 +1,17 @@
 // The backward pass of the gated feed-forward operator over many rows, of at most 64 channels and 256 hidden columns: one
 // pass over x and dout that leaves dx and each workgroup's partial sums of the weights' and biases' gradients.
 //
-// dg and du never leave the CU (written and read again they were 0.6 of the bytes moved: 320000 x 64 -> 256 took 144 us for
-// dg, du and dx, 85 us for the weights' gradients and 7 + 5 us for joins). A workgroup keeps all weights in LDS and takes 32
-// rows at a time (64 where H is at most 128). Each of its eight wavefronts owns 32 hidden columns: it multiplies them,
-// applies the epilogue, adds its dg^T x and du^T x to accumulators that stay in registers for the whole launch, and its
-// column sums too. dg and du go to LDS in 16 bits (operands of 16-bit products, as everywhere in this operator); after one
-// barrier each wavefront takes a 16 x 16 tile of dx, contracted over all of them. With two LDS copies of dg, du and x that is
-// the only barrier of a step: a wavefront writes the next step's while others still read this one's.
+// dg and du never leave the CU: written and read again they were 0.6 of the bytes moved (320000 x 64 -> 256 with its joins, in turn:
+// 156 us, 337 us on tiles). A workgroup keeps all weights in LDS and takes 32 rows at a time (64 where H is at most 128). Each of
+// its eight wavefronts owns 32 hidden columns: it multiplies them, applies the epilogue, adds its dg^T x and du^T x to
+// accumulators that stay in registers for the whole launch, and its column sums too. dg and du go to LDS in 16 bits (operands of
+// 16-bit products, as everywhere in this operator); after one barrier each wavefront takes a 16 x 16 tile of dx, contracted over
+// all of them. With two LDS copies of dg, du and x that is the only barrier of a step: a wavefront writes the next step's while
+// others still read this one's.
 //
-// Measured (MI355X, BF16, SiLU): 320000 x 64 -> 256, 144 us (246 MB are 48 us): vector work 50% of the cycles, matrix products
-// 20%, LDS 42%, with two wavefronts per SIMD to overlap them.
+// Measured (device time of this kernel alone, MI355X, BF16, SiLU): 320000 x 64 -> 256, 124 us after two hundred calls, 162 us in
+// the first calls after a pause (246 MB are 48 us): vector work 50% of the cycles, matrix products 20%, LDS 42%, with two
+// wavefronts per SIMD to overlap them. The joins of the weights' and the biases' partials take 7 + 5 us beside it.
 #pragma once
 
 #include "gated_few.h"

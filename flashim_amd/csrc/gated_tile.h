@@ -13,10 +13,11 @@
 // then on the consumed stage is refilled. One barrier per step.
 //
 // The matrix cores bound it, and below them the loop's LDS reads and the epilogue (the activation's vector work, nothing left to
-// overlap it on a CU's only tile). Measured (MI355X, BF16; a large library product reaches 1440 TFLOP/s): 16384 x 1024 -> 2 x
-// 4096, 256 us (1070 TFLOP/s), its backward's products 220 us (dx, 1250) and 215 us (weights, 1280), dg and du 320 us on
-// 128 x 128 tiles (860: the epilogue has no registers left beside 256 x 256 accumulators, 64 of which spilled); 20000 x 512 ->
-// 2 x 2048 forward 98 us (860).
+// overlap it on a CU's only tile). Measured (device time after a hundred calls, MI355X, BF16; a large library product reaches 1400
+// to 1440 TFLOP/s): 16384 x 1024 -> 2 x 4096 with SiLU, 255 us (1080 TFLOP/s), its backward's products 210 us (dx, 1310) and 208 us
+// (weights, 1320), dg and du 315 us on 128 x 128 tiles (870: the epilogue has no registers left beside 256 x 256 accumulators);
+// 20000 x 512 -> 2 x 2048 forward with GELU and biases 113 us (740). FP16 dx on 256 x 256 tiles spills 64 of its 256 registers
+// around its conversions, and is still ahead of 128 x 128: 237 against 292 us.
 #pragma once
 
 #include "activation.h"

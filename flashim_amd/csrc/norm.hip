@@ -19,26 +19,27 @@
 // cancellation where the mean is large) and merged as means and squared deviations. Small maps take one launch forward
 // (norm_group_kernel).
 //
-// Measured (device time, MI355X; a large copy reaches 5.1 TB/s): 160000 x 64 BF16 with GELU, 15 us for the statistics and 22
-// us for the apply forward, 26 us and 32 us backward, where a map's read or write is 4 us: the activation with its slope is
-// 20 to 40 vector operations a value (8 to 16 us), and each pass starts with a launch, the partials of the pass before and
-// its first round of loads (5 us). 40000 x 128: 12 + 4 (merge) + 14 us. 1024 x 64: 6.7 us in one launch
-// (12 in two), latencies alone.
+// Measured (device time after a hundred calls, MI355X; a large copy reaches 5.1 TB/s): two maps of 160000 x 64 BF16 with GELU,
+// 12 us for the statistics and 21 us for the apply forward, 23 us and 32 us backward, where their read or write is 8 us: the
+// activation with its slope is 20 to 40 vector operations a value (8 to 16 us), and each pass starts with a launch, the
+// partials of the pass before and its first round of loads (5 us). Two of 40000 x 128: 12 + 4 (merge) + 13 us. 1024 x 64: 7.6 us
+// in one launch (13.8 in two), latencies alone.
 #include "activation.h"
 
 namespace fim {
 
 constexpr int NORM_T = 512;           // threads of a workgroup
-// Pixels of a batch of loads (the next batch is loaded while one is worked on), with registers for four wavefronts per SIMD:
-// backward, with two tensors and the activation's slope, 4 took 180 to 230 registers and ran half as many wavefronts
+// Pixels of a batch of loads (the next batch is loaded while one is worked on), for four wavefronts per SIMD (128 registers, of
+// which the applies of 16-bit maps with 8 channels a load spill up to 13 forward and 20 backward): backward, with two tensors and
+// the activation's slope, 4 took 180 to 230 registers and ran half as many wavefronts
 constexpr int NORM_U = 4, NORM_GRAD_U = 2;
 constexpr int NORM_OWN = 8;           // loads of a thread that owns its values (small maps)
 constexpr int NORM_MAX_C = 8192;      // per-channel partials of a workgroup lie in LDS
 constexpr int NORM_MERGE_G = 512;     // groups, and partials, that the workgroups of the second pass add up themselves
 constexpr int64_t NORM_MERGE = 2 << 20;  // (over all workgroups)
 // Bytes of a map that is small. One workgroup per (image, group) reads D channels of each pixel, as little as 16 bytes of a line:
-// against two launches 1024 x 64, 6.7 and 12.1 us; 16 images of it (2 MB), 8.9 and 12.8; 16 x 256 x 512 (4 MB), 11 and 14; 16 x
-// 900 x 196 (5.6 MB), 13.3 and 13.2; 64 x 1024 x 64 (8 MB), 23 and 18 us
+// against two launches 1024 x 64 in 8 groups, 7.6 and 13.8 us; 16 images of it (2 MB), 9.8 and 14.3; 32, 13.5 and 14.9; 40 (5 MB),
+// 19.2 and 17.6; 64, 24.2 and 18.0; 20 images of 256 x 512 in 32 groups (5 MB), 17.8 and 19.1
 constexpr int64_t NORM_SMALL = 5 << 20;
 
 struct NormArgs {

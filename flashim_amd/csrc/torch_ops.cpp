@@ -856,7 +856,8 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch
 // stay, or an output keep the tangent of what it held.
 void refuse_derivatives(at::TensorList tensors) {
   const bool grads = at::GradMode::is_enabled();
-  const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // (no level, no tangents: one look, not one a tensor)
+  // (no level, no tangents: one look a call, not one a tensor)
+  const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
   if (!grads && !tangents) return;
   for (const Tensor& t : tensors) {
     TORCH_CHECK_NOT_IMPLEMENTED(!grads || !t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");

@@ -238,7 +238,8 @@ int fim_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t groups, in
  * per (image, group) over P pixels and C / groups channels out = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]),
  * biased variance, FP32 arithmetic, rounded once to x's type. weight, bias [C] of any float type, or NULL (1, 0).
  * out packed [B, P, C]; stats FP32 [B, groups, 2]: mean and 1 / sqrt(var + eps), which the backward pass reads.
- * C <= 8192 (else 99). No counterpart in the reference. */
+ * C <= 8192, B * C < 2^31 (else 99). A variance that is NaN (an infinity among the values) makes the group NaN; one past FP32's
+ * range makes it act(bias). No counterpart in the reference. */
 int fim_group_norm(const void* x, int dtype, int64_t B, int64_t P, int64_t C, int64_t stride_b, int64_t stride_p,
                    int64_t groups, const void* weight, int weight_dtype, const void* bias, int bias_dtype, float eps,
                    int act, void* out, float* stats, float* workspace, hipStream_t stream);
@@ -265,9 +266,9 @@ int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t x_s
                      const void* b_up, int bias_dtype, int act, void* out, void* workspace, int64_t workspace_bytes,
                      hipStream_t stream);
 
-/* Its gradients: d_out [M, H] (unit column stride, rows less than 2^22 elements apart, else 99); dx packed [M, K], dw_gate and dw_up packed [H, K], db_gate and db_up
- * [H] in the bias type; any of them may be NULL. The pre-activations are computed again; their gradients are rounded to
- * x's type before the products that make dx and the weights' gradients. */
+/* Its gradients: d_out [M, H] (unit column stride, rows less than 2^22 elements apart, else 99); dx packed [M, K], dw_gate and
+ * dw_up packed [H, K], db_gate and db_up [H] in the bias type; any of them may be NULL. The pre-activations are computed
+ * again; their gradients are rounded to x's type before the products that make dx and the weights' gradients. */
 int fim_gated_linear_backward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w_gate,
                               int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int64_t H,
                               const void* b_gate, const void* b_up, int bias_dtype, int act, const void* d_out,
