@@ -899,6 +899,11 @@ Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double no
   return total;
 }
 
+// The backward operators are linear in the incoming gradient, but stop its tangents
+void refuse_tangent(const Tensor& grad, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(grad), name, ": no forward-mode derivative of the backward pass");
+}
+
 struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, int64_t groups,
                                                 const OptTensor& weight, const OptTensor& bias, double eps, int64_t act) {
@@ -914,6 +919,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    refuse_tangent(grads[0], "group_norm_act");
     const auto saved = ctx->get_saved_variables();
     std::optional<at::AutoDispatchBelowAutograd> below;  // (nothing is recorded: past the refusal of second derivatives)
     if (!at::GradMode::is_enabled()) below.emplace();
@@ -958,6 +964,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    refuse_tangent(grads[0], "gated_linear");
     const auto saved = ctx->get_saved_variables();
     std::optional<at::AutoDispatchBelowAutograd> below;  // (nothing is recorded: past the refusal of second derivatives)
     if (!at::GradMode::is_enabled()) below.emplace();

@@ -142,6 +142,18 @@ def test_forward_mode_is_refused(grads):
             assert not call(t).requires_grad
 
 
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_a_tangent_of_the_incoming_gradient_is_refused(create_graph):
+    """The backward passes have no forward-mode derivatives either: a tangent raises there, it is not dropped."""
+    x = torch.empty(3, 16, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.empty(8, 16, device="meta", dtype=torch.bfloat16)
+    for out in (ht.group_norm_act(x, 4), ht.gated_linear(x, w, w)):
+        d = torch.empty_like(out)
+        assert torch.autograd.grad(out, x, d, retain_graph=True)[0].shape == x.shape
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, x, forward_ad.make_dual(d, torch.empty_like(d)), create_graph=create_graph)
+
+
 def test_clip_refuses_tangents():
     """In place, a clipped gradient would keep its unclipped tangent."""
     with forward_ad.dual_level():
