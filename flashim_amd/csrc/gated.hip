@@ -250,6 +250,10 @@ static void with_type(int dtype, F&& f) {
   else f(std::integral_constant<int, FIM_F16>{});
 }
 
+static bool workspace_ok(const Gated& g, const void* workspace, int64_t bytes) {
+  return workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && bytes >= g.total;
+}
+
 static bool rows_wide(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
 static TileArgs gated_forward_args(const Gated& g, const void* b_gate, const void* b_up, int bias_dtype) {
@@ -293,7 +297,7 @@ extern "C" int fim_gated_linear(const void* x, int dtype, int64_t M, int64_t K, 
   if (M == 0) return FIM_OK;
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || out == nullptr) return FIM_ERR_INVALID;
   Gated g = gated_plan(matrix(x, x_stride, M, K), matrix(w_gate, w_gate_stride, H, K), matrix(w_up, w_up_stride, H, K), false);
-  if (g.total > 0 && (workspace == nullptr || workspace_bytes < g.total)) return FIM_ERR_INVALID;
+  if (g.total > 0 && !workspace_ok(g, workspace, workspace_bytes)) return FIM_ERR_INVALID;
   if (g.form == FORM_FEW) {
     FewArgs f{};
     f.x = g.x.p;
@@ -349,7 +353,7 @@ extern "C" int fim_gated_linear_backward(const void* x, int dtype, int64_t M, in
   if (M == 0) return FIM_OK;
   if (x == nullptr || w_gate == nullptr || w_up == nullptr || d_out == nullptr) return FIM_ERR_INVALID;
   Gated g = gated_plan(matrix(x, x_stride, M, K), matrix(w_gate, w_gate_stride, H, K), matrix(w_up, w_up_stride, H, K), true);
-  if (workspace == nullptr || workspace_bytes < g.total) return FIM_ERR_INVALID;
+  if (!workspace_ok(g, workspace, workspace_bytes)) return FIM_ERR_INVALID;
   if (M == 1) d_out_stride = H;
   if (d_out_stride >= (1 << 22)) return FIM_ERR_UNSUPPORTED;  // 32-bit offsets inside a tile
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -221,3 +221,14 @@ def test_c_abi_checks_its_arguments():
     assert lib.fim_grad_norm(1, (ctypes.c_void_p * 1)(fake + 2), types, sizes, 2, fake, fake, None) == _lib.FIM_ERR_INVALID
     assert lib.fim_grad_norm(1, ptrs, types, sizes, 2, None, fake, None) == _lib.FIM_ERR_INVALID
     assert lib.fim_clip_grad_norm(1, ptrs, types, None, types, sizes, 1.0, 2, fake, fake, None) == _lib.FIM_ERR_INVALID
+
+
+def test_c_abi_refuses_a_misaligned_workspace():
+    """The gated product's workspace holds operands of 16-byte loads; both calls return before touching memory."""
+    lib = _lib.load()
+    fake, size = 1 << 20, 1 << 40
+    for off in (2, 8, 16, 128):
+        assert lib.fim_gated_linear(fake, 1, 100, 63, 63, fake, 63, fake, 63, 128, None, None, 0, 0, fake, fake + off, size,
+                                    None) == _lib.FIM_ERR_INVALID
+        assert lib.fim_gated_linear_backward(fake, 1, 100, 64, 64, fake, 64, fake, 64, 128, None, None, 0, 0, fake, 128, fake,
+                                             None, None, None, None, fake + off, size, None) == _lib.FIM_ERR_INVALID
