@@ -23,6 +23,7 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # symbol -> argtypes (all return int)
 SIGNATURES: dict[str, list] = {
@@ -75,6 +76,11 @@ SIGNATURES: dict[str, list] = {
                                   _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "fim_grad_norm_workspace": [_i64, _vp, _vp],
     "fim_grad_norm": [_i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
+    "fim_orthogonalize_workspace": [_i64, _i64, _i64, _vp],
+    "fim_orthogonalize": [_vp, _i32, _i64, _i64, _i64, _i32, _f32, _f32, _f32, _f64, _vp, _i32, _vp, _i64, _vp],
+    "fim_muon_step_workspace": [_i64, _vp, _vp, _vp, _vp],
+    "fim_muon_step": [_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _i32, _f32, _f32, _f32, _f64, _vp,
+                      _i64, _vp],
     "fim_clip_grad_norm": [_i64, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _vp, _vp, _vp],
 }
 

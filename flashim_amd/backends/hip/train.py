@@ -4,7 +4,8 @@ them; here they train a channels-last block before it is quantized, and run it u
 * ``group_norm_act``: group norm and activation of a channels-last map in one pass over it, with its gradients;
 * ``gated_linear``: the gated feed-forward product, both projections, activation and product in one kernel, with its
   gradients;
-* ``grad_norm`` and ``clip_grad_norm_``: the global norm of many gradients, and clipping by it.
+* ``grad_norm`` and ``clip_grad_norm_``: the global norm of many gradients, and clipping by it;
+* ``orthogonalize`` and ``muon_step_``: matrices orthogonalized by Newton-Schulz products, and the optimizer step made of them.
 """
 
 from __future__ import annotations
@@ -22,6 +23,8 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _HALVES = (torch.bfloat16, torch.float16)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # the C ABI's codes
 MAX_CHANNELS = 8192  # of group_norm_act
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # orthogonalize's coefficients: steepest at 0, within 0.7 .. 1.2 near 1
+ADJUST = {"original": 0, "match_rms": 1, "none": 2}  # muon_step_'s factors
 
 
 def group_norm_act(x: Tensor, num_groups: int, weight: Tensor | None = None, bias: Tensor | None = None, *,
@@ -57,6 +60,29 @@ def clip_grad_norm_(grads: Sequence[Tensor], max_norm: float, *, norm_type: floa
         if error_if_nonfinite and not math.isfinite(library.grad_norm(grads, float(norm_type)).item()):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm of type {norm_type} is not finite")
         return library.clip_lists(grads, out, float(max_norm), float(norm_type))
+
+
+def orthogonalize(g: Tensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7,
+                  out_dtype: torch.dtype | None = None) -> Tensor:
+    """Each matrix of ``g`` ``[..., rows, cols]`` with its singular values brought near 1: ``X = g / (|g| + eps)`` (the Frobenius
+    norm), then ``steps`` times ``A = X X^T``, ``X = (a I + b A + c A^2) X`` with ``coefficients = (a, b, c)`` (from the right
+    for tall matrices). Products to FP32's precision, rounded once to ``out_dtype`` (``g``'s). Raises ``UnsupportedShape`` for
+    coefficients by which a singular value of at most 1 passes 6 on its way. Not differentiable."""
+    a, b, c = coefficients
+    return library.orthogonalize(g, steps, a, b, c, eps, out_dtype)
+
+
+def muon_step_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Sequence[Tensor], *, lr: float, momentum: float = 0.95,
+               nesterov: bool = True, weight_decay: float = 0.0, adjust: str = "original", steps: int = 5,
+               coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7) -> None:
+    """One step of ``params`` (matrices, or stacks of them in the leading dimensions, each matrix by itself), in place:
+    ``m = momentum m + g``, ``u = g + momentum m`` (``nesterov``) or ``m``,
+    ``p = p (1 - lr weight_decay) - lr f orthogonalize(u)``. ``momenta`` FP32, the others of any float type. ``f`` by
+    ``adjust``: ``"original"`` sqrt(max(1, rows / cols)), ``"match_rms"`` 0.2 sqrt(max(rows, cols)), ``"none"`` 1. No two of the
+    parameters and momenta overlap. Nothing waits for the GPU."""
+    a, b, c = coefficients
+    with torch.no_grad():
+        library.muon_step_(params, grads, momenta, lr, momentum, nesterov, weight_decay, ADJUST[adjust], steps, a, b, c, eps)
 
 
 # -- eligibility -------------------------------------------------------------------------------------------------------
@@ -102,3 +128,18 @@ def eligible_grad_norm(grads, *, norm_type=2.0) -> bool:
 
 def eligible_clip_grad_norm(grads, max_norm, *, norm_type=2.0, out=None, error_if_nonfinite=False) -> bool:
     return eligible_grad_norm(grads, norm_type=norm_type) and (out is None or (_tensors(out) and len(out) == len(grads)))
+
+
+def _polynomial(steps, coefficients, eps) -> bool:
+    return 1 <= steps <= 100 and len(coefficients) == 3 and eps >= 0
+
+
+def eligible_orthogonalize(g, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out_dtype=None) -> bool:
+    return (isinstance(g, Tensor) and is_gfx950(g.device) and g.ndim >= 2 and g.dtype in _FLOATS
+            and (out_dtype is None or out_dtype in _FLOATS) and _polynomial(steps, coefficients, eps))
+
+
+def eligible_muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="original", steps=5,
+                       coefficients=NEWTON_SCHULZ, eps=1e-7) -> bool:
+    return (all(_tensors(t) and len(t) == len(params) for t in (params, grads, momenta)) and is_gfx950(params[0].device)
+            and params[0].dtype in _FLOATS and adjust in ADJUST and _polynomial(steps, coefficients, eps))

@@ -1,0 +1,279 @@
+// A whole Newton-Schulz iteration, or optimizer step, of a small matrix in one workgroup: X, A and P stay in LDS.
+//
+// At most 64 rows (of the shorter side) whose X fits: read once, written once, and no launch between the 3 `steps` products, which on
+// tiles would be as many launches of one or two workgroups. Eight wavefronts on 16 x 16 x 32 MFMAs: X X^T is split over the columns
+// (each fragment is read once, and is either operand) and the wavefronts' sums are joined pairwise; P X is split over the columns too, and each wavefront
+// replaces the columns it has read.
+#pragma once
+
+#include "ortho.h"
+
+namespace fim {
+
+constexpr int SMALL_WAVES = 8, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
+
+// LDS of a matrix: X [16 T][np] halves; the sums of four wavefronts, or A and P
+inline int64_t small_region(int T) {
+  const int64_t sums = 4 * (T * (T + 1) / 2) * 1024, ap = 2 * (16 * T) * (T > 2 ? 256 : 128);
+  return sums > ap ? sums : ap;
+}
+inline int64_t small_lds(int64_t m, int64_t np) {
+  const int64_t T = cdiv(m, 16);
+  return 16 * T * np * 4 + small_region((int)T) + 64;
+}
+
+// Where a row's 16-byte segments lie in each line, by XOR: eight rows read at one segment, and four rows by 32 bytes of a transposed
+// read, meet different banks.
+__device__ __forceinline__ int small_key(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+__device__ __forceinline__ v4f mfma_small(s16x8 a, s16x8 b, v4f c) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <int T, int LDS>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoStack* __restrict__ table, int count,
+                                                                       OrthoScalars k) {
+  constexpr int MP = 16 * T, LINES = T > 2 ? 2 : 1, PAIRS = T * (T + 1) / 2;  // LINES: of a row of A and P
+  __shared__ __attribute__((aligned(128))) uint8_t lds[LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, g = lane >> 4;
+  const int e = stack_of(table, count, 0, blockIdx.x);
+  const OrthoStack& s = table[e];
+  const int b = (int)(blockIdx.x - s.first[0]);
+  const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np, nb = np >> 5, ld = np * 4;
+  const int n = rows * cols;
+  const int64_t base = (int64_t)b * n;
+  uint8_t* X = lds;
+  uint8_t* A = lds + MP * ld;  // [MP][LINES] lines
+  uint8_t* P = A + MP * LINES * 128;
+  float* sums = reinterpret_cast<float*>(A);  // (A and P are dead while the sums are joined)
+
+  // -- U in 32 bits where X will lie: element (r, c) of X in 4 bytes, the columns of each line rotated by the row
+  for (int i = tid * 16; i < MP * ld; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(X + i) = v4i{0, 0, 0, 0};
+  __syncthreads();
+  double sq = 0.0;
+  for (int i = tid * 4; i < n; i += 64 * SMALL_WAVES * 4) {
+    float u[4];
+    const int left = n - i;
+    load4(s.g, base + i, s.g_type, left, u);
+    if (s.mom != nullptr) {
+      float m[4];
+      load4(s.mom, base + i, FIM_F32, left, m);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        m[q] = fmaf(k.momentum, m[q], u[q]);
+        u[q] = k.nesterov ? fmaf(k.momentum, m[q], u[q]) : m[q];
+      }
+      store4(s.mom, base + i, FIM_F32, left, m);
+    }
+    int r = i / cols, c = i - r * cols;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < left) {
+        sq = fma((double)u[q], (double)u[q], sq);
+        const int xr = s.tall ? c : r, xc = s.tall ? r : c;
+        *reinterpret_cast<float*>(X + xr * ld + (xc >> 5) * 128 + (((xc ^ xr) & 31) << 2)) = u[q];
+      }
+      if (++c == cols) {
+        c = 0;
+        ++r;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o);
+  double* red = reinterpret_cast<double*>(A);
+  if (lane == 0) red[wave] = sq;
+  __syncthreads();
+  sq = red[0];
+#pragma unroll
+  for (int i = 1; i < SMALL_WAVES; ++i) sq += red[i];
+  const float scale = (float)((double)ORTHO_S / (sqrt(sq) + k.eps));
+  // -- S X0 as halves, line by line in place: 8 lanes a line, all of which read before one writes
+  for (int i = tid; i < MP * nb * 8; i += 64 * SMALL_WAVES) {
+    const int q = i & 7, line = i >> 3, r = line / nb;
+    uint8_t* at = X + line * 128;
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float*>(at + (((4 * q + u) ^ (r & 31)) << 2)) * scale;
+    v2i hi, lo;
+    split4(v, hi, lo);
+    const int key = small_key(r);
+    wave_lds_wait();
+    *reinterpret_cast<v2i*>(at + (((q >> 1) ^ key) << 4) + (q & 1) * 8) = hi;
+    *reinterpret_cast<v2i*>(at + (((4 + (q >> 1)) ^ key) << 4) + (q & 1) * 8) = lo;
+  }
+
+  // fragments: lane: row (or column) l % 16, contraction 8 (l / 16) .. + 7 of 32
+  auto along = [&](const uint8_t* p, int row_bytes, int r0, int line, int plane) __attribute__((always_inline)) {
+    const int r = r0 + l16;
+    return *reinterpret_cast<const s16x8*>(p + r * row_bytes + line * 128 + (((4 * plane + g) ^ small_key(r)) << 4));
+  };
+  auto across = [&](int r0, int col16, int plane) __attribute__((always_inline)) {  // X's rows r0 .. r0 + 31 (past MP: any, P is 0)
+    s16x4 half[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      int r = r0 + 8 * g + 4 * q + (l16 >> 2);
+      if (MP % 32 != 0) r = r < MP ? r : r - 16;
+      const int seg = 4 * plane + 2 * (col16 & 1) + ((lane & 3) >> 1);
+      half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)(X + r * ld + (col16 >> 1) * 128 + ((seg ^ small_key(r)) << 4) + (lane & 1) * 8));
+    }
+    return __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // a block's values (lane: row l % 16, columns 4 g ..) into A or P as halves, and their mirror
+  auto put = [&](uint8_t* p, int r, int c, const float (&v)[4], bool mirror) __attribute__((always_inline)) {
+    v2i hi, lo;
+    split4(v, hi, lo);
+    uint8_t* at = p + r * (LINES * 128) + (c >> 5) * 128;
+    const int key = small_key(r), seg = (c & 31) >> 3;
+    *reinterpret_cast<v2i*>(at + ((seg ^ key) << 4) + (c & 7) * 2) = hi;
+    *reinterpret_cast<v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2) = lo;
+    if (mirror) {
+      const s16x4 a4 = __builtin_bit_cast(s16x4, hi), b4 = __builtin_bit_cast(s16x4, lo);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint8_t* o = p + (c + u) * (LINES * 128) + (r >> 5) * 128;
+        const int ko = small_key(c + u), so = (r & 31) >> 3;
+        *reinterpret_cast<int16_t*>(o + ((so ^ ko) << 4) + (r & 7) * 2) = a4[u];
+        *reinterpret_cast<int16_t*>(o + (((4 + so) ^ ko) << 4) + (r & 7) * 2) = b4[u];
+      }
+    }
+  };
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int it = 0; it < k.steps; ++it) {
+    // -- A = X X^T: this wavefront's lines, all pairs of row blocks
+    v4f acc[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) acc[i] = zero;
+    __syncthreads();
+    for (int line = wave; line < nb; line += SMALL_WAVES) {
+      s16x8 f[T][2];
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl) f[i][pl] = along(X, ld, 16 * i, line, pl);
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int i = 0, q = 0; i < T; ++i)
+#pragma unroll
+          for (int j = 0; j <= i; ++j, ++q) acc[q] = mfma_small(f[j][part == 2], f[i][part == 1], acc[q]);
+    }
+    // joined pairwise: 4 wavefronts into 4, 2 into 2, 1 into 1
+#pragma unroll
+    for (int half = 4; half > 0; half >>= 1) {
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + ((wave - half) * PAIRS + i) * 256 + lane * 4) = acc[i];
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) acc[i] += *reinterpret_cast<const v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4);
+      }
+      __syncthreads();
+    }
+    if (T == 1 || T == 3) {  // columns past 16 T of the last line: zero
+      for (int i = tid * 16; i < 2 * MP * LINES * 128; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(A + i) = v4i{0, 0, 0, 0};
+      __syncthreads();
+    }
+    if (wave == 0) {
+#pragma unroll
+      for (int i = 0, q = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j, ++q) {
+          float v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = acc[q][u] * (1.0f / ORTHO_S);
+          put(A, 16 * i + l16, 16 * j + 4 * g, v, i != j);
+        }
+    }
+    __syncthreads();
+    // -- P = a I + b A + c A^2: pairs of blocks over the wavefronts
+#pragma unroll
+    for (int i = 0, q = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j <= i; ++j, ++q)
+        if (q % SMALL_WAVES == wave) {
+          v4f w = zero;
+#pragma unroll
+          for (int line = 0; line < LINES; ++line) {
+            s16x8 fi[2], fj[2];
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl) {
+              fi[pl] = along(A, LINES * 128, 16 * i, line, pl);
+              fj[pl] = along(A, LINES * 128, 16 * j, line, pl);
+            }
+#pragma unroll
+            for (int part = 0; part < 3; ++part) w = mfma_small(fj[part == 2], fi[part == 1], w);
+          }
+          const int r = 16 * i + l16, c = 16 * j + 4 * g, key = small_key(r), seg = (c & 31) >> 3;
+          const uint8_t* at = A + r * (LINES * 128) + (c >> 5) * 128;
+          float old[4], v[4];
+          join4(*reinterpret_cast<const v2i*>(at + ((seg ^ key) << 4) + (c & 7) * 2),
+                *reinterpret_cast<const v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2), old);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            v[u] = fmaf(k.c / ORTHO_S, w[u], k.b * old[u]);
+            if (r == c + u) v[u] += k.a * ORTHO_S;
+          }
+          put(P, r, c, v, i != j);
+        }
+    __syncthreads();
+    // -- X = P X: 16 columns a turn
+    const bool last = it == k.steps - 1;
+    s16x8 fp[T][LINES][2];
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int line = 0; line < LINES; ++line)
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl) fp[i][line][pl] = along(P, LINES * 128, 16 * i, line, pl);
+    for (int c16 = wave; c16 < 2 * nb; c16 += SMALL_WAVES) {
+      v4f y[T];
+#pragma unroll
+      for (int i = 0; i < T; ++i) y[i] = zero;
+#pragma unroll
+      for (int line = 0; line < LINES; ++line) {
+        const s16x8 xh = across(32 * line, c16, 0), xl = across(32 * line, c16, 1);
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int i = 0; i < T; ++i) y[i] = mfma_small(part == 2 ? xl : xh, fp[i][line][part == 1], y[i]);
+      }
+      const int c = 16 * c16 + 4 * g;
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        const int r = 16 * i + l16;
+        float v[4];
+        if (last) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * (1.0f / (ORTHO_S * ORTHO_S));
+          if (s.tall) {
+            if (r < cols) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (c + u < rows) finish1(s, k, base + (int64_t)(c + u) * cols + r, v[u]);
+            }
+          } else if (r < rows && c < cols) {
+            finish4(s, k, base + (int64_t)r * cols + c, cols - c, v);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * (1.0f / ORTHO_S);
+          v2i hi, lo;
+          split4(v, hi, lo);
+          uint8_t* at = X + r * ld + (c >> 5) * 128;
+          const int key = small_key(r), seg = (c & 31) >> 3;
+          *reinterpret_cast<v2i*>(at + ((seg ^ key) << 4) + (c & 7) * 2) = hi;
+          *reinterpret_cast<v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2) = lo;
+        }
+      }
+    }
+  }
+}
+
+}  // namespace fim

@@ -17,7 +17,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <limits>
 #include <optional>
 #include <string>
@@ -730,6 +732,88 @@ Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double norm_type) 
   return clip_grad_norm_out(grads, grads, max_norm, norm_type);
 }
 
+// -- orthogonalized updates -------------------------------------------------------------------------------------------
+
+// The leading dimensions of [..., rows, cols], multiplied
+int64_t stack_size(const Tensor& t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 2 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+
+Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double c, double eps,
+                     std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK_VALUE(g.dim() >= 2, "orthogonalize: expected matrices, got shape ", g.sizes());
+  const c10::DeviceGuard guard(g.device());
+  const Tensor in = g.contiguous();
+  Tensor out = empty(g.sizes(), g, out_dtype.value_or(g.scalar_type()));
+  const int64_t batch = stack_size(g), rows = g.size(-2), cols = g.size(-1);
+  int64_t bytes = 0;
+  check(fim_orthogonalize_workspace(batch, rows, cols, &bytes), "orthogonalize ", g.sizes());
+  const Tensor ws = empty({bytes}, g, at::kByte);
+  check(fim_orthogonalize(in.data_ptr(), dtype_code(in), batch, rows, cols, (int)steps, (float)a, (float)b, (float)c, eps,
+                          out.data_ptr(), dtype_code(out), ws.data_ptr(), bytes, stream_of(g)),
+        "orthogonalize ", g.sizes(), " in ", steps, " steps of ", a, ", ", b, ", ", c);
+  return out;
+}
+
+// adjust 0: sqrt(max(1, rows / cols)), 1: 0.2 sqrt(max(rows, cols)), 2: 1
+float muon_factor(double lr, int64_t adjust, int64_t rows, int64_t cols) {
+  TORCH_CHECK_VALUE(adjust >= 0 && adjust <= 2, "muon_step_: adjustment ", adjust);
+  if (rows == 0 || cols == 0) return 0.0f;
+  const double f = adjust == 0 ? std::sqrt(std::max(1.0, (double)rows / (double)cols))
+                   : adjust == 1 ? 0.2 * std::sqrt((double)std::max(rows, cols))
+                                 : 1.0;
+  return (float)(lr * f);
+}
+
+void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList momenta, double lr, double momentum, bool nesterov,
+                double weight_decay, int64_t adjust, int64_t steps, double a, double b, double c, double eps) {
+  TORCH_CHECK_VALUE(!params.empty(), "muon_step_: no parameters");
+  TORCH_CHECK_VALUE(params.size() == grads.size() && params.size() == momenta.size(), "muon_step_: ", params.size(),
+                    " parameters, ", grads.size(), " gradients and ", momenta.size(), " momenta");
+  const c10::DeviceGuard guard(params[0].device());
+  const size_t n = params.size();
+  std::vector<Tensor> p, g, m;
+  std::vector<void*> pp;
+  std::vector<const void*> gp;
+  std::vector<float*> mp;
+  std::vector<int> pt, gt;
+  std::vector<int64_t> batch, rows, cols;
+  std::vector<float> factors;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &w = params[i], &d = grads[i], &v = momenta[i];
+    for (const Tensor* t : {&w, &d, &v}) check_grad(*t, params[0]);
+    TORCH_CHECK_NOT_IMPLEMENTED(v.scalar_type() == at::kFloat, "no HIP impl applies: a momentum of ", v.scalar_type());
+    TORCH_CHECK_NOT_IMPLEMENTED(w.dim() >= 2 && w.sizes() == d.sizes() && w.sizes() == v.sizes(),
+                                "no HIP impl applies: a parameter of shape ", w.sizes(), ", its gradient of ", d.sizes(),
+                                " and momentum of ", v.sizes());
+    p.push_back(w.is_contiguous() ? w : w.contiguous());
+    g.push_back(d.contiguous());
+    m.push_back(v.is_contiguous() ? v : v.contiguous());
+    pp.push_back(p.back().data_ptr());
+    gp.push_back(g.back().data_ptr());
+    mp.push_back(ptr<float>(m.back()));
+    pt.push_back(dtype_code(w));
+    gt.push_back(dtype_code(d));
+    batch.push_back(stack_size(w));
+    rows.push_back(w.size(-2));
+    cols.push_back(w.size(-1));
+    factors.push_back(muon_factor(lr, adjust, rows.back(), cols.back()));
+  }
+  int64_t bytes = 0;
+  check(fim_muon_step_workspace((int64_t)n, batch.data(), rows.data(), cols.data(), &bytes), "muon_step_");
+  const Tensor ws = empty({bytes}, params[0], at::kByte);
+  check(fim_muon_step((int64_t)n, pp.data(), pt.data(), gp.data(), gt.data(), mp.data(), batch.data(), rows.data(), cols.data(),
+                      factors.data(), (float)momentum, nesterov, (float)(1.0 - lr * weight_decay), (int)steps, (float)a,
+                      (float)b, (float)c, eps, ws.data_ptr(), bytes, stream_of(params[0])),
+        "muon_step_ of ", n, " parameters in ", steps, " steps of ", a, ", ", b, ", ", c);
+  for (size_t i = 0; i < n; ++i) {
+    if (!p[i].is_same(params[i])) params[i].copy_(p[i]);
+    if (!m[i].is_same(momenta[i])) momenta[i].copy_(m[i]);
+  }
+}
+
 }  // namespace
 
 #define FIM_GEO_SCHEMA "SymInt kh, SymInt kw, SymInt sh, SymInt sw, SymInt ph, SymInt pw, SymInt dh, SymInt dw"
@@ -774,12 +858,15 @@ Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double norm_type) 
   X(gated_linear_backward, "(Tensor d_out, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "       \
                            "int act, bool want_x, bool want_weights, bool want_biases) "                               \
                            "-> (Tensor, Tensor, Tensor, Tensor, Tensor)")                                              \
-  X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")
+  X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")                                                          \
+  X(orthogonalize, "(Tensor g, int steps, float a, float b, float c, float eps, ScalarType? out_dtype) -> Tensor")
 
 // those with an autograd kernel of their own (below)
 #define FIM_AUTOGRAD_OPS(X)                                                                                            \
   X(clip_grad_norm_, "(Tensor(a!)[] grads, float max_norm, float norm_type) -> Tensor")                                \
   X(clip_grad_norm_out, "(Tensor[] grads, Tensor(a!)[] out, float max_norm, float norm_type) -> Tensor")               \
+  X(muon_step_, "(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float lr, float momentum, bool nesterov, " \
+                "float weight_decay, int adjust, int steps, float a, float b, float c, float eps) -> ()")              \
   X(group_norm_act, "(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act) -> (Tensor, Tensor)")    \
   X(gated_linear, "(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor")
 
@@ -854,15 +941,15 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch
 // Clipping below autograd, the versions of what it wrote counted: as no_derivative and count_writes do for any operator, but
 // without boxing hundreds of tensors. A tangent is refused whatever the mode: the tensor's values would change and its tangent
 // stay, or an output keep the tangent of what it held.
-void refuse_derivatives(at::TensorList tensors) {
+void refuse_derivatives(at::TensorList tensors, const char* name = "clip_grad_norm_") {
   const bool grads = at::GradMode::is_enabled();
   // (no level, no tangents: one look a call, not one a tensor)
   const bool tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
   if (!grads && !tangents) return;
   for (const Tensor& t : tensors) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!grads || !t.requires_grad(), "clip_grad_norm_: no derivative, and a tensor requires a gradient");
+    TORCH_CHECK_NOT_IMPLEMENTED(!grads || !t.requires_grad(), name, ": no derivative, and a tensor requires a gradient");
     TORCH_CHECK_NOT_IMPLEMENTED(!tangents || !torch::autograd::isFwGradDefined(t),
-                                "clip_grad_norm_: no derivative, and a tensor has a tangent");
+                                name, ": no derivative, and a tensor has a tangent");
   }
 }
 
@@ -897,6 +984,17 @@ Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double no
   Tensor total = op.call(grads, max_norm, norm_type);
   count_writes_to(grads);
   return total;
+}
+
+void muon_step_autograd_(at::TensorList params, at::TensorList grads, at::TensorList momenta, double lr, double momentum,
+                         bool nesterov, double weight_decay, int64_t adjust, int64_t steps, double a, double b, double c,
+                         double eps) {
+  for (const auto& list : {params, grads, momenta}) refuse_derivatives(list, "muon_step_");
+  static const auto op = typed_op<decltype(muon_step_)>("flashim_amd::muon_step_");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  op.call(params, grads, momenta, lr, momentum, nesterov, weight_decay, adjust, steps, a, b, c, eps);
+  count_writes_to(params);
+  count_writes_to(momenta);
 }
 
 // The backward operators are linear in the incoming gradient, but stop its tangents
@@ -1001,10 +1099,11 @@ TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
   m.impl("gated_linear", TORCH_FN(gated_linear_autograd));
   m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_autograd_));
   m.impl("clip_grad_norm_out", TORCH_FN(clip_grad_norm_out_autograd));
+  m.impl("muon_step_", TORCH_FN(muon_step_autograd_));
 }
 
 TORCH_LIBRARY_IMPL(flashim_amd, ADInplaceOrView, m) {
-  for (const char* name : {"int8_linear_quantize_", "clip_grad_norm_", "clip_grad_norm_out"})
+  for (const char* name : {"int8_linear_quantize_", "clip_grad_norm_", "clip_grad_norm_out", "muon_step_"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&count_writes>());
 }
 

@@ -281,6 +281,17 @@ def clip_grad_norm_out(grads, out, max_norm, norm_type):
     return grads[0].new_empty((), dtype=torch.float32)
 
 
+@_fake
+def orthogonalize(g, steps, a, b, c, eps, out_dtype):
+    return g.new_empty(g.shape, dtype=out_dtype or g.dtype)
+
+
+@_fake
+def muon_step_(params, grads, momenta, lr, momentum, nesterov, weight_decay, adjust, steps, a, b, c, eps):
+    """Steps ``params`` and ``momenta`` in place."""
+    return None
+
+
 def clip_lists(grads, out, max_norm: float, norm_type: float):
     """``clip_grad_norm_(grads, ...)`` (``out`` None) or ``clip_grad_norm_out(grads, out, ...)``. Eager lists of plain tensors
     take the library's own entry to those ops, 320 tensors into as many in 65 us of host time instead of 93."""

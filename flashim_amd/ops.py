@@ -42,11 +42,13 @@ conv2d_small_cin_quantize_int8 = Op("conv2d_small_cin_quantize_int8", weights=2)
 bias_relu_quantize_int8 = Op("bias_relu_quantize_int8")
 # this backend's refiner-block producer (folded BatchNorm + GELU)
 depthwise5x5_gelu = Op("depthwise5x5_gelu")
-# this backend's training-step operators (differentiable, but for the last two)
+# this backend's training-step operators (the first two differentiable)
 group_norm_act = Op("group_norm_act")
 gated_linear = Op("gated_linear")
 grad_norm = Op("grad_norm")
 clip_grad_norm_ = Op("clip_grad_norm_")
+orthogonalize = Op("orthogonalize")
+muon_step_ = Op("muon_step_")
 
 ROCM = DeviceSpec("rocm")
 HIP = "hip"
@@ -82,6 +84,8 @@ IMPLS = (
     ("gated_linear", _train.gated_linear, (Feature.HIP,), _train.eligible_gated_linear),
     ("grad_norm", _train.grad_norm, (Feature.HIP,), _train.eligible_grad_norm),
     ("clip_grad_norm_", _train.clip_grad_norm_, (Feature.HIP,), _train.eligible_clip_grad_norm),
+    ("orthogonalize", _train.orthogonalize, (Feature.HIP,), _train.eligible_orthogonalize),
+    ("muon_step_", _train.muon_step_, (Feature.HIP,), _train.eligible_muon_step),
 )
 
 for _name, _fn, _requires, _when in IMPLS:

@@ -227,7 +227,7 @@ int fim_depthwise5x5_relu_pointwise_int8(const uint16_t* x, int64_t B, int64_t H
 int fim_pointwise_bf16(const uint16_t* x, int64_t M, int64_t K, const uint16_t* weight, int64_t N, const void* bias,
                        int bias_dtype, uint16_t* out, hipStream_t stream);
 
-/* ---- training-step operators: group norm with an activation, the gated feed-forward product, gradient clipping --- */
+/* ---- training-step operators: group norm with an activation, the gated feed-forward product, gradient clipping, orthogonalized updates --- */
 
 /* Activation codes: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf form), 4 GELU (tanh form). */
 
@@ -289,6 +289,28 @@ int fim_grad_norm(int64_t count, const void* const* grads, const int* dtypes, co
 int fim_clip_grad_norm(int64_t count, const void* const* grads, const int* dtypes, void* const* out,
                        const int* out_dtypes, const int64_t* numel, float max_norm, int norm, float* total,
                        double* workspace, hipStream_t stream);
+
+/* Bytes of workspace (256-byte aligned) that fim_orthogonalize needs. */
+int fim_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64_t* bytes);
+
+/* Newton-Schulz orthogonalization of `batch` packed matrices [rows, cols] of any float type: X = g / (|g| + eps), |g| the
+ * square root of the sum of squares (summed in 64 bits), of the shorter side's rows; `steps` (1 to 100) times
+ * A = X X^T, X = (a I + b A + c A^2) X, products of operands of 22 bits with FP32 sums; out packed, any float type, rounded
+ * once. Coefficients by which a singular value of at most 1 passes 6, or its factor 48, are refused (99), and so are matrices
+ * of more than 2^29 elements. No counterpart in the reference, as the next two. */
+int fim_orthogonalize(const void* g, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                      double eps, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Bytes of workspace (256-byte aligned) that fim_muon_step needs for stacks of batch[i] matrices [rows[i], cols[i]]. */
+int fim_muon_step_workspace(int64_t count, const int64_t* batch, const int64_t* rows, const int64_t* cols, int64_t* bytes);
+
+/* An optimizer step of `count` stacks of packed matrices (host arrays of device pointers, dtype codes and sizes):
+ * m = momentum m + g (FP32, in place), u = g + momentum m (nesterov) or m, O as above of each u, p = keep p - factors[i] O
+ * (in place). No two of the parameters and momenta overlap. */
+int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, const void* const* grads, const int* grad_dtypes,
+                  float* const* momenta, const int64_t* batch, const int64_t* rows, const int64_t* cols, const float* factors,
+                  float momentum, int nesterov, float keep, int steps, float a, float b, float c, double eps, void* workspace,
+                  int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -102,3 +102,55 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
 
 def clip_scale(total: Tensor, max_norm: float) -> Tensor:
     return torch.clamp(max_norm / (total.double() + 1e-6), max=1.0)
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def schulz_iterates(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> list[Tensor]:
+    """``[X_0, ..., X_steps]`` of one matrix, by its definition from the left (``rows <= cols``) or the right."""
+    a, b, c = coefficients
+    u = u.double()
+    xs = [u / (u.square().sum().sqrt() + eps)]
+    for _ in range(steps):
+        x = xs[-1]
+        if x.shape[0] <= x.shape[1]:
+            gram = x @ x.t()
+            xs.append(a * x + (b * gram + c * gram @ gram) @ x)
+        else:
+            gram = x.t() @ x
+            xs.append(a * x + x @ (b * gram + c * gram @ gram))
+    return xs
+
+
+def orthogonalize(u: Tensor, **kwargs) -> Tensor:
+    """Of ``[..., rows, cols]``."""
+    flat = u.reshape(-1, *u.shape[-2:])
+    return torch.stack([schulz_iterates(m, **kwargs)[-1] for m in flat]).reshape(u.shape)
+
+
+def schulz_bound(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> float:
+    """How far (Frobenius) an iteration of 22-bit operands and FP32 sums may end from one matrix's exact result.
+
+    Step k's rounding is an error of at most e_k |X_k|: each product's operands are off by 2^-23, the dropped product of the
+    low halves by 2^-24, and a sum of K terms, rounded K / 16 times or more at 2^-24 each, by 4 sqrt(K) 2^-24 (independent
+    roundings); three products a step, whose factors a, b |A| and c |A|^2 multiply them by at most |a| + 2 |b| + 2 |c|. Later
+    steps multiply an error by at most the largest slope of the polynomial that is left (of an odd matrix function), between 0
+    and the largest singular value."""
+    a, b, c = coefficients
+    m, n = sorted(u.shape[-2:])
+    e = (2.0**-21 + 4 * math.sqrt(n) * 2.0**-24) * (abs(a) + 2 * abs(b) + 2 * abs(c))
+    xs = schulz_iterates(u, steps, coefficients, eps)
+    total = 0.0
+    for k, x in enumerate(xs[:-1]):
+        top = torch.linalg.matrix_norm(x, ord=2).item() * 1.001
+        grid = torch.linspace(0, max(top, 1e-30), 4097, dtype=torch.float64)
+        slope, at = torch.ones_like(grid), grid
+        slopes = [1.0]
+        for _ in range(steps - k):
+            slope = slope * (a + 3 * b * at**2 + 5 * c * at**4)
+            at = at * (a + b * at**2 + c * at**4)
+            slopes.append(slope.abs().max().item())
+        # (the step's own slope is in the sum above: what is left are the steps after it; X_0's conversion meets all of them)
+        total += e * x.norm().item() * slopes[-2 if k else -1]
+    return total
