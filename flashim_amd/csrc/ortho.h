@@ -6,8 +6,9 @@
 // The products amplify what is small in X0 (by a^steps, 485 times at five steps), and with it any rounding of the large
 // directions: operands of one BF16 each leave 1 to 5% of an output wrong, of one FP16 each 0.3 to 0.6%. So every operand is two FP16
 // numbers, hi + lo, 22 bits, and a product is hi hi + hi lo + lo hi on the matrix cores with FP32 sums: errors of an FP32 product
-// (1e-6 to 5e-6 of an output) at a third of the FP16 rate, which is five times the FP32 rate. What is stored is S = 2^10 times its value:
-// lo's steps are 2^-34 of it, and entries up to 63 fit, which the host checks by the coefficients.
+// (1e-6 to 5e-6 of an output) at a third of the FP16 rate, which is five times the FP32 rate. X, A and P are stored times powers of
+// two, as large as their entries' bounds (by the coefficients, computed on the host) allow, so that lo, too, is seldom below FP16's
+// normal numbers.
 #pragma once
 
 #include <type_traits>
@@ -17,16 +18,14 @@
 
 namespace fim {
 
-constexpr float ORTHO_S = 1024.0f;
-
 // A stack of matrices of one shape, packed row-major; the table lies in the workspace. m <= n: sides, padded mp, np to 32.
 struct OrthoStack {
   const void* g;
   float* mom;     // null: U = g
   void* out;      // O, or the parameters that are stepped in place
-  uint8_t* x[2];  // S X of the first matrix, [mp][np] halves; the others `each` bytes apart
-  uint8_t* a;     // S A, [mp][mp] halves
-  uint8_t* p;     // S P
+  uint8_t* x[2];  // sx X of the first matrix, [mp][np] halves; the others `each` bytes apart
+  uint8_t* a;     // sa A, [mp][mp] halves
+  uint8_t* p;     // sp P
   double* part;   // partial sums of squares, `chunks` a matrix
   int64_t each;
   uint32_t rows, cols, batch, mp, np, chunk, chunks;
@@ -39,6 +38,7 @@ static_assert(sizeof(OrthoStack) % 8 == 0, "");
 struct OrthoScalars {
   float momentum, keep;  // keep = 1 - lr * weight decay
   float a, b, c;
+  float sx, sa, sp;  // powers of two that X, A and P are stored times
   double eps;
   int steps, nesterov, step;  // step: parameters are stepped; else O is written
 };
@@ -51,13 +51,16 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 }
 typedef int v2i __attribute__((ext_vector_type(2)));
 
-// Four values (times S already) as halves
+// Four values as halves. The compiler may not see where they come from: it fuses a product and its conversion into one rounding
+// for hi and not for lo's subtraction, and at a tie lo then belongs to the other neighbour.
 __device__ __forceinline__ void split4(const float (&v)[4], v2i& hi, v2i& lo) {
   _Float16 h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    h[i] = (_Float16)v[i];
-    l[i] = (_Float16)(v[i] - (float)h[i]);
+    float x = v[i];
+    asm("" : "+v"(x));
+    h[i] = (_Float16)x;
+    l[i] = (_Float16)(x - (float)h[i]);
   }
   typedef _Float16 h4 __attribute__((ext_vector_type(4)));
   hi = __builtin_bit_cast(v2i, (h4{h[0], h[1], h[2], h[3]}));

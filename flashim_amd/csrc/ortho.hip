@@ -2,7 +2,7 @@
 //
 // Matrices come as stacks of one shape, many stacks a call; a table of them goes through kernel arguments into the workspace
 // (no upload: capturable), and every launch after that runs over all matrices at once. Small ones take one launch, a workgroup each
-// (ortho_small.h); the others a pass that updates the momentum and sums squares, one that writes S X0 as halves (transposing tall
+// (ortho_small.h); the others a pass that updates the momentum and sums squares, one that writes sx X0 as halves (transposing tall
 // matrices), and three launches of products a step (ortho_tile.h), the last of which writes O or steps the parameters.
 #include <string.h>
 
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(ORTHO_T) void ortho_momentum_kernel(const OrthoStac
   if (threadIdx.x == 0) s.part[local] = sq;
 }
 
-// S U / (|U| + eps) as halves, 64 x 64 of X a workgroup; a tall matrix's through LDS
+// sx U / (|U| + eps) as halves, 64 x 64 of X a workgroup; a tall matrix's through LDS
 __global__ __launch_bounds__(ORTHO_T) void ortho_convert_kernel(const OrthoStack* __restrict__ table, int count,
                                                                 const OrthoScalars k) {
   __shared__ float tile[64 * 65];
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(ORTHO_T) void ortho_convert_kernel(const OrthoStack
   const int r0 = (int)(in / ct) * 64, c0 = (int)(in % ct) * 64;  // of X
   double sq = 0.0;
   for (uint32_t i = threadIdx.x; i < s.chunks; i += ORTHO_T) sq += s.part[b * s.chunks + i];
-  const float scale = (float)((double)ORTHO_S / (sqrt(ortho_sum(sq)) + k.eps));
+  const float scale = (float)((double)k.sx / (sqrt(ortho_sum(sq)) + k.eps));
   const int rows = (int)s.rows, cols = (int)s.cols;
   const int sr0 = s.tall ? c0 : r0, sc0 = s.tall ? r0 : c0;  // of the source
   const int64_t base = (int64_t)b * rows * cols;
@@ -178,23 +178,37 @@ static bool ortho_aligned(const void* p, int t) {
   return p != nullptr && reinterpret_cast<uintptr_t>(p) % (t == FIM_F32 ? 4 : 2) == 0;
 }
 
-// Whether every singular value s <= 1 of X0, and with it every entry, stays where the halves hold it
-static bool ortho_bounded(const OrthoScalars& k) {
-  for (int i = 0; i <= 1024; ++i) {
-    double x = i / 1024.0;
+// The largest power of two that keeps values up to `most` (and a little more) below FP16's largest
+static float ortho_scale(double most) {
+  int e;
+  frexp(60000.0 / (most > 1e-6 ? most : 1e-6), &e);
+  return ldexpf(1.0f, e - 1);
+}
+
+// The scales of X, A and P: no entry of a matrix is larger than its largest singular value, whose path from any s <= 1 is
+// followed here. False where it leaves the halves little room (or does not end at all).
+static bool ortho_scales(OrthoScalars& k) {
+  double most_x = 1.0, most_p = 0.0;
+  for (int i = 0; i <= 256; ++i) {
+    double x = i / 256.0;
     for (int it = 0; it < k.steps; ++it) {
       const double q = x * x, p = k.a + q * (k.b + q * k.c);
-      if (!(fabs(p) <= 48.0)) return false;
+      most_p = fmax(most_p, fabs(p));
       x *= p;
-      if (!(fabs(x) <= 6.0)) return false;
+      if (!(fabs(p) <= 48.0) || !(fabs(x) <= 6.0)) return false;
+      if (it + 1 < k.steps) most_x = fmax(most_x, fabs(x));
     }
   }
+  // (between the grid's points and by rounding a little more)
+  k.sx = ortho_scale(1.1 * most_x);
+  k.sa = ortho_scale(1.25 * most_x * most_x);
+  k.sp = ortho_scale(1.05 * most_p);
   return true;
 }
 
-static int ortho_check(const OrthoCall& c, const OrthoScalars& k) {
+static int ortho_check(const OrthoCall& c, OrthoScalars& k) {
   if (k.steps < 1 || k.steps > 100 || !(k.eps >= 0.0)) return FIM_ERR_INVALID;
-  if (!ortho_bounded(k)) return FIM_ERR_UNSUPPORTED;
+  if (!ortho_scales(k)) return FIM_ERR_UNSUPPORTED;
   if (c.count > 0 && (c.g == nullptr || c.g_type == nullptr || c.out == nullptr || c.out_type == nullptr)) return FIM_ERR_INVALID;
   for (int64_t i = 0; i < c.count; ++i) {
     if (!ortho_type(c.g_type[i]) || !ortho_type(c.out_type[i])) return FIM_ERR_INVALID;
@@ -239,7 +253,7 @@ static void launch_products(const OrthoStack* table, int count, uint32_t sym, ui
 }
 
 // Stacks of one group (a size of small matrices, or all that go on tiles) share their launches
-static int ortho_run(const OrthoCall& c, const OrthoScalars& k, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   int64_t need = 0;
   int rc = ortho_bytes(c, &need);
   if (rc == FIM_OK) rc = ortho_check(c, k);
@@ -345,7 +359,7 @@ extern "C" int fim_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t 
 extern "C" int fim_orthogonalize(const void* g, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
                                  float b, float c, double eps, void* out, int out_dtype, void* workspace,
                                  int64_t workspace_bytes, hipStream_t stream) {
-  const OrthoScalars k{0.0f, 1.0f, a, b, c, eps, steps, 0, 0};
+  const OrthoScalars k{0.0f, 1.0f, a, b, c, 0.0f, 0.0f, 0.0f, eps, steps, 0, 0};
   return ortho_run(OrthoCall{1, &g, &dtype, nullptr, &out, &out_dtype, &batch, &rows, &cols, nullptr}, k, workspace,
                    workspace_bytes, stream);
 }
@@ -362,7 +376,7 @@ extern "C" int fim_muon_step(int64_t count, void* const* params, const int* para
                              float a, float b, float c, double eps, void* workspace, int64_t workspace_bytes,
                              hipStream_t stream) {
   if (count > 0 && (momenta == nullptr || factors == nullptr)) return FIM_ERR_INVALID;
-  const OrthoScalars k{momentum, keep, a, b, c, eps, steps, nesterov, 1};
+  const OrthoScalars k{momentum, keep, a, b, c, 0.0f, 0.0f, 0.0f, eps, steps, nesterov, 1};
   return ortho_run(OrthoCall{count, grads, grad_dtypes, momenta, params, param_dtypes, batch, rows, cols, factors}, k, workspace,
                    workspace_bytes, stream);
 }

@@ -89,8 +89,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   sq = red[0];
 #pragma unroll
   for (int i = 1; i < SMALL_WAVES; ++i) sq += red[i];
-  const float scale = (float)((double)ORTHO_S / (sqrt(sq) + k.eps));
-  // -- S X0 as halves, line by line in place: 8 lanes a line, all of which read before one writes
+  const float scale = (float)((double)k.sx / (sqrt(sq) + k.eps));
+  // -- sx X0 as halves, line by line in place: 8 lanes a line, all of which read before one writes
   for (int i = tid; i < MP * nb * 8; i += 64 * SMALL_WAVES) {
     const int q = i & 7, line = i >> 3, r = line / nb;
     uint8_t* at = X + line * 128;
@@ -142,6 +142,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     }
   };
   const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float gram_scale = k.sa / (k.sx * k.sx), apply_scale = 1.0f / k.sp, last_scale = apply_scale / k.sx;
+  const float sq_scale = k.c * k.sp / (k.sa * k.sa), old_scale = k.b * k.sp / k.sa;
 
   for (int it = 0; it < k.steps; ++it) {
     // -- A = X X^T: this wavefront's lines, all pairs of row blocks
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
         for (int j = 0; j <= i; ++j, ++q) {
           float v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = acc[q][u] * (1.0f / ORTHO_S);
+          for (int u = 0; u < 4; ++u) v[u] = acc[q][u] * gram_scale;
           put(A, 16 * i + l16, 16 * j + 4 * g, v, i != j);
         }
     }
@@ -217,8 +219,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
                 *reinterpret_cast<const v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2), old);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            v[u] = fmaf(k.c / ORTHO_S, w[u], k.b * old[u]);
-            if (r == c + u) v[u] += k.a * ORTHO_S;
+            v[u] = fmaf(sq_scale, w[u], old_scale * old[u]);
+            if (r == c + u) v[u] += k.a * k.sp;
           }
           put(P, r, c, v, i != j);
         }
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
         float v[4];
         if (last) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * (1.0f / (ORTHO_S * ORTHO_S));
+          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * last_scale;
           if (s.tall) {
             if (r < cols) {
 #pragma unroll
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
           }
         } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * (1.0f / ORTHO_S);
+          for (int u = 0; u < 4; ++u) v[u] = y[i][u] * apply_scale;
           v2i hi, lo;
           split4(v, hi, lo);
           uint8_t* at = X + r * ld + (c >> 5) * 128;

@@ -176,7 +176,9 @@ __global__ __launch_bounds__(256, MB > 2 ? 1 : 2) void ortho_tile_kernel(const O
   }
   __builtin_amdgcn_s_waitcnt(tile_wait(0));
 
-  // -- epilogue
+  // -- epilogue; exact scales but for c's and b's own factors
+  const float gram_scale = k.sa / (k.sx * k.sx), apply_scale = 1.0f / k.sp, last_scale = apply_scale / k.sx;
+  const float sq_scale = k.c * k.sp / (k.sa * k.sa), old_scale = k.b * k.sp / k.sa;
   uint8_t* to = (MODE == ORTHO_GRAM ? s.a : MODE == ORTHO_SQUARE ? s.p : s.x[1 - src]) + at;
   const int cols = SYM ? mp : np, ld = cols * 4;
 #pragma unroll
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(256, MB > 2 ? 1 : 2) void ortho_tile_kernel(const O
         for (int u = 0; u < 4; ++u) v[u] = acc[i][j][4 * q + u];
         if constexpr (MODE == ORTHO_LAST) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] *= 1.0f / (ORTHO_S * ORTHO_S);
+          for (int u = 0; u < 4; ++u) v[u] *= last_scale;
           const int64_t base = (int64_t)b * s.rows * s.cols;
           if (s.tall) {
             if (row < (int)s.cols) {
@@ -214,12 +216,12 @@ __global__ __launch_bounds__(256, MB > 2 ? 1 : 2) void ortho_tile_kernel(const O
             join4(*reinterpret_cast<const v2i*>(from), *reinterpret_cast<const v2i*>(from + 64), old);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-              v[u] = fmaf(k.c / ORTHO_S, v[u], k.b * old[u]);
-              if (row == col + u) v[u] += k.a * ORTHO_S;
+              v[u] = fmaf(sq_scale, v[u], old_scale * old[u]);
+              if (row == col + u) v[u] += k.a * k.sp;
             }
           } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] *= 1.0f / ORTHO_S;
+            for (int u = 0; u < 4; ++u) v[u] *= MODE == ORTHO_GRAM ? gram_scale : apply_scale;
           }
           v2i hi, lo;
           split4(v, hi, lo);
