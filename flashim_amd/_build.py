@@ -24,7 +24,7 @@ LIBRARY = PACKAGE / "libflashim_amd.so"
 HOST_LIBRARY = PACKAGE / "libfim_host.so"
 DEVICE_SOURCES = (
     "quantize.hip", "igemm.hip", "deep_plan.hip", "deep_int8.hip", "deep_mx.hip", "depthwise.hip", "dwpw.hip", "mlp.hip",
-    "stem.hip", "pointwise.hip", "norm.hip", "gated.hip", "clip.hip", "ortho.hip", "version.hip",
+    "stem.hip", "pointwise.hip", "norm.hip", "gated.hip", "clip.hip", "ortho.hip", "adapters.hip", "version.hip",
 )
 PROBE_LIBRARY = PACKAGE / "libflashim_amd_probe.so"
 PROBE_SOURCES = ("probe.hip", "deep_plan.hip")

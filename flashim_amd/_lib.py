@@ -81,6 +81,11 @@ SIGNATURES: dict[str, list] = {
     "fim_muon_step_workspace": [_i64, _vp, _vp, _vp, _vp],
     "fim_muon_step": [_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _i32, _f32, _f32, _f32, _f64, _vp,
                       _i64, _vp],
+    "fim_low_rank_adapters": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _f32, _vp,
+                              _vp, _vp],
+    "fim_low_rank_adapters_backward_workspace": [_i64, _i64, _i64, _i64, _i64, _vp],
+    "fim_low_rank_adapters_backward": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp,
+                                       _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "fim_clip_grad_norm": [_i64, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _vp, _vp, _vp],
 }
 

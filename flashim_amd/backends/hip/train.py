@@ -5,7 +5,8 @@ them; here they train a channels-last block before it is quantized, and run it u
 * ``gated_linear``: the gated feed-forward product, both projections, activation and product in one kernel, with its
   gradients;
 * ``grad_norm`` and ``clip_grad_norm_``: the global norm of many gradients, and clipping by it;
-* ``orthogonalize`` and ``muon_step_``: matrices orthogonalized by Newton-Schulz products, and the optimizer step made of them.
+* ``orthogonalize`` and ``muon_step_``: matrices orthogonalized by Newton-Schulz products, and the optimizer step made of them;
+* ``low_rank_adapters``: low-rank adapters of many requests beside a shared projection, with their gradients.
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _HALVES = (torch.bfloat16, torch.float16)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # the C ABI's codes
 MAX_CHANNELS = 8192  # of group_norm_act
+MAX_RANK = 128  # of low_rank_adapters
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # orthogonalize's coefficients: steepest at 0, within 0.7 .. 1.2 near 1
 ADJUST = {"original": 0, "match_rms": 1, "none": 2}  # muon_step_'s factors
 
@@ -85,6 +87,18 @@ def muon_step_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seque
         library.muon_step_(params, grads, momenta, lr, momentum, nesterov, weight_decay, ADJUST[adjust], steps, a, b, c, eps)
 
 
+def low_rank_adapters(base: Tensor | None, x: Tensor, a: Tensor, b: Tensor, index: Tensor, *,
+                      scale: float | Tensor = 1.0) -> Tensor:
+    """``base + s_j (x A_j^T) B_j^T`` for each row of ``x`` ``[..., K]``, beside a shared projection's output ``base``
+    ``[..., N]`` (None: zeros) of any kind. ``a`` ``[J, R, K]`` and ``b`` ``[J, N, R]`` (rank ``R`` at most 128), all BF16 or
+    all FP16; ``index`` (int32 or int64) has the shape of some of ``x``'s leading dimensions and names each entry's adapter:
+    one a row, or one an image, or one for all. A value outside ``[0, J)`` means none: the row keeps ``base``. ``scale``: a
+    number, or FP32 ``[J]``. FP32 sums, rounded once. Differentiable in ``base``, ``x``, ``a`` and ``b``."""
+    scales, factor = (scale, 1.0) if isinstance(scale, Tensor) else (None, float(scale))
+    save = torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)
+    return library.low_rank_adapters(base, x, a, b, index, scales, factor, save)[0]
+
+
 # -- eligibility -------------------------------------------------------------------------------------------------------
 
 
@@ -143,3 +157,17 @@ def eligible_muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=Tr
                        coefficients=NEWTON_SCHULZ, eps=1e-7) -> bool:
     return (all(_tensors(t) and len(t) == len(params) for t in (params, grads, momenta)) and is_gfx950(params[0].device)
             and params[0].dtype in _FLOATS and adjust in ADJUST and _polynomial(steps, coefficients, eps))
+
+
+def eligible_low_rank_adapters(base, x, a, b, index, *, scale=1.0) -> bool:
+    return (
+        isinstance(x, Tensor) and is_gfx950(x.device) and x.ndim >= 1 and x.dtype in _HALVES and x.shape[-1] > 0
+        and all(isinstance(t, Tensor) and t.ndim == 3 and t.dtype == x.dtype and t.device == x.device for t in (a, b))
+        and a.shape[2] == x.shape[-1] and b.shape[0] == a.shape[0] > 0 and b.shape[2] == a.shape[1] and b.shape[1] > 0
+        and 0 < a.shape[1] <= MAX_RANK
+        and (base is None or (isinstance(base, Tensor) and base.dtype == x.dtype and base.device == x.device
+                              and base.shape == (*x.shape[:-1], b.shape[1])))
+        and isinstance(index, Tensor) and index.dtype in (torch.int32, torch.int64) and index.device == x.device
+        and index.ndim < x.ndim and index.shape == x.shape[:index.ndim]
+        and (not isinstance(scale, Tensor) or _vector(scale, a.shape[0], x, (torch.float32,)))
+    )

@@ -1,0 +1,178 @@
+// Low-rank adapters of many requests beside a shared projection: out = base + s_j (x A_j^T) B_j^T, j by row or by leading entry, and
+// the gradients of x, A and B (formulas and layouts: adapters_rows.h, adapters_grad.h).
+#include <type_traits>
+
+#include "adapters_grad.h"
+#include "adapters_rows.h"
+#include "gated_plan.h"
+
+namespace fim {
+
+constexpr int ADAPTER_RANK = 128;
+
+static int adapter_blocks(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }  // of 16 ranks, as compiled
+
+struct AdapterSizes {
+  int64_t M, K, N, J, R, entries;
+};
+
+static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
+  if (s.M < 0 || s.K < 1 || s.N < 1 || s.J < 1 || s.R < 1 || s.entries < 0 || (wide != 0 && wide != 1)) return FIM_ERR_INVALID;
+  if (s.M > 0 && (s.entries < 1 || s.M % s.entries != 0)) return FIM_ERR_INVALID;
+  if (dtype != FIM_BF16 && dtype != FIM_F16) return dtype == FIM_F32 ? FIM_ERR_UNSUPPORTED : FIM_ERR_INVALID;
+  constexpr int64_t most = int64_t{1} << 31;
+  if (s.R > ADAPTER_RANK || s.M >= most / 2 || s.K >= 1 << 24 || s.N >= 1 << 24 || s.J >= 1 << 20 || s.J * s.R >= most ||
+      s.J * (s.K + s.N) >= most)
+    return FIM_ERR_UNSUPPORTED;
+  return FIM_OK;
+}
+
+// Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of 16 would
+// go through them one after the other. Else tiles of 16 rows, four wavefronts each until tiles fill the CUs.
+template <int DT, int NR>
+static void launch_rows(AdapterArgs& p, hipStream_t stream) {
+  const int64_t cus = device_cus(), blocks = cdiv(p.N, 32);
+  const bool one = p.index.per < 16 && p.M <= 512;
+  const int64_t tiles = one ? p.M : cdiv(p.M, 16);
+  const bool four = one || tiles < 8 * cus;
+  // parts of the columns: enough wavefronts for the card, each with four blocks at least
+  int64_t parts = cdiv(8 * cus, tiles * (four ? 4 : 1));
+  const int64_t most = cdiv(blocks, four ? 16 : 4);
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  p.parts = (int)(four ? 4 * parts : parts);
+  const dim3 grid((unsigned)(four ? tiles : cdiv(tiles, 4)), (unsigned)parts);
+  if (one) adapter_rows_kernel<DT, NR, 4, true><<<grid, dim3(256), 0, stream>>>(p);
+  else if (four) adapter_rows_kernel<DT, NR, 4, false><<<grid, dim3(256), 0, stream>>>(p);
+  else adapter_rows_kernel<DT, NR, 1, false><<<grid, dim3(256), 0, stream>>>(p);
+}
+
+template <typename F>
+static void by_type(int dtype, int64_t R, F&& f) {
+  auto ranks = [&](auto dt) {
+    switch (adapter_blocks(R)) {
+      case 1: return f(dt, std::integral_constant<int, 1>{});
+      case 2: return f(dt, std::integral_constant<int, 2>{});
+      case 4: return f(dt, std::integral_constant<int, 4>{});
+      default: return f(dt, std::integral_constant<int, 8>{});
+    }
+  };
+  if (dtype == FIM_BF16) ranks(std::integral_constant<int, FIM_BF16>{});
+  else ranks(std::integral_constant<int, FIM_F16>{});
+}
+
+static void adapter_rows(AdapterArgs& p, int dtype, hipStream_t stream) {
+  by_type(dtype, p.R, [&](auto dt, auto nr) { launch_rows<decltype(dt)::value, decltype(nr)::value>(p, stream); });
+}
+
+struct AdapterGradPlan {
+  int64_t chunk, chunks, at, bt, t, part, counts, bytes;
+  int xt, ct;
+};
+
+static AdapterGradPlan grad_plan(const AdapterSizes& s) {
+  AdapterGradPlan g;
+  g.xt = (int)cdiv(s.K, GRAD_COLS);
+  g.ct = g.xt + (int)cdiv(s.N, GRAD_COLS);
+  // workgroups for the card if all adapters have rows in every chunk; 256 rows a chunk at least
+  int64_t chunks = cdiv(8 * (int64_t)device_cus(), g.ct * s.J);
+  if (chunks > cdiv(s.M, 256)) chunks = cdiv(s.M, 256);
+  if (chunks < 1) chunks = 1;
+  g.chunk = cdiv(cdiv(s.M, chunks), 256) * 256;
+  if (g.chunk > GRAD_CHUNK) g.chunk = GRAD_CHUNK;
+  if (g.chunk < 256) g.chunk = 256;
+  g.chunks = cdiv(s.M, g.chunk);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += align256(bytes);
+    return from;
+  };
+  g.at = take(s.J * s.R * s.K * 2);
+  g.bt = take(s.J * s.R * s.N * 2);
+  g.t = take(s.M * 16 * adapter_blocks(s.R) * 4);
+  g.part = take(g.chunks > 1 ? s.J * g.chunks * s.R * (s.K + s.N) * 4 : 0);
+  g.counts = take(g.chunks > 1 ? s.J * g.chunks * 4 : 0);
+  g.bytes = at;
+  return g;
+}
+
+}  // namespace fim
+
+using namespace fim;
+
+extern "C" int fim_low_rank_adapters(const void* base, int64_t base_stride, const void* x, int64_t x_stride, int dtype, int64_t M,
+                                     int64_t K, int64_t N, const void* a, const void* b, int64_t J, int64_t R,
+                                     const void* index, int index_wide, int64_t entries, const float* scales, float scale,
+                                     void* out, float* h, hipStream_t stream) {
+  const AdapterSizes s{M, K, N, J, R, entries};
+  const int rc = adapter_check(s, dtype, index_wide);
+  if (rc != FIM_OK) return rc;
+  if (M == 0) return FIM_OK;
+  if (x == nullptr || a == nullptr || b == nullptr || index == nullptr || out == nullptr) return FIM_ERR_INVALID;
+  for (const void* t : {base, x, a, b, static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(t) % 2) return FIM_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(index) % (index_wide ? 8 : 4) || reinterpret_cast<uintptr_t>(h) % 16) return FIM_ERR_INVALID;
+  AdapterArgs p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(base), static_cast<const uint16_t*>(a),
+                static_cast<const uint16_t*>(b), x_stride, base_stride, static_cast<uint16_t*>(out), h,
+                AdapterIndex{index, index_wide, (uint32_t)(M / entries), (int)J}, scales, scale, (uint32_t)M, (int)K, (int)N,
+                (int)R, 1};
+  adapter_rows(p, dtype, stream);
+  return launch_status();
+}
+
+extern "C" int fim_low_rank_adapters_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t J, int64_t R, int64_t* bytes) {
+  if (bytes == nullptr) return FIM_ERR_INVALID;
+  const AdapterSizes s{M, K, N, J, R, M};
+  const int rc = adapter_check(s, FIM_BF16, 0);
+  if (rc != FIM_OK) return rc;
+  *bytes = M > 0 ? grad_plan(s).bytes : 0;
+  return FIM_OK;
+}
+
+extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_stride, const void* x, int64_t x_stride, int dtype,
+                                              int64_t M, int64_t K, int64_t N, const void* a, const void* b, int64_t J, int64_t R,
+                                              const void* index, int index_wide, int64_t entries, const float* scales, float scale,
+                                              const float* h, void* dx, void* da, void* db, void* workspace,
+                                              int64_t workspace_bytes, hipStream_t stream) {
+  const AdapterSizes s{M, K, N, J, R, entries};
+  int rc = adapter_check(s, dtype, index_wide);
+  if (rc != FIM_OK) return rc;
+  if (M == 0) return FIM_ERR_INVALID;  // (there is no row to sum over: the caller's zeros)
+  if (d_out == nullptr || x == nullptr || a == nullptr || b == nullptr || index == nullptr || (da == nullptr) != (db == nullptr) ||
+      (da != nullptr && h == nullptr))
+    return FIM_ERR_INVALID;
+  for (const void* t : {d_out, x, a, b, static_cast<const void*>(dx), static_cast<const void*>(da), static_cast<const void*>(db)})
+    if (reinterpret_cast<uintptr_t>(t) % 2) return FIM_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(index) % (index_wide ? 8 : 4) || reinterpret_cast<uintptr_t>(h) % 16) return FIM_ERR_INVALID;
+  const AdapterGradPlan g = grad_plan(s);
+  if (workspace == nullptr || workspace_bytes < g.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return FIM_ERR_INVALID;
+  if (dx == nullptr && da == nullptr) return FIM_OK;
+  const int64_t na = J * R * K, nb = J * R * N, outputs = J * R * (K + N);
+  if (cdiv(na + nb, 256) >= int64_t{1} << 31 || J * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint16_t *at = reinterpret_cast<uint16_t*>(ws + g.at), *bt = reinterpret_cast<uint16_t*>(ws + g.bt);
+  float* t = reinterpret_cast<float*>(ws + g.t);
+  const AdapterIndex rows{index, index_wide, (uint32_t)(M / entries), (int)J};
+  adapter_transpose_kernel<<<dim3((unsigned)cdiv(na + nb, 256)), dim3(256), 0, stream>>>(
+      static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), at, bt, (int)K, (int)N, (int)R, na, nb);
+  // t = s d_out B and dx = t A: the forward pass over d_out (without dx: over one column)
+  AdapterArgs p{static_cast<const uint16_t*>(d_out), nullptr, bt, at, d_out_stride, 0, static_cast<uint16_t*>(dx), t, rows, scales,
+                scale, (uint32_t)M, (int)N, dx == nullptr ? 0 : (int)K, (int)R, 1};
+  adapter_rows(p, dtype, stream);
+  if (da != nullptr) {
+    float* part = g.chunks > 1 ? reinterpret_cast<float*>(ws + g.part) : nullptr;
+    int* counts = g.chunks > 1 ? reinterpret_cast<int*>(ws + g.counts) : nullptr;
+    const AdapterGradArgs q{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(d_out), x_stride, d_out_stride, t, h, rows,
+                            static_cast<uint16_t*>(da), static_cast<uint16_t*>(db), part, counts, (uint32_t)M, (uint32_t)g.chunk,
+                            (int)g.chunks, (int)K, (int)N, (int)R, g.xt, g.ct};
+    by_type(dtype, R, [&](auto dt, auto nr) {
+      constexpr int DT = decltype(dt)::value;
+      adapter_grad_kernel<DT, decltype(nr)::value><<<dim3((unsigned)(J * g.chunks * g.ct)), dim3(256), 0, stream>>>(q);
+      if (part != nullptr)
+        adapter_join_kernel<DT><<<dim3((unsigned)cdiv(outputs, 256)), dim3(256), 0, stream>>>(
+            part, counts, (int)g.chunks, (int)J, (int)K, (int)N, (int)R, q.da, q.db);
+    });
+  }
+  return launch_status();
+}

@@ -814,6 +814,99 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   }
 }
 
+// -- low-rank adapters ------------------------------------------------------------------------------------------------
+
+struct Adapters {
+  Tensor x, a, b, index;
+  OptTensor scales;
+  int64_t m, k, n, j, r, entries;
+  bool wide;
+  Adapters(const Tensor& x_in, const Tensor& a_in, const Tensor& b_in, const Tensor& index_in, const OptTensor& scales_in) {
+    x = matrix_rows(x_in, "low_rank_adapters");
+    m = x.size(0);
+    k = x.size(1);
+    check_dims(a_in, 3, "low_rank_adapters: a");
+    check_dims(b_in, 3, "low_rank_adapters: b");
+    j = a_in.size(0);
+    r = a_in.size(1);
+    n = b_in.size(1);
+    TORCH_CHECK_VALUE(a_in.size(2) == k && b_in.size(0) == j && b_in.size(2) == r, "low_rank_adapters: adapters of shape ",
+                      a_in.sizes(), " and ", b_in.sizes(), " for ", k, " channels");
+    check_same(a_in, x.scalar_type(), x, "low_rank_adapters: a");
+    check_same(b_in, x.scalar_type(), x, "low_rank_adapters: b");
+    TORCH_CHECK_TYPE(index_in.scalar_type() == at::kInt || index_in.scalar_type() == at::kLong,
+                     "low_rank_adapters: an index of ", index_in.scalar_type());
+    TORCH_CHECK_VALUE(index_in.device() == x.device() && index_in.dim() < x_in.dim() &&
+                          index_in.sizes() == x_in.sizes().slice(0, index_in.dim()),
+                      "low_rank_adapters: an index of shape ", index_in.sizes(), " for ", x_in.sizes());
+    check_vector(scales_in, j, x, "low_rank_adapters: scale");
+    TORCH_CHECK_TYPE(!scales_in || scales_in->scalar_type() == at::kFloat, "low_rank_adapters: scales of ",
+                     scales_in->scalar_type());
+    a = a_in.contiguous();
+    b = b_in.contiguous();
+    index = index_in.contiguous();
+    scales = dense(scales_in);
+    entries = index.numel();
+    wide = index.scalar_type() == at::kLong;
+  }
+  int64_t ranks() const { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+};
+
+std::tuple<Tensor, Tensor> low_rank_adapters(const OptTensor& base, const Tensor& x, const Tensor& a, const Tensor& b,
+                                             const Tensor& index, const OptTensor& scales, double scale, bool save) {
+  const c10::DeviceGuard guard(x.device());
+  const Adapters g(x, a, b, index, scales);
+  const auto sizes = with_last(x, g.n);
+  Tensor rows;
+  if (base) {
+    TORCH_CHECK_VALUE(base->sizes() == at::IntArrayRef(sizes), "low_rank_adapters: a base of shape ", base->sizes(), ", expected ",
+                      at::IntArrayRef(sizes));
+    check_same(*base, x.scalar_type(), x, "low_rank_adapters: base");
+    rows = matrix_rows(*base, "low_rank_adapters");
+  }
+  Tensor out = empty(sizes, x, x.scalar_type());
+  Tensor h = save ? empty({g.m, g.ranks()}, x, at::kFloat) : empty({0}, x, at::kFloat);
+  check(fim_low_rank_adapters(base ? rows.data_ptr() : nullptr, base ? rows.stride(0) : 0, g.x.data_ptr(), g.x.stride(0),
+                              dtype_code(x), g.m, g.k, g.n, g.a.data_ptr(), g.b.data_ptr(), g.j, g.r, g.index.data_ptr(), g.wide,
+                              g.entries, ptr<const float>(g.scales), (float)scale, out.data_ptr(), save ? ptr<float>(h) : nullptr,
+                              stream_of(x)),
+        "low_rank_adapters ", x.sizes(), " x ", a.sizes(), " -> ", g.n);
+  return {out, h};
+}
+
+// Gradients that are not wanted come back empty.
+std::tuple<Tensor, Tensor, Tensor> low_rank_adapters_backward(const Tensor& d_out, const Tensor& x, const Tensor& a,
+                                                              const Tensor& b, const Tensor& index, const OptTensor& scales,
+                                                              double scale, const Tensor& h, bool want_x, bool want_adapters) {
+  const c10::DeviceGuard guard(x.device());
+  const Adapters g(x, a, b, index, scales);
+  TORCH_CHECK_VALUE(d_out.sizes() == at::IntArrayRef(with_last(x, g.n)), "low_rank_adapters: gradient of shape ", d_out.sizes(),
+                    " for ", x.sizes(), " -> ", g.n);
+  check_same(d_out, x.scalar_type(), x, "low_rank_adapters: gradient");
+  if (want_adapters) {
+    check_same(h, at::kFloat, x, "low_rank_adapters: saved products");
+    TORCH_CHECK_VALUE(h.dim() == 2 && h.size(0) == g.m && h.size(1) == g.ranks() && h.is_contiguous(),
+                      "low_rank_adapters: saved products of shape ", h.sizes());
+  }
+  const Tensor d = matrix_rows(d_out, "low_rank_adapters");
+  auto grad = [](const Tensor& t, bool want) { return want ? empty(t.sizes(), t, t.scalar_type()) : empty({0}, t, t.scalar_type()); };
+  Tensor dx = grad(x, want_x), da = grad(a, want_adapters), db = grad(b, want_adapters);
+  if (g.m == 0) {
+    for (Tensor* t : {&da, &db}) t->zero_();
+    return {dx, da, db};
+  }
+  int64_t bytes = 0;
+  check(fim_low_rank_adapters_backward_workspace(g.m, g.k, g.n, g.j, g.r, &bytes), "low_rank_adapters backward");
+  const Tensor ws = empty({bytes}, x, at::kByte);
+  check(fim_low_rank_adapters_backward(d.data_ptr(), d.stride(0), g.x.data_ptr(), g.x.stride(0), dtype_code(x), g.m, g.k, g.n,
+                                       g.a.data_ptr(), g.b.data_ptr(), g.j, g.r, g.index.data_ptr(), g.wide, g.entries,
+                                       ptr<const float>(g.scales), (float)scale, want_adapters ? ptr<float>(h) : nullptr,
+                                       want_x ? dx.data_ptr() : nullptr, want_adapters ? da.data_ptr() : nullptr,
+                                       want_adapters ? db.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(x)),
+        "low_rank_adapters backward ", x.sizes(), " x ", a.sizes(), " -> ", g.n);
+  return {dx, da, db};
+}
+
 }  // namespace
 
 #define FIM_GEO_SCHEMA "SymInt kh, SymInt kw, SymInt sh, SymInt sw, SymInt ph, SymInt pw, SymInt dh, SymInt dw"
@@ -858,6 +951,8 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   X(gated_linear_backward, "(Tensor d_out, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "       \
                            "int act, bool want_x, bool want_weights, bool want_biases) "                               \
                            "-> (Tensor, Tensor, Tensor, Tensor, Tensor)")                                              \
+  X(low_rank_adapters_backward, "(Tensor d_out, Tensor x, Tensor a, Tensor b, Tensor index, Tensor? scales, "          \
+                                "float scale, Tensor h, bool want_x, bool want_adapters) -> (Tensor, Tensor, Tensor)") \
   X(grad_norm, "(Tensor[] grads, float norm_type) -> Tensor")                                                          \
   X(orthogonalize, "(Tensor g, int steps, float a, float b, float c, float eps, ScalarType? out_dtype) -> Tensor")
 
@@ -868,7 +963,9 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   X(muon_step_, "(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, float lr, float momentum, bool nesterov, " \
                 "float weight_decay, int adjust, int steps, float a, float b, float c, float eps) -> ()")              \
   X(group_norm_act, "(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act) -> (Tensor, Tensor)")    \
-  X(gated_linear, "(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor")
+  X(gated_linear, "(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor")           \
+  X(low_rank_adapters, "(Tensor? base, Tensor x, Tensor a, Tensor b, Tensor index, Tensor? scales, float scale, "      \
+                       "bool save) -> (Tensor, Tensor)")
 
 TORCH_LIBRARY(flashim_amd, m) {
 #define X(name, schema) m.def(#name schema, {at::Tag::pt2_compliant_tag});
@@ -1089,6 +1186,55 @@ Tensor gated_linear_autograd(const Tensor& x, const Tensor& w_gate, const Tensor
   return GatedLinear::apply(x, w_gate, w_up, b_gate, b_up, act);
 }
 
+struct LowRankAdapters : torch::autograd::Function<LowRankAdapters> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const OptTensor& base, const Tensor& x,
+                                                const Tensor& a, const Tensor& b, const Tensor& index, const OptTensor& scales,
+                                                double scale, bool save) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(low_rank_adapters)>("flashim_amd::low_rank_adapters");
+    auto [out, h] = op.call(base, x, a, b, index, scales, scale, save);
+    ctx->save_for_backward({x, a, b, index, as_tensor(scales), h});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["base"] = base && base->defined();
+    ctx->mark_non_differentiable({h});
+    return {out, h};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list result(8);
+    if (!grads[0].defined()) return result;
+    refuse_tangent(grads[0], "low_rank_adapters");
+    const auto saved = ctx->get_saved_variables();
+    const int first = ctx->saved_data["base"].toBool();  // (the edges count the tensors that are there)
+    const bool want_x = ctx->needs_input_grad(first), want_ab = ctx->needs_input_grad(first + 1) || ctx->needs_input_grad(first + 2);
+    if (first && ctx->needs_input_grad(0)) result[0] = grads[0];
+    if (!want_x && !want_ab) return result;
+    std::optional<at::AutoDispatchBelowAutograd> below;  // (nothing is recorded: past the refusal of second derivatives)
+    if (!at::GradMode::is_enabled()) below.emplace();
+    static const auto op = typed_op<decltype(low_rank_adapters_backward)>("flashim_amd::low_rank_adapters_backward");
+    auto [dx, da, db] = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], as_optional(saved[4]),
+                                ctx->saved_data["scale"].toDouble(), saved[5], want_x, want_ab);
+    if (want_x) result[1] = dx;
+    if (want_ab) {
+      result[2] = da;
+      result[3] = db;
+    }
+    return result;
+  }
+};
+
+std::tuple<Tensor, Tensor> low_rank_adapters_autograd(const OptTensor& base, const Tensor& x, const Tensor& a, const Tensor& b,
+                                                      const Tensor& index, const OptTensor& scales, double scale, bool save) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!records(scales), "low_rank_adapters: no derivative of the scales, and they require one");
+  if (!records(base, x, a, b)) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = typed_op<decltype(low_rank_adapters)>("flashim_amd::low_rank_adapters");
+    return op.call(base, x, a, b, index, scales, scale, save);
+  }
+  auto out = LowRankAdapters::apply(base, x, a, b, index, scales, scale, save || a.requires_grad() || b.requires_grad());
+  return {out[0], out[1]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
@@ -1097,6 +1243,7 @@ TORCH_LIBRARY_IMPL(flashim_amd, Autograd, m) {
 #undef X
   m.impl("group_norm_act", TORCH_FN(group_norm_act_autograd));
   m.impl("gated_linear", TORCH_FN(gated_linear_autograd));
+  m.impl("low_rank_adapters", TORCH_FN(low_rank_adapters_autograd));
   m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_autograd_));
   m.impl("clip_grad_norm_out", TORCH_FN(clip_grad_norm_out_autograd));
   m.impl("muon_step_", TORCH_FN(muon_step_autograd_));

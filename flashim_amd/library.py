@@ -292,6 +292,26 @@ def muon_step_(params, grads, momenta, lr, momentum, nesterov, weight_decay, adj
     return None
 
 
+@_fake
+def low_rank_adapters(base, x, a, b, index, scales, scale, save):
+    """``base + s (x A^T) B^T`` by row, and (``save``) ``s x A^T`` in FP32, which the backward pass reads; differentiable in
+    ``base``, ``x``, ``a`` and ``b``."""
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty((*x.shape[:-1], b.shape[1])),
+            x.new_empty((rows, _ranks(a.shape[1])) if save else (0,), dtype=torch.float32))
+
+
+@_fake
+def low_rank_adapters_backward(d_out, x, a, b, index, scales, scale, h, want_x, want_adapters):
+    """The gradients of x, a and b; those not wanted come back empty."""
+    return (x.new_empty(x.shape if want_x else (0,)), *(t.new_empty(t.shape if want_adapters else (0,)) for t in (a, b)))
+
+
+def _ranks(rank):
+    """Ranks that the kernels compute: 16, 32, 64 or 128."""
+    return 16 if rank <= 16 else 32 if rank <= 32 else 64 if rank <= 64 else 128
+
+
 def clip_lists(grads, out, max_norm: float, norm_type: float):
     """``clip_grad_norm_(grads, ...)`` (``out`` None) or ``clip_grad_norm_out(grads, out, ...)``. Eager lists of plain tensors
     take the library's own entry to those ops, 320 tensors into as many in 65 us of host time instead of 93."""
@@ -312,9 +332,10 @@ def _clip_lists():
 
 
 # ``torch.ops.flashim_amd`` is there on import. A library that is built later is loaded on first use, and so is one that
-# does not load now (built against another torch, a missing HIP runtime): the first op raises the loader's error.
+# does not load now (built against another torch or from older sources, a missing HIP runtime): the first op raises the
+# loader's error.
 if TORCH_LIBRARY.is_file():
     try:
         load()
-    except OSError as error:
+    except (OSError, RuntimeError) as error:
         logger.warning("%s does not load: %s", TORCH_LIBRARY, error)

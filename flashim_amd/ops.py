@@ -49,6 +49,8 @@ grad_norm = Op("grad_norm")
 clip_grad_norm_ = Op("clip_grad_norm_")
 orthogonalize = Op("orthogonalize")
 muon_step_ = Op("muon_step_")
+# this backend's low-rank adapters beside a shared projection (differentiable)
+low_rank_adapters = Op("low_rank_adapters")
 
 ROCM = DeviceSpec("rocm")
 HIP = "hip"
@@ -86,6 +88,7 @@ IMPLS = (
     ("clip_grad_norm_", _train.clip_grad_norm_, (Feature.HIP,), _train.eligible_clip_grad_norm),
     ("orthogonalize", _train.orthogonalize, (Feature.HIP,), _train.eligible_orthogonalize),
     ("muon_step_", _train.muon_step_, (Feature.HIP,), _train.eligible_muon_step),
+    ("low_rank_adapters", _train.low_rank_adapters, (Feature.HIP,), _train.eligible_low_rank_adapters),
 )
 
 for _name, _fn, _requires, _when in IMPLS:

@@ -154,3 +154,53 @@ def schulz_bound(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: flo
         # (the step's own slope is in the sum above: what is left are the steps after it; X_0's conversion meets all of them)
         total += e * x.norm().item() * slopes[-2 if k else -1]
     return total
+
+
+def _sum_error(n: int) -> float:
+    """Of FP32 sums of n terms, relative to the terms' magnitudes: independent roundings of 2^-24, four standard deviations."""
+    return 4 * math.sqrt(n + 4) * 2.0**-24
+
+
+def low_rank_adapters(base: Tensor | None, x: Tensor, a: Tensor, b: Tensor, index: Tensor, scale, d_out: Tensor | None = None,
+                      half: float = 2.0**-16) -> dict[str, Tensor]:
+    """``out`` and, with ``d_out``, the gradients ``x``, ``a``, ``b``, float64, row by row; ``*_error`` what FP32 sums and a
+    product's operand kept to ``half`` may change. (``half`` covers operands of two 16-bit numbers, and 2^-20 of a row's largest
+    for FP16 values that are small beside it.)"""
+    k, n, (j, r) = x.shape[-1], b.shape[1], a.shape[:2]
+    rows = x.double().reshape(-1, k)
+    which = index.reshape(-1).repeat_interleave(rows.shape[0] // max(1, index.numel()))
+    scales = (scale.double() if isinstance(scale, Tensor) else torch.full((j,), float(scale), dtype=torch.float64))
+    d = None if d_out is None else d_out.double().reshape(-1, n)
+    out = torch.zeros(rows.shape[0], n, dtype=torch.float64) if base is None else base.double().reshape(-1, n).clone()
+    got = {"out": out, "out_error": 2.0**-24 * out.abs()}
+    if d is not None:
+        got |= {"x": torch.zeros_like(rows), "x_error": torch.zeros_like(rows)}
+        got |= {name + kind: torch.zeros_like(t, dtype=torch.float64) for name, t in (("a", a), ("b", b)) for kind in ("", "_error")}
+
+    def product(u, v, w, s, sums):  # s (u v^T) w^T, its error's bound, and the middle
+        mid, terms = s * u @ v.t(), abs(s) * (u.abs() @ v.abs().t())
+        off = (_sum_error(sums) + 2.0**-23) * terms + half * mid.abs() + 2.0**-20 * mid.abs().amax(1, keepdim=True)
+        return mid @ w.t(), off @ w.abs().t() + _sum_error(r) * (mid.abs() @ w.abs().t()), mid, off
+
+    for i in range(j):
+        at = (which == i).nonzero().squeeze(1)
+        if at.numel() == 0:
+            continue
+        xi, ai, bi, s = rows[at], a[i].double(), b[i].double(), scales[i].item()
+        low, error, h, h_off = product(xi, ai, bi, s, k)
+        got["out"][at] += low
+        got["out_error"][at] += error + 2.0**-24 * low.abs()
+        if d is None:
+            continue
+        di = d[at]
+        got["x"][at], got["x_error"][at], t, t_off = product(di, bi.t(), ai.t(), s, n)
+        m = at.numel()
+        for name, u, u_off, v in (("a", t, t_off, xi), ("b", h, h_off, di)):
+            total = u.t() @ v
+            off = u_off.t() @ v.abs() + (_sum_error(m) + half) * (u.abs().t() @ v.abs())
+            got[name][i], got[name + "_error"][i] = (total, off) if name == "a" else (total.t(), off.t())
+    for name, shape in (("out", (*x.shape[:-1], n)), ("x", x.shape)):
+        for kind in ("", "_error"):
+            if name + kind in got:
+                got[name + kind] = got[name + kind].reshape(shape)
+    return got
