@@ -28,13 +28,15 @@ static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
 }
 
 // Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of 16 would
-// go through them one after the other. Else tiles of 16 rows, four wavefronts each until tiles fill the CUs.
+// go through them one after the other. Else tiles of 16 rows: four wavefronts each until tiles fill the CUs, and beyond that where
+// all four have a part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange
+// nothing (320000 x 64 -> 256 forward and dx: 77 us each, 106 with four).
 template <int DT, int NR>
 static void launch_rows(AdapterArgs& p, hipStream_t stream) {
   const int64_t cus = device_cus(), blocks = cdiv(p.N, 32);
   const bool one = p.index.per < 16 && p.M <= 512;
   const int64_t tiles = one ? p.M : cdiv(p.M, 16);
-  const bool four = one || tiles < 8 * cus;
+  const bool four = one || tiles < 8 * cus || (blocks >= 16 && p.K >= 128);
   // parts of the columns: enough wavefronts for the card, each with four blocks at least
   int64_t parts = cdiv(8 * cus, tiles * (four ? 4 : 1));
   const int64_t most = cdiv(blocks, four ? 16 : 4);
@@ -42,9 +44,14 @@ static void launch_rows(AdapterArgs& p, hipStream_t stream) {
   if (parts < 1) parts = 1;
   p.parts = (int)(four ? 4 * parts : parts);
   const dim3 grid((unsigned)(four ? tiles : cdiv(tiles, 4)), (unsigned)parts);
-  if (one) adapter_rows_kernel<DT, NR, 4, true><<<grid, dim3(256), 0, stream>>>(p);
-  else if (four) adapter_rows_kernel<DT, NR, 4, false><<<grid, dim3(256), 0, stream>>>(p);
-  else adapter_rows_kernel<DT, NR, 1, false><<<grid, dim3(256), 0, stream>>>(p);
+  auto launch = [&](auto quads) {
+    constexpr bool Q = decltype(quads)::value;
+    if (one) adapter_rows_kernel<DT, NR, 4, true, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else if (four) adapter_rows_kernel<DT, NR, 4, false, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else adapter_rows_kernel<DT, NR, 1, false, Q><<<grid, dim3(256), 0, stream>>>(p);
+  };
+  if (p.R % 4 == 0) launch(std::integral_constant<bool, true>{});
+  else launch(std::integral_constant<bool, false>{});
 }
 
 template <typename F>
@@ -74,9 +81,10 @@ static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   AdapterGradPlan g;
   g.xt = (int)cdiv(s.K, GRAD_COLS);
   g.ct = g.xt + (int)cdiv(s.N, GRAD_COLS);
-  // workgroups for the card if all adapters have rows in every chunk; 256 rows a chunk at least
-  int64_t chunks = cdiv(8 * (int64_t)device_cus(), g.ct * s.J);
-  if (chunks > cdiv(s.M, 256)) chunks = cdiv(s.M, 256);
+  // workgroups for the card where a chunk's rows have one adapter, but at most 64 MB of partial sums should they have all
+  int64_t chunks = cdiv(4 * (int64_t)device_cus(), g.ct);
+  const int64_t most = (int64_t{64} << 20) / (s.J * s.R * (s.K + s.N) * 4);
+  if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
   g.chunk = cdiv(cdiv(s.M, chunks), 256) * 256;
   if (g.chunk > GRAD_CHUNK) g.chunk = GRAD_CHUNK;
@@ -149,7 +157,7 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
   if (workspace == nullptr || workspace_bytes < g.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return FIM_ERR_INVALID;
   if (dx == nullptr && da == nullptr) return FIM_OK;
   const int64_t na = J * R * K, nb = J * R * N, outputs = J * R * (K + N);
-  if (cdiv(na + nb, 256) >= int64_t{1} << 31 || J * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
+  if (cdiv(na + nb, 64) >= int64_t{1} << 31 || J * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint16_t *at = reinterpret_cast<uint16_t*>(ws + g.at), *bt = reinterpret_cast<uint16_t*>(ws + g.bt);
   float* t = reinterpret_cast<float*>(ws + g.t);
@@ -170,7 +178,7 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
       constexpr int DT = decltype(dt)::value;
       adapter_grad_kernel<DT, decltype(nr)::value><<<dim3((unsigned)(J * g.chunks * g.ct)), dim3(256), 0, stream>>>(q);
       if (part != nullptr)
-        adapter_join_kernel<DT><<<dim3((unsigned)cdiv(outputs, 256)), dim3(256), 0, stream>>>(
+        adapter_join_kernel<DT><<<dim3((unsigned)cdiv(outputs, 64)), dim3(64 * JOIN_WAVES), 0, stream>>>(
             part, counts, (int)g.chunks, (int)J, (int)K, (int)N, (int)R, q.da, q.db);
     });
   }

@@ -172,18 +172,36 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
   }
 }
 
-// The chunks' partial sums, added up in order
+// The chunks' partial sums, added up in order: each wavefront a run of chunks of 64 outputs, then the wavefronts' sums
+constexpr int JOIN_WAVES = 8;
 template <int DT>
-__global__ __launch_bounds__(256) void adapter_join_kernel(const float* __restrict__ part, const int* __restrict__ counts,
-                                                           int chunks, int J, int K, int N, int R, uint16_t* da, uint16_t* db) {
-  const int width = K + N;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)J * R * width) return;
-  const int j = (int)(i / ((int64_t)R * width)), in = (int)(i - (int64_t)j * R * width), r = in / width, c = in - r * width;
+__global__ __launch_bounds__(64 * JOIN_WAVES) void adapter_join_kernel(const float* __restrict__ part, const int* __restrict__ counts,
+                                                                       int chunks, int J, int K, int N, int R, uint16_t* da,
+                                                                       uint16_t* db) {
+  __shared__ float sums[JOIN_WAVES][64];
+  const int width = K + N, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t of = (int64_t)J * R * width, i = (int64_t)blockIdx.x * 64 + lane, at = i < of ? i : of - 1;
+  const int j = (int)(at / ((int64_t)R * width)), in = (int)(at - (int64_t)j * R * width), r = in / width, c = in - r * width;
+  const int from = chunks * wave / JOIN_WAVES, to = chunks * (wave + 1) / JOIN_WAVES;
   float v = 0.0f;
-#pragma unroll 4
-  for (int k = 0; k < chunks; ++k)
-    if (counts[j * chunks + k] > 0) v += part[((int64_t)(j * chunks + k) * R + r) * width + c];
+  constexpr int U = 16;  // chunks whose partials are in flight; those of empty chunks were never written
+  for (int k = from; k < to; k += U) {
+    float w[U];
+    int n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t slot = (int64_t)j * chunks + (k + u < to ? k + u : k);
+      n[u] = k + u < to ? counts[slot] : 0;
+      w[u] = part[slot * R * width + in];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) v += n[u] > 0 ? w[u] : 0.0f;
+  }
+  sums[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0 || i >= of) return;
+#pragma unroll
+  for (int w = 1; w < JOIN_WAVES; ++w) v += sums[w][lane];
   if (c < K) da[((int64_t)j * R + r) * K + c] = to16<DT>(v);
   else db[((int64_t)j * N + c - K) * R + r] = to16<DT>(v);
 }

@@ -24,8 +24,10 @@ struct AdapterArgs {
   int K, N, R, parts;  // parts: of the columns
 };
 
-template <int DT, int NR, int W, bool ONE>
+// QUADS: R is a multiple of 4, so that a lane's 4 ranks of B_j lie in one row.
+template <int DT, int NR, int W, bool ONE, bool QUADS>
 __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) {
+  constexpr int GROUP = NR <= 2 && W > 1 ? 4 : 2;  // blocks of 32 columns whose operands are in flight
   __shared__ __attribute__((aligned(16))) float sums[W > 1 ? W * NR * 256 : 4];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -43,6 +45,19 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
   // this part's columns, in blocks of 32, and this wavefront's steps of the contraction
   const int blocks = (p.N + 31) / 32, n_from = (int)((int64_t)blocks * part / p.parts), n_to = (int)((int64_t)blocks * (part + 1) / p.parts);
   const int steps = (p.K + 31) / 32, k_from = W > 1 ? steps * wave / W : 0, k_to = W > 1 ? steps * (wave + 1) / W : steps;
+  const int n_full = n_to < p.N / 32 ? n_to : p.N / 32;  // blocks before this one are whole
+  const bool writes = !ONE || l16 == 0;
+
+  s16x8 old[2][GROUP];
+  auto load_base = [&](int nb, s16x8 (&v)[GROUP]) __attribute__((always_inline)) {  // of whole blocks; past them any
+    if (base == nullptr) return;
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u) {
+      const int at = nb + u < n_full ? nb + u : n_full - 1;
+      v[u] = *reinterpret_cast<const s16x8_any*>(base + 32 * at + 8 * g);
+    }
+  };
+  if (n_from < n_full) load_base(n_from, old[0]);
 
   uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(there) & 0xffff;  // rows to do
   while (left != 0) {
@@ -50,14 +65,42 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
     const bool own = which == j;
     left &= ~(uint32_t)__builtin_amdgcn_ballot_w64(own);
     if (j < 0) {  // no adapter: base, or zeros
+#pragma unroll 4
       for (int nb = n_from; nb < n_to; ++nb) {
         const int n = 32 * nb + 8 * g;
         s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
         if (base != nullptr && n < p.N) v = load_some<8>(base + n, p.N - n);
-        if (own && n < p.N && (!ONE || l16 == 0)) store_some<8>(out + n, p.N - n, v);
+        if (own && n < p.N && writes) store_some<8>(out + n, p.N - n, v);
       }
       continue;
     }
+    const uint16_t* b = p.b + (int64_t)j * p.N * p.R;
+    // B_j's operands of column c: 4 ranks of each 16
+    auto load_b = [&](int c, s16x4 (&v)[NR]) __attribute__((always_inline)) {
+      const uint16_t* from = b + (int64_t)c * p.R;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int r = 16 * i + 4 * g;
+        if constexpr (QUADS) {
+          const s16x4 w = *reinterpret_cast<const s16x4_any*>(from + (r < p.R ? r : 0));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[i][q] = r < p.R ? w[q] : (short)0;
+        } else {
+          v[i] = load_some<4>(from + r, p.R - r);
+        }
+      }
+    };
+    auto load_group = [&](int nb, s16x4 (&v)[GROUP][2][NR]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < GROUP; ++u) {
+        const int at = nb + u < n_full ? nb + u : n_full - 1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) load_b(32 * at + 8 * (l16 >> 2) + 4 * t + (l16 & 3), v[u][t]);
+      }
+    };
+    s16x4 bv[2][GROUP][2][NR];
+    if (n_from < n_full) load_group(n_from, bv[0]);
+
     // -- h: accumulators: lane: row l % 16, ranks 16 i + 4 (l / 16) ..
     v4f h[NR];
     const uint16_t* a[NR];
@@ -83,10 +126,10 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
     }
     if constexpr (W > 1) {
       v4f* to = reinterpret_cast<v4f*>(sums);
-      __syncthreads();  // (the sums of the adapter before have been read)
+      lds_barrier();  // (the sums of the adapter before have been read)
 #pragma unroll
       for (int i = 0; i < NR; ++i) to[(wave * NR + i) * 64 + lane] = h[i];
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         h[i] = to[i * 64 + lane];
@@ -103,7 +146,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
         h[i][q] = 16 * i + 4 * g + q < p.R ? h[i][q] * scale : 0.0f;
         most = __builtin_elementwise_maximum(most, fabsf(h[i][q]));
       }
-    if (p.h != nullptr && part == 0 && own && (!ONE || l16 == 0)) {
+    if (p.h != nullptr && part == 0 && own && writes) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) *reinterpret_cast<v4f*>(p.h + (int64_t)row * (16 * NR) + 16 * i + 4 * g) = h[i];
     }
@@ -124,45 +167,52 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
         hf[i][4 + q] = lo;
       }
     // -- out: two products of 16 columns whose rows interleave, so that a lane gets 8 neighbours
-    const uint16_t* b = p.b + (int64_t)j * p.N * p.R;
-    auto columns = [&](int nb, auto full_c) __attribute__((always_inline)) {
-      constexpr bool FULL = decltype(full_c)::value;
-      const int n = 32 * nb + 8 * g;
-      v4f d[2];
+    auto block = [&](const s16x4 (&v)[2][NR], s16x8 from) __attribute__((always_inline)) {
+      float o[8];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        d[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        int c = 32 * nb + 8 * (l16 >> 2) + 4 * t + (l16 & 3);
-        if (!FULL) c = c < p.N ? c : p.N - 1;
-        const uint16_t* from = b + (int64_t)c * p.R + 4 * g;
+        v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-          const s16x4 v = load_some<4>(from + 16 * i, p.R - 16 * i - 4 * g);
-          d[t] = mfma_rank<DT>(__builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, 6, 7), hf[i], d[t]);
+        for (int i = 0; i < NR; ++i) d = mfma_rank<DT>(__builtin_shufflevector(v[t][i], v[t][i], 0, 1, 2, 3, 4, 5, 6, 7), hf[i], d);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float z = from16<DT>((uint16_t)from[4 * t + q]);
+          if (base == nullptr) o[4 * t + q] = DT == FIM_F16 ? d[q] * down : d[q];
+          else o[4 * t + q] = DT == FIM_F16 ? fmaf(d[q], down, z) : d[q] + z;
         }
       }
-      s16x8 old = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (base != nullptr && (FULL || n < p.N)) {
-        if (FULL) old = *reinterpret_cast<const s16x8_any*>(base + n);
-        else old = load_some<8>(base + n, p.N - n);
+      const v4i w = {(int)to16x2<DT>(o[0], o[1]), (int)to16x2<DT>(o[2], o[3]), (int)to16x2<DT>(o[4], o[5]), (int)to16x2<DT>(o[6], o[7])};
+      return __builtin_bit_cast(s16x8, w);
+    };
+    auto group = [&](int nb, int cur) __attribute__((always_inline)) {
+      if (nb + GROUP < n_full) {
+        load_base(nb + GROUP, old[cur ^ 1]);
+        load_group(nb + GROUP, bv[cur ^ 1]);
       }
-      float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float o = from16<DT>((uint16_t)old[q]), m = d[q >> 2][q & 3];
-        v[q] = base == nullptr ? (DT == FIM_F16 ? m * down : m) : (DT == FIM_F16 ? fmaf(m, down, o) : m + o);
-      }
-      const v4i w = {(int)to16x2<DT>(v[0], v[1]), (int)to16x2<DT>(v[2], v[3]), (int)to16x2<DT>(v[4], v[5]), (int)to16x2<DT>(v[6], v[7])};
-      if (own && (!ONE || l16 == 0)) {
-        if (FULL) *reinterpret_cast<s16x8_any*>(out + n) = __builtin_bit_cast(s16x8, w);
-        else if (n < p.N) store_some<8>(out + n, p.N - n, __builtin_bit_cast(s16x8, w));
+      for (int u = 0; u < GROUP; ++u) {
+        const s16x8 w = block(bv[cur][u], old[cur][u]);
+        if (own && writes && nb + u < n_full) *reinterpret_cast<s16x8_any*>(out + 32 * (nb + u) + 8 * g) = w;
       }
     };
-    int nb = n_from;
-    const int full = n_to < p.N / 32 ? n_to : p.N / 32;
-#pragma unroll 2
-    for (; nb < full; ++nb) columns(nb, std::integral_constant<bool, true>{});
-    if (nb < n_to) columns(nb, std::integral_constant<bool, false>{});
+    for (int nb = n_from; nb < n_full; nb += 2 * GROUP) {
+      group(nb, 0);
+      if (nb + GROUP < n_full) group(nb + GROUP, 1);
+    }
+    if (n_full < n_to) {  // the last columns
+      const int n = 32 * n_full + 8 * g;
+      s16x4 v[2][NR];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int c = 32 * n_full + 8 * (l16 >> 2) + 4 * t + (l16 & 3);
+        load_b(c < p.N ? c : p.N - 1, v[t]);
+      }
+      s16x8 from = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (base != nullptr && n < p.N) from = load_some<8>(base + n, p.N - n);
+      const s16x8 w = block(v, from);
+      if (own && writes && n < p.N) store_some<8>(out + n, p.N - n, w);
+    }
+    if (left != 0 && n_from < n_full) load_base(n_from, old[0]);  // for the next adapter's rows
   }
 }
 
