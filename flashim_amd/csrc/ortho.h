@@ -30,8 +30,8 @@ struct OrthoStack {
   int64_t each;
   uint32_t rows, cols, batch, mp, np, chunk, chunks;
   float factor;     // O's factor in a step
-  uint32_t first[4];  // first workgroup of a pass over: elements, conversion tiles, symmetric products, X's products
-  uint8_t g_type, out_type, tall, pad[5];
+  uint32_t first[5];  // first workgroup of a pass over: elements, conversion tiles, tiles of A, of P, of P X
+  uint8_t g_type, out_type, tall, pad;
 };
 static_assert(sizeof(OrthoStack) % 8 == 0, "");
 

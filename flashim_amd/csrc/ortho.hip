@@ -39,7 +39,7 @@ __device__ __forceinline__ double ortho_sum(double v) {
 // Momentum in place, and each chunk's sum of squares of U
 __global__ __launch_bounds__(ORTHO_T) void ortho_momentum_kernel(const OrthoStack* __restrict__ table, int count,
                                                                  const OrthoScalars k) {
-  const OrthoStack& s = table[stack_of(table, count, 0, blockIdx.x)];
+  const OrthoStack s = table[stack_of(table, count, 0, blockIdx.x)];
   const uint32_t local = blockIdx.x - s.first[0], b = local / s.chunks, c = local - b * s.chunks;
   const int64_t n = (int64_t)s.rows * s.cols, begin = (int64_t)c * s.chunk;
   const int64_t base = b * n + begin;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(ORTHO_T) void ortho_momentum_kernel(const OrthoStac
 __global__ __launch_bounds__(ORTHO_T) void ortho_convert_kernel(const OrthoStack* __restrict__ table, int count,
                                                                 const OrthoScalars k) {
   __shared__ float tile[64 * 65];
-  const OrthoStack& s = table[stack_of(table, count, 1, blockIdx.x)];
+  const OrthoStack s = table[stack_of(table, count, 1, blockIdx.x)];
   const uint32_t rt = (s.mp + 63) / 64, ct = (s.np + 63) / 64, local = blockIdx.x - s.first[1];
   const uint32_t b = local / (rt * ct), in = local - b * rt * ct;
   const int r0 = (int)(in / ct) * 64, c0 = (int)(in % ct) * 64;  // of X
@@ -154,6 +154,8 @@ static OrthoShape ortho_shape(int64_t rows, int64_t cols) {
 
 static bool ortho_empty(const OrthoCall& c, int64_t i) { return c.batch[i] == 0 || c.rows[i] == 0 || c.cols[i] == 0; }
 
+static int64_t ortho_part_bytes(const OrthoCall& c);
+
 // Sizes and the workspace's bytes: the table, then sums of squares and halves of the matrices on tiles
 static int ortho_bytes(const OrthoCall& c, int64_t* bytes) {
   if (c.count < 0 || (c.count > 0 && (c.batch == nullptr || c.rows == nullptr || c.cols == nullptr))) return FIM_ERR_INVALID;
@@ -169,6 +171,7 @@ static int ortho_bytes(const OrthoCall& c, int64_t* bytes) {
     total += c.batch[i] * s.each + cdiv(c.batch[i] * s.chunks * 8, 256) * 256;
     if (total > int64_t{1} << 46) return FIM_ERR_UNSUPPORTED;
   }
+  total += cdiv(ortho_part_bytes(c), 256) * 256;
   *bytes = total;
   return FIM_OK;
 }
@@ -239,16 +242,78 @@ static void launch_small(int T, bool half, const OrthoStack* table, int count, u
   }
 }
 
-template <int MB>
-static void launch_products(const OrthoStack* table, int count, uint32_t sym, uint32_t all, const OrthoScalars& k,
+// The products' tiles, of 64 `side` squared, and how many parts their contraction has; `deep`: four LDS stages, not two
+struct OrthoTiles {
+  int side;
+  int64_t tiles, splits;
+  bool deep;
+};
+struct OrthoPlan {
+  OrthoTiles gram, square, apply;
+};
+
+// Tiles of 128 move half the operands of 64, but a product needs enough of them for the card. By time measured (us a product; m x n):
+// * A = X X^T, three of 1024 x 4096: 128 in 4 parts 42 + 9 to join, in 2 parts 46 + 7, whole 75; 64 whole 55. One: 128 in 4 parts
+//   20 + 5, 64 whole 28. 196 x 523: 64 whole 7, in parts 5 + 5. 96 matrices of 512 x 2048 and smaller: 128 whole 79, 64 whole 82.
+// * P: its contraction is short, and the epilogue costs as much: three of 1024: 64 whole 21, 128 in 2 parts 18 + 9, whole 29; the 96
+//   matrices: 64 whole 28, 128 whole 32.
+// * P X: three of 1024 x 4096: 128 71, 64 97; the 96 matrices 107, 152; 196 x 523: 64 6, 128 10.
+// Four stages cover a workgroup's latencies where it is alone on its CU; two leave room for another.
+static OrthoPlan ortho_plan(const OrthoCall& c) {
+  int64_t t1 = 0, t2 = 0, a1 = 0, a2 = 0, most = 0;  // tiles of 64 and 128: symmetric, all; the longest contraction
+  const int64_t cus = device_cus();
+  for (int64_t i = 0; i < c.count; ++i) {
+    if (ortho_empty(c, i)) continue;
+    const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
+    if (s.small) continue;
+    const int64_t m1 = cdiv(s.mp, 64), m2 = cdiv(s.mp, 128);
+    t1 += c.batch[i] * (m1 * (m1 + 1) / 2);
+    t2 += c.batch[i] * (m2 * (m2 + 1) / 2);
+    a1 += c.batch[i] * m1 * cdiv(s.np, 64);
+    a2 += c.batch[i] * m2 * cdiv(s.np, 128);
+    if (s.np > most) most = s.np;
+  }
+  auto of = [&](int side, int64_t tiles, int64_t splits) {
+    const int64_t n = tiles * splits;
+    return OrthoTiles{side, tiles, splits, n <= (side == 1 ? 2 * cus : cus)};
+  };
+  int64_t splits = cdiv(3 * cus / 2, t2 > 0 ? t2 : 1);
+  if (splits > most / 256) splits = most / 256;  // (eight steps at least)
+  OrthoPlan p;
+  p.gram = t2 >= cus ? of(2, t2, 1) : most <= 1024 || splits <= 1 ? of(1, t1, 1) : of(2, t2, splits);
+  p.square = t2 >= 2 * cus ? of(2, t2, 1) : of(1, t1, 1);
+  p.apply = a2 >= cus / 2 ? of(2, a2, 1) : of(1, a1, 1);
+  return p;
+}
+
+static int64_t ortho_part_bytes(const OrthoCall& c) {
+  const OrthoTiles g = ortho_plan(c).gram;
+  return g.splits > 1 ? g.splits * g.tiles * (64 * g.side) * (64 * g.side) * 4 : 0;
+}
+
+template <int MODE>
+static void launch_product(const OrthoStack* table, int count, const OrthoTiles& t, float* part, int src, const OrthoScalars& k,
+                           hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(t.tiles * t.splits, 8) * 8), block(256);
+  const uint32_t tiles = (uint32_t)t.tiles;
+  const int splits = (int)t.splits;
+  if (t.side == 2 && t.deep) ortho_tile_kernel<MODE, 2, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  else if (t.side == 2) ortho_tile_kernel<MODE, 2, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  else if (t.deep) ortho_tile_kernel<MODE, 1, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  else ortho_tile_kernel<MODE, 1, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+}
+
+static void launch_products(const OrthoStack* table, int count, const OrthoPlan& p, float* part, const OrthoScalars& k,
                             hipStream_t stream) {
-  const dim3 gs((unsigned)cdiv(sym, 8) * 8), ga((unsigned)cdiv(all, 8) * 8), block(256);
   for (int it = 0; it < k.steps; ++it) {
     const int src = it & 1;
-    ortho_tile_kernel<ORTHO_GRAM, MB><<<gs, block, 0, stream>>>(table, count, sym, src, k);
-    ortho_tile_kernel<ORTHO_SQUARE, MB><<<gs, block, 0, stream>>>(table, count, sym, src, k);
-    if (it + 1 < k.steps) ortho_tile_kernel<ORTHO_APPLY, MB><<<ga, block, 0, stream>>>(table, count, all, src, k);
-    else ortho_tile_kernel<ORTHO_LAST, MB><<<ga, block, 0, stream>>>(table, count, all, src, k);
+    launch_product<ORTHO_GRAM>(table, count, p.gram, part, src, k, stream);
+    if (p.gram.splits > 1)  // (tiles of 128)
+      ortho_join_kernel<<<dim3((unsigned)(p.gram.tiles * 4)), dim3(256), 0, stream>>>(table, count, (uint32_t)p.gram.tiles,
+                                                                                      (int)p.gram.splits, part, k);
+    launch_product<ORTHO_SQUARE>(table, count, p.square, nullptr, src, k, stream);
+    if (it + 1 < k.steps) launch_product<ORTHO_APPLY>(table, count, p.apply, nullptr, src, k, stream);
+    else launch_product<ORTHO_LAST>(table, count, p.apply, nullptr, src, k, stream);
   }
 }
 
@@ -278,16 +343,11 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
     const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
     return s.small ? 2 * s.T + (small_lds(s.m, s.np) <= SMALL_LDS / 2) : 0;
   };
-  // tiles of 64 or 128: the larger ones where they still cover the CUs
-  int64_t tiles128 = 0;
-  for (int64_t i = 0; i < c.count; ++i)
-    if (!ortho_empty(c, i) && group_of(i) == 0) {
-      const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
-      tiles128 += c.batch[i] * cdiv(s.mp, 128) * cdiv(s.np, 128);
-    }
-  const int mb = tiles128 >= device_cus() ? 2 : 1;
+  const OrthoPlan plan = ortho_plan(c);
+  float* part = reinterpret_cast<float*>(free_at);
+  free_at += cdiv(ortho_part_bytes(c), 256) * 256;
   for (int group = 0; group < 10; ++group) {
-    int64_t first[4] = {0, 0, 0, 0};
+    int64_t first[5] = {0, 0, 0, 0, 0};
     const int start = written + filled;
     for (int64_t i = 0; i < c.count; ++i) {
       if (ortho_empty(c, i) || group_of(i) != group) continue;
@@ -307,7 +367,7 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
       e.g_type = (uint8_t)c.g_type[i];
       e.out_type = (uint8_t)c.out_type[i];
       e.tall = c.rows[i] > c.cols[i];
-      for (int p = 0; p < 4; ++p) e.first[p] = (uint32_t)first[p];
+      for (int p = 0; p < 5; ++p) e.first[p] = (uint32_t)first[p];
       if (group == 0) {
         e.part = reinterpret_cast<double*>(free_at);
         free_at += cdiv(batch * s.chunks * 8, 256) * 256;
@@ -319,15 +379,19 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
         free_at += batch * s.each;
         e.chunk = (uint32_t)s.chunk;
         e.chunks = (uint32_t)s.chunks;
-        const int64_t bm = 64 * mb, mt = cdiv(s.mp, bm);
+        auto triangle = [&](int side) {
+          const int64_t n = cdiv(s.mp, 64 * side);
+          return n * (n + 1) / 2;
+        };
         first[0] += batch * s.chunks;
         first[1] += batch * cdiv(s.mp, 64) * cdiv(s.np, 64);
-        first[2] += batch * (mt * (mt + 1) / 2);
-        first[3] += batch * mt * cdiv(s.np, bm);
+        first[2] += batch * triangle(plan.gram.side);
+        first[3] += batch * triangle(plan.square.side);
+        first[4] += batch * cdiv(s.mp, 64 * plan.apply.side) * cdiv(s.np, 64 * plan.apply.side);
       } else {
         first[0] += batch;
       }
-      for (int p = 0; p < 4; ++p)
+      for (int p = 0; p < 5; ++p)
         if (first[p] >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
       if (++filled == ORTHO_FILL) flush();
     }
@@ -341,8 +405,7 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
     }
     ortho_momentum_kernel<<<dim3((unsigned)first[0]), dim3(ORTHO_T), 0, stream>>>(t, n, k);
     ortho_convert_kernel<<<dim3((unsigned)first[1]), dim3(ORTHO_T), 0, stream>>>(t, n, k);
-    if (mb == 2) launch_products<2>(t, n, (uint32_t)first[2], (uint32_t)first[3], k, stream);
-    else launch_products<1>(t, n, (uint32_t)first[2], (uint32_t)first[3], k, stream);
+    launch_products(t, n, plan, part, k, stream);
   }
   return launch_status();
 }

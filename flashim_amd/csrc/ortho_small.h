@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int e = stack_of(table, count, 0, blockIdx.x);
-  const OrthoStack& s = table[e];
+  const OrthoStack s = table[e];
   const int b = (int)(blockIdx.x - s.first[0]);
   const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np, nb = np >> 5, ld = np * 4;
   const int n = rows * cols;
