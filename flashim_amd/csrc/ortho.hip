@@ -17,11 +17,11 @@ struct OrthoFill {
 };
 static_assert(sizeof(OrthoFill) <= 4000, "kernel arguments");
 
-__global__ __launch_bounds__(64) void ortho_fill_kernel(const OrthoFill f, OrthoStack* table, int n) {
+__global__ __launch_bounds__(ORTHO_T) void ortho_fill_kernel(const OrthoFill f, OrthoStack* table, int n) {
   constexpr int WORDS = sizeof(OrthoStack) / 4;
   const uint32_t* from = reinterpret_cast<const uint32_t*>(&f);
   uint32_t* to = reinterpret_cast<uint32_t*>(table);
-  for (int i = threadIdx.x; i < n * WORDS; i += 64) to[i] = from[i];
+  for (int i = threadIdx.x; i < n * WORDS; i += ORTHO_T) to[i] = from[i];
 }
 
 __device__ __forceinline__ double ortho_sum(double v) {
@@ -294,7 +294,7 @@ static int64_t ortho_part_bytes(const OrthoCall& c) {
 template <int MODE>
 static void launch_product(const OrthoStack* table, int count, const OrthoTiles& t, float* part, int src, const OrthoScalars& k,
                            hipStream_t stream) {
-  const dim3 grid((unsigned)cdiv(t.tiles * t.splits, 8) * 8), block(256);
+  const dim3 grid((unsigned)(cdiv(t.tiles * t.splits, 8 * ORTHO_RUN) * 8 * ORTHO_RUN)), block(256);
   const uint32_t tiles = (uint32_t)t.tiles;
   const int splits = (int)t.splits;
   if (t.side == 2 && t.deep) ortho_tile_kernel<MODE, 2, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
@@ -334,7 +334,7 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
   int filled = 0;  // entries of `fill` that the device's table does not hold yet
   int written = 0;
   auto flush = [&]() {
-    if (filled > 0) ortho_fill_kernel<<<dim3(1), dim3(64), 0, stream>>>(fill, table + written, filled);
+    if (filled > 0) ortho_fill_kernel<<<dim3(1), dim3(ORTHO_T), 0, stream>>>(fill, table + written, filled);
     written += filled;
     filled = 0;
   };

@@ -1,16 +1,17 @@
 // A whole Newton-Schulz iteration, or optimizer step, of a small matrix in one workgroup: X, A and P stay in LDS.
 //
 // At most 64 rows (of the shorter side) whose X fits: read once, written once, and no launch between the 3 `steps` products, which on
-// tiles would be as many launches of one or two workgroups. Eight wavefronts on 16 x 16 x 32 MFMAs: X X^T is split over the columns
-// (each fragment is read once, and is either operand) and the wavefronts' sums are joined pairwise; P X is split over the columns too, and each wavefront
-// replaces the columns it has read.
+// tiles would be as many launches of one or two workgroups. Sixteen wavefronts (eight took 46 us
+// for 39) on 16 x 16 x 32 MFMAs: X X^T is split over the columns of eight (each fragment is read once, and is either operand), four wavefronts' sums meet the other four's in LDS, and each wavefront adds up
+// one of the 16 blocks, those above the diagonal from the ones below, read across; P X is split over the columns too, and each
+// wavefront replaces the columns it has read.
 #pragma once
 
 #include "ortho.h"
 
 namespace fim {
 
-constexpr int SMALL_WAVES = 8, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
+constexpr int SMALL_WAVES = 16, SMALL_SUMS = 8, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
 // LDS of a matrix: X [16 T][np] halves; the sums of four wavefronts, or A and P
 inline int64_t small_region(int T) {
@@ -50,37 +51,68 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   float* sums = reinterpret_cast<float*>(A);  // (A and P are dead while the sums are joined)
 
   // -- U in 32 bits where X will lie: element (r, c) of X in 4 bytes, the columns of each line rotated by the row
-  for (int i = tid * 16; i < MP * ld; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(X + i) = v4i{0, 0, 0, 0};
-  __syncthreads();
-  double sq = 0.0;
-  for (int i = tid * 4; i < n; i += 64 * SMALL_WAVES * 4) {
-    float u[4];
-    const int left = n - i;
-    load4(s.g, base + i, s.g_type, left, u);
-    if (s.mom != nullptr) {
-      float m[4];
-      load4(s.mom, base + i, FIM_F32, left, m);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        m[q] = fmaf(k.momentum, m[q], u[q]);
-        u[q] = k.nesterov ? fmaf(k.momentum, m[q], u[q]) : m[q];
-      }
-      store4(s.mom, base + i, FIM_F32, left, m);
-    }
-    int r = i / cols, c = i - r * cols;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (q < left) {
-        sq = fma((double)u[q], (double)u[q], sq);
-        const int xr = s.tall ? c : r, xc = s.tall ? r : c;
-        *reinterpret_cast<float*>(X + xr * ld + (xc >> 5) * 128 + (((xc ^ xr) & 31) << 2)) = u[q];
-      }
-      if (++c == cols) {
-        c = 0;
-        ++r;
-      }
-    }
+  if (rows < cols ? rows < MP || cols < np : cols < MP || rows < np) {
+    for (int i = tid * 16; i < MP * ld; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(X + i) = v4i{0, 0, 0, 0};
+    __syncthreads();
   }
+  double sq = 0.0;
+  auto load_all = [&](auto dt, auto mom_c) __attribute__((always_inline)) {
+    constexpr int DT = decltype(dt)::value, STEP = 64 * SMALL_WAVES * 4, U = 4;  // U loads in flight: stores may alias them
+    constexpr bool MOM = decltype(mom_c)::value;
+    int r = tid * 4 / cols, c = tid * 4 - r * cols;
+    const int dr = STEP / cols, dc = STEP - dr * cols;
+    for (int i0 = tid * 4; i0 < n; i0 += U * STEP) {
+      float u[U][4], m[MOM ? U : 1][4];
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        const int i = i0 + t * STEP;
+        if (i < n) {
+          load4(s.g, base + i, DT, n - i, u[t]);
+          if constexpr (MOM) load4(s.mom, base + i, FIM_F32, n - i, m[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        const int i = i0 + t * STEP, left = n - i;
+        if (left > 0) {
+          if constexpr (MOM) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              m[t][q] = fmaf(k.momentum, m[t][q], u[t][q]);
+              u[t][q] = k.nesterov ? fmaf(k.momentum, m[t][q], u[t][q]) : m[t][q];
+            }
+            store4(s.mom, base + i, FIM_F32, left, m[t]);
+          }
+          int rr = r, cc = c;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q < left) {
+              sq = fma((double)u[t][q], (double)u[t][q], sq);
+              const int xr = s.tall ? cc : rr, xc = s.tall ? rr : cc;
+              *reinterpret_cast<float*>(X + xr * ld + (xc >> 5) * 128 + (((xc ^ xr) & 31) << 2)) = u[t][q];
+            }
+            if (++cc == cols) {
+              cc = 0;
+              ++rr;
+            }
+          }
+        }
+        r += dr;
+        c += dc;
+        if (c >= cols) {
+          c -= cols;
+          ++r;
+        }
+      }
+    }
+  };
+  auto load_of = [&](auto dt) __attribute__((always_inline)) {
+    if (s.mom != nullptr) load_all(dt, std::integral_constant<bool, true>{});
+    else load_all(dt, std::integral_constant<bool, false>{});
+  };
+  if (s.g_type == FIM_F32) load_of(std::integral_constant<int, FIM_F32>{});
+  else if (s.g_type == FIM_BF16) load_of(std::integral_constant<int, FIM_BF16>{});
+  else load_of(std::integral_constant<int, FIM_F16>{});
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o);
   double* red = reinterpret_cast<double*>(A);
@@ -91,6 +123,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   for (int i = 1; i < SMALL_WAVES; ++i) sq += red[i];
   const float scale = (float)((double)k.sx / (sqrt(sq) + k.eps));
   // -- sx X0 as halves, line by line in place: 8 lanes a line, all of which read before one writes
+#pragma unroll 4
   for (int i = tid; i < MP * nb * 8; i += 64 * SMALL_WAVES) {
     const int q = i & 7, line = i >> 3, r = line / nb;
     uint8_t* at = X + line * 128;
@@ -122,25 +155,16 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     }
     return __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  // a block's values (lane: row l % 16, columns 4 g ..) into A or P as halves, and their mirror
-  auto put = [&](uint8_t* p, int r, int c, const float (&v)[4], bool mirror) __attribute__((always_inline)) {
+  // a block's values (lane: row l % 16, columns 4 g ..) into A or P as halves
+  auto put = [&](uint8_t* p, int r, int c, const float (&v)[4]) __attribute__((always_inline)) {
     v2i hi, lo;
     split4(v, hi, lo);
     uint8_t* at = p + r * (LINES * 128) + (c >> 5) * 128;
     const int key = small_key(r), seg = (c & 31) >> 3;
     *reinterpret_cast<v2i*>(at + ((seg ^ key) << 4) + (c & 7) * 2) = hi;
     *reinterpret_cast<v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2) = lo;
-    if (mirror) {
-      const s16x4 a4 = __builtin_bit_cast(s16x4, hi), b4 = __builtin_bit_cast(s16x4, lo);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        uint8_t* o = p + (c + u) * (LINES * 128) + (r >> 5) * 128;
-        const int ko = small_key(c + u), so = (r & 31) >> 3;
-        *reinterpret_cast<int16_t*>(o + ((so ^ ko) << 4) + (r & 7) * 2) = a4[u];
-        *reinterpret_cast<int16_t*>(o + (((4 + so) ^ ko) << 4) + (r & 7) * 2) = b4[u];
-      }
-    }
   };
+  constexpr int OWN = (T * T + SMALL_WAVES - 1) / SMALL_WAVES;  // blocks of A and P of a wavefront
   const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
   const float gram_scale = k.sa / (k.sx * k.sx), apply_scale = 1.0f / k.sp, last_scale = apply_scale / k.sx;
   const float sq_scale = k.c * k.sp / (k.sa * k.sa), old_scale = k.b * k.sp / k.sa;
@@ -151,7 +175,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) acc[i] = zero;
     __syncthreads();
-    for (int line = wave; line < nb; line += SMALL_WAVES) {
+    for (int line = wave; line < nb && wave < SMALL_SUMS; line += SMALL_SUMS) {
       s16x8 f[T][2];
 #pragma unroll
       for (int i = 0; i < T; ++i)
@@ -164,76 +188,78 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
           for (int j = 0; j <= i; ++j, ++q) acc[q] = mfma_small(f[j][part == 2], f[i][part == 1], acc[q]);
     }
-    // joined pairwise: 4 wavefronts into 4, 2 into 2, 1 into 1
+    // four sums of two wavefronts each
+    if (wave >= 4 && wave < SMALL_SUMS) {
 #pragma unroll
-    for (int half = 4; half > 0; half >>= 1) {
-      if (wave >= half && wave < 2 * half) {
-#pragma unroll
-        for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + ((wave - half) * PAIRS + i) * 256 + lane * 4) = acc[i];
-      }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int i = 0; i < PAIRS; ++i) acc[i] += *reinterpret_cast<const v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4);
-      }
-      __syncthreads();
+      for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + ((wave - 4) * PAIRS + i) * 256 + lane * 4) = acc[i];
     }
+    __syncthreads();
+    if (wave < 4) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) acc[i] += *reinterpret_cast<const v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4) = acc[i];
+    }
+    __syncthreads();
+    float own[OWN][4];
+#pragma unroll
+    for (int t = 0; t < OWN; ++t) {
+      const int q = wave + SMALL_WAVES * t, i = q / T, j = q % T;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) own[t][u] = 0.0f;
+      if (q < T * T) {
+        const int hi = i > j ? i : j, lo = i > j ? j : i;
+        const float* from = sums + (hi * (hi + 1) / 2 + lo) * 256;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)  // above the diagonal: row l % 16, column 4 g + u of the block below, across
+            own[t][u] += from[w * PAIRS * 256 + (i >= j ? lane * 4 + u : ((l16 >> 2) * 16 + 4 * g + u) * 4 + (l16 & 3))];
+      }
+    }
+    __syncthreads();  // (A and P lie where the sums lay)
     if (T == 1 || T == 3) {  // columns past 16 T of the last line: zero
       for (int i = tid * 16; i < 2 * MP * LINES * 128; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(A + i) = v4i{0, 0, 0, 0};
       __syncthreads();
     }
-    if (wave == 0) {
 #pragma unroll
-      for (int i = 0, q = 0; i < T; ++i)
+    for (int t = 0; t < OWN; ++t) {
+      const int q = wave + SMALL_WAVES * t;
 #pragma unroll
-        for (int j = 0; j <= i; ++j, ++q) {
-          float v[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = acc[q][u] * gram_scale;
-          put(A, 16 * i + l16, 16 * j + 4 * g, v, i != j);
-        }
+      for (int u = 0; u < 4; ++u) own[t][u] *= gram_scale;
+      if (q < T * T) put(A, 16 * (q / T) + l16, 16 * (q % T) + 4 * g, own[t]);
     }
     __syncthreads();
-    // -- P = a I + b A + c A^2: pairs of blocks over the wavefronts
+    // -- P = a I + b A + c A^2
 #pragma unroll
-    for (int i = 0, q = 0; i < T; ++i)
+    for (int t = 0; t < OWN; ++t) {
+      const int q = wave + SMALL_WAVES * t, i = q / T, j = q % T;
+      if (q < T * T) {
+        v4f w[3] = {zero, zero, zero};
 #pragma unroll
-      for (int j = 0; j <= i; ++j, ++q)
-        if (q % SMALL_WAVES == wave) {
-          v4f w = zero;
+        for (int line = 0; line < LINES; ++line) {
+          s16x8 fi[2], fj[2];
 #pragma unroll
-          for (int line = 0; line < LINES; ++line) {
-            s16x8 fi[2], fj[2];
-#pragma unroll
-            for (int pl = 0; pl < 2; ++pl) {
-              fi[pl] = along(A, LINES * 128, 16 * i, line, pl);
-              fj[pl] = along(A, LINES * 128, 16 * j, line, pl);
-            }
-#pragma unroll
-            for (int part = 0; part < 3; ++part) w = mfma_small(fj[part == 2], fi[part == 1], w);
+          for (int pl = 0; pl < 2; ++pl) {
+            fi[pl] = along(A, LINES * 128, 16 * i, line, pl);
+            fj[pl] = along(A, LINES * 128, 16 * j, line, pl);
           }
-          const int r = 16 * i + l16, c = 16 * j + 4 * g, key = small_key(r), seg = (c & 31) >> 3;
-          const uint8_t* at = A + r * (LINES * 128) + (c >> 5) * 128;
-          float old[4], v[4];
-          join4(*reinterpret_cast<const v2i*>(at + ((seg ^ key) << 4) + (c & 7) * 2),
-                *reinterpret_cast<const v2i*>(at + (((4 + seg) ^ key) << 4) + (c & 7) * 2), old);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            v[u] = fmaf(sq_scale, w[u], old_scale * old[u]);
-            if (r == c + u) v[u] += k.a * k.sp;
-          }
-          put(P, r, c, v, i != j);
+          for (int part = 0; part < 3; ++part) w[part] = mfma_small(fj[part == 2], fi[part == 1], w[part]);
         }
+        const int r = 16 * i + l16, c = 16 * j + 4 * g;
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          v[u] = fmaf(sq_scale, w[0][u] + (w[1][u] + w[2][u]), old_scale * own[t][u]);
+          if (r == c + u) v[u] += k.a * k.sp;
+        }
+        put(P, r, c, v);
+      }
+    }
     __syncthreads();
     // -- X = P X: 16 columns a turn
     const bool last = it == k.steps - 1;
-    s16x8 fp[T][LINES][2];
-#pragma unroll
-    for (int i = 0; i < T; ++i)
-#pragma unroll
-      for (int line = 0; line < LINES; ++line)
-#pragma unroll
-        for (int pl = 0; pl < 2; ++pl) fp[i][line][pl] = along(P, LINES * 128, 16 * i, line, pl);
     for (int c16 = wave; c16 < 2 * nb; c16 += SMALL_WAVES) {
       v4f y[T];
 #pragma unroll
@@ -241,10 +267,15 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
       for (int line = 0; line < LINES; ++line) {
         const s16x8 xh = across(32 * line, c16, 0), xl = across(32 * line, c16, 1);
+        s16x8 fp[T][2];
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) fp[i][pl] = along(P, LINES * 128, 16 * i, line, pl);
 #pragma unroll
         for (int part = 0; part < 3; ++part)
 #pragma unroll
-          for (int i = 0; i < T; ++i) y[i] = mfma_small(part == 2 ? xl : xh, fp[i][line][part == 1], y[i]);
+          for (int i = 0; i < T; ++i) y[i] = mfma_small(part == 2 ? xl : xh, fp[i][part == 1], y[i]);
       }
       const int c = 16 * c16 + 4 * g;
 #pragma unroll

@@ -18,6 +18,10 @@ enum { ORTHO_GRAM, ORTHO_SQUARE, ORTHO_APPLY, ORTHO_LAST };
 
 __device__ __forceinline__ v16f mfma_halves(s16x8 a, s16x8 b, v16f c) { return mfma16<FIM_F16>(a, b, c); }
 
+// Neighbouring tiles of an XCD. Whole eighths of the tiles gave some XCDs the long contractions of the first stacks (96 matrices:
+// P X 110 us, the last one 192; 102 and 173 with runs of 16 or 32); runs of 4 and 8 share less in the L2 (111 and 110).
+constexpr uint32_t ORTHO_RUN = 16;
+
 // Scales of the accumulators, exact but for c's and b's own factors
 struct OrthoOut {
   float gram, apply, last, square, old;
@@ -174,8 +178,8 @@ __global__ __launch_bounds__(256, 128 * MB * 128 * NS > 80 * 1024 ? 1 : 2) void 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1, h = lane >> 5;
 
-  // workgroups go round the 8 XCDs: each takes a contiguous run of tiles
-  uint32_t t = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  // workgroups go round the 8 XCDs: each takes runs of ORTHO_RUN tiles, which share operands in its L2
+  uint32_t t = ((blockIdx.x >> 3) / ORTHO_RUN * 8 + (blockIdx.x & 7)) * ORTHO_RUN + (blockIdx.x >> 3) % ORTHO_RUN;
   if (t >= tiles * (SYM ? splits : 1)) return;
   const int split = SYM ? __builtin_amdgcn_readfirstlane((int)(t / tiles)) : 0;
   t -= split * tiles;
