@@ -83,6 +83,7 @@ SIGNATURES: dict[str, list] = {
                       _i64, _vp],
     "fim_low_rank_adapters": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _f32, _vp,
                               _vp, _vp],
+    "fim_low_rank_adapters_saved": [_i64, _i64, _i64, _vp],
     "fim_low_rank_adapters_backward_workspace": [_i64, _i64, _i64, _i64, _i64, _vp],
     "fim_low_rank_adapters_backward": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp,
                                        _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],

@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "adapters_grad.h"
+#include "adapters_narrow.h"
 #include "adapters_rows.h"
 #include "gated_plan.h"
 
@@ -75,20 +76,29 @@ static void adapter_rows(AdapterArgs& p, int dtype, hipStream_t stream) {
 struct AdapterGradPlan {
   int64_t chunk, chunks, at, bt, t, part, counts, bytes;
   int xt, ct;
+  bool narrow;
 };
+
+// Whether the backward pass is one pass over x and d_out
+static bool adapter_narrow(int64_t K, int64_t N, int64_t R) {
+  return R <= 32 && cdiv(K, 32) * 32 + cdiv(N, 32) * 32 <= NARROW_WIDTH;
+}
 
 static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   AdapterGradPlan g;
   g.xt = (int)cdiv(s.K, GRAD_COLS);
   g.ct = g.xt + (int)cdiv(s.N, GRAD_COLS);
-  // workgroups for the card where a chunk's rows have one adapter, but at most 64 MB of partial sums should they have all
-  int64_t chunks = cdiv(4 * (int64_t)device_cus(), g.ct);
-  const int64_t most = (int64_t{64} << 20) / (s.J * s.R * (s.K + s.N) * 4);
+  g.narrow = adapter_narrow(s.K, s.N, s.R);
+  // workgroups for the card where a chunk's rows have one adapter (narrow: two a CU), but at most 64 MB of partial sums
+  // should they have all
+  int64_t chunks = g.narrow ? 2 * (int64_t)device_cus() : cdiv(4 * (int64_t)device_cus(), g.ct);
+  const int64_t most = (int64_t{64} << 20) / (s.J * s.R * (s.K + s.N) * 4), step = g.narrow ? NARROW_ROWS : 256;
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
-  g.chunk = cdiv(cdiv(s.M, chunks), 256) * 256;
-  if (g.chunk > GRAD_CHUNK) g.chunk = GRAD_CHUNK;
-  if (g.chunk < 256) g.chunk = 256;
+  g.chunk = cdiv(cdiv(s.M, chunks), step) * step;
+  if (g.chunk < 256) g.chunk = 256;  // (a workgroup's weights cost as much)
+  const int64_t longest = g.narrow ? NARROW_CHUNK : GRAD_CHUNK;
+  if (g.chunk > longest) g.chunk = longest;
   g.chunks = cdiv(s.M, g.chunk);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -96,9 +106,9 @@ static AdapterGradPlan grad_plan(const AdapterSizes& s) {
     at += align256(bytes);
     return from;
   };
-  g.at = take(s.J * s.R * s.K * 2);
-  g.bt = take(s.J * s.R * s.N * 2);
-  g.t = take(s.M * 16 * adapter_blocks(s.R) * 4);
+  g.at = take(g.narrow ? 0 : s.J * s.R * s.K * 2);
+  g.bt = take(g.narrow ? 0 : s.J * s.R * s.N * 2);
+  g.t = take(g.narrow ? 0 : s.M * 16 * adapter_blocks(s.R) * 4);
   g.part = take(g.chunks > 1 ? s.J * g.chunks * s.R * (s.K + s.N) * 4 : 0);
   g.counts = take(g.chunks > 1 ? s.J * g.chunks * 4 : 0);
   g.bytes = at;
@@ -129,6 +139,13 @@ extern "C" int fim_low_rank_adapters(const void* base, int64_t base_stride, cons
   return launch_status();
 }
 
+extern "C" int fim_low_rank_adapters_saved(int64_t K, int64_t N, int64_t R, int64_t* columns) {
+  if (K < 1 || N < 1 || R < 1 || columns == nullptr) return FIM_ERR_INVALID;
+  if (R > ADAPTER_RANK || K >= 1 << 24 || N >= 1 << 24) return FIM_ERR_UNSUPPORTED;
+  *columns = adapter_narrow(K, N, R) ? 0 : 16 * adapter_blocks(R);
+  return FIM_OK;
+}
+
 extern "C" int fim_low_rank_adapters_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t J, int64_t R, int64_t* bytes) {
   if (bytes == nullptr) return FIM_ERR_INVALID;
   const AdapterSizes s{M, K, N, J, R, M};
@@ -148,17 +165,43 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
   if (rc != FIM_OK) return rc;
   if (M == 0) return FIM_ERR_INVALID;  // (there is no row to sum over: the caller's zeros)
   if (d_out == nullptr || x == nullptr || a == nullptr || b == nullptr || index == nullptr || (da == nullptr) != (db == nullptr) ||
-      (da != nullptr && h == nullptr))
+      (da != nullptr && h == nullptr && !adapter_narrow(K, N, R)))
     return FIM_ERR_INVALID;
   for (const void* t : {d_out, x, a, b, static_cast<const void*>(dx), static_cast<const void*>(da), static_cast<const void*>(db)})
     if (reinterpret_cast<uintptr_t>(t) % 2) return FIM_ERR_INVALID;
   if (reinterpret_cast<uintptr_t>(index) % (index_wide ? 8 : 4) || reinterpret_cast<uintptr_t>(h) % 16) return FIM_ERR_INVALID;
   const AdapterGradPlan g = grad_plan(s);
-  if (workspace == nullptr || workspace_bytes < g.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return FIM_ERR_INVALID;
+  if (g.bytes > 0 && (workspace == nullptr || workspace_bytes < g.bytes || reinterpret_cast<uintptr_t>(workspace) % 256))
+    return FIM_ERR_INVALID;
   if (dx == nullptr && da == nullptr) return FIM_OK;
-  const int64_t na = J * R * K, nb = J * R * N, outputs = J * R * (K + N);
-  if (cdiv(na + nb, 64) >= int64_t{1} << 31 || J * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
+  const int64_t na = J * R * K, nb = J * R * N;
+  if (J * cdiv(R * (K + N), 64) >= int64_t{1} << 31 || (J + 1) * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* part = da != nullptr && g.chunks > 1 ? reinterpret_cast<float*>(ws + g.part) : nullptr;
+  int* counts = part != nullptr ? reinterpret_cast<int*>(ws + g.counts) : nullptr;
+  auto join = [&]() {
+    if (part == nullptr) return;
+    const auto kernel = dtype == FIM_BF16 ? adapter_join_kernel<FIM_BF16> : adapter_join_kernel<FIM_F16>;
+    kernel<<<dim3((unsigned)(J * cdiv(R * (K + N), 64))), dim3(64 * JOIN_WAVES), 0, stream>>>(
+        part, counts, (int)g.chunks, (int)K, (int)N, (int)R, static_cast<uint16_t*>(da), static_cast<uint16_t*>(db));
+  };
+  if (g.narrow) {
+    const AdapterNarrowArgs q{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(a),
+                              static_cast<const uint16_t*>(b), x_stride, d_out_stride,
+                              AdapterIndex{index, index_wide, (uint32_t)(M / entries), (int)J}, scales, scale,
+                              static_cast<uint16_t*>(dx), static_cast<uint16_t*>(da), static_cast<uint16_t*>(db), part, counts,
+                              (uint32_t)M, (uint32_t)g.chunk, (int)g.chunks, (int)K, (int)N, (int)R};
+    const dim3 grid((unsigned)((J + (dx != nullptr)) * g.chunks));  // (rows without an adapter: zeros of dx)
+    auto launch = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      if (R > 16) adapter_narrow_kernel<DT, 2><<<grid, dim3(256), 0, stream>>>(q);
+      else adapter_narrow_kernel<DT, 1><<<grid, dim3(256), 0, stream>>>(q);
+    };
+    if (dtype == FIM_BF16) launch(std::integral_constant<int, FIM_BF16>{});
+    else launch(std::integral_constant<int, FIM_F16>{});
+    join();
+    return launch_status();
+  }
   uint16_t *at = reinterpret_cast<uint16_t*>(ws + g.at), *bt = reinterpret_cast<uint16_t*>(ws + g.bt);
   float* t = reinterpret_cast<float*>(ws + g.t);
   const AdapterIndex rows{index, index_wide, (uint32_t)(M / entries), (int)J};
@@ -169,18 +212,14 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
                 scale, (uint32_t)M, (int)N, dx == nullptr ? 0 : (int)K, (int)R, 1};
   adapter_rows(p, dtype, stream);
   if (da != nullptr) {
-    float* part = g.chunks > 1 ? reinterpret_cast<float*>(ws + g.part) : nullptr;
-    int* counts = g.chunks > 1 ? reinterpret_cast<int*>(ws + g.counts) : nullptr;
     const AdapterGradArgs q{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(d_out), x_stride, d_out_stride, t, h, rows,
                             static_cast<uint16_t*>(da), static_cast<uint16_t*>(db), part, counts, (uint32_t)M, (uint32_t)g.chunk,
                             (int)g.chunks, (int)K, (int)N, (int)R, g.xt, g.ct};
     by_type(dtype, R, [&](auto dt, auto nr) {
       constexpr int DT = decltype(dt)::value;
       adapter_grad_kernel<DT, decltype(nr)::value><<<dim3((unsigned)(J * g.chunks * g.ct)), dim3(256), 0, stream>>>(q);
-      if (part != nullptr)
-        adapter_join_kernel<DT><<<dim3((unsigned)cdiv(outputs, 64)), dim3(64 * JOIN_WAVES), 0, stream>>>(
-            part, counts, (int)g.chunks, (int)J, (int)K, (int)N, (int)R, q.da, q.db);
     });
+    join();
   }
   return launch_status();
 }

@@ -172,36 +172,40 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
   }
 }
 
-// The chunks' partial sums, added up in order: each wavefront a run of chunks of 64 outputs, then the wavefronts' sums
-constexpr int JOIN_WAVES = 8;
+// The chunks' partial sums of 64 outputs of an adapter, added up in order: each wavefront a run of chunks, of which the empty ones
+// (never written) are passed over, then the wavefronts' sums
+constexpr int JOIN_WAVES = 16;
 template <int DT>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void adapter_join_kernel(const float* __restrict__ part, const int* __restrict__ counts,
-                                                                       int chunks, int J, int K, int N, int R, uint16_t* da,
-                                                                       uint16_t* db) {
+                                                                       int chunks, int K, int N, int R, uint16_t* da, uint16_t* db) {
   __shared__ float sums[JOIN_WAVES][64];
-  const int width = K + N, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t of = (int64_t)J * R * width, i = (int64_t)blockIdx.x * 64 + lane, at = i < of ? i : of - 1;
-  const int j = (int)(at / ((int64_t)R * width)), in = (int)(at - (int64_t)j * R * width), r = in / width, c = in - r * width;
-  const int from = chunks * wave / JOIN_WAVES, to = chunks * (wave + 1) / JOIN_WAVES;
+  const int width = K + N, of = R * width, blocks = (of + 63) / 64, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = (int)(blockIdx.x / (unsigned)blocks);
+  const int i = (int)(blockIdx.x - (unsigned)j * blocks) * 64 + lane, at = i < of ? i : of - 1;
+  const int from = (int)((int64_t)chunks * wave / JOIN_WAVES), to = (int)((int64_t)chunks * (wave + 1) / JOIN_WAVES);
+  const float* mine = part + (int64_t)j * chunks * of + at;
   float v = 0.0f;
-  constexpr int U = 16;  // chunks whose partials are in flight; those of empty chunks were never written
-  for (int k = from; k < to; k += U) {
-    float w[U];
-    int n[U];
+  for (int k0 = from; k0 < to; k0 += 64) {
+    uint64_t some = __builtin_amdgcn_ballot_w64(k0 + lane < to && counts[(int64_t)j * chunks + (k0 + lane < to ? k0 + lane : k0)] > 0);
+    while (some != 0) {
+      constexpr int U = 8;  // loads in flight
+      float w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t slot = (int64_t)j * chunks + (k + u < to ? k + u : k);
-      n[u] = k + u < to ? counts[slot] : 0;
-      w[u] = part[slot * R * width + in];
+      for (int u = 0; u < U; ++u) {
+        w[u] = 0.0f;
+        if (some != 0) w[u] = mine[(int64_t)(k0 + __builtin_ctzll(some)) * of];
+        some &= some - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) v += w[u];
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) v += n[u] > 0 ? w[u] : 0.0f;
   }
   sums[wave][lane] = v;
   __syncthreads();
   if (wave != 0 || i >= of) return;
 #pragma unroll
   for (int w = 1; w < JOIN_WAVES; ++w) v += sums[w][lane];
+  const int r = i / width, c = i - r * width;
   if (c < K) da[((int64_t)j * R + r) * K + c] = to16<DT>(v);
   else db[((int64_t)j * N + c - K) * R + r] = to16<DT>(v);
 }

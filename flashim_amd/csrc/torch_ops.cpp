@@ -849,7 +849,11 @@ struct Adapters {
     entries = index.numel();
     wide = index.scalar_type() == at::kLong;
   }
-  int64_t ranks() const { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+  int64_t saved() const {
+    int64_t columns = 0;
+    check(fim_low_rank_adapters_saved(k, n, r, &columns), "low_rank_adapters of rank ", r);
+    return columns;
+  }
 };
 
 std::tuple<Tensor, Tensor> low_rank_adapters(const OptTensor& base, const Tensor& x, const Tensor& a, const Tensor& b,
@@ -865,10 +869,10 @@ std::tuple<Tensor, Tensor> low_rank_adapters(const OptTensor& base, const Tensor
     rows = matrix_rows(*base, "low_rank_adapters");
   }
   Tensor out = empty(sizes, x, x.scalar_type());
-  Tensor h = save ? empty({g.m, g.ranks()}, x, at::kFloat) : empty({0}, x, at::kFloat);
+  Tensor h = empty({save ? g.m : 0, g.saved()}, x, at::kFloat);
   check(fim_low_rank_adapters(base ? rows.data_ptr() : nullptr, base ? rows.stride(0) : 0, g.x.data_ptr(), g.x.stride(0),
                               dtype_code(x), g.m, g.k, g.n, g.a.data_ptr(), g.b.data_ptr(), g.j, g.r, g.index.data_ptr(), g.wide,
-                              g.entries, ptr<const float>(g.scales), (float)scale, out.data_ptr(), save ? ptr<float>(h) : nullptr,
+                              g.entries, ptr<const float>(g.scales), (float)scale, out.data_ptr(), h.numel() ? ptr<float>(h) : nullptr,
                               stream_of(x)),
         "low_rank_adapters ", x.sizes(), " x ", a.sizes(), " -> ", g.n);
   return {out, h};
@@ -885,7 +889,7 @@ std::tuple<Tensor, Tensor, Tensor> low_rank_adapters_backward(const Tensor& d_ou
   check_same(d_out, x.scalar_type(), x, "low_rank_adapters: gradient");
   if (want_adapters) {
     check_same(h, at::kFloat, x, "low_rank_adapters: saved products");
-    TORCH_CHECK_VALUE(h.dim() == 2 && h.size(0) == g.m && h.size(1) == g.ranks() && h.is_contiguous(),
+    TORCH_CHECK_VALUE(h.dim() == 2 && h.size(0) == g.m && h.size(1) == g.saved() && h.is_contiguous(),
                       "low_rank_adapters: saved products of shape ", h.sizes());
   }
   const Tensor d = matrix_rows(d_out, "low_rank_adapters");
@@ -900,7 +904,7 @@ std::tuple<Tensor, Tensor, Tensor> low_rank_adapters_backward(const Tensor& d_ou
   const Tensor ws = empty({bytes}, x, at::kByte);
   check(fim_low_rank_adapters_backward(d.data_ptr(), d.stride(0), g.x.data_ptr(), g.x.stride(0), dtype_code(x), g.m, g.k, g.n,
                                        g.a.data_ptr(), g.b.data_ptr(), g.j, g.r, g.index.data_ptr(), g.wide, g.entries,
-                                       ptr<const float>(g.scales), (float)scale, want_adapters ? ptr<float>(h) : nullptr,
+                                       ptr<const float>(g.scales), (float)scale, want_adapters && h.numel() ? ptr<float>(h) : nullptr,
                                        want_x ? dx.data_ptr() : nullptr, want_adapters ? da.data_ptr() : nullptr,
                                        want_adapters ? db.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(x)),
         "low_rank_adapters backward ", x.sizes(), " x ", a.sizes(), " -> ", g.n);

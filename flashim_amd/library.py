@@ -298,7 +298,7 @@ def low_rank_adapters(base, x, a, b, index, scales, scale, save):
     ``base``, ``x``, ``a`` and ``b``."""
     rows = x.numel() // x.shape[-1]
     return (x.new_empty((*x.shape[:-1], b.shape[1])),
-            x.new_empty((rows, _ranks(a.shape[1])) if save else (0,), dtype=torch.float32))
+            x.new_empty((rows if save else 0, _saved(x.shape[-1], b.shape[1], a.shape[1])), dtype=torch.float32))
 
 
 @_fake
@@ -307,8 +307,12 @@ def low_rank_adapters_backward(d_out, x, a, b, index, scales, scale, h, want_x, 
     return (x.new_empty(x.shape if want_x else (0,)), *(t.new_empty(t.shape if want_adapters else (0,)) for t in (a, b)))
 
 
-def _ranks(rank):
-    """Ranks that the kernels compute: 16, 32, 64 or 128."""
+def _saved(k, n, rank):
+    """Columns of ``s x A^T`` that the backward pass reads: ranks as the kernels compute them, or none where it computes them
+    again (``fim_low_rank_adapters_saved``)."""
+    width = -(-k // 32) * 32 + -(-n // 32) * 32
+    if rank <= 32 and width <= 384:
+        return 0
     return 16 if rank <= 16 else 32 if rank <= 32 else 64 if rank <= 64 else 128
 
 

@@ -318,16 +318,21 @@ int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, c
  * elements), a packed [J, R, K], b packed [J, N, R], all BF16 or FP16 (else 99), R <= 128; j = index[r / (M / entries)]
  * for row r (int32, or int64 with index_wide; M a multiple of entries), a row whose j is outside [0, J) keeps its base;
  * s_j = scale * scales[j] (scales FP32 [J], or NULL: 1). Sums and x A^T in FP32 (split in two 16-bit operands for the second
- * product), rounded once. out packed [M, N]; h, if not NULL (16-byte aligned), FP32 [M, 16 ceil'(R / 16)], s_j x A_j^T for the backward
- * pass (ceil' rounds up to 1, 2, 4 or 8; rows without an adapter are not written). No counterpart in the reference, as the next two. */
+ * product), rounded once. out packed [M, N]; h, if not NULL (16-byte aligned), FP32 [M, columns of
+ * fim_low_rank_adapters_saved], s_j x A_j^T for the backward pass (rows without an adapter are not written). No counterpart in
+ * the reference, as the next three. */
 int fim_low_rank_adapters(const void* base, int64_t base_stride, const void* x, int64_t x_stride, int dtype, int64_t M, int64_t K,
                           int64_t N, const void* a, const void* b, int64_t J, int64_t R, const void* index, int index_wide,
                           int64_t entries, const float* scales, float scale, void* out, float* h, hipStream_t stream);
 
+/* Columns of h that the backward pass needs for the adapters' gradients: R rounded up to 16, 32, 64 or 128, or 0 where it computes
+ * h again (narrow projections). */
+int fim_low_rank_adapters_saved(int64_t K, int64_t N, int64_t R, int64_t* columns);
+
 /* Bytes of workspace (256-byte aligned) that fim_low_rank_adapters_backward needs. */
 int fim_low_rank_adapters_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t J, int64_t R, int64_t* bytes);
 
-/* The gradients of x, a and b (packed; dx alone may be NULL, or da and db together, and h with those), from d_out [M, N], M >= 1,
+/* The gradients of x, a and b (packed; dx alone may be NULL, or da and db together; h where it is not needed), from d_out [M, N], M >= 1,
  * and the forward pass's h: t = s_j d_out B_j, dx = t A_j, dA_j = t^T x, dB_j = d_out^T h over the rows of j. */
 int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_stride, const void* x, int64_t x_stride, int dtype, int64_t M,
                                    int64_t K, int64_t N, const void* a, const void* b, int64_t J, int64_t R, const void* index,
