@@ -7,6 +7,11 @@ Training: :class:`GatedBlock` is an ordinary module; :func:`train_step` takes it
 and steps the optimizer. Inference: :class:`QuantizedGatedBlock` keeps the norm and the gated product, quantizes the hidden
 map with static scales from one calibration pass, and contracts it with the INT8 or MXFP8 1x1 convolution and its fused
 residual, as the refiner blocks (:mod:`flashim_amd.blocks`) do.
+
+Adapting: :class:`Adapters` are low-rank changes of the contraction, one of them for each image of a batch (``index``).
+:class:`AdaptedGatedBlock` trains them beside a frozen block (``train_step`` with :class:`flashim_amd.optim.Muon`, say), and
+:class:`QuantizedGatedBlock` takes them beside its INT8 or MXFP8 contraction: many requests' adapters at once, one set of
+quantized weights.
 """
 
 from __future__ import annotations
@@ -62,9 +67,40 @@ def train_step(module: nn.Module, optimizer: torch.optim.Optimizer, loss: Callab
     return value.detach(), norm
 
 
+class Adapters(nn.Module):
+    """``count`` adapters of a block's contraction, ``scale (h A_j^T) B_j^T`` beside ``h Wd^T``: ``a`` random, ``b`` zero (no
+    change) at first."""
+
+    def __init__(self, block: GatedBlock, count: int, rank: int, *, scale: float = 1.0,
+                 generator: torch.Generator | None = None) -> None:
+        super().__init__()
+        channels, hidden = block.w_down.shape
+        like = dict(dtype=block.w_down.dtype, device=block.w_down.device)
+        self.a = nn.Parameter((torch.randn(count, rank, hidden, generator=generator) * hidden ** -0.5).to(**like))
+        self.b = nn.Parameter(torch.zeros(count, channels, rank, **like))
+        self.scale = scale
+
+    def forward(self, base: Tensor, hidden: Tensor, index: Tensor) -> Tensor:
+        """``base`` and each image's adapter of ``hidden``; ``index`` ``[B]``, outside ``[0, count)`` for none."""
+        return ops.low_rank_adapters(base, hidden, self.a, self.b, index, scale=self.scale)
+
+
+class AdaptedGatedBlock(nn.Module):
+    """``block``, whose parameters this freezes, with ``adapters`` that train."""
+
+    def __init__(self, block: GatedBlock, adapters: Adapters) -> None:
+        super().__init__()
+        self.block, self.adapters = block.requires_grad_(False), adapters
+
+    def forward(self, x: Tensor, index: Tensor) -> Tensor:
+        hidden = self.block.hidden(x)
+        return self.adapters(x + F.linear(hidden, self.block.w_down, self.block.b_down), hidden, index)
+
+
 class QuantizedGatedBlock:
     """A trained block with its contraction in ``preset`` ``"int8"`` or ``"mxfp8"``; ``sample`` gives the hidden map's static
-    scale. BF16, ``hidden`` a multiple of 32."""
+    scale. BF16, ``hidden`` a multiple of 32. A call with ``adapters`` and ``index`` ``[B]`` adds each image's adapter, from the
+    hidden map as it was before its quantization."""
 
     def __init__(self, block: GatedBlock, preset: str, sample: Tensor) -> None:
         if preset not in ("int8", "mxfp8"):
@@ -80,12 +116,16 @@ class QuantizedGatedBlock:
                 self.scale = (hidden.float().abs().amax() / quant.INT8_MAX).clamp_min(1e-8).reshape(())
 
     @torch.no_grad()
-    def __call__(self, x: Tensor) -> Tensor:
+    def __call__(self, x: Tensor, adapters: Adapters | None = None, index: Tensor | None = None) -> Tensor:
+        if (adapters is None) != (index is None):
+            raise ValueError("adapters come with an index of them")
         hidden, bias = self.block.hidden(x), self.block.b_down.detach()
         if self.preset == "mxfp8":
             q = ops.quantize_mxfp8(hidden, self.scale)
-            return ops.mxfp8_conv2d(q.values, self.scale, self.weight.values, self.weight.scale_exponent, bias, *_POINTWISE,
-                                    residual=x)
-        codes, weight_scale = self.weight
-        q = ops.quantize_int8(hidden, self.scale)
-        return ops.int8_conv2d(q.values, codes, self.scale, weight_scale, bias, *_POINTWISE, residual=x)
+            out = ops.mxfp8_conv2d(q.values, self.scale, self.weight.values, self.weight.scale_exponent, bias, *_POINTWISE,
+                                   residual=x)
+        else:
+            codes, weight_scale = self.weight
+            q = ops.quantize_int8(hidden, self.scale)
+            out = ops.int8_conv2d(q.values, codes, self.scale, weight_scale, bias, *_POINTWISE, residual=x)
+        return out if adapters is None else adapters(out, hidden, index)
