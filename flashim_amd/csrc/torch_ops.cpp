@@ -801,6 +801,12 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
     cols.push_back(w.size(-1));
     factors.push_back(muon_factor(lr, adjust, rows.back(), cols.back()));
   }
+  std::vector<const void*> written;  // (empty tensors have none)
+  for (size_t i = 0; i < n; ++i)
+    if (p[i].numel() > 0) written.insert(written.end(), {pp[i], mp[i]});
+  std::sort(written.begin(), written.end());
+  TORCH_CHECK_VALUE(std::adjacent_find(written.begin(), written.end()) == written.end(),
+                    "muon_step_: a parameter or momentum is there twice");
   int64_t bytes = 0;
   check(fim_muon_step_workspace((int64_t)n, batch.data(), rows.data(), cols.data(), &bytes), "muon_step_");
   const Tensor ws = empty({bytes}, params[0], at::kByte);

@@ -134,7 +134,9 @@ def schulz_bound(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: flo
 
     Step k's rounding is an error of at most e_k |X_k|: each product's operands are off by 2^-23, the dropped product of the
     low halves by 2^-24, and a sum of K terms, rounded K / 16 times or more at 2^-24 each, by 4 sqrt(K) 2^-24 (independent
-    roundings); three products a step, whose factors a, b |A| and c |A|^2 multiply them by at most |a| + 2 |b| + 2 |c|. Later
+    roundings); three products a step, whose factors a, b |A| and c |A|^2 multiply them by at most |a| + 2 |b| + 2 |c|. Besides, a low half
+    below FP16's normal numbers, 2^-14, may count as zero: with the scales of 2^13 and more that go with singular values of at
+    most 2, 2^-27 of each entry. Later
     steps multiply an error by at most the largest slope of the polynomial that is left (of an odd matrix function), between 0
     and the largest singular value."""
     a, b, c = coefficients
@@ -152,7 +154,7 @@ def schulz_bound(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: flo
             at = at * (a + b * at**2 + c * at**4)
             slopes.append(slope.abs().max().item())
         # (the step's own slope is in the sum above: what is left are the steps after it; X_0's conversion meets all of them)
-        total += e * x.norm().item() * slopes[-2 if k else -1]
+        total += (e * x.norm().item() + 2.0**-27 * math.sqrt(x.numel())) * slopes[-2 if k else -1]
     return total
 
 

@@ -32,6 +32,9 @@ def _close(name, got, want, error):
     got = got.detach().double().cpu()
     bound = error + HALF_STEP[dtype] * (want.abs() + error) + TINY[dtype]
     off = (got - want).abs()
+    # a value past the type's range rounds to infinity: 65520 and more in FP16, its largest 65504 and half of its last step 32
+    most = torch.finfo(dtype).max * (1 + HALF_STEP[dtype] / 2)
+    off[torch.isinf(got) & (got.sign() == want.sign()) & (want.abs() + bound >= most)] = 0
     assert (off <= bound).all(), (name, (off / bound).max().item(), (off > bound).sum().item(), off.numel())
 
 
@@ -109,3 +112,204 @@ def test_values_that_name_no_adapter():
     index = torch.tensor([2**32, -(2**32), 2**32 + 1, 2**40, 3, -1])  # whose low halves would name one
     out, grads = _run(base, x, a, b, index, 1.0, d_out)
     assert torch.equal(out.cpu(), base) and all((grads[n] == 0).all() for n in ("x", "a", "b"))
+
+
+def test_gradients_against_differences():
+    """Directional differences of the float64 forward, and the kernel's gradients: second-order terms vanish (each input enters
+    linearly), so the two agree to the gradient's own error."""
+    base, x, a, b, d_out = _inputs((4, 25), 48, 40, 8, 3, BF16, seed=4)
+    index = torch.tensor([2, 0, 2, -1])
+    _, grads = _run(base, x, a, b, index, 0.5, d_out)
+    want = ref.low_rank_adapters(base, x, a, b, index, 0.5, d_out)
+    g = torch.Generator().manual_seed(5)
+
+    def value(x, a, b):
+        return (ref.low_rank_adapters(base, x, a, b, index, 0.5)["out"] * d_out.double()).sum()
+
+    for i, name in enumerate(("x", "a", "b")):
+        at = [t.double() for t in (x, a, b)]
+        v = torch.randn(at[i].shape, generator=g, dtype=torch.float64)
+        plus, minus = ([t + s * v if k == i else t for k, t in enumerate(at)] for s in (0.5, -0.5))
+        difference = value(*plus) - value(*minus)
+        bound = ((want[name + "_error"] + HALF_STEP[BF16] * want[name].abs() * 1.01) * v.abs()).sum()
+        assert (grads[name].double().cpu() * v).sum().sub(difference).abs() <= bound, name
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("width", [(64, 256), (200, 520)])
+def test_small_and_large_values(width, dtype):
+    """Gradients of 1e-6 and activations of 1e3: FP16 holds neither x A^T nor d_out B as they are."""
+    k, n = width
+    for d, up in ((1e-6, 1.0), (1.0, 1e3)):
+        base, x, a, b, d_out = _inputs((2, 300), k, n, 8, 3, dtype, seed=6, d=d)
+        x = (x.float() * up).to(dtype)
+        a = (a.float() * (30.0 if up > 1 else 1.0)).to(dtype)
+        b = (b.float() * (1e-3 if up > 1 else 1.0)).to(dtype)
+        _check(base, x, a, b, torch.tensor([1, 2]), 1.0, d_out)
+
+
+@pytest.mark.parametrize("kind", ["image", "row"])
+def test_infinite_and_nan_rows_stay_alone(kind):
+    base, x, a, b, _ = _inputs((6, 40), 64, 96, 8, 3, BF16, seed=7)
+    index = _index(kind, (6, 40), 3, seed=7)
+    want = _run(base, x, a, b, index, 1.0)[0]
+    bad = x.clone()
+    bad[2, 5, 3], bad[4, 39, 60], bad[0, 0, 0] = math.nan, math.inf, -math.inf
+    got = _run(base, bad, a, b, index, 1.0)[0]
+    rows = torch.ones(6, 40, dtype=torch.bool)
+    rows[2, 5] = rows[4, 39] = rows[0, 0] = False
+    assert torch.equal(got.cpu()[rows], want.cpu()[rows])
+    for at in ((2, 5), (4, 39), (0, 0)):
+        j = index[at] if kind == "row" else index[at[0]]
+        if j >= 0:
+            exact = base[at].double() + (bad[at].double() @ a[j].double().t()) @ b[j].double().t()
+            assert torch.equal(torch.isfinite(got[at].cpu()), torch.isfinite(exact))
+
+
+def test_layouts():
+    """Rows apart in memory, leading dimensions that do not merge, expanded bases and gradients, transposed adapters."""
+    base, x, a, b, d_out = _inputs((3, 30), 64, 96, 8, 4, BF16, seed=8)
+    index = torch.tensor([3, 1, 0])
+    want, want_grads = _run(base, x, a, b, index, 0.5, d_out)
+
+    def apart(t):
+        return torch.cat([t, t + 1], -1)[..., :t.shape[-1]]
+
+    def turned(t):
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    for view in (apart, turned, lambda t: torch.cat([t[..., :1], t], -1)[..., 1:]):
+        dev = [view(t.to(DEV)) for t in (base, x, a, b)]
+        leaves = [t.detach().requires_grad_() for t in dev]
+        out = ops.low_rank_adapters(*leaves, index.to(DEV), scale=0.5)
+        assert torch.equal(out, want)
+        for g, name in zip(torch.autograd.grad(out, leaves, view(d_out.to(DEV))), ("base", "x", "a", "b")):
+            assert torch.equal(g, want_grads[name]), name
+    one = base[:1, :1].to(DEV)
+    expanded = ops.low_rank_adapters(one.expand(3, 30, 96), x.to(DEV), a.to(DEV), b.to(DEV), index.to(DEV), scale=0.5)
+    assert torch.equal(expanded, ops.low_rank_adapters(one.expand(3, 30, 96).contiguous(), x.to(DEV), a.to(DEV), b.to(DEV),
+                                                       index.to(DEV), scale=0.5))
+    leaf = one.clone().requires_grad_()
+    out = ops.low_rank_adapters(leaf.expand(3, 30, 96), x.to(DEV), a.to(DEV), b.to(DEV), index.to(DEV), scale=0.5)
+    torch.testing.assert_close(torch.autograd.grad(out, leaf, torch.ones_like(out))[0], torch.full_like(leaf, 90.0))
+
+
+@pytest.mark.parametrize("wanted", ["x", "a", "b", "base", "xa", "ab"])
+@pytest.mark.parametrize("width", [(64, 96), (300, 260)])
+def test_gradients_wanted_alone(width, wanted):
+    k, n = width
+    base, x, a, b, d_out = _inputs((2, 350), k, n, 8, 3, BF16, seed=9)
+    index = torch.tensor([1, 2], device=DEV)
+    names = ["base", "x", "a", "b"]
+    every = dict(zip(names, (t.to(DEV) for t in (base, x, a, b))))
+    whole = {m: t.clone().requires_grad_() for m, t in every.items()}
+    want = dict(zip(names, torch.autograd.grad(ops.low_rank_adapters(*whole.values(), index), list(whole.values()), d_out.to(DEV))))
+    chosen = ["base"] if wanted == "base" else list(wanted)
+    some = {m: t.clone().requires_grad_(m in chosen) for m, t in every.items()}
+    got = torch.autograd.grad(ops.low_rank_adapters(*some.values(), index), [some[m] for m in chosen], d_out.to(DEV))
+    assert all(torch.equal(g, want[m]) for g, m in zip(got, chosen))
+
+
+def test_no_rows():
+    base, x, a, b, _ = (t.to(DEV) for t in _inputs((0, 5), 16, 24, 4, 3, BF16))
+    leaves = [t.requires_grad_() for t in (base, x, a, b)]
+    out = ops.low_rank_adapters(*leaves, torch.zeros(0, dtype=torch.int64, device=DEV))
+    assert out.shape == (0, 5, 24)
+    grads = torch.autograd.grad(out, leaves, torch.zeros_like(out))
+    assert all((g == 0).all() and g.shape == t.shape for g, t in zip(grads, leaves))
+
+
+def test_rows_past_32_bit_offsets():
+    """600 rows 2^22 elements apart (5 GB): forward and both forms of the backward pass."""
+    for k, n in ((64, 96), (200, 520)):
+        base, x, a, b, d_out = _inputs((600,), k, n, 8, 3, BF16, seed=10)
+        index = torch.arange(600) % 4 - 1
+        memory = torch.empty(600, 1 << 22, dtype=BF16, device=DEV)
+        far = memory[:, 5:5 + k]
+        far.copy_(x)
+        memory[:, 5000:5000 + n].copy_(base)
+        memory[:, 10000:10000 + n].copy_(d_out)
+        want, want_grads = _run(base, x, a, b, index, 1.0, d_out)
+        leaves = [t.to(DEV).requires_grad_() for t in (a, b)]
+        x_leaf = far.detach().requires_grad_()
+        out = ops.low_rank_adapters(memory[:, 5000:5000 + n], x_leaf, *leaves, index.to(DEV))
+        assert torch.equal(out, want)
+        d = memory[:, 10000:10000 + n]
+        for g, name in zip(torch.autograd.grad(out, [x_leaf, *leaves], d), ("x", "a", "b")):
+            assert torch.equal(g, want_grads[name]), name
+        del memory, far, x_leaf, d, out
+
+
+def test_more_adapters_than_rows_and_many_chunks():
+    base, x, a, b, d_out = _inputs((40,), 96, 64, 4, 300, BF16, seed=11)
+    _check(base, x, a, b, torch.randint(0, 300, (40,), generator=torch.Generator().manual_seed(0)), 1.0, d_out)
+    base, x, a, b, d_out = _inputs((9000,), 40, 500, 4, 2, BF16, seed=12)
+    _check(base, x, a, b, (torch.arange(9000) // 5000), 1.0, d_out)
+
+
+def test_same_bits_on_any_stream():
+    base, x, a, b, d_out = _inputs((3, 3000), 64, 256, 8, 3, BF16, seed=13)
+    index = torch.tensor([0, 2, 0])
+    want, want_grads = _run(base, x, a, b, index, 1.0, d_out)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out, grads = _run(base, x, a, b, index, 1.0, d_out)
+        side.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(grads[m], want_grads[m]) for m in grads)
+
+
+@pytest.mark.parametrize("width", [(64, 256), (300, 260)])
+def test_graph_capture(width):
+    k, n = width
+    base, x, a, b, d_out = (t.to(DEV) for t in _inputs((3, 500), k, n, 8, 4, BF16, seed=14))
+    index = torch.tensor([0, 3, -1], device=DEV)
+    leaves = [t.requires_grad_() for t in (base, x, a, b)]
+
+    def both():
+        out = ops.low_rank_adapters(*leaves, index, scale=0.5)
+        return out.detach(), *torch.autograd.grad(out, leaves, d_out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = both()
+    for seed in range(3):
+        with torch.no_grad():
+            leaves[1].copy_(_inputs((3, 500), k, n, 8, 4, BF16, seed=20 + seed)[1])
+            index.copy_(torch.tensor([seed, -1, 3 - seed]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(c, e) for c, e in zip(captured, both()))
+
+
+def test_refusals():
+    base, x, a, b, _ = (t.to(DEV) for t in _inputs((2, 10), 64, 48, 8, 3, BF16))
+    index = torch.tensor([0, 1], device=DEV)
+    wide = torch.zeros(3, 129, 64, device=DEV, dtype=BF16), torch.zeros(3, 48, 129, device=DEV, dtype=BF16)
+    bad = [(base.float(), x.float(), a.float(), b.float(), index), (base, x, a.to(F16), b, index), (base.to(F16), x, a, b, index),
+           (base[..., :40], x, a, b, index), (base, x, a[:, :, :32], b, index), (base, x, a[:2], b, index), (base, x, a, b[..., :4], index),
+           (base, x, a, b, index[:1]), (base, x, a, b, index.float()), (base, x, a, b, index.cpu()), (base, x, a, b, index[:, None]),
+           (base, x, a[0], b[0], index), (base, x, *wide, index), (base, x, a[:0], b[:0], index), (base, x.cpu(), a, b, index),
+           (base, x, a, b, torch.zeros(2, 10, 64, dtype=torch.int32, device=DEV))]
+    for args in bad:
+        with pytest.raises(NotImplementedError, match="no HIP impl"):
+            ops.low_rank_adapters(*args)
+    for scale in (torch.ones(2, device=DEV), torch.ones(3, device=DEV, dtype=BF16), torch.ones(3)):
+        with pytest.raises(NotImplementedError, match="no HIP impl"):
+            ops.low_rank_adapters(base, x, a, b, index, scale=scale)
+    with pytest.raises((TypeError, ValueError)):
+        torch.ops.flashim_amd.low_rank_adapters(base, x, a.to(F16), b, index, None, 1.0, False)
+    with pytest.raises(ValueError):
+        torch.ops.flashim_amd.low_rank_adapters(base, x, a, b, index[:1], None, 1.0, False)
+    with pytest.raises(NotImplementedError, match="scales"):
+        ops.low_rank_adapters(base, x, a, b, index, scale=torch.ones(3, device=DEV, requires_grad=True))
+    leaf = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(ops.low_rank_adapters(base, leaf, a, b, index).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        g.sum().backward()

@@ -60,3 +60,206 @@ def test_stacks(shape):
 def test_large():
     g = _gradient(520, 2100, seed=5, dtype=BF16)
     _check(ops.orthogonalize(g.to(DEV), out_dtype=F32), g)
+
+
+@pytest.mark.parametrize("shape", [(5, 7), (64, 256), (70, 600), (300, 90)])
+def test_conversion_keeps_fp32(shape):
+    """One step of X = 1 X: what the halves hold, element by element: 2^-23 of each, twice (X and a product of 1), 2^-24 where a
+    term of the low halves is left out, and the sums' own roundings; a thousandth part of lo below FP16's normal numbers."""
+    g = _gradient(*shape, seed=7)
+    got = ops.orthogonalize(g.to(DEV), steps=1, coefficients=(1.0, 0.0, 0.0)).double().cpu()
+    want = g.double() / (g.double().norm() + 1e-7)
+    assert ((got - want).abs() <= 2.0**-20 * want.abs() + 2.0**-28).all()
+
+
+@pytest.mark.parametrize("steps, coefficients", [(1, (1.5, -0.5, 0.0)), (12, (1.5, -0.5, 0.0)), (3, (0.0, 0.0, 1.0)),
+                                                 (10, (1.875, -1.25, 0.375)), (6, (2.0, -1.5, 0.5)), (4, (-1.5, 0.5, 0.0))])
+@pytest.mark.parametrize("shape", [(24, 40), (100, 600)])
+def test_coefficients(shape, steps, coefficients):
+    g = _gradient(*shape, seed=8)
+    _check(ops.orthogonalize(g.to(DEV), steps=steps, coefficients=coefficients), g, steps=steps, coefficients=coefficients)
+
+
+@pytest.mark.parametrize("shape", [(24, 40), (130, 200)])
+@pytest.mark.parametrize("scale", [1e-30, 1e-9, 1e12, 1e30])
+def test_magnitudes(shape, scale):
+    """Squares past FP32's range; a norm near eps and below it."""
+    g = (_gradient(*shape, seed=9) * scale).float()
+    _check(ops.orthogonalize(g.to(DEV)), g)
+    _check(ops.orthogonalize(g.to(DEV), eps=1e-3), g, eps=1e-3)
+
+
+@pytest.mark.parametrize("shape", [(24, 40), (40, 24), (130, 200)])
+def test_zeros_and_nonfinite(shape):
+    zero = torch.zeros(shape, device=DEV)
+    assert (ops.orthogonalize(zero) == 0).all()
+    stack = torch.stack([_gradient(*shape, seed=10).to(DEV) for _ in range(4)])
+    want = ops.orthogonalize(stack)
+    stack[1, 3, 5], stack[2, 0, 0] = math.nan, math.inf
+    got = ops.orthogonalize(stack)
+    assert torch.isnan(got[1]).all() and torch.isnan(got[2]).all()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 4, 4), (3, 0, 4)])
+def test_empty(shape):
+    g = torch.empty(shape, device=DEV)
+    assert ops.orthogonalize(g).shape == g.shape
+    ops.muon_step_([g], [g.clone()], [g.clone()], lr=0.1)
+
+
+def test_layouts():
+    """Transposed and strided gradients, and views at odd offsets: the values of their packed copies."""
+    base = _gradient(90, 150, seed=11, dtype=BF16).to(DEV)
+    for view in (base.t(), base[::2, 1:91], base[3:40], base.reshape(-1)[7:7 + 80 * 33].view(80, 33),
+                 base.reshape(-1)[1:1 + 12 * 9 * 30].view(12, 9, 30).transpose(0, 1)):
+        assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(view.contiguous()))
+
+
+def test_many_small_ones():
+    g = _gradient(700, 9, 14, seed=12)
+    _check(ops.orthogonalize(g.to(DEV)), g)
+
+
+# -- the step ------------------------------------------------------------------------------------------------------------
+
+
+def _step(p, g, m, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="original", steps=5):
+    """One matrix or stack, float64: the parameter, the momentum, and the parameter's bound."""
+    m = momentum * m.double() + g.double()
+    u = g.double() + momentum * m if nesterov else m
+    rows, cols = p.shape[-2:]
+    f = {"original": max(1.0, rows / cols) ** 0.5, "match_rms": 0.2 * max(rows, cols) ** 0.5, "none": 1.0}[adjust]
+    flat = u.reshape(-1, rows, cols)
+    o = torch.stack([ref.orthogonalize(x, steps=steps) for x in flat]).reshape(u.shape)
+    # u itself is rounded to FP32, one or two FMAs: as any operand's error
+    off = torch.tensor([2 * ref.schulz_bound(x, steps=steps) for x in flat]).reshape(*u.shape[:-2], 1, 1)
+    return p.double() * (1 - lr * weight_decay) - lr * f * o, m, lr * f * off
+
+
+def _check_step(params, grads, momenta, **kwargs):
+    before = [[t.cpu().clone() for t in ts] for ts in (params, grads, momenta)]
+    ops.muon_step_(params, grads, momenta, **kwargs)
+    for p, g, m, p0, g0, m0 in zip(params, grads, momenta, *before):
+        want, want_m, off = _step(p0, g0, m0, **kwargs)
+        assert torch.equal(g.cpu(), g0)
+        assert ((m.double().cpu() - want_m).abs() <= 2.0**-22 * (m0.double().abs() + g0.double().abs())).all()
+        error = (p.double().cpu() - want)
+        per = error.reshape(-1, *error.shape[-2:]).norm(dim=(1, 2))
+        bound = off.reshape(-1) + (2 * U[p.dtype] + 2.0**-22) * (want.abs() + p0.double().abs()).reshape(-1, *error.shape[-2:]).norm(dim=(1, 2))
+        assert (per <= bound).all(), (p.shape, (per / bound).max())
+
+
+def _triples(shapes, p_dtype, g_dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    params = [(torch.randn(s, generator=g) * s[-1] ** -0.5).to(p_dtype).to(DEV) for s in shapes]
+    grads = [_gradient(*s, seed=seed + i, dtype=g_dtype).to(DEV) for i, s in enumerate(shapes)]
+    momenta = [5 * _gradient(*s, seed=seed + 50 + i).to(DEV) for i, s in enumerate(shapes)]
+    return params, grads, momenta
+
+
+MIXED = [(64, 256), (256, 64), (17, 5), (1, 9), (90, 90), (3, 20, 30), (130, 260), (260, 130), (2, 70, 300), (16, 700), (33, 40)]
+
+
+@pytest.mark.parametrize("p_dtype, g_dtype", [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (BF16, F32), (F16, BF16)])
+def test_step(p_dtype, g_dtype):
+    _check_step(*_triples(MIXED, p_dtype, g_dtype), lr=0.3, weight_decay=0.2)
+
+
+@pytest.mark.parametrize("kwargs", [dict(nesterov=False), dict(momentum=0.0), dict(momentum=0.5, steps=2), dict(adjust="match_rms"),
+                                    dict(adjust="none", weight_decay=1.0), dict(lr=0.0, weight_decay=0.5)])
+def test_step_options(kwargs):
+    _check_step(*_triples([(24, 40), (130, 70), (40, 24)], F32, F32, seed=1), **{"lr": 0.1, **kwargs})
+
+
+def test_step_of_many_matrices():
+    """More than one launch's table."""
+    _check_step(*_triples([(12 + i % 5, 20 + i % 7) for i in range(70)] + [(100, 68)] * 30, F32, F32, seed=2), lr=0.1)
+
+
+def test_packed_views_at_odd_offsets_and_strided_tensors():
+    shapes = [(7, 9), (65, 70), (20, 31)]
+    sizes = [a * b for a, b in shapes]
+    buckets = [torch.full((sum(sizes) + 4,), 9.0, dtype=t, device=DEV) for t in (BF16, F16, F32)]
+    views = [[b[1:1 + sum(sizes)].split(sizes)[i].view(s) for i, s in enumerate(shapes)] for b in buckets]
+    for view, new in zip(views, _triples(shapes, BF16, F16, seed=3)):
+        for v, n in zip(view, new):
+            v.copy_(n)
+    _check_step(*views, lr=0.1)
+    assert all((b[:1] == 9).all() and (b[-3:] == 9).all() for b in buckets)
+    big = torch.randn(3, 40, 60, device=DEV)
+    strided = [[big[i].t()[:, ::2]] for i in range(3)]
+    rest = big.clone()
+    _check_step(*strided, lr=0.1)
+    assert torch.equal(big[0][1::2], rest[0][1::2]) and torch.equal(big[2][1::2], rest[2][1::2])
+
+
+def test_same_bits_on_any_stream_and_versions():
+    args = _triples([(64, 256), (130, 260)], F32, F32, seed=4)
+    copies = [[[t.clone() for t in ts] for ts in args] for _ in range(3)]
+    side = torch.cuda.Stream()
+    for c in copies:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.muon_step_(*c, lr=0.1)
+        side.synchronize()
+    for c in copies[1:]:
+        assert all(torch.equal(a, b) for x, y in zip(c, copies[0]) for a, b in zip(x, y))
+    versions = [[t._version for t in ts] for ts in args]
+    ops.muon_step_(*args, lr=0.1)
+    assert [[t._version - v for t, v in zip(ts, vs)] for ts, vs in zip(args, versions)] == [[1, 1], [0, 0], [1, 1]]
+
+
+def test_graph_capture():
+    """Replayed on new gradients with eager work and synchronizations between, against eager steps from the same state."""
+    shapes = [(64, 256), (130, 260), (512, 1100)]
+    params, grads, momenta = _triples(shapes, F32, F32, seed=5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.muon_step_([p.clone() for p in params], grads, [m.clone() for m in momenta], lr=0.1)
+        ops.orthogonalize(grads[2])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step_(params, grads, momenta, lr=0.1)
+        o = ops.orthogonalize(grads[2])
+    eager = [[t.clone() for t in ts] for ts in (params, momenta)]
+    for seed in range(3):
+        for g, new in zip(grads, _triples(shapes, F32, F32, seed=20 + seed)[1]):
+            g.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.muon_step_(eager[0], grads, eager[1], lr=0.1)
+        assert torch.equal(o, ops.orthogonalize(grads[2]))
+        assert all(torch.equal(a, b) for a, b in zip(params + momenta, eager[0] + eager[1]))
+
+
+def test_refusals():
+    g = torch.ones(4, 5, device=DEV)
+    for bad in (g.double(), g[0], g.cpu(), g.long()):
+        with pytest.raises(NotImplementedError, match="no HIP impl"):
+            ops.orthogonalize(bad)
+    for kwargs in (dict(steps=0), dict(steps=101), dict(coefficients=(1.0, 2.0)), dict(eps=-1.0), dict(out_dtype=torch.float64)):
+        with pytest.raises(NotImplementedError, match="no HIP impl"):
+            ops.orthogonalize(g, **kwargs)
+    from flashim_amd._lib import UnsupportedShape
+
+    for coefficients in ((9.0, -20.0, 9.0), (3.0, 1.0, 1.0), (math.nan, 0.0, 0.0), (100.0, 0.0, 0.0)):
+        with pytest.raises(UnsupportedShape):
+            ops.orthogonalize(g, coefficients=coefficients)
+    p, m = g.clone(), g.clone()
+    for args in (([p], [g], []), ([p], [g[:3]], [m]), ([p], [g], [m.bfloat16()]), ([p[0]], [g[0]], [m[0]]), ([p], [g.cpu()], [m]),
+                 ([], [], []), ([p.double()], [g], [m]), (p, g, m)):
+        with pytest.raises(NotImplementedError, match="no HIP impl"):
+            ops.muon_step_(*args, lr=0.1)
+    with pytest.raises(NotImplementedError, match="no HIP impl"):
+        ops.muon_step_([p], [g], [m], lr=0.1, adjust="half")
+    with pytest.raises(ValueError, match="twice"):
+        ops.muon_step_([p, p], [g, g], [m, m.clone()], lr=0.1)
+    leaf = g.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="not implemented"):
+        ops.orthogonalize(leaf).sum().backward()
+    with pytest.raises(NotImplementedError, match="no derivative"):
+        torch.ops.flashim_amd.muon_step_([leaf], [g], [m], 0.1, 0.9, True, 0.0, 0, 5, 3.0, -3.0, 1.0, 1e-7)
+    assert torch.equal(p, g) and torch.equal(m, g)
