@@ -223,22 +223,23 @@ static int ortho_check(const OrthoCall& c, OrthoScalars& k) {
 }
 
 template <int T, int LDS>
-static void launch_small(const OrthoStack* table, int count, uint32_t grid, const OrthoScalars& k, hipStream_t stream) {
-  ortho_small_kernel<T, LDS><<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(table, count, k);
+static void launch_small(const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid, const OrthoScalars& k,
+                         hipStream_t stream) {
+  ortho_small_kernel<T, LDS><<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(few, table, count, k);
 }
 
 // LDS classes: 160 KB is a CU's; matrices of at most half of it run two to a CU
-static void launch_small(int T, bool half, const OrthoStack* table, int count, uint32_t grid, const OrthoScalars& k,
-                         hipStream_t stream) {
+static void launch_small(int T, bool half, const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid,
+                         const OrthoScalars& k, hipStream_t stream) {
   switch (T * 2 + half) {
-    case 2: return launch_small<1, SMALL_LDS>(table, count, grid, k, stream);
-    case 3: return launch_small<1, SMALL_LDS / 2>(table, count, grid, k, stream);
-    case 4: return launch_small<2, SMALL_LDS>(table, count, grid, k, stream);
-    case 5: return launch_small<2, SMALL_LDS / 2>(table, count, grid, k, stream);
-    case 6: return launch_small<3, SMALL_LDS>(table, count, grid, k, stream);
-    case 7: return launch_small<3, SMALL_LDS / 2>(table, count, grid, k, stream);
-    case 8: return launch_small<4, SMALL_LDS>(table, count, grid, k, stream);
-    case 9: return launch_small<4, SMALL_LDS / 2>(table, count, grid, k, stream);
+    case 2: return launch_small<1, SMALL_LDS>(few, table, count, grid, k, stream);
+    case 3: return launch_small<1, SMALL_LDS / 2>(few, table, count, grid, k, stream);
+    case 4: return launch_small<2, SMALL_LDS>(few, table, count, grid, k, stream);
+    case 5: return launch_small<2, SMALL_LDS / 2>(few, table, count, grid, k, stream);
+    case 6: return launch_small<3, SMALL_LDS>(few, table, count, grid, k, stream);
+    case 7: return launch_small<3, SMALL_LDS / 2>(few, table, count, grid, k, stream);
+    case 8: return launch_small<4, SMALL_LDS>(few, table, count, grid, k, stream);
+    case 9: return launch_small<4, SMALL_LDS / 2>(few, table, count, grid, k, stream);
   }
 }
 
@@ -331,6 +332,7 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
   uint8_t* free_at = static_cast<uint8_t*>(workspace) + cdiv(c.count * (int64_t)sizeof(OrthoStack), 256) * 256;
 
   OrthoFill fill;
+  memset(&fill, 0, sizeof(fill));
   int filled = 0;  // entries of `fill` that the device's table does not hold yet
   int written = 0;
   auto flush = [&]() {
@@ -397,12 +399,17 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
     }
     const int n = written + filled - start;
     if (n == 0) continue;
-    flush();
-    const OrthoStack* t = table + start;
     if (group > 0) {
-      launch_small(group / 2, group & 1, t, n, (uint32_t)first[0], k, stream);
+      OrthoFew few;
+      const bool args = n <= SMALL_FEW && n == filled;  // (no table: neither its launch nor its latency)
+      memcpy(few.s, fill.s, sizeof(few));
+      if (args) filled = 0;
+      else flush();
+      launch_small(group / 2, group & 1, few, args ? nullptr : table + start, n, (uint32_t)first[0], k, stream);
       continue;
     }
+    flush();
+    const OrthoStack* t = table + start;
     ortho_momentum_kernel<<<dim3((unsigned)first[0]), dim3(ORTHO_T), 0, stream>>>(t, n, k);
     ortho_convert_kernel<<<dim3((unsigned)first[1]), dim3(ORTHO_T), 0, stream>>>(t, n, k);
     launch_products(t, n, plan, part, k, stream);

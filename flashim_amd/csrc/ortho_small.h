@@ -1,9 +1,10 @@
 // A whole Newton-Schulz iteration, or optimizer step, of a small matrix in one workgroup: X, A and P stay in LDS.
 //
 // At most 64 rows (of the shorter side) whose X fits: read once, written once, and no launch between the 3 `steps` products, which on
-// tiles would be as many launches of one or two workgroups. Sixteen wavefronts (eight took 46 us
-// for 39) on 16 x 16 x 32 MFMAs: X X^T is split over the columns of eight (each fragment is read once, and is either operand), four wavefronts' sums meet the other four's in LDS, and each wavefront adds up
-// one of the 16 blocks, those above the diagonal from the ones below, read across; P X is split over the columns too, and each
+// tiles would be as many launches of one or two workgroups. Sixteen wavefronts on
+// 16 x 16 x 32 MFMAs: X X^T is split over the columns of four (each fragment is read once, and is either operand), whose sums meet in
+// LDS; each wavefront adds up one of the 16 blocks, those above the diagonal from the ones below, read across; P X is split over the
+// columns too, and each
 // wavefront replaces the columns it has read.
 #pragma once
 
@@ -11,11 +12,12 @@
 
 namespace fim {
 
-constexpr int SMALL_WAVES = 16, SMALL_SUMS = 8, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
+// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once. FEW: stacks that travel in kernel arguments
+constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
-// LDS of a matrix: X [16 T][np] halves; the sums of four wavefronts, or A and P
+// LDS of a matrix: X [16 T][np] halves; the wavefronts' sums, or A and P
 inline int64_t small_region(int T) {
-  const int64_t sums = 4 * (T * (T + 1) / 2) * 1024, ap = 2 * (16 * T) * (T > 2 ? 256 : 128);
+  const int64_t sums = SMALL_SUMS * (T * (T + 1) / 2) * 1024, ap = 2 * (16 * T) * (T > 2 ? 256 : 128);
   return sums > ap ? sums : ap;
 }
 inline int64_t small_lds(int64_t m, int64_t np) {
@@ -32,15 +34,27 @@ __device__ __forceinline__ v4f mfma_small(s16x8 a, s16x8 b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
+struct OrthoFew {
+  OrthoStack s[SMALL_FEW];
+};
+
+// The stacks: in the arguments, or in `table` where they are more
 template <int T, int LDS>
-__global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoStack* __restrict__ table, int count,
-                                                                       OrthoScalars k) {
-  constexpr int MP = 16 * T, LINES = T > 2 ? 2 : 1, PAIRS = T * (T + 1) / 2;  // LINES: of a row of A and P
+__global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoFew few, const OrthoStack* __restrict__ table,
+                                                                       int count, OrthoScalars k) {
+  constexpr int SUMS = SMALL_SUMS, MP = 16 * T, LINES = T > 2 ? 2 : 1, PAIRS = T * (T + 1) / 2;  // LINES: of a row of A and P
   __shared__ __attribute__((aligned(128))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int e = stack_of(table, count, 0, blockIdx.x);
-  const OrthoStack s = table[e];
+  OrthoStack s;
+  if (table == nullptr) {
+    int e = 0;
+#pragma unroll
+    for (int i = 1; i < SMALL_FEW; ++i) e += i < count && few.s[i].first[0] <= blockIdx.x;
+    s = few.s[e];
+  } else {
+    s = table[stack_of(table, count, 0, blockIdx.x)];
+  }
   const int b = (int)(blockIdx.x - s.first[0]);
   const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np, nb = np >> 5, ld = np * 4;
   const int n = rows * cols;
@@ -175,7 +189,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) acc[i] = zero;
     __syncthreads();
-    for (int line = wave; line < nb && wave < SMALL_SUMS; line += SMALL_SUMS) {
+    for (int line = wave; line < nb && wave < SUMS; line += SUMS) {
       s16x8 f[T][2];
 #pragma unroll
       for (int i = 0; i < T; ++i)
@@ -188,15 +202,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
           for (int j = 0; j <= i; ++j, ++q) acc[q] = mfma_small(f[j][part == 2], f[i][part == 1], acc[q]);
     }
-    // four sums of two wavefronts each
-    if (wave >= 4 && wave < SMALL_SUMS) {
-#pragma unroll
-      for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + ((wave - 4) * PAIRS + i) * 256 + lane * 4) = acc[i];
-    }
-    __syncthreads();
-    if (wave < 4) {
-#pragma unroll
-      for (int i = 0; i < PAIRS; ++i) acc[i] += *reinterpret_cast<const v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4);
+    if (wave < SUMS) {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4) = acc[i];
     }
@@ -211,7 +217,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
         const int hi = i > j ? i : j, lo = i > j ? j : i;
         const float* from = sums + (hi * (hi + 1) / 2 + lo) * 256;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < SUMS; ++w)
 #pragma unroll
           for (int u = 0; u < 4; ++u)  // above the diagonal: row l % 16, column 4 g + u of the block below, across
             own[t][u] += from[w * PAIRS * 256 + (i >= j ? lane * 4 + u : ((l16 >> 2) * 16 + 4 * g + u) * 4 + (l16 & 3))];
