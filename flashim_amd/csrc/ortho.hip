@@ -225,7 +225,8 @@ static int ortho_check(const OrthoCall& c, OrthoScalars& k) {
 template <int T, int LDS>
 static void launch_small(const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid, const OrthoScalars& k,
                          hipStream_t stream) {
-  ortho_small_kernel<T, LDS><<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(few, table, count, k);
+  const auto kernel = table == nullptr ? ortho_small_kernel<T, LDS, true> : ortho_small_kernel<T, LDS, false>;
+  kernel<<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(few, table, count, k);
 }
 
 // LDS classes: 160 KB is a CU's; matrices of at most half of it run two to a CU

@@ -12,7 +12,8 @@
 
 namespace fim {
 
-// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once. FEW: stacks that travel in kernel arguments
+// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once. SMALL_FEW: stacks that travel in kernel
+// arguments
 constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
 // LDS of a matrix: X [16 T][np] halves; the wavefronts' sums, or A and P
@@ -38,23 +39,22 @@ struct OrthoFew {
   OrthoStack s[SMALL_FEW];
 };
 
-// The stacks: in the arguments, or in `table` where they are more
-template <int T, int LDS>
+// FEW: the stacks are in the arguments, which takes less than a table's launch and its latency; else in `table`
+template <int T, int LDS, bool FEW>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoFew few, const OrthoStack* __restrict__ table,
                                                                        int count, OrthoScalars k) {
   constexpr int SUMS = SMALL_SUMS, MP = 16 * T, LINES = T > 2 ? 2 : 1, PAIRS = T * (T + 1) / 2;  // LINES: of a row of A and P
   __shared__ __attribute__((aligned(128))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  OrthoStack s;
-  if (table == nullptr) {
-    int e = 0;
+  int e = 0;
+  if constexpr (FEW) {
 #pragma unroll
     for (int i = 1; i < SMALL_FEW; ++i) e += i < count && few.s[i].first[0] <= blockIdx.x;
-    s = few.s[e];
   } else {
-    s = table[stack_of(table, count, 0, blockIdx.x)];
+    e = stack_of(table, count, 0, blockIdx.x);
   }
+  const OrthoStack s = FEW ? few.s[e] : table[e];
   const int b = (int)(blockIdx.x - s.first[0]);
   const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np, nb = np >> 5, ld = np * 4;
   const int n = rows * cols;
