@@ -22,6 +22,7 @@ from flashim_amd.platforms import is_gfx950
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _HALVES = (torch.bfloat16, torch.float16)
+_INDEX = (torch.int32, torch.int64)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # the C ABI's codes
 MAX_CHANNELS = 8192  # of group_norm_act
 MAX_RANK = 128  # of low_rank_adapters
@@ -160,14 +161,21 @@ def eligible_muon_step(params, grads, momenta, *, lr, momentum=0.95, nesterov=Tr
 
 
 def eligible_low_rank_adapters(base, x, a, b, index, *, scale=1.0) -> bool:
-    return (
-        isinstance(x, Tensor) and is_gfx950(x.device) and x.ndim >= 1 and x.dtype in _HALVES and x.shape[-1] > 0
-        and all(isinstance(t, Tensor) and t.ndim == 3 and t.dtype == x.dtype and t.device == x.device for t in (a, b))
-        and a.shape[2] == x.shape[-1] and b.shape[0] == a.shape[0] > 0 and b.shape[2] == a.shape[1] and b.shape[1] > 0
-        and 0 < a.shape[1] <= MAX_RANK
-        and (base is None or (isinstance(base, Tensor) and base.dtype == x.dtype and base.device == x.device
-                              and base.shape == (*x.shape[:-1], b.shape[1])))
-        and isinstance(index, Tensor) and index.dtype in (torch.int32, torch.int64) and index.device == x.device
-        and index.ndim < x.ndim and index.shape == x.shape[:index.ndim]
-        and (not isinstance(scale, Tensor) or _vector(scale, a.shape[0], x, (torch.float32,)))
-    )
+    # (each attribute read once: a call's launch is no longer than this)
+    if not (isinstance(x, Tensor) and isinstance(a, Tensor) and isinstance(b, Tensor) and isinstance(index, Tensor)):
+        return False
+    device, dtype = x.device, x.dtype
+    if not is_gfx950(device) or dtype not in _HALVES or a.dtype is not dtype or b.dtype is not dtype:
+        return False
+    xs, sa, sb, si = x.shape, a.shape, b.shape, index.shape
+    if len(sa) != 3 or len(sb) != 3 or not 1 <= len(xs) > len(si) or si != xs[:len(si)]:
+        return False
+    (adapters, rank, k), n = sa, sb[1]
+    if xs[-1] != k or sb[0] != adapters or sb[2] != rank or not (0 < rank <= MAX_RANK and k > 0 and n > 0 and adapters > 0):
+        return False
+    if a.device != device or b.device != device or index.device != device or index.dtype not in _INDEX:
+        return False
+    if base is not None and not (isinstance(base, Tensor) and base.dtype is dtype and base.device == device
+                                 and base.shape == xs[:-1] + (n,)):
+        return False
+    return not isinstance(scale, Tensor) or _vector(scale, adapters, x, (torch.float32,))
