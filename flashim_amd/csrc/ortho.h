@@ -29,6 +29,7 @@ struct OrthoStack {
   double* part;   // partial sums of squares, `chunks` a matrix
   int64_t each;
   uint32_t rows, cols, batch, mp, np, chunk, chunks;
+  uint32_t slab, slabs;  // thin matrices: lines of 32 columns a workgroup, and workgroups a matrix; a and p: parts of X X^T
   float factor;     // O's factor in a step
   uint32_t first[5];  // first workgroup of a pass over: elements, conversion tiles, tiles of A, of P, of P X
   uint8_t g_type, out_type, tall, pad;

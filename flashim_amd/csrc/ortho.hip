@@ -1,8 +1,8 @@
 // Orthogonalized matrices by Newton-Schulz products, and the optimizer step made of them (formulas and precision: ortho.h).
 //
 // Matrices come as stacks of one shape, many stacks a call; a table of them goes through kernel arguments into the workspace
-// (no upload: capturable), and every launch after that runs over all matrices at once. Small ones take one launch, a workgroup each
-// (ortho_small.h); the others a pass that updates the momentum and sums squares, one that writes sx X0 as halves (transposing tall
+// (no upload: capturable), and every launch after that runs over all matrices at once. Small ones take one launch, a workgroup each,
+// and longer ones of as few rows a launch a step (ortho_small.h); the others a pass that updates the momentum and sums squares, one that writes sx X0 as halves (transposing tall
 // matrices), and three launches of products a step (ortho_tile.h), the last of which writes O or steps the parameters.
 #include <string.h>
 
@@ -129,10 +129,12 @@ struct OrthoCall {
 };
 
 struct OrthoShape {
-  int64_t m, n, mp, np, each, chunk, chunks;
-  bool small;
+  int64_t m, n, mp, np, each, chunk, chunks, slab, slabs;
+  bool small, thin;  // one launch; a launch a step
   int T;
 };
+
+enum { ORTHO_TILES, ORTHO_HALF, ORTHO_WHOLE, ORTHO_THIN };  // how a matrix is computed
 
 constexpr int64_t ORTHO_MOST = int64_t{1} << 29;  // padded elements of a matrix: 31-bit offsets into its halves
 
@@ -144,7 +146,13 @@ static OrthoShape ortho_shape(int64_t rows, int64_t cols) {
   s.np = cdiv(s.n, 32) * 32;
   s.T = (int)cdiv(s.m, 16);
   s.small = s.m <= SMALL_ROWS && small_lds(s.m, s.np) <= SMALL_LDS;
-  s.each = s.small ? 0 : cdiv((2 * s.mp * s.np + 2 * s.mp * s.mp) * 4, 256) * 256;
+  s.thin = !s.small && s.m <= SMALL_ROWS;
+  // about 16 workgroups a matrix, each of which reads all their parts; four lines a workgroup at least
+  const int64_t lines = s.np / 32, most = (SMALL_LDS - small_region(s.T) - 64) / (16 * s.T * 128);
+  s.slab = cdiv(lines, 16) < 4 ? 4 : cdiv(lines, 16) > most ? most : cdiv(lines, 16);
+  s.slabs = cdiv(lines, s.slab);
+  s.each = s.small ? 0 : s.thin ? cdiv(s.mp * s.np * 4 + 2 * s.slabs * s.T * s.T * 1024, 256) * 256
+                                : cdiv((2 * s.mp * s.np + 2 * s.mp * s.mp) * 4, 256) * 256;
   // at least 8192 elements, at most 512 chunks a matrix
   s.chunk = cdiv(cdiv(rows * cols, 512), 4096) * 4096;
   if (s.chunk < 8192) s.chunk = 8192;
@@ -222,25 +230,30 @@ static int ortho_check(const OrthoCall& c, OrthoScalars& k) {
   return FIM_OK;
 }
 
-template <int T, int LDS>
-static void launch_small(const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid, const OrthoScalars& k,
+template <int T, int LDS, int MODE>
+static void launch_small(const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid, int step, const OrthoScalars& k,
                          hipStream_t stream) {
-  const auto kernel = table == nullptr ? ortho_small_kernel<T, LDS, true> : ortho_small_kernel<T, LDS, false>;
-  kernel<<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(few, table, count, k);
+  const auto kernel = table == nullptr ? ortho_small_kernel<T, LDS, MODE, true> : ortho_small_kernel<T, LDS, MODE, false>;
+  kernel<<<dim3(grid), dim3(64 * SMALL_WAVES), 0, stream>>>(few, table, count, step, k);
 }
 
 // LDS classes: 160 KB is a CU's; matrices of at most half of it run two to a CU
-static void launch_small(int T, bool half, const OrthoFew& few, const OrthoStack* table, int count, uint32_t grid,
+template <int T>
+static void launch_small(int kind, const OrthoFew& few, const OrthoStack* table, int count, const uint32_t (&grid)[2],
                          const OrthoScalars& k, hipStream_t stream) {
-  switch (T * 2 + half) {
-    case 2: return launch_small<1, SMALL_LDS>(few, table, count, grid, k, stream);
-    case 3: return launch_small<1, SMALL_LDS / 2>(few, table, count, grid, k, stream);
-    case 4: return launch_small<2, SMALL_LDS>(few, table, count, grid, k, stream);
-    case 5: return launch_small<2, SMALL_LDS / 2>(few, table, count, grid, k, stream);
-    case 6: return launch_small<3, SMALL_LDS>(few, table, count, grid, k, stream);
-    case 7: return launch_small<3, SMALL_LDS / 2>(few, table, count, grid, k, stream);
-    case 8: return launch_small<4, SMALL_LDS>(few, table, count, grid, k, stream);
-    case 9: return launch_small<4, SMALL_LDS / 2>(few, table, count, grid, k, stream);
+  if (kind == ORTHO_HALF) return launch_small<T, SMALL_LDS / 2, SMALL_WHOLE>(few, table, count, grid[0], 0, k, stream);
+  if (kind == ORTHO_WHOLE) return launch_small<T, SMALL_LDS, SMALL_WHOLE>(few, table, count, grid[0], 0, k, stream);
+  launch_small<T, SMALL_LDS, THIN_FIRST>(few, table, count, grid[1], 0, k, stream);
+  for (int it = 0; it < k.steps; ++it) launch_small<T, SMALL_LDS, THIN_STEP>(few, table, count, grid[1], it, k, stream);
+}
+
+static void launch_small(int T, int kind, const OrthoFew& few, const OrthoStack* table, int count, const uint32_t (&grid)[2],
+                         const OrthoScalars& k, hipStream_t stream) {
+  switch (T) {
+    case 1: return launch_small<1>(kind, few, table, count, grid, k, stream);
+    case 2: return launch_small<2>(kind, few, table, count, grid, k, stream);
+    case 3: return launch_small<3>(kind, few, table, count, grid, k, stream);
+    default: return launch_small<4>(kind, few, table, count, grid, k, stream);
   }
 }
 
@@ -267,7 +280,7 @@ static OrthoPlan ortho_plan(const OrthoCall& c) {
   for (int64_t i = 0; i < c.count; ++i) {
     if (ortho_empty(c, i)) continue;
     const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
-    if (s.small) continue;
+    if (s.small || s.thin) continue;
     const int64_t m1 = cdiv(s.mp, 64), m2 = cdiv(s.mp, 128);
     t1 += c.batch[i] * (m1 * (m1 + 1) / 2);
     t2 += c.batch[i] * (m2 * (m2 + 1) / 2);
@@ -341,15 +354,17 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
     written += filled;
     filled = 0;
   };
-  // group 2 T + half: small matrices; 0: tiles, of 64 MB
+  // group: 4 T + kind, or 0 for tiles
   auto group_of = [&](int64_t i) {
     const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
-    return s.small ? 2 * s.T + (small_lds(s.m, s.np) <= SMALL_LDS / 2) : 0;
+    if (s.thin) return 4 * s.T + ORTHO_THIN;
+    return !s.small ? 0 : 4 * s.T + (small_lds(s.m, s.np) <= SMALL_LDS / 2 ? ORTHO_HALF : ORTHO_WHOLE);
   };
   const OrthoPlan plan = ortho_plan(c);
   float* part = reinterpret_cast<float*>(free_at);
   free_at += cdiv(ortho_part_bytes(c), 256) * 256;
-  for (int group = 0; group < 10; ++group) {
+  for (int group = 0; group < 4 * (SMALL_ROWS / 16 + 1); ++group) {
+    const int kind = group % 4;
     int64_t first[5] = {0, 0, 0, 0, 0};
     const int start = written + filled;
     for (int64_t i = 0; i < c.count; ++i) {
@@ -371,17 +386,24 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
       e.out_type = (uint8_t)c.out_type[i];
       e.tall = c.rows[i] > c.cols[i];
       for (int p = 0; p < 5; ++p) e.first[p] = (uint32_t)first[p];
-      if (group == 0) {
+      if (kind == ORTHO_TILES || kind == ORTHO_THIN) {
         e.part = reinterpret_cast<double*>(free_at);
         free_at += cdiv(batch * s.chunks * 8, 256) * 256;
         e.x[0] = free_at;
-        e.x[1] = e.x[0] + s.mp * s.np * 4;
-        e.a = e.x[1] + s.mp * s.np * 4;
-        e.p = e.a + s.mp * s.mp * 4;
+        e.x[1] = e.x[0] + s.mp * s.np * 4;  // (thin: the parts)
+        e.a = kind == ORTHO_THIN ? e.x[1] : e.x[1] + s.mp * s.np * 4;
+        e.p = e.a + (kind == ORTHO_THIN ? s.slabs * s.T * s.T * 1024 : s.mp * s.mp * 4);
         e.each = s.each;
         free_at += batch * s.each;
         e.chunk = (uint32_t)s.chunk;
         e.chunks = (uint32_t)s.chunks;
+        e.slab = (uint32_t)s.slab;
+        e.slabs = (uint32_t)s.slabs;
+      }
+      if (kind == ORTHO_THIN) {
+        first[0] += batch * s.chunks;
+        first[1] += batch * s.slabs;
+      } else if (kind == ORTHO_TILES) {
         auto triangle = [&](int side) {
           const int64_t n = cdiv(s.mp, 64 * side);
           return n * (n + 1) / 2;
@@ -400,13 +422,16 @@ static int ortho_run(const OrthoCall& c, OrthoScalars k, void* workspace, int64_
     }
     const int n = written + filled - start;
     if (n == 0) continue;
-    if (group > 0) {
+    if (kind != ORTHO_TILES) {
       OrthoFew few;
       const bool args = n <= SMALL_FEW && n == filled;  // (no table: neither its launch nor its latency)
       memcpy(few.s, fill.s, sizeof(few));
-      if (args) filled = 0;
+      if (args && kind != ORTHO_THIN) filled = 0;
       else flush();
-      launch_small(group / 2, group & 1, few, args ? nullptr : table + start, n, (uint32_t)first[0], k, stream);
+      const OrthoStack* t = table + start;
+      if (kind == ORTHO_THIN) ortho_momentum_kernel<<<dim3((unsigned)first[0]), dim3(ORTHO_T), 0, stream>>>(t, n, k);
+      const uint32_t grid[2] = {(uint32_t)first[0], (uint32_t)first[1]};
+      launch_small(group / 4, kind, few, args ? nullptr : t, n, grid, k, stream);
       continue;
     }
     flush();

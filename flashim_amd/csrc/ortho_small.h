@@ -39,10 +39,17 @@ struct OrthoFew {
   OrthoStack s[SMALL_FEW];
 };
 
+// WHOLE: the iteration in one launch. A longer matrix goes through it in slabs of columns, a workgroup each, a launch a step: FIRST writes
+// a slab of X0 and its part of X X^T; STEP adds up all slabs' parts, in order and in every workgroup, replaces its slab by P X and
+// leaves its part of the next X X^T, or O. (Seven launches for the 17 of the tiles, whose products of such a matrix have a
+// tile or two: 7 x 3696 120 -> 61 us.)
+enum { SMALL_WHOLE, THIN_FIRST, THIN_STEP };
+
 // FEW: the stacks are in the arguments, which takes less than a table's launch and its latency; else in `table`
-template <int T, int LDS, bool FEW>
+template <int T, int LDS, int MODE, bool FEW>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoFew few, const OrthoStack* __restrict__ table,
-                                                                       int count, OrthoScalars k) {
+                                                                       int count, int step, OrthoScalars k) {
+  constexpr int PASS = MODE == SMALL_WHOLE ? 0 : 1;
   constexpr int SUMS = SMALL_SUMS, MP = 16 * T, LINES = T > 2 ? 2 : 1, PAIRS = T * (T + 1) / 2;  // LINES: of a row of A and P
   __shared__ __attribute__((aligned(128))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -50,22 +57,26 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   int e = 0;
   if constexpr (FEW) {
 #pragma unroll
-    for (int i = 1; i < SMALL_FEW; ++i) e += i < count && few.s[i].first[0] <= blockIdx.x;
+    for (int i = 1; i < SMALL_FEW; ++i) e += i < count && few.s[i].first[PASS] <= blockIdx.x;
   } else {
-    e = stack_of(table, count, 0, blockIdx.x);
+    e = stack_of(table, count, PASS, blockIdx.x);
   }
   const OrthoStack s = FEW ? few.s[e] : table[e];
-  const int b = (int)(blockIdx.x - s.first[0]);
-  const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np, nb = np >> 5, ld = np * 4;
-  const int n = rows * cols;
-  const int64_t base = (int64_t)b * n;
+  const uint32_t local = blockIdx.x - s.first[PASS];
+  const int b = (int)(MODE == SMALL_WHOLE ? local : local / s.slabs);
+  const int line0 = MODE == SMALL_WHOLE ? 0 : (int)(local - (uint32_t)b * s.slabs) * (int)s.slab;  // this workgroup's lines
+  const int rows = (int)s.rows, cols = (int)s.cols, np = (int)s.np;
+  const int nb = MODE == SMALL_WHOLE || (np >> 5) - line0 < (int)s.slab ? (np >> 5) - line0 : (int)s.slab, ld = nb * 128;
+  const int64_t n = (int64_t)rows * cols, base = b * n;
   uint8_t* X = lds;
   uint8_t* A = lds + MP * ld;  // [MP][LINES] lines
   uint8_t* P = A + MP * LINES * 128;
   float* sums = reinterpret_cast<float*>(A);  // (A and P are dead while the sums are joined)
 
+  if constexpr (MODE != THIN_STEP) {
   // -- U in 32 bits where X will lie: element (r, c) of X in 4 bytes, the columns of each line rotated by the row
-  if (rows < cols ? rows < MP || cols < np : cols < MP || rows < np) {
+  const int short_side = s.tall ? cols : rows, long_side = s.tall ? rows : cols;
+  if (short_side < MP || long_side < (line0 + nb) * 32) {
     for (int i = tid * 16; i < MP * ld; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(X + i) = v4i{0, 0, 0, 0};
     __syncthreads();
   }
@@ -75,19 +86,19 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     constexpr bool MOM = decltype(mom_c)::value;
     int r = tid * 4 / cols, c = tid * 4 - r * cols;
     const int dr = STEP / cols, dc = STEP - dr * cols;
-    for (int i0 = tid * 4; i0 < n; i0 += U * STEP) {
+    for (int i0 = tid * 4; i0 < (int)n; i0 += U * STEP) {
       float u[U][4], m[MOM ? U : 1][4];
 #pragma unroll
       for (int t = 0; t < U; ++t) {
         const int i = i0 + t * STEP;
-        if (i < n) {
-          load4(s.g, base + i, DT, n - i, u[t]);
-          if constexpr (MOM) load4(s.mom, base + i, FIM_F32, n - i, m[t]);
+        if (i < (int)n) {
+          load4(s.g, base + i, DT, (int)n - i, u[t]);
+          if constexpr (MOM) load4(s.mom, base + i, FIM_F32, (int)n - i, m[t]);
         }
       }
 #pragma unroll
       for (int t = 0; t < U; ++t) {
-        const int i = i0 + t * STEP, left = n - i;
+        const int i = i0 + t * STEP, left = (int)n - i;
         if (left > 0) {
           if constexpr (MOM) {
 #pragma unroll
@@ -120,13 +131,49 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
       }
     }
   };
+  // a slab's elements, row by row of the source; the momentum has been updated and the squares summed by a launch before
+  auto load_slab = [&](auto dt, auto mom_c) __attribute__((always_inline)) {
+    constexpr int DT = decltype(dt)::value, STEP = 64 * SMALL_WAVES, U = 4;
+    constexpr bool MOM = decltype(mom_c)::value;
+    const int slab_long = long_side - line0 * 32 < nb * 32 ? long_side - line0 * 32 : nb * 32;
+    const int width = s.tall ? cols : slab_long, height = s.tall ? slab_long : rows, quads = (width + 3) / 4;
+    const int64_t from = base + (s.tall ? (int64_t)line0 * 32 * cols : line0 * 32);
+    for (int i0 = tid; i0 < height * quads; i0 += U * STEP) {
+      float u[U][4], m[MOM ? U : 1][4];
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        const int i = i0 + t * STEP, r = i / quads, c = (i - r * quads) * 4;
+        if (r < height) {
+          load4(s.g, from + (int64_t)r * cols + c, DT, width - c, u[t]);
+          if constexpr (MOM) load4(s.mom, from + (int64_t)r * cols + c, FIM_F32, width - c, m[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        const int i = i0 + t * STEP, r = i / quads, c = (i - r * quads) * 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (r < height && c + q < width) {
+            const float v = !MOM ? u[t][q] : k.nesterov ? fmaf(k.momentum, m[MOM ? t : 0][q], u[t][q]) : m[MOM ? t : 0][q];
+            const int xr = s.tall ? c + q : r, xc = s.tall ? r : c + q;
+            *reinterpret_cast<float*>(X + xr * ld + (xc >> 5) * 128 + (((xc ^ xr) & 31) << 2)) = v;
+          }
+      }
+    }
+  };
   auto load_of = [&](auto dt) __attribute__((always_inline)) {
-    if (s.mom != nullptr) load_all(dt, std::integral_constant<bool, true>{});
-    else load_all(dt, std::integral_constant<bool, false>{});
+    auto load = [&](auto mom) __attribute__((always_inline)) {
+      if constexpr (MODE == SMALL_WHOLE) load_all(dt, mom);
+      else load_slab(dt, mom);
+    };
+    if (s.mom != nullptr) load(std::integral_constant<bool, true>{});
+    else load(std::integral_constant<bool, false>{});
   };
   if (s.g_type == FIM_F32) load_of(std::integral_constant<int, FIM_F32>{});
   else if (s.g_type == FIM_BF16) load_of(std::integral_constant<int, FIM_BF16>{});
   else load_of(std::integral_constant<int, FIM_F16>{});
+  if constexpr (MODE == THIN_FIRST)
+    for (uint32_t i = tid; i < s.chunks; i += 64 * SMALL_WAVES) sq += s.part[b * s.chunks + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o);
   double* red = reinterpret_cast<double*>(A);
@@ -151,6 +198,21 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     *reinterpret_cast<v2i*>(at + (((q >> 1) ^ key) << 4) + (q & 1) * 8) = hi;
     *reinterpret_cast<v2i*>(at + (((4 + (q >> 1)) ^ key) << 4) + (q & 1) * 8) = lo;
   }
+  }
+
+  // the slab's lines as the workspace has them, without the swizzle
+  uint8_t* stored = MODE == SMALL_WHOLE ? nullptr : s.x[0] + b * s.each + line0 * 128;
+  auto move_slab = [&](bool out) __attribute__((always_inline)) {
+#pragma unroll 4
+    for (int i = tid; i < MP * nb * 8; i += 64 * SMALL_WAVES) {
+      const int line = i >> 3, r = line / nb;
+      v4i* global = reinterpret_cast<v4i*>(stored + (int64_t)r * np * 4 + (line - r * nb) * 128 + (i & 7) * 16);
+      v4i* local_at = reinterpret_cast<v4i*>(X + line * 128 + (((i & 7) ^ small_key(r)) << 4));
+      if (out) *global = *local_at;
+      else *local_at = *global;
+    }
+  };
+  if constexpr (MODE == THIN_STEP) move_slab(false);
 
   // fragments: lane: row (or column) l % 16, contraction 8 (l / 16) .. + 7 of 32
   auto along = [&](const uint8_t* p, int row_bytes, int r0, int line, int plane) __attribute__((always_inline)) {
@@ -183,7 +245,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   const float gram_scale = k.sa / (k.sx * k.sx), apply_scale = 1.0f / k.sp, last_scale = apply_scale / k.sx;
   const float sq_scale = k.c * k.sp / (k.sa * k.sa), old_scale = k.b * k.sp / k.sa;
 
-  for (int it = 0; it < k.steps; ++it) {
+  float own[OWN][4];  // this wavefront's blocks of X X^T
+  auto gram = [&]() __attribute__((always_inline)) {
     // -- A = X X^T: this wavefront's lines, all pairs of row blocks
     v4f acc[PAIRS];
 #pragma unroll
@@ -207,7 +270,6 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
       for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<v4f*>(sums + (wave * PAIRS + i) * 256 + lane * 4) = acc[i];
     }
     __syncthreads();
-    float own[OWN][4];
 #pragma unroll
     for (int t = 0; t < OWN; ++t) {
       const int q = wave + SMALL_WAVES * t, i = q / T, j = q % T;
@@ -223,6 +285,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
             own[t][u] += from[w * PAIRS * 256 + (i >= j ? lane * 4 + u : ((l16 >> 2) * 16 + 4 * g + u) * 4 + (l16 & 3))];
       }
     }
+  };
+  auto polynomial = [&]() __attribute__((always_inline)) {
     __syncthreads();  // (A and P lie where the sums lay)
     if (T == 1 || T == 3) {  // columns past 16 T of the last line: zero
       for (int i = tid * 16; i < 2 * MP * LINES * 128; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(A + i) = v4i{0, 0, 0, 0};
@@ -264,8 +328,9 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
       }
     }
     __syncthreads();
+  };
+  auto apply = [&](bool last) __attribute__((always_inline)) {
     // -- X = P X: 16 columns a turn
-    const bool last = it == k.steps - 1;
     for (int c16 = wave; c16 < 2 * nb; c16 += SMALL_WAVES) {
       v4f y[T];
 #pragma unroll
@@ -283,7 +348,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
 #pragma unroll
           for (int i = 0; i < T; ++i) y[i] = mfma_small(part == 2 ? xl : xh, fp[i][part == 1], y[i]);
       }
-      const int c = 16 * c16 + 4 * g;
+      const int c = 16 * c16 + 4 * g, cx = line0 * 32 + c;  // of the slab, of X
 #pragma unroll
       for (int i = 0; i < T; ++i) {
         const int r = 16 * i + l16;
@@ -295,10 +360,10 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
             if (r < cols) {
 #pragma unroll
               for (int u = 0; u < 4; ++u)
-                if (c + u < rows) finish1(s, k, base + (int64_t)(c + u) * cols + r, v[u]);
+                if (cx + u < rows) finish1(s, k, base + (int64_t)(cx + u) * cols + r, v[u]);
             }
-          } else if (r < rows && c < cols) {
-            finish4(s, k, base + (int64_t)r * cols + c, cols - c, v);
+          } else if (r < rows && cx < cols) {
+            finish4(s, k, base + (int64_t)r * cols + cx, cols - cx, v);
           }
         } else {
 #pragma unroll
@@ -312,6 +377,48 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
         }
       }
     }
+  };
+
+  if constexpr (MODE == SMALL_WHOLE) {
+    for (int it = 0; it < k.steps; ++it) {
+      gram();
+      polynomial();
+      apply(it == k.steps - 1);
+    }
+    return;
+  }
+  // parts of X X^T: [slab][T T][256], two of them in turn: a workgroup of this launch may still read the last ones
+  auto parts = [&](int turn) __attribute__((always_inline)) {
+    return reinterpret_cast<float*>((turn & 1 ? s.p : s.a) + b * s.each) + lane * 4;
+  };
+  if constexpr (MODE == THIN_STEP) {
+#pragma unroll
+    for (int t = 0; t < OWN; ++t) {
+      const int q = wave + SMALL_WAVES * t;
+      v4f sum = zero;
+      if (q < T * T) {
+#pragma unroll 8
+        for (uint32_t i = 0; i < s.slabs; ++i) sum += *reinterpret_cast<const v4f*>(parts(step) + ((int64_t)i * (T * T) + q) * 256);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) own[t][u] = sum[u];
+    }
+    polynomial();
+    const bool last = step == k.steps - 1;
+    apply(last);
+    if (last) return;
+    __syncthreads();
+  } else {
+    __syncthreads();
+  }
+  move_slab(true);
+  gram();
+#pragma unroll
+  for (int t = 0; t < OWN; ++t) {
+    const int q = wave + SMALL_WAVES * t;
+    if (q < T * T)
+      *reinterpret_cast<v4f*>(parts(MODE == THIN_FIRST ? 0 : step + 1) + ((int64_t)(line0 / (int)s.slab) * (T * T) + q) * 256) =
+          v4f{own[t][0], own[t][1], own[t][2], own[t][3]};
   }
 }
 

@@ -116,6 +116,21 @@ def test_layouts():
         assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(view.contiguous()))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(7, 3696), (2500, 30), (16, 2400), (40, 1500), (1300, 48), (64, 449), (4000, 63), (3, 20000), (2, 33, 1300)])
+def test_thin(shape, dtype):
+    """Few rows or columns, too long for one workgroup: slabs of the other side."""
+    g = _gradient(*shape, seed=13, dtype=dtype)
+    _check(ops.orthogonalize(g.to(DEV)), g)
+
+
+def test_steps_of_thin_ones():
+    shapes = [(16, 2400), (2400, 16), (3, 32, 1300), (64, 600), (700, 50), (5, 4000), (40, 1200), (1200, 33)]
+    for p_dtype, g_dtype in ((F32, BF16), (BF16, F32)):
+        _check_step(*_triples(shapes, p_dtype, g_dtype, seed=6), lr=0.3, weight_decay=0.2)
+    _check_step(*_triples(shapes, F32, F32, seed=7), lr=0.3, nesterov=False, steps=1)
+
+
 def test_many_small_ones():
     g = _gradient(700, 9, 14, seed=12)
     _check(ops.orthogonalize(g.to(DEV)), g)
