@@ -16,6 +16,7 @@ namespace fim {
 // arguments
 constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
+// (Three blocks of 16 rows spill some 30 registers, and are still ahead: 48 x 600 49 us, 62 in slabs, which four would need.)
 // LDS of a matrix: X [16 T][np] halves; the wavefronts' sums, or A and P
 inline int64_t small_region(int T) {
   const int64_t sums = SMALL_SUMS * (T * (T + 1) / 2) * 1024, ap = 2 * (16 * T) * (T > 2 ? 256 : 128);
