@@ -81,8 +81,8 @@ def muon_step_(params: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seque
     """One step of ``params`` (matrices, or stacks of them in the leading dimensions, each matrix by itself), in place:
     ``m = momentum m + g``, ``u = g + momentum m`` (``nesterov``) or ``m``,
     ``p = p (1 - lr weight_decay) - lr f orthogonalize(u)``. ``momenta`` FP32, the others of any float type. ``f`` by
-    ``adjust``: ``"original"`` sqrt(max(1, rows / cols)), ``"match_rms"`` 0.2 sqrt(max(rows, cols)), ``"none"`` 1. No two of the
-    parameters and momenta overlap. Nothing waits for the GPU."""
+    ``adjust``: ``"original"`` sqrt(max(1, rows / cols)), ``"match_rms"`` 0.2 sqrt(max(rows, cols)), ``"none"`` 1. No
+    parameter or momentum overlaps another tensor of the call. Nothing waits for the GPU."""
     a, b, c = coefficients
     with torch.no_grad():
         library.muon_step_(params, grads, momenta, lr, momentum, nesterov, weight_decay, ADJUST[adjust], steps, a, b, c, eps)

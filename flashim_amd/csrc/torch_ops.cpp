@@ -5,6 +5,7 @@
 // contiguity, devices); 1-byte float formats cross as they are or as their uint8 views (the bodies read bytes), and come
 // back as uint8.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -757,6 +758,32 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double 
   return out;
 }
 
+// The memory of a call's tensors: none that is written may overlap another. (Of a tensor that is not contiguous, whose rows may
+// lie between another's, the first element.)
+struct Extents {
+  struct Extent {
+    uintptr_t from, to;
+    bool written;
+  };
+  std::vector<Extent> all;
+  void add(const Tensor& t, bool written) {
+    if (written) at::assert_no_internal_overlap(t);
+    if (t.numel() == 0) return;
+    const auto from = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    all.push_back({from, from + (t.is_contiguous() ? t.nbytes() : t.element_size()), written});
+  }
+  bool apart() {
+    std::sort(all.begin(), all.end(), [](const Extent& a, const Extent& b) { return a.from < b.from; });
+    uintptr_t end = 0, written = 0;
+    for (const Extent& e : all) {
+      if (e.from < (e.written ? end : written)) return false;
+      end = std::max(end, e.to);
+      if (e.written) written = std::max(written, e.to);
+    }
+    return true;
+  }
+};
+
 // adjust 0: sqrt(max(1, rows / cols)), 1: 0.2 sqrt(max(rows, cols)), 2: 1
 float muon_factor(double lr, int64_t adjust, int64_t rows, int64_t cols) {
   TORCH_CHECK_VALUE(adjust >= 0 && adjust <= 2, "muon_step_: adjustment ", adjust);
@@ -781,6 +808,7 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   std::vector<int> pt, gt;
   std::vector<int64_t> batch, rows, cols;
   std::vector<float> factors;
+  Extents extents;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &w = params[i], &d = grads[i], &v = momenta[i];
     for (const Tensor* t : {&w, &d, &v}) check_grad(*t, params[0]);
@@ -788,6 +816,9 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
     TORCH_CHECK_NOT_IMPLEMENTED(w.dim() >= 2 && w.sizes() == d.sizes() && w.sizes() == v.sizes(),
                                 "no HIP impl applies: a parameter of shape ", w.sizes(), ", its gradient of ", d.sizes(),
                                 " and momentum of ", v.sizes());
+    extents.add(w, true);
+    extents.add(d, false);
+    extents.add(v, true);
     p.push_back(w.is_contiguous() ? w : w.contiguous());
     g.push_back(d.contiguous());
     m.push_back(v.is_contiguous() ? v : v.contiguous());
@@ -801,12 +832,7 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
     cols.push_back(w.size(-1));
     factors.push_back(muon_factor(lr, adjust, rows.back(), cols.back()));
   }
-  std::vector<const void*> written;  // (empty tensors have none)
-  for (size_t i = 0; i < n; ++i)
-    if (p[i].numel() > 0) written.insert(written.end(), {pp[i], mp[i]});
-  std::sort(written.begin(), written.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(written.begin(), written.end()) == written.end(),
-                    "muon_step_: a parameter or momentum is there twice");
+  TORCH_CHECK_VALUE(extents.apart(), "muon_step_: a parameter or momentum is there twice, or overlaps another tensor");
   int64_t bytes = 0;
   check(fim_muon_step_workspace((int64_t)n, batch.data(), rows.data(), cols.data(), &bytes), "muon_step_");
   const Tensor ws = empty({bytes}, params[0], at::kByte);

@@ -278,3 +278,32 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="no derivative"):
         torch.ops.flashim_amd.muon_step_([leaf], [g], [m], 0.1, 0.9, True, 0.0, 0, 5, 3.0, -3.0, 1.0, 1e-7)
     assert torch.equal(p, g) and torch.equal(m, g)
+
+
+@pytest.mark.parametrize("shape", [(64, 70000), (64, 140000), (12, 300000), (140000, 40)])
+def test_long_matrices_of_few_rows(shape):
+    """On both sides of the length up to which slabs' workgroups read each other's parts."""
+    g = _gradient(*shape, seed=31)
+    _check(ops.orthogonalize(g.to(DEV)), g)
+
+
+def test_tensors_that_overlap_are_refused():
+    w = torch.randn(4, 16, 32, device=DEV)
+    g, m = torch.randn_like(w), torch.zeros_like(w)
+    square = torch.randn(16, 16, device=DEV)
+    before = [t.clone() for t in (w, g, m, square)]
+    for params, grads, momenta in (([w, w[1]], [g, g[1]], [m, m[1].clone()]),  # a part of another
+                                   ([w[0], w[1]], [g[0], g[1]], [m[0], m[0]]),  # a momentum twice
+                                   ([w], [w], [m]), ([w], [m], [m]),  # the gradient is written
+                                   ([w], [g], [w]),
+                                   ([square, square.t()], [g[0, :, :16], g[1, :, :16]], [m[0, :, :16], m[1, :, :16]]),
+                                   ([w[:2], w[1:3]], [g[:2], g[1:3]], [m[:2], m[:2].clone()])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.muon_step_(params, grads, momenta, lr=0.1)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        ops.muon_step_([square[:1].expand(16, 16)], [g[0, :, :16]], [torch.zeros(16, 16, device=DEV)], lr=0.1)
+    assert all(torch.equal(t, b) for t, b in zip((w, g, m, square), before))
+    # neighbours, halves of one matrix's columns and a gradient for two parameters are apart
+    ops.muon_step_([w[0], w[1], w[2, :, :16], w[2, :, 16:]], [g[0], g[0], g[2, :, :16], g[2, :, 16:]],
+                   [m[0], m[1], m[2, :, :16], m[2, :, 16:]], lr=0.1)
+    assert torch.equal(w[3], before[0][3]) and not torch.equal(w[2], before[0][2])
