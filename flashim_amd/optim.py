@@ -17,18 +17,19 @@ from flashim_amd.backends.hip.train import NEWTON_SCHULZ
 class Muon(torch.optim.Optimizer):
     """Parameters of two dimensions or more (leading ones: stacks of matrices, each stepped by itself) take
     ``ops.muon_step_`` with an FP32 momentum; the others (norms' weights, biases) take AdamW with ``adam_lr``, ``adam_betas``
-    and ``adam_eps``. Every option may differ by parameter group. All matrices of a group are stepped in the same launches, and
-    nothing waits for the GPU."""
+    and ``adam_eps``. Every option may differ by parameter group. All matrices of a group (on one GPU) are stepped in the same launches, and
+    nothing waits for the GPU. A step in a captured graph needs one before it, which makes its state, and ``capturable=True`` where
+    AdamW's parameters are among them: their step counts then lie on the GPU."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, adjust: str = "original", steps: int = 5, coefficients=NEWTON_SCHULZ,
                  eps: float = 1e-7, adam_lr: float = 1e-3, adam_betas: tuple[float, float] = (0.9, 0.95),
-                 adam_eps: float = 1e-8) -> None:
+                 adam_eps: float = 1e-8, capturable: bool = False) -> None:
         if lr < 0 or adam_lr < 0 or weight_decay < 0 or not 0 <= momentum < 1:
             raise ValueError(f"Muon: lr {lr}, adam_lr {adam_lr}, weight_decay {weight_decay}, momentum {momentum}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, adjust=adjust,
                                       steps=steps, coefficients=coefficients, eps=eps, adam_lr=adam_lr, adam_betas=adam_betas,
-                                      adam_eps=adam_eps))
+                                      adam_eps=adam_eps, capturable=capturable))
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As any optimizer's, but with states of its own (none is shared with the optimizer they came from), and momenta that
@@ -52,6 +53,8 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             with_grad = [p for p in group["params"] if p.grad is not None]
             matrices = [p for p in with_grad if p.ndim >= 2]
+            if with_grad and with_grad[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                self._check_capture(group, with_grad)
             if matrices:
                 ops.muon_step_(matrices, [p.grad for p in matrices], [self._momentum(p) for p in matrices], lr=group["lr"],
                                momentum=group["momentum"], nesterov=group["nesterov"], weight_decay=group["weight_decay"],
@@ -59,6 +62,12 @@ class Muon(torch.optim.Optimizer):
                                eps=group["eps"])
             self._adam(group, [p for p in with_grad if p.ndim < 2])
         return loss
+
+    def _check_capture(self, group: dict, params: list[Tensor]) -> None:
+        if not all(p in self.state for p in params):
+            raise RuntimeError("Muon: a first step in a captured graph (every replay would start from its zeros); take one before it")
+        if not group["capturable"] and any(p.ndim < 2 for p in params):
+            raise RuntimeError("Muon: AdamW's step counts would stand still in a captured graph; construct with capturable=True")
 
     def _momentum(self, p: Tensor) -> Tensor:
         state = self.state[p]
@@ -72,9 +81,10 @@ class Muon(torch.optim.Optimizer):
         states = [self.state[p] for p in params]
         for p, state in zip(params, states):
             if not state:
-                state |= {"step": torch.zeros((), dtype=torch.float32), "exp_avg": torch.zeros_like(p),
+                on = p.device if group["capturable"] else None
+                state |= {"step": torch.zeros((), dtype=torch.float32, device=on), "exp_avg": torch.zeros_like(p),
                           "exp_avg_sq": torch.zeros_like(p)}
         beta1, beta2 = group["adam_betas"]
         adamw(params, [p.grad for p in params], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], [],
-              [s["step"] for s in states], amsgrad=False, beta1=beta1, beta2=beta2, lr=group["adam_lr"],
-              weight_decay=group["weight_decay"], eps=group["adam_eps"], maximize=False)
+              [s["step"] for s in states], capturable=group["capturable"], amsgrad=False, beta1=beta1, beta2=beta2,
+              lr=group["adam_lr"], weight_decay=group["weight_decay"], eps=group["adam_eps"], maximize=False)

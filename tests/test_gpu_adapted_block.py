@@ -155,3 +155,53 @@ def test_compiled_step_equals_eager():
     for a, b in zip(copies[0], copies[1]):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
     assert not torch.equal(copies[0][0][0], tensors[0][0])
+
+
+def test_captured_optimizer_steps_equal_eager_ones():
+    """Matrices and vectors: replays count AdamW's steps, and start from no zeros."""
+    block, other = _block(seed=17), _block(seed=17)
+    captured, eager = (optim.Muon(b.parameters(), lr=0.03, weight_decay=0.1, capturable=True) for b in (block, other))
+
+    def gradients(seed):
+        g = torch.Generator().manual_seed(seed)
+        for p, q in zip(block.parameters(), other.parameters()):
+            new = torch.randn(p.shape, generator=g).to(p)
+            for t in (p, q):
+                if t.grad is None:
+                    t.grad = torch.empty_like(t)
+                t.grad.copy_(new)
+
+    gradients(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured.step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for seed in range(1, 4):
+        gradients(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.step()
+        for p, q in zip(block.parameters(), other.parameters()):
+            assert torch.equal(p, q)
+            assert all(torch.equal(captured.state[p][k], v) for k, v in eager.state[q].items())
+
+
+@pytest.mark.parametrize("state", [False, True])
+def test_captures_that_would_replay_wrong_steps_are_refused(state):
+    block = _block(seed=18)
+    optimizer = optim.Muon(block.parameters())
+    for p in block.parameters():
+        p.grad = torch.ones_like(p)
+    if state:
+        optimizer.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capturable" if state else "first step"), torch.cuda.graph(graph):
+        optimizer.step()
+    optimizer.step()
+    assert all(torch.isfinite(p).all() for p in block.parameters())
