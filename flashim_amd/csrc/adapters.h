@@ -71,11 +71,13 @@ __device__ __forceinline__ void split16(float v, short& hi, short& lo) {
   lo = (short)to16<DT>(fabsf(rest) < __builtin_inff() ? rest : 0.0f);  // (infinity less infinity would be NaN)
 }
 
+// For the largest of finite values: an infinity or NaN beside them stays one whatever it is scaled by.
+__device__ __forceinline__ float finite_abs(float v) { return fabsf(v) < __builtin_inff() ? fabsf(v) : 0.0f; }
+
 // A power of two that brings values of at most `most` near FP16's upper end, and its inverse: FP16 has the range of neither large
 // nor small FP32 values (gradients of 1e-6), and BF16 needs none.
 __device__ __forceinline__ float half_scale(float most, float& inverse) {
-  const int e = (int)(f2u(most) >> 23 & 255) - 127;  // (infinities and NaN: 128)
-  int up = e == 128 ? 0 : 14 - e;
+  int up = 14 - ((int)(f2u(most) >> 23 & 255) - 127);
   up = up > 100 ? 100 : up;
   inverse = u2f((uint32_t)(127 - up) << 23);
   return u2f((uint32_t)(127 + up) << 23);

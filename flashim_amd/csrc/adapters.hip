@@ -21,8 +21,8 @@ static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
   if (s.M < 0 || s.K < 1 || s.N < 1 || s.J < 1 || s.R < 1 || s.entries < 0 || (wide != 0 && wide != 1)) return FIM_ERR_INVALID;
   if (s.M > 0 && (s.entries < 1 || s.M % s.entries != 0)) return FIM_ERR_INVALID;
   if (dtype != FIM_BF16 && dtype != FIM_F16) return dtype == FIM_F32 ? FIM_ERR_UNSUPPORTED : FIM_ERR_INVALID;
-  constexpr int64_t most = int64_t{1} << 31;
-  if (s.R > ADAPTER_RANK || s.M >= most / 2 || s.K >= 1 << 24 || s.N >= 1 << 24 || s.J >= 1 << 20 || s.J * s.R >= most ||
+  constexpr int64_t most = int64_t{1} << 31;  // (rows: 16 a workgroup, whose threads a launch counts in 32 bits)
+  if (s.R > ADAPTER_RANK || s.M >= most / 8 || s.K >= 1 << 24 || s.N >= 1 << 24 || s.J >= 1 << 20 || s.J * s.R >= most ||
       s.J * (s.K + s.N) >= most)
     return FIM_ERR_UNSUPPORTED;
   return FIM_OK;
@@ -89,16 +89,17 @@ static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   g.xt = (int)cdiv(s.K, GRAD_COLS);
   g.ct = g.xt + (int)cdiv(s.N, GRAD_COLS);
   g.narrow = adapter_narrow(s.K, s.N, s.R);
-  // workgroups for the card where a chunk's rows have one adapter (narrow: two a CU), but at most 64 MB of partial sums
-  // should they have all
+  // workgroups for the card where a chunk's rows have one adapter (narrow: two a CU), lists no longer than their room if the partial
+  // sums of all adapters are 256 MB or less then; else fewer and longer chunks (lists in pieces)
   int64_t chunks = g.narrow ? 2 * (int64_t)device_cus() : cdiv(4 * (int64_t)device_cus(), g.ct);
-  const int64_t most = (int64_t{64} << 20) / (s.J * s.R * (s.K + s.N) * 4), step = g.narrow ? NARROW_ROWS : 256;
+  const int64_t step = g.narrow ? NARROW_ROWS : 256, longest = g.narrow ? NARROW_CHUNK : GRAD_CHUNK;
+  const int64_t most = (int64_t{256} << 20) / (s.J * s.R * (s.K + s.N) * 4), fits = cdiv(s.M, longest);
+  if (chunks < fits) chunks = fits;
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
   g.chunk = cdiv(cdiv(s.M, chunks), step) * step;
   if (g.chunk < 256) g.chunk = 256;  // (a workgroup's weights cost as much)
-  const int64_t longest = g.narrow ? NARROW_CHUNK : GRAD_CHUNK;
-  if (g.chunk > longest) g.chunk = longest;
+  if (g.chunk > longest) g.chunk = cdiv(g.chunk, longest) * longest;
   g.chunks = cdiv(s.M, g.chunk);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -132,7 +133,8 @@ extern "C" int fim_low_rank_adapters(const void* base, int64_t base_stride, cons
     if (reinterpret_cast<uintptr_t>(t) % 2) return FIM_ERR_INVALID;
   if (reinterpret_cast<uintptr_t>(index) % (index_wide ? 8 : 4) || reinterpret_cast<uintptr_t>(h) % 16) return FIM_ERR_INVALID;
   AdapterArgs p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(base), static_cast<const uint16_t*>(a),
-                static_cast<const uint16_t*>(b), x_stride, base_stride, static_cast<uint16_t*>(out), h,
+                static_cast<const uint16_t*>(b), x_stride, base_stride, static_cast<uint16_t*>(out),
+                adapter_narrow(K, N, R) ? nullptr : h,  // (no columns are saved)
                 AdapterIndex{index, index_wide, (uint32_t)(M / entries), (int)J}, scales, scale, (uint32_t)M, (int)K, (int)N,
                 (int)R, 1};
   adapter_rows(p, dtype, stream);
@@ -175,15 +177,19 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
     return FIM_ERR_INVALID;
   if (dx == nullptr && da == nullptr) return FIM_OK;
   const int64_t na = J * R * K, nb = J * R * N;
-  if (J * cdiv(R * (K + N), 64) >= int64_t{1} << 31 || (J + 1) * g.chunks * g.ct >= int64_t{1} << 31) return FIM_ERR_UNSUPPORTED;
+  // (a launch counts its threads in 32 bits)
+  if (na + nb >= int64_t{1} << 32 || R * (K + N) >= int64_t{1} << 30 || (J + 1) * g.chunks * (g.narrow ? 1 : g.ct) >= 1 << 24)
+    return FIM_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* part = da != nullptr && g.chunks > 1 ? reinterpret_cast<float*>(ws + g.part) : nullptr;
   int* counts = part != nullptr ? reinterpret_cast<int*>(ws + g.counts) : nullptr;
   auto join = [&]() {
     if (part == nullptr) return;
     const auto kernel = dtype == FIM_BF16 ? adapter_join_kernel<FIM_BF16> : adapter_join_kernel<FIM_F16>;
-    kernel<<<dim3((unsigned)(J * cdiv(R * (K + N), 64))), dim3(64 * JOIN_WAVES), 0, stream>>>(
-        part, counts, (int)g.chunks, (int)K, (int)N, (int)R, static_cast<uint16_t*>(da), static_cast<uint16_t*>(db));
+    const int64_t blocks = J * cdiv(R * (K + N), 64);
+    kernel<<<dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(64 * JOIN_WAVES), 0, stream>>>(
+        part, counts, (int)g.chunks, (int)J, (int)K, (int)N, (int)R,
+        static_cast<uint16_t*>(da), static_cast<uint16_t*>(db));
   };
   if (g.narrow) {
     const AdapterNarrowArgs q{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(a),
@@ -192,13 +198,21 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
                               static_cast<uint16_t*>(dx), static_cast<uint16_t*>(da), static_cast<uint16_t*>(db), part, counts,
                               (uint32_t)M, (uint32_t)g.chunk, (int)g.chunks, (int)K, (int)N, (int)R};
     const dim3 grid((unsigned)((J + (dx != nullptr)) * g.chunks));  // (rows without an adapter: zeros of dx)
-    auto launch = [&](auto dt) {
+    auto launch = [&](auto dt, auto whole, auto pieces) {
       constexpr int DT = decltype(dt)::value;
-      if (R > 16) adapter_narrow_kernel<DT, 2><<<grid, dim3(256), 0, stream>>>(q);
-      else adapter_narrow_kernel<DT, 1><<<grid, dim3(256), 0, stream>>>(q);
+      constexpr bool W = decltype(whole)::value, P = decltype(pieces)::value;
+      if (R > 16) adapter_narrow_kernel<DT, 2, W, P><<<grid, dim3(256), 0, stream>>>(q);
+      else adapter_narrow_kernel<DT, 1, W, P><<<grid, dim3(256), 0, stream>>>(q);
     };
-    if (dtype == FIM_BF16) launch(std::integral_constant<int, FIM_BF16>{});
-    else launch(std::integral_constant<int, FIM_F16>{});
+    const auto yes = std::integral_constant<bool, true>{};
+    const auto no = std::integral_constant<bool, false>{};
+    auto of_type = [&](auto dt) {
+      const bool whole = K % 32 == 0 && N % 32 == 0, pieces = g.chunk > NARROW_CHUNK;
+      if (whole) pieces ? launch(dt, yes, yes) : launch(dt, yes, no);
+      else pieces ? launch(dt, no, yes) : launch(dt, no, no);
+    };
+    if (dtype == FIM_BF16) of_type(std::integral_constant<int, FIM_BF16>{});
+    else of_type(std::integral_constant<int, FIM_F16>{});
     join();
     return launch_status();
   }
@@ -217,7 +231,9 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
                             (int)g.chunks, (int)K, (int)N, (int)R, g.xt, g.ct};
     by_type(dtype, R, [&](auto dt, auto nr) {
       constexpr int DT = decltype(dt)::value;
-      adapter_grad_kernel<DT, decltype(nr)::value><<<dim3((unsigned)(J * g.chunks * g.ct)), dim3(256), 0, stream>>>(q);
+      const auto kernel = g.chunk > GRAD_CHUNK ? adapter_grad_kernel<DT, decltype(nr)::value, true>
+                                               : adapter_grad_kernel<DT, decltype(nr)::value, false>;
+      kernel<<<dim3((unsigned)(J * g.chunks * g.ct)), dim3(256), 0, stream>>>(q);
     });
     join();
   }

@@ -11,6 +11,7 @@
 
 namespace fim {
 
+// GRAD_CHUNK: rows that the list has room for; a longer chunk's are listed and summed in pieces
 constexpr int GRAD_COLS = 128, GRAD_ROWS = 32, GRAD_CHUNK = 4096;
 
 struct AdapterGradArgs {
@@ -25,7 +26,8 @@ struct AdapterGradArgs {
   int chunks, K, N, R, xt, ct;  // column tiles of x, and of both
 };
 
-template <int DT, int NR>
+// PIECES: chunks are longer than the list (one piece, known as such: 16800 x 196 -> 523 21 us, 28 not)
+template <int DT, int NR, bool PIECES>
 __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][GRAD_ROWS * GRAD_COLS * 2];
   __shared__ uint16_t rows[GRAD_CHUNK];
@@ -34,33 +36,10 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ct = (int)(blockIdx.x % (unsigned)p.ct);
   const int slot = (int)(blockIdx.x / (unsigned)p.ct), j = slot / p.chunks, chunk = slot - j * p.chunks;
-  const uint32_t r0 = (uint32_t)chunk * p.chunk, r1 = r0 + p.chunk < p.M ? r0 + p.chunk : p.M;
-  // -- the chunk's rows of this adapter, in order: each wavefront counts a quarter, then lists it
-  const uint32_t quarter = p.chunk / 4, q0 = r0 + wave * quarter < r1 ? r0 + wave * quarter : r1, q1 = q0 + quarter < r1 ? q0 + quarter : r1;
-  int n = 0;
-#pragma unroll 4
-  for (uint32_t r = q0 + lane; r - lane < q1; r += 64)
-    n += __popcll(__builtin_amdgcn_ballot_w64(r < q1 && adapter_of(p.index, r < q1 ? r : r0) == j));
-  if (lane == 0) counted[wave] = n;
-  __syncthreads();
-  int at = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    at += w < wave ? counted[w] : 0;
-    total += counted[w];
-  }
-  if (ct == 0 && tid == 0 && p.counts != nullptr) p.counts[slot] = total;
-  if (total == 0 && p.part != nullptr) return;
-#pragma unroll 4
-  for (uint32_t r = q0 + lane; r - lane < q1; r += 64) {
-    const bool own = r < q1 && adapter_of(p.index, r < q1 ? r : r0) == j;
-    const uint64_t all = __builtin_amdgcn_ballot_w64(own);
-    if (own) rows[at + __popcll(all & ((uint64_t{1} << lane) - 1))] = (uint16_t)(r - r0);
-    at += __popcll(all);
-  }
-  __syncthreads();
-  total = __builtin_amdgcn_readfirstlane(total);
-
+  const uint32_t begin = (uint32_t)chunk * p.chunk, end = begin + p.chunk < p.M ? begin + p.chunk : p.M;
+  const uint32_t piece = PIECES ? GRAD_CHUNK : p.chunk;  // rows listed at a time
+  uint32_t r0 = begin;
+  int total = 0, all = 0;  // of this piece's rows, of all before it
   const bool of_x = ct < p.xt;
   const int width = of_x ? p.K : p.N, c0 = (of_x ? ct : ct - p.xt) * GRAD_COLS;
   const uint16_t* y = of_x ? p.x : p.d;
@@ -100,59 +79,92 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
 #pragma unroll
     for (int c = 0; c < 2; ++c) acc[i][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   s16x8 yv[2];
-  load_y(0, yv);
-  load_t(0);
   int buf = 0;
-  for (int from = 0; from < total; from += GRAD_ROWS, buf ^= 1) {
-    put_y(buf, yv);
-    float up = 1.0f, down = 1.0f;
-    if constexpr (DT == FIM_F16) {
-      float most = 0.0f;
+  do {
+    const uint32_t r1 = r0 + piece < end ? r0 + piece : end;
+    if constexpr (PIECES) __syncthreads();  // (the list before has been read)
+    // -- the piece's rows of this adapter, in order: each wavefront counts a quarter, then lists it
+    const uint32_t quarter = piece / 4, q0 = r0 + wave * quarter < r1 ? r0 + wave * quarter : r1;
+    const uint32_t q1 = q0 + quarter < r1 ? q0 + quarter : r1;
+    int n = 0;
+#pragma unroll 4
+    for (uint32_t r = q0 + lane; r - lane < q1; r += 64)
+      n += __popcll(__builtin_amdgcn_ballot_w64(r < q1 && adapter_of(p.index, r < q1 ? r : r0) == j));
+    if (lane == 0) counted[wave] = n;
+    __syncthreads();
+    int at = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      at += w < wave ? counted[w] : 0;
+      total += counted[w];
+    }
+    if (total == 0) continue;
+#pragma unroll 4
+    for (uint32_t r = q0 + lane; r - lane < q1; r += 64) {
+      const bool own = r < q1 && adapter_of(p.index, r < q1 ? r : r0) == j;
+      const uint64_t owned = __builtin_amdgcn_ballot_w64(own);
+      if (own) rows[at + __popcll(owned & ((uint64_t{1} << lane) - 1))] = (uint16_t)(r - r0);
+      at += __popcll(owned);
+    }
+    __syncthreads();
+    total = __builtin_amdgcn_readfirstlane(total);
+    all += total;
+    load_y(0, yv);
+    load_t(0);
+    for (int from = 0; from < total; from += GRAD_ROWS, buf ^= 1) {
+      put_y(buf, yv);
+      float up = 1.0f, down = 1.0f;
+      if constexpr (DT == FIM_F16) {
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) most = fmaxf(most, finite_abs(tv[i][q]));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+        up = half_scale(most, down);
+      }
+      s16x8 th[NR], tl[NR];
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) most = __builtin_elementwise_maximum(most, fabsf(tv[i][q]));
+        for (int q = 0; q < 8; ++q) {
+          short hi, lo;
+          split16<DT>(DT == FIM_F16 ? tv[i][q] * up : tv[i][q], hi, lo);
+          th[i][q] = hi;
+          tl[i][q] = lo;
+        }
+      load_y(from + GRAD_ROWS, yv);
+      load_t(from + GRAD_ROWS);
+      lds_barrier();  // (two stages: one barrier a turn)
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) most = __builtin_elementwise_maximum(most, __shfl_xor(most, o));
-      up = half_scale(most, down);
-    }
-    s16x8 th[NR], tl[NR];
+      for (int c = 0; c < 2; ++c) {
+        s16x4 half[2];
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
+        for (int q = 0; q < 2; ++q) {
+          const int r = 8 * g + 4 * q + (l16 >> 2);
+          half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4*)(stage[buf] + r * 256 + ((wave ^ (r & 3)) << 6) + c * 32 + (lane & 3) * 8));
+        }
+        const s16x8 v = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        short hi, lo;
-        split16<DT>(DT == FIM_F16 ? tv[i][q] * up : tv[i][q], hi, lo);
-        th[i][q] = hi;
-        tl[i][q] = lo;
-      }
-    load_y(from + GRAD_ROWS, yv);
-    load_t(from + GRAD_ROWS);
-    lds_barrier();  // (two stages: one barrier a turn)
+        for (int i = 0; i < NR; ++i) {
+          if constexpr (DT == FIM_F16) {
+            v4f s = mfma_rank<DT>(th[i], v, v4f{0.0f, 0.0f, 0.0f, 0.0f});
+            s = mfma_rank<DT>(tl[i], v, s);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      s16x4 half[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = 8 * g + 4 * q + (l16 >> 2);
-        half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4*)(stage[buf] + r * 256 + ((wave ^ (r & 3)) << 6) + c * 32 + (lane & 3) * 8));
-      }
-      const s16x8 v = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        if constexpr (DT == FIM_F16) {
-          v4f s = mfma_rank<DT>(th[i], v, v4f{0.0f, 0.0f, 0.0f, 0.0f});
-          s = mfma_rank<DT>(tl[i], v, s);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][c][q] = fmaf(s[q], down, acc[i][c][q]);
-        } else {
-          acc[i][c] = mfma_rank<DT>(th[i], v, acc[i][c]);
-          acc[i][c] = mfma_rank<DT>(tl[i], v, acc[i][c]);
+            for (int q = 0; q < 4; ++q) acc[i][c][q] = fmaf(s[q], down, acc[i][c][q]);
+          } else {
+            acc[i][c] = mfma_rank<DT>(th[i], v, acc[i][c]);
+            acc[i][c] = mfma_rank<DT>(tl[i], v, acc[i][c]);
+          }
         }
       }
     }
-  }
+  } while (PIECES && (r0 += piece) < end);
+  if (ct == 0 && tid == 0 && p.counts != nullptr) p.counts[slot] = all;
+  if (all == 0 && p.part != nullptr) return;
   // -- lane: column l % 16 of 16, ranks 4 (l / 16) ..
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -177,37 +189,42 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
 constexpr int JOIN_WAVES = 16;
 template <int DT>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void adapter_join_kernel(const float* __restrict__ part, const int* __restrict__ counts,
-                                                                       int chunks, int K, int N, int R, uint16_t* da, uint16_t* db) {
+                                                                       int chunks, int J, int K, int N, int R, uint16_t* da,
+                                                                       uint16_t* db) {
   __shared__ float sums[JOIN_WAVES][64];
   const int width = K + N, of = R * width, blocks = (of + 63) / 64, lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), j = (int)(blockIdx.x / (unsigned)blocks);
-  const int i = (int)(blockIdx.x - (unsigned)j * blocks) * 64 + lane, at = i < of ? i : of - 1;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int from = (int)((int64_t)chunks * wave / JOIN_WAVES), to = (int)((int64_t)chunks * (wave + 1) / JOIN_WAVES);
-  const float* mine = part + (int64_t)j * chunks * of + at;
-  float v = 0.0f;
-  for (int k0 = from; k0 < to; k0 += 64) {
-    uint64_t some = __builtin_amdgcn_ballot_w64(k0 + lane < to && counts[(int64_t)j * chunks + (k0 + lane < to ? k0 + lane : k0)] > 0);
-    while (some != 0) {
-      constexpr int U = 8;  // loads in flight
-      float w[U];
+  for (int64_t block = blockIdx.x; block < (int64_t)J * blocks; block += gridDim.x) {
+    const int j = (int)(block / blocks), i = (int)(block - (int64_t)j * blocks) * 64 + lane, at = i < of ? i : of - 1;
+    const float* mine = part + (int64_t)j * chunks * of + at;
+    float v = 0.0f;
+    for (int k0 = from; k0 < to; k0 += 64) {
+      uint64_t some = __builtin_amdgcn_ballot_w64(k0 + lane < to && counts[(int64_t)j * chunks + (k0 + lane < to ? k0 + lane : k0)] > 0);
+      while (some != 0) {
+        constexpr int U = 8;  // loads in flight
+        float w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        w[u] = 0.0f;
-        if (some != 0) w[u] = mine[(int64_t)(k0 + __builtin_ctzll(some)) * of];
-        some &= some - 1;
+        for (int u = 0; u < U; ++u) {
+          w[u] = 0.0f;
+          if (some != 0) w[u] = mine[(int64_t)(k0 + __builtin_ctzll(some)) * of];
+          some &= some - 1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) v += w[u];
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) v += w[u];
     }
-  }
-  sums[wave][lane] = v;
-  __syncthreads();
-  if (wave != 0 || i >= of) return;
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && i < of) {
 #pragma unroll
-  for (int w = 1; w < JOIN_WAVES; ++w) v += sums[w][lane];
-  const int r = i / width, c = i - r * width;
-  if (c < K) da[((int64_t)j * R + r) * K + c] = to16<DT>(v);
-  else db[((int64_t)j * N + c - K) * R + r] = to16<DT>(v);
+      for (int w = 1; w < JOIN_WAVES; ++w) v += sums[w][lane];
+      const int r = i / width, c = i - r * width;
+      if (c < K) da[((int64_t)j * R + r) * K + c] = to16<DT>(v);
+      else db[((int64_t)j * N + c - K) * R + r] = to16<DT>(v);
+    }
+    __syncthreads();
+  }
 }
 
 // at[j][k][r] = a[j][r][k] and bt[j][r][n] = b[j][n][r]

@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         h[i][q] = 16 * i + 4 * g + q < p.R ? h[i][q] * scale : 0.0f;
-        most = __builtin_elementwise_maximum(most, fabsf(h[i][q]));
+        most = fmaxf(most, finite_abs(h[i][q]));
       }
     if (p.h != nullptr && part == 0 && own && writes) {
 #pragma unroll
@@ -152,8 +152,8 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(const AdapterArgs p) 
     }
     float up = 1.0f, down = 1.0f;
     if constexpr (DT == FIM_F16) {
-      most = __builtin_elementwise_maximum(most, __shfl_xor(most, 16));
-      most = __builtin_elementwise_maximum(most, __shfl_xor(most, 32));
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
       up = half_scale(most, down);
     }
     s16x8 hf[NR];

@@ -297,7 +297,7 @@ int fim_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64
  * square root of the sum of squares (summed in 64 bits), of the shorter side's rows; `steps` (1 to 100) times
  * A = X X^T, X = (a I + b A + c A^2) X, products of operands of 22 bits with FP32 sums; out packed, any float type, rounded
  * once. Coefficients by which a singular value of at most 1 passes 6, or its factor 48, are refused (99), and so are matrices
- * of more than 2^29 elements. No counterpart in the reference, as the next two. */
+ * of more than 2^29 elements and 2^22 matrices or more. No counterpart in the reference, as the next two. */
 int fim_orthogonalize(const void* g, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                       double eps, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
@@ -306,7 +306,7 @@ int fim_muon_step_workspace(int64_t count, const int64_t* batch, const int64_t* 
 
 /* An optimizer step of `count` stacks of packed matrices (host arrays of device pointers, dtype codes and sizes):
  * m = momentum m + g (FP32, in place), u = g + momentum m (nesterov) or m, O as above of each u, p = keep p - factors[i] O
- * (in place). No two of the parameters and momenta overlap. */
+ * (in place). No parameter or momentum overlaps another array of the call. */
 int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, const void* const* grads, const int* grad_dtypes,
                   float* const* momenta, const int64_t* batch, const int64_t* rows, const int64_t* cols, const float* factors,
                   float momentum, int nesterov, float keep, int steps, float a, float b, float c, double eps, void* workspace,
@@ -319,14 +319,14 @@ int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, c
  * for row r (int32, or int64 with index_wide; M a multiple of entries), a row whose j is outside [0, J) keeps its base;
  * s_j = scale * scales[j] (scales FP32 [J], or NULL: 1). Sums and x A^T in FP32 (split in two 16-bit operands for the second
  * product), rounded once. out packed [M, N]; h, if not NULL (16-byte aligned), FP32 [M, columns of
- * fim_low_rank_adapters_saved], s_j x A_j^T for the backward pass (rows without an adapter are not written). No counterpart in
- * the reference, as the next three. */
+ * fim_low_rank_adapters_saved], s_j x A_j^T for the backward pass (rows without an adapter are not written, and nothing where
+ * there are 0 columns). M below 2^28 (else 99). No counterpart in the reference, as the next three. */
 int fim_low_rank_adapters(const void* base, int64_t base_stride, const void* x, int64_t x_stride, int dtype, int64_t M, int64_t K,
                           int64_t N, const void* a, const void* b, int64_t J, int64_t R, const void* index, int index_wide,
                           int64_t entries, const float* scales, float scale, void* out, float* h, hipStream_t stream);
 
-/* Columns of h that the backward pass needs for the adapters' gradients: R rounded up to 16, 32, 64 or 128, or 0 where it computes
- * h again (narrow projections). */
+/* Columns of h that the backward pass needs for the adapters' gradients: R rounded up to 16, 32, 64 or 128, or 0
+ * where it computes h again (narrow projections). */
 int fim_low_rank_adapters_saved(int64_t K, int64_t N, int64_t R, int64_t* columns);
 
 /* Bytes of workspace (256-byte aligned) that fim_low_rank_adapters_backward needs. */

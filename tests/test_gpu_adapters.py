@@ -247,6 +247,38 @@ def test_more_adapters_than_rows_and_many_chunks():
     _check(base, x, a, b, (torch.arange(9000) // 5000), 1.0, d_out)
 
 
+@pytest.mark.parametrize("size", [((2, 20000), 96, 160, 24, 400), ((20000,), 300, 340, 100, 400)])
+def test_chunks_of_several_lists(size):
+    """So many adapters that the partial sums of all take few, long chunks: their rows are listed in pieces."""
+    lead, k, n, r, j = size
+    base, x, a, b, d_out = _inputs(lead, k, n, r, j, BF16, seed=21)
+    index = _index("row", lead, j, seed=22)
+    index[..., : lead[-1] // 3] = 7  # one adapter's rows fill lists
+    _check(base, x, a, b, index, 0.5, d_out)
+
+
+@pytest.mark.parametrize("width", [(64, 256), (200, 520)])
+def test_rows_of_different_magnitude_in_fp16(width):
+    """A row's dx keeps its precision beside rows of 2^20 times its gradient."""
+    k, n = width
+    base, x, a, b, d_out = _inputs((300,), k, n, 8, 2, F16, seed=23)
+    d_out = (d_out.double() * 2.0 ** (-20 * (torch.arange(300) % 3 == 0).double())[:, None] * 16).to(F16)
+    _check(base, x, (a * 64).to(F16), b, _index("row", (300,), 2, seed=24), 1.0, d_out)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_an_infinite_row_leaves_the_others_their_precision(bad):
+    """FP16 gradients of 1e-6 beside one that is not finite."""
+    base, x, a, b, d_out = _inputs((200,), 64, 256, 8, 1, F16, seed=25, d=1e-6)
+    index, a = torch.tensor(0), (a * 64).to(F16)
+    d_out[77, 3] = bad
+    _, grads = _run(base, x, a, b, index, 1.0, d_out)
+    keep = torch.arange(200) != 77
+    want = ref.low_rank_adapters(base[keep], x[keep], a, b, index, 1.0, d_out[keep])
+    _close("x", grads["x"][keep.to(DEV)], want["x"], want["x_error"])
+    assert not torch.isfinite(grads["x"][77]).any()
+
+
 def test_same_bits_on_any_stream():
     base, x, a, b, d_out = _inputs((3, 3000), 64, 256, 8, 3, BF16, seed=13)
     index = torch.tensor([0, 2, 0])

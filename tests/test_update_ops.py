@@ -232,3 +232,22 @@ def test_c_abi_checks_its_arguments():
     assert backward(h=None) == backward(da=None) == backward(db=None) == backward(ws=None) == backward(ws=fake + 8) == backward(size=0) == bad
     assert backward(m=0) == bad
     assert backward(dx=None, da=None, db=None) == 0  # nothing to do
+
+
+def test_c_abi_refuses_what_one_launch_cannot_hold():
+    lib = _lib.load()
+    fake, out = 1 << 20, ctypes.c_int64()
+    at, no = ctypes.byref(out), _lib.FIM_ERR_UNSUPPORTED
+    assert lib.fim_orthogonalize_workspace(1 << 22, 16, 16, at) == no
+    assert lib.fim_orthogonalize_workspace(1 << 20, 16, 16, at) == 0
+    assert lib.fim_low_rank_adapters(fake, 8, fake, 8, 1, 1 << 28, 8, 8, fake, fake, 1, 4, fake, 1, 1, None, 1.0, fake, None, None) == no
+    assert lib.fim_low_rank_adapters_backward(fake, 600, fake, 600, 1, 64, 600, 1 << 23, fake, fake, 100, 128, fake, 1, 1, None, 1.0,
+                                              fake, fake, fake, fake, fake, 1 << 50, None) == no
+
+
+def test_partial_sums_of_many_adapters_stay_small():
+    """However long the input: chunks are fewer and longer, so that all adapters' sums take at most 256 MB."""
+    lib, out = _lib.load(), ctypes.c_int64()
+    for m, k, n, j, r in ((1 << 20, 64, 256, 1000, 8), (1 << 21, 128, 256, 100, 32), (1 << 24, 64, 64, 2000, 16)):
+        assert lib.fim_low_rank_adapters_backward_workspace(m, k, n, j, r, ctypes.byref(out)) == 0
+        assert out.value <= (256 << 20) + j * 1024 * 4 + 4096
