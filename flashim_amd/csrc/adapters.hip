@@ -28,16 +28,19 @@ static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
   return FIM_OK;
 }
 
-// Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of 16 would
-// go through them one after the other. Else tiles of 16 rows: four wavefronts each until tiles fill the CUs, and beyond that where
-// all four have a part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange
-// nothing (320000 x 64 -> 256 forward and dx: 77 us each, 106 with four).
+// Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of rows would
+// go through them one after the other. Else tiles, four wavefronts each until rows fill the CUs, and beyond that where all four have a
+// part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange nothing
+// (320000 x 64 -> 256 77 us, 106 with four). A tile of two sets of 16 rows halves the reads of A_j and B_j from the caches, once
+// there are enough: 512 -> 2048, 16384 rows of ranks 32, 64, 128: 30, 40 and 64 us, of one set 45, 52 and 113; 4096 rows 15, 21, 35
+// and 18, 19, 41. At rank 16 it gains where a wavefront has the tile (320000 x 64 -> 256: 92 -> 84 us; 40000 x 512 -> 2048: 94 -> 97).
 template <int DT, int NR>
 static void launch_rows(AdapterArgs& p, hipStream_t stream) {
   const int64_t cus = device_cus(), blocks = cdiv(p.N, 32);
   const bool one = p.index.per < 16 && p.M <= 512;
-  const int64_t tiles = one ? p.M : cdiv(p.M, 16);
-  const bool four = one || tiles < 8 * cus || (blocks >= 16 && p.K >= 128);
+  const bool four = one || p.M < 128 * cus || (blocks >= 16 && p.K >= 128);
+  const bool two = !one && (NR == 1 ? !four : p.M >= (NR == 4 ? 64 : 8) * cus);
+  const int64_t tiles = one ? p.M : cdiv(p.M, two ? 32 : 16);
   // parts of the columns: enough wavefronts for the card, each with four blocks at least
   int64_t parts = cdiv(8 * cus, tiles * (four ? 4 : 1));
   const int64_t most = cdiv(blocks, four ? 16 : 4);
@@ -47,11 +50,13 @@ static void launch_rows(AdapterArgs& p, hipStream_t stream) {
   const dim3 grid((unsigned)(four ? tiles : cdiv(tiles, 4)), (unsigned)parts);
   auto launch = [&](auto quads) {
     constexpr bool Q = decltype(quads)::value;
-    if (one) adapter_rows_kernel<DT, NR, 4, true, Q><<<grid, dim3(256), 0, stream>>>(p);
-    else if (four) adapter_rows_kernel<DT, NR, 4, false, Q><<<grid, dim3(256), 0, stream>>>(p);
-    else adapter_rows_kernel<DT, NR, 1, false, Q><<<grid, dim3(256), 0, stream>>>(p);
+    if (one) adapter_rows_kernel<DT, NR, 4, 0, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else if (four && two) adapter_rows_kernel<DT, NR, 4, 2, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else if (four) adapter_rows_kernel<DT, NR, 4, 1, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else if (two) adapter_rows_kernel<DT, NR, 1, 2, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else adapter_rows_kernel<DT, NR, 1, 1, Q><<<grid, dim3(256), 0, stream>>>(p);
   };
-  if (p.R % 4 == 0) launch(std::integral_constant<bool, true>{});
+  if (p.R % (NR == 1 ? 4 : 8) == 0) launch(std::integral_constant<bool, true>{});
   else launch(std::integral_constant<bool, false>{});
 }
 
