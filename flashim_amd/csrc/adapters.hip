@@ -1,5 +1,5 @@
-// Low-rank adapters of many requests beside a shared projection: out = base + s_j (x A_j^T) B_j^T, j by row or by leading entry, and
-// the gradients of x, A and B (formulas and layouts: adapters_rows.h, adapters_grad.h).
+// Low-rank adapters of many requests beside a shared projection: out = base + s_j (x A_j^T) B_j^T, j by row or by leading entry,
+// and the gradients of x, A and B (formulas and layouts: adapters_rows.h, adapters_grad.h).
 #include <type_traits>
 
 #include "adapters_grad.h"
@@ -28,12 +28,13 @@ static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
   return FIM_OK;
 }
 
-// Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of rows would
-// go through them one after the other. Else tiles, four wavefronts each until rows fill the CUs, and beyond that where all four have a
-// part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange nothing
+// Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of rows would go
+// through them one after the other. Else tiles, four wavefronts each until rows fill the CUs, and beyond that where all four have
+// a part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange nothing
 // (320000 x 64 -> 256 77 us, 106 with four). A tile of two sets of 16 rows halves the reads of A_j and B_j from the caches, once
-// there are enough: 512 -> 2048, 16384 rows of ranks 32, 64, 128: 30, 40 and 64 us, of one set 45, 52 and 113; 4096 rows 15, 21, 35
-// and 18, 19, 41. At rank 16 it gains where a wavefront has the tile (320000 x 64 -> 256: 92 -> 84 us; 40000 x 512 -> 2048: 94 -> 97).
+// there are enough: 512 -> 2048, 16384 rows of ranks 32, 64, 128: 30, 40 and 64 us, of one set 45, 52 and 113; 4096 rows 15, 21,
+// 35 and 18, 19, 41. At rank 16 it gains where a wavefront has the tile (320000 x 64 -> 256: 92 -> 84 us; 40000 x 512 -> 2048: 94
+// -> 97).
 template <int DT, int NR>
 static void launch_rows(AdapterArgs& p, hipStream_t stream) {
   const int64_t cus = device_cus(), blocks = cdiv(p.N, 32);

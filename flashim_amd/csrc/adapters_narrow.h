@@ -1,12 +1,12 @@
 // The whole backward pass of low-rank adapters beside a narrow projection in one pass over x and d_out: dx, and each workgroup's
 // partial sums of dA_j and dB_j.
 //
-// A workgroup takes an adapter and a chunk of rows and lists the chunk's rows of its adapter (a long chunk's in pieces). A_j and B_j^T lie in LDS, and so do 64
-// rows of x and d_out at a time, read once from memory and used three times: each wavefront multiplies 16 of them into h and t and
-// its rows of dx; then t and h (hi and lo) meet all 64 rows, read transposed, in accumulators that stay in registers for the
-// chunk. Passes of their own (adapters_rows.h, adapters_grad.h) read d_out twice and write and read t and h in FP32: 320000 x 64 ->
-// 256 at rank 8 took 77 + 55 us and 22 to join, and takes 61 and 5 to join here: 246 MB at 4.0 TB/s, of the 5.1 of a large copy; the
-// rest is the turns' barriers, with two workgroups a CU to cover them.
+// A workgroup takes an adapter and a chunk of rows and lists the chunk's rows of its adapter (a long chunk's in pieces). A_j and
+// B_j^T lie in LDS, and so do 64 rows of x and d_out at a time, read once from memory and used three times: each wavefront
+// multiplies 16 of them into h and t and its rows of dx; then t and h (hi and lo) meet all 64 rows, read transposed, in
+// accumulators that stay in registers for the chunk. Passes of their own (adapters_rows.h, adapters_grad.h) read d_out twice and
+// write and read t and h in FP32: 320000 x 64 -> 256 at rank 8 took 77 + 55 us and 22 to join, and takes 61 and 5 to join here:
+// 246 MB at 4.0 TB/s, of the 5.1 of a large copy; the rest is the turns' barriers, with two workgroups a CU to cover them.
 #pragma once
 
 #include "adapters.h"
@@ -37,7 +37,8 @@ struct AdapterNarrowArgs {
 template <int DT, int NR, bool WHOLE, bool PIECES>
 __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrowArgs p) {
   constexpr int W = NARROW_WIDTH, CB = W / 64;                          // 16-column blocks of a wavefront
-  constexpr int STRIDE = W * 2 + 16, TS = 128 * NR + 16;  // bytes of a row; an odd number of 16s: rows at one column meet different banks
+  // bytes of a row; an odd number of 16s: rows at one column meet different banks
+  constexpr int STRIDE = W * 2 + 16, TS = 128 * NR + 16;
   __shared__ __attribute__((aligned(16))) uint8_t rows_at[NARROW_ROWS * STRIDE];  // x, then d_out, then zeros up to 32 columns
   __shared__ __attribute__((aligned(16))) uint8_t weights[16 * NR * STRIDE];      // A_j, then B_j^T
   __shared__ __attribute__((aligned(16))) uint8_t ts[NARROW_ROWS * TS];           // t hi, t lo, h hi, h lo
@@ -244,8 +245,10 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
 #pragma unroll
             for (int q = 0; q < 4; ++q) o[4 * u + q] = DT == FIM_F16 ? d[q] * down_r : d[q];
           }
-          const v4i w = {(int)to16x2<DT>(o[0], o[1]), (int)to16x2<DT>(o[2], o[3]), (int)to16x2<DT>(o[4], o[5]), (int)to16x2<DT>(o[6], o[7])};
-          if (there && (WHOLE || c + 8 * g < p.K)) store_some<8>(out + c, WHOLE ? 8 : p.K - c - 8 * g, __builtin_bit_cast(s16x8, w));
+          const v4i w = {(int)to16x2<DT>(o[0], o[1]), (int)to16x2<DT>(o[2], o[3]), (int)to16x2<DT>(o[4], o[5]),
+                         (int)to16x2<DT>(o[6], o[7])};
+          const int left = WHOLE ? 8 : p.K - c - 8 * g;
+          if (there && left > 0) store_some<8>(out + c, left, __builtin_bit_cast(s16x8, w));
         }
       }
       lds_barrier();

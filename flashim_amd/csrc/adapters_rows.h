@@ -7,9 +7,9 @@
 // and then lo of the 4 beside the same 4 of B_j twice; so h keeps 16 bits or more and nothing is exchanged. Rows of several
 // adapters in a tile: once for each adapter that occurs, rows of others computed and not stored.
 //
-// Bound by memory at low ranks: 40000 x 512 -> 2048 at rank 16, 369 MB in 92 us, 4.0 TB/s of the 5.1 of a large copy; 320000 x 64 ->
-// 256 at rank 8 as many in 84. By the caches' reads of A_j and B_j at high ones: rank 32 104 us, 64 155, 128 202 (171, 278 and 434
-// with 8-byte loads of B_j and 16 rows). 64 rows of adapters of their own, 1024 -> 4096 at rank 16: 12 MB in 7 us, latency.
+// Bound by memory at low ranks: 40000 x 512 -> 2048 at rank 16, 369 MB in 92 us, 4.0 TB/s of the 5.1 of a large copy; 320000 x 64
+// -> 256 at rank 8 as many in 84. By the caches' reads of A_j and B_j at high ones: rank 32 104 us, 64 155, 128 202 (171, 278 and
+// 434 with 8-byte loads of B_j and 16 rows). 64 rows of adapters of their own, 1024 -> 4096 at rank 16: 12 MB in 7 us, latency.
 #pragma once
 
 #include "adapters.h"
@@ -40,7 +40,8 @@ template <int DT, int NR, int W, int SETS, bool EVEN>
 __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_rows_kernel(const AdapterArgs p) {
   constexpr bool ONE = SETS == 0;
   constexpr int S = ONE ? 1 : SETS;
-  constexpr int GROUP = NR <= 2 && W > 1 && S == 1 ? 4 : NR == 4 || S * NR >= 8 ? 1 : 2;  // blocks of 32 columns whose operands are in flight
+  // blocks of 32 columns whose operands are in flight
+  constexpr int GROUP = NR <= 2 && W > 1 && S == 1 ? 4 : NR == 4 || S * NR >= 8 ? 1 : 2;
   __shared__ __attribute__((aligned(16))) float sums[W > 1 ? W * S * NR * 256 : 4];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -65,7 +66,8 @@ __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_row
     left |= ((uint32_t)__builtin_amdgcn_ballot_w64(there) & 0xffff) << (16 * z);
   }
   // this part's columns, in blocks of 32, and this wavefront's steps of the contraction
-  const int blocks = (p.N + 31) / 32, n_from = (int)((int64_t)blocks * part / p.parts), n_to = (int)((int64_t)blocks * (part + 1) / p.parts);
+  const int blocks = (p.N + 31) / 32;
+  const int n_from = (int)((int64_t)blocks * part / p.parts), n_to = (int)((int64_t)blocks * (part + 1) / p.parts);
   const int steps = (p.K + 31) / 32, k_from = W > 1 ? steps * wave / W : 0, k_to = W > 1 ? steps * (wave + 1) / W : steps;
   const int n_full = n_to < p.N / 32 ? n_to : p.N / 32;  // blocks before this one are whole
   const bool writes = !ONE || l16 == 0;
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_row
       for (int t = 0; t < 2; ++t) {
         v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NR; ++i) d = mfma_rank<DT>(__builtin_shufflevector(v[t][i], v[t][i], 0, 1, 2, 3, 4, 5, 6, 7), hf[z][i], d);
+        for (int i = 0; i < NR; ++i)
+          d = mfma_rank<DT>(__builtin_shufflevector(v[t][i], v[t][i], 0, 1, 2, 3, 4, 5, 6, 7), hf[z][i], d);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float y = from16<DT>((uint16_t)from[4 * t + q]);
@@ -241,7 +244,8 @@ __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_row
           else o[4 * t + q] = DT == FIM_F16 ? fmaf(d[q], down[z], y) : d[q] + y;
         }
       }
-      const v4i w = {(int)to16x2<DT>(o[0], o[1]), (int)to16x2<DT>(o[2], o[3]), (int)to16x2<DT>(o[4], o[5]), (int)to16x2<DT>(o[6], o[7])};
+      const v4i w = {(int)to16x2<DT>(o[0], o[1]), (int)to16x2<DT>(o[2], o[3]), (int)to16x2<DT>(o[4], o[5]),
+                     (int)to16x2<DT>(o[6], o[7])};
       return __builtin_bit_cast(s16x8, w);
     };
     auto group = [&](int nb, int cur) __attribute__((always_inline)) {

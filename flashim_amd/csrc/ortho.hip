@@ -139,7 +139,7 @@ struct OrthoShape {
 
 enum { ORTHO_TILES, ORTHO_HALF, ORTHO_WHOLE, ORTHO_THIN };  // how a matrix is computed
 
-constexpr int64_t ORTHO_MOST = int64_t{1} << 29;  // padded elements of a matrix: 31-bit offsets into its halves
+constexpr int64_t ORTHO_MOST = int64_t{1} << 29;  // padded elements of a matrix are fewer: 31-bit offsets into its halves
 
 static OrthoShape ortho_shape(int64_t rows, int64_t cols) {
   OrthoShape s;
@@ -180,7 +180,7 @@ static int ortho_bytes(const OrthoCall& c, int64_t* bytes) {
     if (ortho_empty(c, i)) continue;
     if (c.batch[i] >= 1 << 24 || c.rows[i] >= 1 << 24 || c.cols[i] >= 1 << 24) return FIM_ERR_UNSUPPORTED;
     const OrthoShape s = ortho_shape(c.rows[i], c.cols[i]);
-    if (s.mp * s.np > ORTHO_MOST) return FIM_ERR_UNSUPPORTED;
+    if (s.mp * s.np >= ORTHO_MOST) return FIM_ERR_UNSUPPORTED;
     small += s.small ? c.batch[i] : s.thin ? c.batch[i] * s.slabs : 0;
     tiles += s.small ? 0 : c.batch[i] * (cdiv(s.mp, 64) * cdiv(s.np, 64) + s.chunks);
     if (small >= 1 << 22 || tiles >= 1 << 24) return FIM_ERR_UNSUPPORTED;

@@ -1,11 +1,13 @@
 // A whole Newton-Schulz iteration, or optimizer step, of a small matrix in one workgroup: X, A and P stay in LDS.
 //
 // At most 64 rows (of the shorter side) whose X fits: read once, written once, and no launch between the 3 `steps` products, which on
-// tiles would be as many launches of one or two workgroups. Sixteen wavefronts on
-// 16 x 16 x 32 MFMAs: X X^T is split over the columns of four (each fragment is read once, and is either operand), whose sums meet in
-// LDS; each wavefront adds up one of the 16 blocks, those above the diagonal from the ones below, read across; P X is split over the
-// columns too, and each
-// wavefront replaces the columns it has read.
+// tiles would be as many launches of one or two workgroups. Sixteen wavefronts on 16 x 16 x 32 MFMAs: X X^T is split over the
+// columns of four (each fragment is read once, and is either operand), whose sums meet in LDS; each wavefront adds up one of the 16
+// blocks, those above the diagonal from the ones below, read across; P X is split over the columns too, and each wavefront replaces
+// the columns it has read.
+//
+// Bound by the chain of dependent products, each of LDS latencies and two or three barriers: 64 x 256 32 us, about 6 a step; 64
+// matrices of 16 x 512 beside each other 16.
 #pragma once
 
 #include "ortho.h"
@@ -40,10 +42,10 @@ struct OrthoFew {
   OrthoStack s[SMALL_FEW];
 };
 
-// WHOLE: the iteration in one launch. A longer matrix goes through it in slabs of columns, a workgroup each, a launch a step: FIRST writes
-// a slab of X0 and its part of X X^T; STEP adds up all slabs' parts, in order and in every workgroup, replaces its slab by P X and
-// leaves its part of the next X X^T, or O. (Seven launches for the 17 of the tiles, whose products of such a matrix have a
-// tile or two: 7 x 3696 120 -> 47 us.)
+// WHOLE: the iteration in one launch. A longer matrix goes through it in slabs of columns, a workgroup each, a launch a step:
+// FIRST writes a slab of X0 and its part of X X^T; STEP adds up all slabs' parts, in order and in every workgroup, replaces its
+// slab by P X and leaves its part of the next X X^T, or O. (Seven launches for the 17 of the tiles, whose products of such a
+// matrix have a tile or two: 7 x 3696 120 -> 47 us.)
 enum { SMALL_WHOLE, THIN_FIRST, THIN_STEP };
 
 // FEW: the stacks are in the arguments, which takes less than a table's launch and its latency; else in `table`

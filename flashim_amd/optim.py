@@ -17,8 +17,8 @@ from flashim_amd.backends.hip.train import NEWTON_SCHULZ
 class Muon(torch.optim.Optimizer):
     """Parameters of two dimensions or more (leading ones: stacks of matrices, each stepped by itself) take
     ``ops.muon_step_`` with an FP32 momentum; the others (norms' weights, biases) take AdamW with ``adam_lr``, ``adam_betas``
-    and ``adam_eps``. Every option may differ by parameter group. All matrices of a group (on one GPU) are stepped in the same launches, and
-    nothing waits for the GPU. A step in a captured graph needs one before it, which makes its state, and ``capturable=True`` where
+    and ``adam_eps``. Every option may differ by parameter group. All matrices of a group (on one GPU) are stepped in the
+    same launches, and nothing waits for the GPU. A step in a captured graph needs one before it, which makes its state, and ``capturable=True`` where
     AdamW's parameters are among them: their step counts then lie on the GPU."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True,
@@ -65,7 +65,7 @@ class Muon(torch.optim.Optimizer):
 
     def _check_capture(self, group: dict, params: list[Tensor]) -> None:
         if not all(p in self.state for p in params):
-            raise RuntimeError("Muon: a first step in a captured graph (every replay would start from its zeros); take one before it")
+            raise RuntimeError("Muon: a first step in a captured graph, whose replays would all start from its zeros")
         if not group["capturable"] and any(p.ndim < 2 for p in params):
             raise RuntimeError("Muon: AdamW's step counts would stand still in a captured graph; construct with capturable=True")
 

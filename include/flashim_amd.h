@@ -297,7 +297,7 @@ int fim_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int64
  * square root of the sum of squares (summed in 64 bits), of the shorter side's rows; `steps` (1 to 100) times
  * A = X X^T, X = (a I + b A + c A^2) X, products of operands of 22 bits with FP32 sums; out packed, any float type, rounded
  * once. Coefficients by which a singular value of at most 1 passes 6, or its factor 48, are refused (99), and so are matrices
- * of more than 2^29 elements and 2^22 matrices or more. No counterpart in the reference, as the next two. */
+ * of 2^29 elements or more (sides rounded up to 32) and 2^22 matrices or more. No counterpart in the reference, as the next two. */
 int fim_orthogonalize(const void* g, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                       double eps, void* out, int out_dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 

@@ -287,6 +287,22 @@ def test_long_matrices_of_few_rows(shape):
     _check(ops.orthogonalize(g.to(DEV)), g)
 
 
+@pytest.mark.parametrize("shape", [(70, 5_500_000), (5_500_000, 70), (12, 5_000_000), (40, 8_000_000)])
+def test_offsets_past_31_bits(shape):
+    """Zero but for some columns at the ends and between: exact zeros there, and the others' own matrix orthogonalized."""
+    m, n = min(shape), max(shape)
+    g = torch.Generator().manual_seed(32)
+    at = torch.cat([torch.arange(60), torch.randint(60, n - 60, (100,), generator=g).unique(), torch.arange(n - 60, n)])
+    few = _gradient(m, at.numel(), seed=33)
+    u = torch.zeros(m, n, device=DEV)
+    u[:, at.to(DEV)] = few.to(DEV)
+    got = ops.orthogonalize(u.t().contiguous() if shape[0] > shape[1] else u)
+    del u
+    got = got.t() if shape[0] > shape[1] else got
+    _check(got[:, at.to(DEV)], few)
+    assert got.count_nonzero().item() == got[:, at.to(DEV)].count_nonzero().item()
+
+
 def test_tensors_that_overlap_are_refused():
     w = torch.randn(4, 16, 32, device=DEV)
     g, m = torch.randn_like(w), torch.zeros_like(w)
