@@ -14,15 +14,16 @@
 
 namespace fim {
 
-// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once. SMALL_FEW: stacks that travel in kernel
+// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once (64 matrices of 16 x 512 15.8 us; by 8 16.0, 16 16.9). SMALL_FEW: stacks that travel in kernel
 // arguments
 constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
 // (Three blocks of 16 rows spill some 30 registers, and are still ahead: 48 x 600 49 us, 62 in slabs, which four would need.)
-// LDS of a matrix: X [16 T][np] halves; the wavefronts' sums, or A and P
+// LDS of a matrix: X [16 T][np] halves; the wavefronts' sums, or A and P (one block of 16 rows: both, so that A's and P's
+// columns past 16 stay zero and no barrier parts them from the sums: 64 matrices of 16 x 512 16.2 -> 15.7 us)
 inline int64_t small_region(int T) {
   const int64_t sums = SMALL_SUMS * (T * (T + 1) / 2) * 1024, ap = 2 * (16 * T) * (T > 2 ? 256 : 128);
-  return sums > ap ? sums : ap;
+  return T == 1 ? sums + ap : sums > ap ? sums : ap;
 }
 inline int64_t small_lds(int64_t m, int64_t np) {
   const int64_t T = cdiv(m, 16);
@@ -72,9 +73,12 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   const int nb = MODE == SMALL_WHOLE || (np >> 5) - line0 < (int)s.slab ? (np >> 5) - line0 : (int)s.slab, ld = nb * 128;
   const int64_t n = (int64_t)rows * cols, base = b * n;
   uint8_t* X = lds;
-  uint8_t* A = lds + MP * ld;  // [MP][LINES] lines
+  constexpr bool APART = T == 1 && MODE == SMALL_WHOLE;
+  float* sums = reinterpret_cast<float*>(lds + MP * ld);
+  uint8_t* A = lds + MP * ld + (APART ? SUMS * PAIRS * 1024 : 0);  // [MP][LINES] lines
   uint8_t* P = A + MP * LINES * 128;
-  float* sums = reinterpret_cast<float*>(A);  // (A and P are dead while the sums are joined)
+  if constexpr (APART)
+    for (int i = tid * 16; i < 2 * MP * LINES * 128; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(A + i) = v4i{0, 0, 0, 0};
 
   if constexpr (MODE != THIN_STEP) {
   // -- U in 32 bits where X will lie: element (r, c) of X in 4 bytes, the columns of each line rotated by the row
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     for (uint32_t i = tid; i < s.chunks; i += 64 * SMALL_WAVES) sq += s.part[b * s.chunks + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sq += __shfl_xor(sq, o);
-  double* red = reinterpret_cast<double*>(A);
+  double* red = reinterpret_cast<double*>(sums);
   if (lane == 0) red[wave] = sq;
   __syncthreads();
   sq = red[0];
@@ -290,8 +294,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     }
   };
   auto polynomial = [&]() __attribute__((always_inline)) {
-    __syncthreads();  // (A and P lie where the sums lay)
-    if (T == 1 || T == 3) {  // columns past 16 T of the last line: zero
+    if constexpr (!APART) __syncthreads();  // (A and P lie where the sums lay)
+    if (!APART && (T == 1 || T == 3)) {  // columns past 16 T of the last line: zero
       for (int i = tid * 16; i < 2 * MP * LINES * 128; i += 64 * SMALL_WAVES * 16) *reinterpret_cast<v4i*>(A + i) = v4i{0, 0, 0, 0};
       __syncthreads();
     }
