@@ -14,8 +14,8 @@
 
 namespace fim {
 
-// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once (64 matrices of 16 x 512 15.8 us; by 8 16.0, 16 16.9). SMALL_FEW: stacks that travel in kernel
-// arguments
+// SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once (64 matrices of 16 x 512 15.8 us; by 8 16.0, by 16
+// 16.9). SMALL_FEW: stacks that travel in kernel arguments
 constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
 // (Three blocks of 16 rows spill some 30 registers, and are still ahead: 48 x 600 49 us, 62 in slabs, which four would need.)
