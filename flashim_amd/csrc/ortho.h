@@ -74,6 +74,18 @@ __device__ __forceinline__ void join4(v2i hi, v2i lo, float (&v)[4]) {
   for (int i = 0; i < 4; ++i) v[i] = (float)h[i] + (float)l[i];
 }
 
+// sx / (|U| + eps) as two FP32 factors, the first a power of two: 1 in the range where FP32 holds the quotient with room. (A sum
+// below FP32's smallest number is eps beside a zero matrix, or zero, whose 0 / 0 is NaN.)
+struct OrthoScale {
+  float first, second;
+  __device__ OrthoScale(double norm_eps, float sx) {
+    const double s = (double)sx / (norm_eps > 0.0 && norm_eps < 1e-60 ? 1e-60 : norm_eps);
+    first = s > 0x1p100 ? 0x1p100f : s < 0x1p-100 ? 0x1p-60f : 1.0f;
+    second = (float)(s / (double)first);
+  }
+  __device__ float operator()(float u) const { return u * first * second; }
+};
+
 // Up to four neighbours of a tensor of type dt, in one access where the address allows
 __device__ __forceinline__ void load4(const void* p, int64_t i, int dt, int n, float (&v)[4]) {
   const int es = dt == FIM_F32 ? 4 : 2;

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(ORTHO_T) void ortho_convert_kernel(const OrthoStack
   const int r0 = (int)(in / ct) * 64, c0 = (int)(in % ct) * 64;  // of X
   double sq = 0.0;
   for (uint32_t i = threadIdx.x; i < s.chunks; i += ORTHO_T) sq += s.part[b * s.chunks + i];
-  const float scale = (float)((double)k.sx / (sqrt(ortho_sum(sq)) + k.eps));
+  const OrthoScale scaled(sqrt(ortho_sum(sq)) + k.eps, k.sx);
   const int rows = (int)s.rows, cols = (int)s.cols;
   const int sr0 = s.tall ? c0 : r0, sc0 = s.tall ? r0 : c0;  // of the source
   const int64_t base = (int64_t)b * rows * cols;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(ORTHO_T) void ortho_convert_kernel(const OrthoStack
     if (r >= (int)s.mp || c >= (int)s.np) continue;
     float v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = tile[lr * 65 + lc + q] * scale;
+    for (int q = 0; q < 4; ++q) v[q] = scaled(tile[lr * 65 + lc + q]);
     v2i hi, lo;
     split4(v, hi, lo);
     uint8_t* at = X + (int64_t)r * s.np * 4 + line_of(c);

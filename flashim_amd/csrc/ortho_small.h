@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
   sq = red[0];
 #pragma unroll
   for (int i = 1; i < SMALL_WAVES; ++i) sq += red[i];
-  const float scale = (float)((double)k.sx / (sqrt(sq) + k.eps));
+  const OrthoScale scaled(sqrt(sq) + k.eps, k.sx);
   // -- sx X0 as halves, line by line in place: 8 lanes a line, all of which read before one writes
 #pragma unroll 4
   for (int i = tid; i < MP * nb * 8; i += 64 * SMALL_WAVES) {
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     uint8_t* at = X + line * 128;
     float v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float*>(at + (((4 * q + u) ^ (r & 31)) << 2)) * scale;
+    for (int u = 0; u < 4; ++u) v[u] = scaled(*reinterpret_cast<const float*>(at + (((4 * q + u) ^ (r & 31)) << 2)));
     v2i hi, lo;
     split4(v, hi, lo);
     const int key = small_key(r);

@@ -323,3 +323,21 @@ def test_tensors_that_overlap_are_refused():
     ops.muon_step_([w[0], w[1], w[2, :, :16], w[2, :, 16:]], [g[0], g[0], g[2, :, :16], g[2, :, 16:]],
                    [m[0], m[1], m[2, :, :16], m[2, :, 16:]], lr=0.1)
     assert torch.equal(w[3], before[0][3]) and not torch.equal(w[2], before[0][2])
+
+
+@pytest.mark.parametrize("shape", [(4, 4), (24, 40), (40, 24), (7, 3696), (130, 200), (200, 130)])
+def test_norms_whose_scale_fp32_does_not_hold(shape):
+    """2^13 / |g| is past FP32's largest number, or near its smallest; an eps beside which only a zero matrix counts."""
+    for scale in (1e-34, 1e-41, 1e38):
+        g = (_gradient(*shape, seed=41).double() * scale).float()
+        assert g.count_nonzero() > 0
+        _check(ops.orthogonalize(g.to(DEV), eps=0.0), g, scale, eps=0.0)
+        _check(ops.orthogonalize(g.to(DEV), eps=1e-40), g, scale, eps=1e-40)
+    zero = torch.zeros(shape, device=DEV)
+    for eps in (1e-40, 5e-324):
+        assert (ops.orthogonalize(zero, eps=eps) == 0).all()
+    assert torch.isnan(ops.orthogonalize(zero, eps=0.0)).all()  # 0 / 0
+    momentum = torch.zeros(shape, device=DEV)
+    p = torch.ones(shape, device=DEV)
+    ops.muon_step_([p], [zero], [momentum], lr=0.5, eps=1e-40)
+    assert (p == 1).all()
