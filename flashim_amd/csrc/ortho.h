@@ -80,8 +80,9 @@ struct OrthoScale {
   float first, second;
   __device__ OrthoScale(double norm_eps, float sx) {
     const double s = (double)sx / (norm_eps > 0.0 && norm_eps < 1e-60 ? 1e-60 : norm_eps);
-    first = s > 0x1p100 ? 0x1p100f : s < 0x1p-100 ? 0x1p-60f : 1.0f;
-    second = (float)(s / (double)first);
+    const bool large = s > 0x1p100, small = s < 0x1p-100;
+    first = large ? 0x1p100f : small ? 0x1p-60f : 1.0f;
+    second = (float)(s * (large ? 0x1p-100 : small ? 0x1p60 : 1.0));
   }
   __device__ float operator()(float u) const { return u * first * second; }
 };
