@@ -170,13 +170,16 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
           }
         }
       if (from + NARROW_ROWS < total) load_rows(from + NARROW_ROWS);
+      // (ranks past R and rows past the list are zero: an infinity times the zeros there is NaN, which would meet all sums)
+      const bool there = from + 16 * wave + l16 < total;
       float most_t = 0.0f, most_h = 0.0f;
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          h[i][q] *= scale;
-          t[i][q] *= scale;
+          const bool part = there && 16 * i + 4 * g + q < p.R;
+          h[i][q] = part ? h[i][q] * scale : 0.0f;
+          t[i][q] = part ? t[i][q] * scale : 0.0f;
           most_t = fmaxf(most_t, finite_abs(t[i][q]));
           most_h = fmaxf(most_h, finite_abs(h[i][q]));
         }
@@ -229,7 +232,6 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
       }
       // -- dx: columns interleaved as in adapters_rows.h, A_j's ranks read down its columns
       if (p.dx != nullptr) {
-        const bool there = from + 16 * wave + l16 < total;
         uint16_t* out = p.dx + (int64_t)(r0 + (there ? list[from + 16 * wave + l16] : 0)) * p.K + 8 * g;
         for (int c = 0; c < p.K; c += 32) {
           float o[8];

@@ -345,3 +345,36 @@ def test_refusals():
     (g,) = torch.autograd.grad(ops.low_rank_adapters(base, leaf, a, b, index).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="not implemented"):
         g.sum().backward()
+
+
+def _positive(lead, k, n, r, j, dtype, seed):
+    """Inputs above zero, so that an infinity meets no other of its sign's opposite: what it reaches is +infinity."""
+    base, x, a, b, d_out = ((t.float().abs() + 0.125).to(dtype) for t in _inputs(lead, k, n, r, j, dtype, seed=seed))
+    return base, x, a, b, d_out / 16  # (sums within FP16)
+
+
+def _infinite_as_defined(bad, width, r, dtype, names, lead=(70,)):
+    """An infinity in one operand, and the named results against float64's: infinities, NaN and finite values where it has them."""
+    k, n = width
+    base, x, a, b, d_out = _positive(lead, k, n, r, 3, dtype, seed=26)
+    {"x": x, "d": d_out, "a": a[1], "b": b[1]}[bad].view(-1)[5 % min(k, n)] = math.inf
+    index = torch.arange(lead[0]) % 3
+    index[0] = 1 if bad in "ab" else index[0]
+    out, grads = _run(base, x, a, b, index, 0.5, d_out)
+    want = ref.low_rank_adapters(base, x, a, b, index, 0.5, d_out)
+    for name, got in {"out": out, **grads}.items():
+        if name in names:
+            w, g = want[name], got.double().cpu()
+            assert torch.equal(torch.isposinf(g), torch.isposinf(w)) and torch.equal(torch.isnan(g), torch.isnan(w)), (name, bad)
+            assert not torch.isneginf(g).any()
+            at = torch.isfinite(w) & torch.isfinite(want[name + "_error"])
+            _close(name, got.cpu()[at], w[at], want[name + "_error"][at])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("r", [1, 5, 8, 24])
+@pytest.mark.parametrize("bad, names", [("d", ("x", "a")), ("a", ("b",)), ("b", ("a",))])
+def test_infinities_beside_padding(bad, names, r, dtype):
+    """Ranks past R and rows past a turn's last are no part of the narrow backward pass: infinities there are the definition's."""
+    _infinite_as_defined(bad, (64, 96), r, dtype, names)
+    _infinite_as_defined(bad, (41, 50), r, dtype, names)
