@@ -71,6 +71,30 @@ __device__ __forceinline__ void split16(float v, short& hi, short& lo) {
   lo = (short)to16<DT>(fabsf(rest) < __builtin_inff() ? rest : 0.0f);  // (infinity less infinity would be NaN)
 }
 
+// What lo meets of an operand that meets hi and lo: the same, but one in the place of an infinity. hi makes the infinity; lo, zero
+// or of the other sign, would make NaN of it. (A NaN may become anything: hi makes it, too.)
+template <int DT, typename T>
+__device__ __forceinline__ T beside_hi(T v) {
+  constexpr int N = sizeof(T) / 4;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef int words __attribute__((ext_vector_type(N)));
+  constexpr uint16_t most = DT == FIM_BF16 ? 0x7f7f : 0x7bff;
+  words w = __builtin_bit_cast(words, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int both = w[i], size = both & 0x7fff7fff;
+    const u16x2 past = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, size), u16x2{most, most});
+    const u16x2 one = __builtin_bit_cast(u16x2, both) - (past << (uint16_t)14);
+    w[i] = __builtin_bit_cast(int, one);
+  }
+  return __builtin_bit_cast(T, w);
+}
+// Four values of the second operand twice, for hi and lo of four of the first
+template <int DT>
+__device__ __forceinline__ s16x8 beside_halves(s16x4 v) {
+  return __builtin_shufflevector(v, beside_hi<DT>(v), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // For the largest of finite values: an infinity or NaN beside them stays one whatever it is scaled by.
 __device__ __forceinline__ float finite_abs(float v) { return fabsf(v) < __builtin_inff() ? fabsf(v) : 0.0f; }
 

@@ -150,17 +150,17 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(const AdapterGradArgs
           half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (lds_s16x4*)(stage[buf] + r * 256 + ((wave ^ (r & 3)) << 6) + c * 32 + (lane & 3) * 8));
         }
-        const s16x8 v = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const s16x8 v = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7), vl = beside_hi<DT>(v);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           if constexpr (DT == FIM_F16) {
             v4f s = mfma_rank<DT>(th[i], v, v4f{0.0f, 0.0f, 0.0f, 0.0f});
-            s = mfma_rank<DT>(tl[i], v, s);
+            s = mfma_rank<DT>(tl[i], vl, s);
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[i][c][q] = fmaf(s[q], down, acc[i][c][q]);
           } else {
             acc[i][c] = mfma_rank<DT>(th[i], v, acc[i][c]);
-            acc[i][c] = mfma_rank<DT>(tl[i], v, acc[i][c]);
+            acc[i][c] = mfma_rank<DT>(tl[i], vl, acc[i][c]);
           }
         }
       }

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
             for (int i = 0; i < NR; ++i) {
               const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                   (lds_s16x4*)(weights + (16 * i + 4 * g + (l16 >> 2)) * STRIDE + (c + 8 * (lane & 3) + 4 * u) * 2));
-              d = mfma_rank<DT>(__builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, 6, 7), tf[i], d);
+              d = mfma_rank<DT>(beside_halves<DT>(v), tf[i], d);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) o[4 * u + q] = DT == FIM_F16 ? d[q] * down_r : d[q];
@@ -276,18 +276,18 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
             const uint8_t* src = rows_at + r * STRIDE + col * 2 + (lane & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 4 * STRIDE));
-            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), vl = beside_hi<DT>(v);
             const bool of_x = col < xcols;
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
               const s16x8 fh = of_x ? f[0][i] : f[2][i], fl = of_x ? f[1][i] : f[3][i];
               if constexpr (DT == FIM_F16) {
-                const v4f z = mfma_rank<DT>(fl, v, mfma_rank<DT>(fh, v, zero));
+                const v4f z = mfma_rank<DT>(fl, vl, mfma_rank<DT>(fh, v, zero));
                 const float down = of_x ? down_t : down_h;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc[i][c][q] = fmaf(z[q], down, acc[i][c][q]);
               } else {
-                acc[i][c] = mfma_rank<DT>(fl, v, mfma_rank<DT>(fh, v, acc[i][c]));
+                acc[i][c] = mfma_rank<DT>(fl, vl, mfma_rank<DT>(fh, v, acc[i][c]));
               }
             }
           }

@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_row
         v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NR; ++i)
-          d = mfma_rank<DT>(__builtin_shufflevector(v[t][i], v[t][i], 0, 1, 2, 3, 4, 5, 6, 7), hf[z][i], d);
+          d = mfma_rank<DT>(beside_halves<DT>(v[t][i]), hf[z][i], d);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float y = from16<DT>((uint16_t)from[4 * t + q]);

@@ -378,3 +378,14 @@ def test_infinities_beside_padding(bad, names, r, dtype):
     """Ranks past R and rows past a turn's last are no part of the narrow backward pass: infinities there are the definition's."""
     _infinite_as_defined(bad, (64, 96), r, dtype, names)
     _infinite_as_defined(bad, (41, 50), r, dtype, names)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("width, r", [((64, 96), 1), ((64, 96), 8), ((41, 50), 5), ((64, 96), 24), ((200, 520), 5), ((200, 520), 8),
+                                      ((200, 520), 24), ((200, 523), 40), ((96, 200), 100)])
+@pytest.mark.parametrize("bad", ["x", "d", "a", "b"])
+def test_infinities_meet_both_halves(bad, width, r, dtype):
+    """h and t go into products as two numbers of 16 bits, whose second may be zero or negative: an infinity on the other side
+    stays the one that it makes with the first."""
+    for lead in ((70,), (600,), (9, 40)):
+        _infinite_as_defined(bad, width, r, dtype, ("out", "x", "a", "b"), lead)
