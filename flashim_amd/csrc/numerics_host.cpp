@@ -1,6 +1,7 @@
 // Host build of numerics.h (the scalar rules every kernel uses), exported over arrays so the CPU test suite can check
-// them against torch exhaustively without a GPU. Not part of the device library.
+// them against torch exhaustively without a GPU, and of overlap.h. Not part of the device library.
 #include "numerics.h"
+#include "overlap.h"
 
 extern "C" {
 
@@ -40,6 +41,21 @@ void fim_host_int8_quotient(const float* x, int64_t n, float scale, int8_t* out)
 }
 void fim_host_quantize_int8(const float* x, int64_t n, float scale, int8_t* out) {
   for (int64_t i = 0; i < n; ++i) out[i] = fim::quantize_int8_value(x[i], scale);
+}
+
+// 1 where no written tensor of `count` meets another or itself: at, es, written, dims a tensor; strides (bytes) and sizes of all
+int fim_host_apart(int64_t count, const int64_t* at, const int64_t* es, const uint8_t* written, const int64_t* dims,
+                   const int64_t* strides, const int64_t* sizes) {
+  fim::Extents extents;
+  for (int64_t i = 0; i < count; ++i) {
+    fim::Strided t;
+    t.at = at[i];
+    t.es = es[i];
+    for (int64_t k = 0; k < dims[i]; ++k, ++strides, ++sizes)
+      if (*sizes > 1) t.dims.push_back({*strides, *sizes});
+    extents.add(t, written[i] != 0);
+  }
+  return extents.apart() ? 1 : 0;
 }
 
 }  // extern "C"

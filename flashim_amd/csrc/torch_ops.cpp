@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "../../include/flashim_amd.h"
+#include "overlap.h"
 
 namespace {
 
@@ -758,31 +759,21 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double 
   return out;
 }
 
-// The memory of a call's tensors: none that is written may overlap another. (Of a tensor that is not contiguous, whose rows may
-// lie between another's, the first element.)
-struct Extents {
-  struct Extent {
-    uintptr_t from, to;
-    bool written;
-  };
-  std::vector<Extent> all;
-  void add(const Tensor& t, bool written) {
-    if (written) at::assert_no_internal_overlap(t);
-    if (t.numel() == 0) return;
-    const auto from = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    all.push_back({from, from + (t.is_contiguous() ? t.nbytes() : t.element_size()), written});
+// A tensor's memory, in bytes; neighbouring dimensions that step as one are one
+fim::Strided memory_of(const Tensor& t) {
+  fim::Strided s;
+  s.at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.const_data_ptr()));
+  s.es = t.is_contiguous() ? t.nbytes() : t.element_size();
+  for (int64_t i = 0; i < t.dim() && !t.is_contiguous(); ++i) {
+    const fim::Strided::Dim d{t.stride(i) * s.es, t.size(i)};
+    if (d.size == 1) continue;
+    if (!s.dims.empty() && s.dims.back().stride == d.stride * d.size)
+      s.dims.back() = {d.stride, d.size * s.dims.back().size};
+    else
+      s.dims.push_back(d);
   }
-  bool apart() {
-    std::sort(all.begin(), all.end(), [](const Extent& a, const Extent& b) { return a.from < b.from; });
-    uintptr_t end = 0, written = 0;
-    for (const Extent& e : all) {
-      if (e.from < (e.written ? end : written)) return false;
-      end = std::max(end, e.to);
-      if (e.written) written = std::max(written, e.to);
-    }
-    return true;
-  }
-};
+  return s;
+}
 
 // adjust 0: sqrt(max(1, rows / cols)), 1: 0.2 sqrt(max(rows, cols)), 2: 1
 float muon_factor(double lr, int64_t adjust, int64_t rows, int64_t cols) {
@@ -808,7 +799,11 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   std::vector<int> pt, gt;
   std::vector<int64_t> batch, rows, cols;
   std::vector<float> factors;
-  Extents extents;
+  fim::Extents extents;
+  auto add = [&](const Tensor& t, bool written) {
+    if (written) at::assert_no_internal_overlap(t);
+    if (t.numel() > 0) extents.add(memory_of(t), written);
+  };
   for (size_t i = 0; i < n; ++i) {
     const Tensor &w = params[i], &d = grads[i], &v = momenta[i];
     for (const Tensor* t : {&w, &d, &v}) check_grad(*t, params[0]);
@@ -816,9 +811,9 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
     TORCH_CHECK_NOT_IMPLEMENTED(w.dim() >= 2 && w.sizes() == d.sizes() && w.sizes() == v.sizes(),
                                 "no HIP impl applies: a parameter of shape ", w.sizes(), ", its gradient of ", d.sizes(),
                                 " and momentum of ", v.sizes());
-    extents.add(w, true);
-    extents.add(d, false);
-    extents.add(v, true);
+    add(w, true);
+    add(d, false);
+    add(v, true);
     p.push_back(w.is_contiguous() ? w : w.contiguous());
     g.push_back(d.contiguous());
     m.push_back(v.is_contiguous() ? v : v.contiguous());

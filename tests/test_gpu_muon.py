@@ -341,3 +341,30 @@ def test_norms_whose_scale_fp32_does_not_hold(shape):
     p = torch.ones(shape, device=DEV)
     ops.muon_step_([p], [zero], [momentum], lr=0.5, eps=1e-40)
     assert (p == 1).all()
+
+
+def test_strided_tensors_that_overlap_are_refused():
+    """Views with gaps, between whose rows another's may lie: what counts are the elements."""
+    big, flat = torch.randn(40, 128, device=DEV), torch.randn(4000, device=DEV)
+    g, m = torch.randn(40, 128, device=DEV), torch.zeros(40, 128, device=DEV)
+    before = big.clone()
+
+    def step(*params):
+        grads = [g.reshape(-1)[:p.numel()].reshape(p.shape) for p in params]
+        ops.muon_step_(list(params), grads, [torch.zeros_like(t) for t in grads], lr=0.1)
+
+    for params in ((big[:, :64], big[:, 32:96]), (big[:, ::2], big[:, 2::4]), (big[::2, :10], big[10:11, 9:]), (big[:, :64], big[:, 63:].t()),
+                   (flat.as_strided((5, 9), (30, 2)), flat.as_strided((4, 7), (13, 3), 1)), (big, flat.new_empty(3, 3), big[5:, 5:9])):
+        with pytest.raises(ValueError, match="overlaps"):
+            step(*params)
+    with pytest.raises(ValueError, match="overlaps"):  # a gradient's elements
+        ops.muon_step_([big[:, :64]], [big[:, 32:96]], [m[:, :64]], lr=0.1)
+    with pytest.raises(ValueError, match="overlaps"):  # one tensor's own
+        step(flat.as_strided((8, 8), (3, 2)))
+    assert torch.equal(big, before)
+    # apart, however their addresses interleave
+    step(big[:, :64], big[:, 64:])
+    step(big[:, ::2], big[:, 1::2].t())
+    step(big[::2, :100], big[1::2], big[::2, 100:].t())
+    step(flat.as_strided((5, 9), (90, 4)), flat.as_strided((4, 7), (90, 8), 2), flat.as_strided((9, 9), (11, 1), 3000))
+    ops.muon_step_([big[:, :64]], [big[:, 64:]], [m[:, 3:67]], lr=0.1)

@@ -251,3 +251,74 @@ def test_partial_sums_of_many_adapters_stay_small():
     for m, k, n, j, r in ((1 << 20, 64, 256, 1000, 8), (1 << 21, 128, 256, 100, 32), (1 << 24, 64, 64, 2000, 16)):
         assert lib.fim_low_rank_adapters_backward_workspace(m, k, n, j, r, ctypes.byref(out)) == 0
         assert out.value <= (256 << 20) + j * 1024 * 4 + 4096
+
+
+# -- memory of a step's tensors --------------------------------------------------------------------------------------------
+
+
+def _apart(tensors):
+    """``fim_host_apart`` of ``(address, element bytes, written, [(stride in bytes, size)])``."""
+    fn, i64 = _lib.load_host().fim_host_apart, ctypes.c_int64
+
+    def array(kind, values):
+        return (kind * max(1, len(values)))(*values)
+
+    dims = [d for t in tensors for d in t[3]]
+    return fn(i64(len(tensors)), array(i64, [t[0] for t in tensors]), array(i64, [t[1] for t in tensors]),
+              array(ctypes.c_uint8, [t[2] for t in tensors]), array(i64, [len(t[3]) for t in tensors]),
+              array(i64, [d[0] for d in dims]), array(i64, [d[1] for d in dims])) == 1
+
+
+def _apart_by_bytes(tensors):
+    """The same, byte by byte."""
+    seen, read = set(), set()
+    for address, size, written, dims in tensors:
+        at = [address]
+        for stride, n in dims:
+            at = [x + stride * i for x in at for i in range(n)]
+        own = [x + i for x in at for i in range(size)]
+        if written and (len(set(own)) < len(own) or not read.isdisjoint(own)) or not seen.isdisjoint(own):
+            return False
+        (seen if written else read).update(own)
+    return True
+
+
+def test_overlaps_of_strided_tensors_are_found_exactly():
+    """Two or three tensors of up to three dimensions, random and nested strides: byte by byte the same answer, both often."""
+    g = torch.Generator().manual_seed(0)
+
+    def pick(*values):
+        return values[torch.randint(0, len(values), (), generator=g).item()]
+
+    answers = [0, 0]
+    for trial in range(4000):
+        tensors = []
+        row = pick(24, 40, 64)  # bytes of a row of a shared buffer
+        for _ in range(pick(2, 2, 3)):
+            es = pick(2, 4)
+            if trial % 2:  # views of rows
+                step, cols = es * pick(1, 1, 2, 3), pick(1, 2, 3, 5)
+                dims = [(row * pick(1, 2), pick(1, 3, 4)), (step, cols)]
+                dims = dims[::-1] if pick(0, 1) else dims
+                address = row * pick(0, 0, 1) + es * pick(0, 1, 2, 4, 6, 8)
+            else:
+                dims = [(es * pick(0, 1, 2, 3, 5, 7, 11, 13), pick(1, 2, 3, 4)) for _ in range(pick(0, 1, 2, 3))]
+                address = es * torch.randint(0, 60, (), generator=g).item()
+            tensors.append((address, es, pick(0, 1, 1), dims))
+        want = _apart_by_bytes(tensors)
+        answers[want] += 1
+        assert _apart(tensors) == want, tensors
+    assert min(answers) > 800, answers
+
+
+def test_overlaps_of_large_tensors_are_found_in_few_steps():
+    """Halves of a matrix's columns, its transposes and interleaved slices at full size; strides that do not nest count as overlapping
+    once the search grows long."""
+    n = 1 << 20
+    left, right = (0, 4, 1, [(8 * n, n), (4, n)]), (4 * n, 4, 1, [(4, n), (8 * n, n)])
+    assert _apart([left, right]) and not _apart([left, (4 * n - 4, 4, 1, right[3])])
+    assert _apart([(0, 4, 1, [(8, n)]), (4, 4, 1, [(8, n)]), (8 * n, 2, 0, [(0, n), (2, n)])])
+    assert not _apart([(0, 4, 1, [(8, n)]), (4 * n, 2, 0, [(4, n)])])
+    assert not _apart([(0, 4, 1, [(12, n), (8, n)])])
+    assert not _apart([(0, 2, 1, [(10**6 + 2, 1000), (10**6 - 2, 999), (10**6 + 6, 998)]),
+                       (2, 2, 1, [(10**6 + 4, 1000), (10**6 - 8, 999), (10**6 + 14, 998)])])
