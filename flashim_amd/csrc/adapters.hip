@@ -90,6 +90,8 @@ static bool adapter_narrow(int64_t K, int64_t N, int64_t R) {
   return R <= 32 && cdiv(K, 32) * 32 + cdiv(N, 32) * 32 <= NARROW_WIDTH;
 }
 
+constexpr int64_t GRAD_GRID = 1 << 24;  // workgroups of 256 threads, which a launch counts in 32 bits: fewer
+
 static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   AdapterGradPlan g;
   g.xt = (int)cdiv(s.K, GRAD_COLS);
@@ -101,7 +103,9 @@ static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   const int64_t step = g.narrow ? NARROW_ROWS : 256, longest = g.narrow ? NARROW_CHUNK : GRAD_CHUNK;
   const int64_t most = (int64_t{256} << 20) / (s.J * s.R * (s.K + s.N) * 4), fits = cdiv(s.M, longest);
   if (chunks < fits) chunks = fits;
+  const int64_t grid = (GRAD_GRID - 1) / ((s.J + 1) * (g.narrow ? 1 : g.ct));
   if (chunks > most) chunks = most;
+  if (chunks > grid) chunks = grid;
   if (chunks < 1) chunks = 1;
   g.chunk = cdiv(cdiv(s.M, chunks), step) * step;
   if (g.chunk < 256) g.chunk = 256;  // (a workgroup's weights cost as much)
@@ -120,6 +124,13 @@ static AdapterGradPlan grad_plan(const AdapterSizes& s) {
   g.counts = take(g.chunks > 1 ? s.J * g.chunks * 4 : 0);
   g.bytes = at;
   return g;
+}
+
+// What one launch of the backward pass cannot hold
+static int grad_check(const AdapterSizes& s, const AdapterGradPlan& g) {
+  const bool no = s.J * s.R * (s.K + s.N) >= int64_t{1} << 32 || s.R * (s.K + s.N) >= int64_t{1} << 30 ||
+                  (s.J + 1) * g.chunks * (g.narrow ? 1 : g.ct) >= GRAD_GRID;
+  return no ? FIM_ERR_UNSUPPORTED : FIM_OK;
 }
 
 }  // namespace fim
@@ -159,8 +170,11 @@ extern "C" int fim_low_rank_adapters_backward_workspace(int64_t M, int64_t K, in
   const AdapterSizes s{M, K, N, J, R, M};
   const int rc = adapter_check(s, FIM_BF16, 0);
   if (rc != FIM_OK) return rc;
-  *bytes = M > 0 ? grad_plan(s).bytes : 0;
-  return FIM_OK;
+  *bytes = 0;
+  if (M == 0) return FIM_OK;
+  const AdapterGradPlan g = grad_plan(s);
+  *bytes = g.bytes;
+  return grad_check(s, g);
 }
 
 extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_stride, const void* x, int64_t x_stride, int dtype,
@@ -182,10 +196,9 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
   if (g.bytes > 0 && (workspace == nullptr || workspace_bytes < g.bytes || reinterpret_cast<uintptr_t>(workspace) % 256))
     return FIM_ERR_INVALID;
   if (dx == nullptr && da == nullptr) return FIM_OK;
+  rc = grad_check(s, g);
+  if (rc != FIM_OK) return rc;
   const int64_t na = J * R * K, nb = J * R * N;
-  // (a launch counts its threads in 32 bits)
-  if (na + nb >= int64_t{1} << 32 || R * (K + N) >= int64_t{1} << 30 || (J + 1) * g.chunks * (g.narrow ? 1 : g.ct) >= 1 << 24)
-    return FIM_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* part = da != nullptr && g.chunks > 1 ? reinterpret_cast<float*>(ws + g.part) : nullptr;
   int* counts = part != nullptr ? reinterpret_cast<int*>(ws + g.counts) : nullptr;
@@ -227,7 +240,7 @@ extern "C" int fim_low_rank_adapters_backward(const void* d_out, int64_t d_out_s
   const AdapterIndex rows{index, index_wide, (uint32_t)(M / entries), (int)J};
   adapter_transpose_kernel<<<dim3((unsigned)cdiv(na + nb, 256)), dim3(256), 0, stream>>>(
       static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), at, bt, (int)K, (int)N, (int)R, na, nb);
-  // t = s d_out B and dx = t A: the forward pass over d_out (without dx: over one column)
+  // t = s d_out B and dx = t A: the forward pass over d_out (without dx: over no columns)
   AdapterArgs p{static_cast<const uint16_t*>(d_out), nullptr, bt, at, d_out_stride, 0, static_cast<uint16_t*>(dx), t, rows, scales,
                 scale, (uint32_t)M, (int)N, dx == nullptr ? 0 : (int)K, (int)R, 1};
   adapter_rows(p, dtype, stream);

@@ -1224,6 +1224,12 @@ struct LowRankAdapters : torch::autograd::Function<LowRankAdapters> {
     at::AutoDispatchBelowAutograd guard;
     static const auto op = typed_op<decltype(low_rank_adapters)>("flashim_amd::low_rank_adapters");
     auto [out, h] = op.call(base, x, a, b, index, scales, scale, save);
+    // (sizes past a launch of the backward pass: refused before a step depends on it)
+    if (x.is_cuda() && !x.key_set().has(c10::DispatchKey::Python) && x.numel() > 0) {
+      int64_t bytes = 0;
+      check(fim_low_rank_adapters_backward_workspace(x.numel() / x.size(-1), x.size(-1), b.size(1), b.size(0), b.size(2), &bytes),
+            "low_rank_adapters backward ", x.sizes(), " x ", a.sizes(), " -> ", b.size(1));
+    }
     ctx->save_for_backward({x, a, b, index, as_tensor(scales), h});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["base"] = base && base->defined();

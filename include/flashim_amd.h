@@ -329,7 +329,8 @@ int fim_low_rank_adapters(const void* base, int64_t base_stride, const void* x, 
  * where it computes h again (narrow projections). */
 int fim_low_rank_adapters_saved(int64_t K, int64_t N, int64_t R, int64_t* columns);
 
-/* Bytes of workspace (256-byte aligned) that fim_low_rank_adapters_backward needs. */
+/* Bytes of workspace (256-byte aligned) that fim_low_rank_adapters_backward needs; 99 for sizes that a launch of it cannot hold:
+ * adapters of 2^32 elements or more together, or one of 2^30. */
 int fim_low_rank_adapters_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t J, int64_t R, int64_t* bytes);
 
 /* The gradients of x, a and b (packed; dx alone may be NULL, or da and db together; h where it is not needed), from d_out [M, N], M >= 1,

@@ -389,3 +389,18 @@ def test_infinities_meet_both_halves(bad, width, r, dtype):
     stays the one that it makes with the first."""
     for lead in ((70,), (600,), (9, 40)):
         _infinite_as_defined(bad, width, r, dtype, ("out", "x", "a", "b"), lead)
+
+
+@pytest.mark.parametrize("wanted", ["x", "a"])
+def test_what_the_backward_pass_cannot_hold_is_refused_by_the_forward_pass(wanted):
+    """Adapters of 2^32 elements and more (their transposes' launch): served, but not trained or trained through."""
+    from flashim_amd._lib import UnsupportedShape
+
+    j, r, k, n = 1024, 128, 32768 - 32, 64
+    a, b = torch.empty(j, r, k, dtype=BF16, device=DEV), torch.zeros(j, n, r, dtype=BF16, device=DEV)
+    x, index = torch.zeros(3, k, dtype=BF16, device=DEV), torch.tensor([5, -1, 1023], device=DEV)
+    a[[5, 1023]] = 1.0
+    assert (ops.low_rank_adapters(None, x, a, b, index) == 0).all()
+    (x if wanted == "x" else a).requires_grad_()
+    with pytest.raises(UnsupportedShape, match="backward"):
+        ops.low_rank_adapters(None, x, a, b, index)

@@ -322,3 +322,18 @@ def test_overlaps_of_large_tensors_are_found_in_few_steps():
     assert not _apart([(0, 4, 1, [(12, n), (8, n)])])
     assert not _apart([(0, 2, 1, [(10**6 + 2, 1000), (10**6 - 2, 999), (10**6 + 6, 998)]),
                        (2, 2, 1, [(10**6 + 4, 1000), (10**6 - 8, 999), (10**6 + 14, 998)])])
+
+
+def test_adapters_whose_gradients_one_launch_cannot_hold_are_refused_by_the_workspace():
+    lib, out = _lib.load(), ctypes.c_int64()
+    at, no = ctypes.byref(out), _lib.FIM_ERR_UNSUPPORTED
+
+    def workspace(m, k, n, j, r):
+        return lib.fim_low_rank_adapters_backward_workspace(m, k, n, j, r, at)
+
+    assert workspace(3, 32768 - 64, 64, 1024, 128) == no  # 2^32 elements of adapters
+    assert workspace(3, 32768 - 65, 64, 1024, 128) == 0
+    assert workspace(3, 1 << 23, 1, 1, 128) == no  # 2^30 of one
+    # many tiny adapters: fewer chunks, not more workgroups than a launch has
+    for j in (1 << 15, 1 << 17, (1 << 20) - 1):
+        assert workspace(1 << 20, 1, 1, j, 1) == 0 and workspace(1 << 20, 8, 400, j, 1) == 0
