@@ -15,11 +15,15 @@ from flashim_amd.backends.hip.train import NEWTON_SCHULZ
 
 
 class Muon(torch.optim.Optimizer):
-    """Parameters of two dimensions or more (leading ones: stacks of matrices, each stepped by itself) take
-    ``ops.muon_step_`` with an FP32 momentum; the others (norms' weights, biases) take AdamW with ``adam_lr``, ``adam_betas``
-    and ``adam_eps``. Every option may differ by parameter group. All matrices of a group (on one GPU) are stepped in the
-    same launches, and nothing waits for the GPU. A step in a captured graph needs one before it, which makes its state, and ``capturable=True`` where
-    AdamW's parameters are among them: their step counts then lie on the GPU."""
+    """Matrices, and parameters of three dimensions as stacks of matrices, each stepped by itself, take ``ops.muon_step_`` with
+    an FP32 momentum; the others (norms' weights, biases) take AdamW with ``adam_lr``, ``adam_betas`` and ``adam_eps``. Parameters of
+    more dimensions are refused: a convolution's weight is one matrix of its output channels by the rest, and not a stack of
+    its kernels. Every option may differ by parameter group. All matrices of a group (on one GPU) are stepped in the same
+    launches, and nothing waits for the GPU.
+
+    A step in a captured graph needs one before it, which makes its state, and ``capturable=True`` where AdamW's parameters are
+    among them: their step counts then lie on the GPU. Replays keep the options of the capture, its learning rates among them: a
+    schedule that changes them needs a capture for each."""
 
     def __init__(self, params: Iterable, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, adjust: str = "original", steps: int = 5, coefficients=NEWTON_SCHULZ,
@@ -30,6 +34,14 @@ class Muon(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, adjust=adjust,
                                       steps=steps, coefficients=coefficients, eps=eps, adam_lr=adam_lr, adam_betas=adam_betas,
                                       adam_eps=adam_eps, capturable=capturable))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.ndim > 3:
+                self.param_groups.pop()
+                raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)}: neither a matrix nor a stack of them (a convolution's "
+                                 "weight would be one matrix, a view of two dimensions)")
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As any optimizer's, but with states of its own (none is shared with the optimizer they came from), and momenta that

@@ -337,3 +337,16 @@ def test_adapters_whose_gradients_one_launch_cannot_hold_are_refused_by_the_work
     # many tiny adapters: fewer chunks, not more workgroups than a launch has
     for j in (1 << 15, 1 << 17, (1 << 20) - 1):
         assert workspace(1 << 20, 1, 1, j, 1) == 0 and workspace(1 << 20, 8, 400, j, 1) == 0
+
+
+def test_optimizer_refuses_what_is_neither_a_matrix_nor_a_stack():
+    """A convolution's weight, of which the stack would be its kernels; a group that is refused leaves the optimizer as it was."""
+    conv = torch.nn.Conv2d(3, 4, 3)
+    with pytest.raises(ValueError, match="neither a matrix"):
+        optim.Muon(conv.parameters())
+    opt = optim.Muon([conv.bias])
+    with pytest.raises(ValueError, match="neither a matrix"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2, 3)), conv.weight]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": torch.nn.Parameter(conv.weight.detach().flatten(1))})
+    assert len(opt.param_groups) == 2
