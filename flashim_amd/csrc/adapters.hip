@@ -54,8 +54,7 @@ static void launch_rows(AdapterArgs& p, hipStream_t stream) {
     if (one) adapter_rows_kernel<DT, NR, 4, 0, Q><<<grid, dim3(256), 0, stream>>>(p);
     else if (four && two) adapter_rows_kernel<DT, NR, 4, 2, Q><<<grid, dim3(256), 0, stream>>>(p);
     else if (four) adapter_rows_kernel<DT, NR, 4, 1, Q><<<grid, dim3(256), 0, stream>>>(p);
-    else if (two) adapter_rows_kernel<DT, NR, 1, 2, Q><<<grid, dim3(256), 0, stream>>>(p);
-    else adapter_rows_kernel<DT, NR, 1, 1, Q><<<grid, dim3(256), 0, stream>>>(p);
+    else adapter_rows_kernel<DT, NR, 1, 2, Q><<<grid, dim3(256), 0, stream>>>(p);  // (so many rows are always two sets)
   };
   if (p.R % (NR == 1 ? 4 : 8) == 0) launch(std::integral_constant<bool, true>{});
   else launch(std::integral_constant<bool, false>{});

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, SETS == 2 && NR <= 4 ? 2 : 1) void adapter_row
   constexpr bool ONE = SETS == 0;
   constexpr int S = ONE ? 1 : SETS;
   // blocks of 32 columns whose operands are in flight
-  constexpr int GROUP = NR <= 2 && W > 1 && S == 1 ? 4 : NR == 4 || S * NR >= 8 ? 1 : 2;
+  constexpr int GROUP = NR <= 2 && S == 1 ? 4 : NR == 4 || S * NR >= 8 ? 1 : 2;
   __shared__ __attribute__((aligned(16))) float sums[W > 1 ? W * S * NR * 256 : 4];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);

@@ -321,10 +321,17 @@ static void launch_product(const OrthoStack* table, int count, const OrthoTiles&
   const dim3 grid((unsigned)(cdiv(t.tiles * t.splits, 8 * ORTHO_RUN) * 8 * ORTHO_RUN)), block(256);
   const uint32_t tiles = (uint32_t)t.tiles;
   const int splits = (int)t.splits;
-  if (t.side == 2 && t.deep) ortho_tile_kernel<MODE, 2, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
-  else if (t.side == 2) ortho_tile_kernel<MODE, 2, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
-  else if (t.deep) ortho_tile_kernel<MODE, 1, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
-  else ortho_tile_kernel<MODE, 1, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  // (P on tiles of 128 has two a CU and more, and P X on tiles of 64 at most two: their stages are 2 and 4)
+  constexpr bool ALWAYS_2 = MODE == ORTHO_SQUARE, ALWAYS_4 = MODE == ORTHO_APPLY || MODE == ORTHO_LAST;
+  if (t.side == 2) {
+    if constexpr (!ALWAYS_2)
+      if (t.deep) return ortho_tile_kernel<MODE, 2, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+    ortho_tile_kernel<MODE, 2, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  } else {
+    if constexpr (!ALWAYS_4)
+      if (!t.deep) return ortho_tile_kernel<MODE, 1, 2><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+    ortho_tile_kernel<MODE, 1, 4><<<grid, block, 0, stream>>>(table, count, tiles, splits, part, src, k);
+  }
 }
 
 static void launch_products(const OrthoStack* table, int count, const OrthoPlan& p, float* part, const OrthoScalars& k,
