@@ -158,6 +158,43 @@ def schulz_bound(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: flo
     return total
 
 
+def schulz_halves(u: Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7, leave_out: str = "") -> Tensor:
+    """One matrix's iteration as FP32 arithmetic on operands of two FP16 halves computes it, in some order of its sums: X, A and P
+    times powers of two that keep a little more than their largest entries below FP16's largest number, each product hi hi + hi lo +
+    lo hi with FP32 sums. How far this ends from the exact result is how far such an iteration may end. ``leave_out``: a
+    product (``"gram"``, ``"square"`` or ``"apply"``) whose low halves are dropped, a mistake to be noticed."""
+    a, b, c = coefficients
+    grid = torch.linspace(0, 1, 257, dtype=torch.float64)
+    most_x, most_p = 1.0, 0.0
+    for k in range(steps):
+        p = a + b * grid**2 + c * grid**4
+        grid = grid * p
+        most_p = max(most_p, p.abs().max().item())
+        most_x = max(most_x, grid.abs().max().item()) if k + 1 < steps else most_x
+    sx, sa, sp = (2.0 ** math.floor(math.log2(60000.0 / m)) for m in (1.1 * most_x, 1.25 * most_x**2, 1.05 * most_p))
+
+    def halves(t, scale):
+        t = t.float() * scale
+        hi = t.half().float()
+        return hi, (t - hi).half().float()
+
+    def product(s, t, name):
+        hi, lo = s[0] @ t[0], s[0] @ t[1] + s[1] @ t[0]
+        return (hi if leave_out == name else hi + lo).double()
+
+    tall = u.shape[0] > u.shape[1]
+    u = (u.t() if tall else u).double()
+    eye = torch.eye(u.shape[0], dtype=torch.float64, device=u.device)
+    x = halves(u / (u.square().sum().sqrt() + eps), sx)
+    for k in range(steps):
+        gram = product(x, [t.t() for t in x], "gram") / sx**2
+        half = halves(gram, sa)
+        square = product(half, half, "square") / sa**2
+        y = product(halves(a * eye + b * gram + c * square, sp), x, "apply") / (sp * sx)
+        x = halves(y, sx)
+    return y.t() if tall else y
+
+
 def _sum_error(n: int) -> float:
     """Of FP32 sums of n terms, relative to the terms' magnitudes: independent roundings of 2^-24, four standard deviations."""
     return 4 * math.sqrt(n + 4) * 2.0**-24

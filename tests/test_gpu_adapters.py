@@ -404,3 +404,15 @@ def test_what_the_backward_pass_cannot_hold_is_refused_by_the_forward_pass(wante
     (x if wanted == "x" else a).requires_grad_()
     with pytest.raises(UnsupportedShape, match="backward"):
         ops.low_rank_adapters(None, x, a, b, index)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("size", [((2100,), 200, 523, 24, 3), ((2100,), 200, 523, 100, 3), ((17000,), 72, 520, 40, 3),
+                                  ((17000,), 196, 300, 64, 5), ((33000,), 64, 256, 8, 4), ((33000,), 41, 50, 5, 4),
+                                  ((33000,), 64, 100, 24, 3), ((33000,), 64, 100, 40, 3), ((33000,), 72, 100, 100, 3),
+                                  ((33000,), 130, 520, 12, 3)])
+def test_every_form_of_the_tiles(size, dtype):
+    """Two sets of 16 rows at any rank, and a wavefront a tile, on the other side of the rows they begin at (8, 64 and 128 a CU)."""
+    lead, k, n, r, j = size
+    base, x, a, b, d_out = _inputs(lead, k, n, r, j, dtype, seed=27, d=0.125)
+    _check(base, x, a, b, _index("runs", lead, j, seed=28), 0.5, d_out)

@@ -368,3 +368,45 @@ def test_strided_tensors_that_overlap_are_refused():
     step(big[::2, :100], big[1::2], big[::2, 100:].t())
     step(flat.as_strided((5, 9), (90, 4)), flat.as_strided((4, 7), (90, 8), 2), flat.as_strided((9, 9), (11, 1), 3000))
     ops.muon_step_([big[:, :64]], [big[:, 64:]], [m[:, 3:67]], lr=0.1)
+
+
+# -- precision of the products, and every form of them ------------------------------------------------------------------------
+
+
+def _check_halves(got, u, **kwargs):
+    """Each matrix of ``got`` (FP32) as near float64's result as FP32 arithmetic on two halves ends (``schulz_halves``), times 4: both
+    are sums of hundreds and more of independent roundings of the same sizes, which pass through the same steps, in other orders.
+    Half a step of the output's own besides. (What a product without its low halves would be off by is at least twice that at up to 130 rows:
+    ``test_oracle_tells_a_product_without_its_low_halves``.)"""
+    got = got.reshape(-1, *u.shape[-2:])
+    for i, m in enumerate(u.reshape(-1, *u.shape[-2:])):
+        m = m.to(DEV if m.numel() > 1 << 18 else "cpu")
+        want = ref.orthogonalize(m, **kwargs)
+        off, halves = ((t.to(want) - want).norm().item() for t in (got[i], ref.schulz_halves(m, **kwargs)))
+        assert off <= 4 * halves + U[F32] * want.norm().item(), (i, off, halves)
+
+
+@pytest.mark.parametrize("shape", [(16, 512), (64, 256), (256, 64), (48, 100), (40, 1500), (1500, 40), (7, 3696), (96, 96), (65, 65),
+                                   (100, 200), (150, 130), (20, 64, 64), (300, 1000), (520, 2100)])
+def test_products_keep_both_halves(shape):
+    g = _gradient(*shape, seed=42)
+    _check_halves(ops.orthogonalize(g.to(DEV)), g)
+
+
+# (X X^T on tiles of 64 and 128, with two and four stages, whole and in parts; P and P X on either tile; by tiles a call, at 256 CUs)
+PLANS = {"gram 64, square 64, two stages": [(200, 100, 200)], "gram 128, square 128": [(171, 130, 150)],
+         "gram 128 with four stages": [(85, 130, 150), (100, 120)], "gram 128, square 64": [(100, 130, 150)],
+         "apply 128 with four stages": [(33, 130, 150)], "gram in parts, two stages": [(1000, 4000)],
+         "gram in parts, four stages": [(1000, 1300)], "tall, mixed": [(60, 150, 130), (4, 600, 260), (30, 90, 70)]}
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_every_form_of_the_products(plan):
+    """A step from zeros is -O."""
+    grads = [_gradient(*s, seed=43 + i) for i, s in enumerate(PLANS[plan])]
+    params, momenta = ([torch.zeros(s, device=DEV) for s in PLANS[plan]] for _ in range(2))
+    ops.muon_step_(params, [g.to(DEV) for g in grads], momenta, lr=1.0, adjust="none", nesterov=False)
+    for p, g in zip(params, grads):
+        _check_halves(-p, g)
+    if len(grads) == 1:
+        assert torch.equal(ops.orthogonalize(grads[0].to(DEV)), -params[0])

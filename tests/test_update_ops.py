@@ -350,3 +350,20 @@ def test_optimizer_refuses_what_is_neither_a_matrix_nor_a_stack():
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": torch.nn.Parameter(conv.weight.detach().flatten(1))})
     assert len(opt.param_groups) == 2
+
+
+@pytest.mark.parametrize("shape", [(16, 512), (64, 256), (48, 100), (40, 1500), (7, 3696), (96, 96), (65, 65), (100, 200), (130, 150)])
+def test_oracle_tells_a_product_without_its_low_halves(shape):
+    """Of matrices as gradients are: an iteration that drops the low halves of one of its products ends at least twice as far from
+    the exact result as 4 times one that keeps them, the tolerance of the tests that hold the kernels to it."""
+    g = torch.Generator().manual_seed(3)
+    few = min(6, *shape)
+    strong = torch.randn(shape[0], few, generator=g) * torch.exp(-0.5 * torch.arange(few))
+    u = strong @ torch.randn(few, shape[1], generator=g) + 0.05 * torch.randn(shape, generator=g)
+    want = ref.orthogonalize(u)
+    off = {name: (ref.schulz_halves(u, leave_out=name) - want).norm() for name in ("", "gram", "square", "apply")}
+    assert off[""] <= 1e-5 * want.norm()
+    for name in ("gram", "square", "apply"):
+        assert off[name] >= 8 * off[""], (name, off)
+    if shape[0] != shape[1]:  # (a tall one's is the other's; a square one's sums run otherwise)
+        torch.testing.assert_close(ref.schulz_halves(u.t()), ref.schulz_halves(u).t())
