@@ -45,6 +45,7 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
   __shared__ uint16_t list[NARROW_CHUNK];
   __shared__ int counted[4];
   __shared__ float largest[2][4];
+  __shared__ int infinities[4];  // whether a wavefront's rows hold some
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int slot = (int)blockIdx.x, j = slot / p.chunks, chunk = slot - j * p.chunks;  // j = J: rows without an adapter
@@ -170,6 +171,14 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
           }
         }
       if (from + NARROW_ROWS < total) load_rows(from + NARROW_ROWS);
+      // (an infinity in a row makes one or NaN of all its sums)
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum += h[i][q] + t[i][q];
+      const uint64_t found = __builtin_amdgcn_ballot_w64(!(fabsf(sum) < __builtin_inff()));
+      if (lane == 0) infinities[wave] = found != 0;
       // (ranks past R and rows past the list are zero: an infinity times the zeros there is NaN, which would meet all sums)
       const bool there = from + 16 * wave + l16 < total;
       float most_t = 0.0f, most_h = 0.0f;
@@ -255,7 +264,7 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
       }
       lds_barrier();
       // -- dA and dB: 64 rows, 32 a product; this wavefront's 16-column blocks of x and d_out
-      if (p.da != nullptr) {
+      auto sums = [&](auto beside) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int r = 32 * s + 8 * g + (l16 >> 2), xcols = kp, most = kp + np;
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
             const uint8_t* src = rows_at + r * STRIDE + col * 2 + (lane & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 4 * STRIDE));
-            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), vl = beside_hi<DT>(v);
+            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), vl = beside(v);
             const bool of_x = col < xcols;
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
@@ -292,6 +301,11 @@ __global__ __launch_bounds__(256) void adapter_narrow_kernel(const AdapterNarrow
             }
           }
         }
+      };
+      if (p.da != nullptr) {  // (infinities apart: 320000 x 64 -> 256 62 us, 68 in one)
+        if (__builtin_amdgcn_readfirstlane(infinities[0] | infinities[1] | infinities[2] | infinities[3]))
+          sums([](s16x8 v) { return beside_hi<DT>(v); });
+        else sums([](s16x8 v) { return v; });
       }
       lds_barrier();
     }
