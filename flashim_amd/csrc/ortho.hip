@@ -149,10 +149,13 @@ static OrthoShape ortho_shape(int64_t rows, int64_t cols) {
   s.np = cdiv(s.n, 32) * 32;
   s.T = (int)cdiv(s.m, 16);
   s.small = s.m <= SMALL_ROWS && small_lds(s.m, s.np) <= SMALL_LDS;
-  // about 16 workgroups a matrix, each of which reads all their parts; four lines a workgroup at least
-  const int64_t lines = s.np / 32, most = (SMALL_LDS - small_region(s.T) - 64) / (16 * s.T * 128);
-  s.slab = cdiv(lines, 16) < 4 ? 4 : cdiv(lines, 16) > most ? most : cdiv(lines, 16);
-  s.slabs = cdiv(lines, s.slab);
+  s.slab = s.slabs = 0;
+  if (s.m <= SMALL_ROWS) {  // (more rows' sums leave no room for a line, and are on tiles)
+    // about 16 workgroups a matrix, each of which reads all their parts; four lines a workgroup at least
+    const int64_t lines = s.np / 32, most = (SMALL_LDS - small_region(s.T) - 64) / (16 * s.T * 128);
+    s.slab = cdiv(lines, 16) < 4 ? 4 : cdiv(lines, 16) > most ? most : cdiv(lines, 16);
+    s.slabs = cdiv(lines, s.slab);
+  }
   // (all their reads of all parts grow with the slabs squared: at most 2 MB each. 64 x 65536 in 121 slabs 201 us, 367 on tiles;
   // 64 x 131072 in 241 slabs 596, 545; 16 x 262144 120, 549)
   s.thin = !s.small && s.m <= SMALL_ROWS && s.slabs * s.T * s.T <= 2048;

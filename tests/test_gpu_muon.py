@@ -410,3 +410,11 @@ def test_every_form_of_the_products(plan):
         _check_halves(-p, g)
     if len(grads) == 1:
         assert torch.equal(ops.orthogonalize(grads[0].to(DEV)), -params[0])
+
+
+@pytest.mark.parametrize("shape", [(128, 2048), (1600, 113), (116, 2635), (129, 2048), (112, 2048)])
+def test_a_hundred_rows_and_long(shape):
+    """Eight blocks of 16 rows, whose sums would leave a slab no room for a line."""
+    g = _gradient(*shape, seed=44)
+    _check_halves(ops.orthogonalize(g.to(DEV)), g)
+    _check_step(*_triples([shape, (2, *shape)], F32, BF16, seed=45), lr=0.1)

@@ -367,3 +367,16 @@ def test_oracle_tells_a_product_without_its_low_halves(shape):
         assert off[name] >= 8 * off[""], (name, off)
     if shape[0] != shape[1]:  # (a tall one's is the other's; a square one's sums run otherwise)
         torch.testing.assert_close(ref.schulz_halves(u.t()), ref.schulz_halves(u).t())
+
+
+def test_workspaces_of_every_shape_are_found():
+    """Each number of rows past and below what a workgroup holds, beside lengths on both sides of every rule (128 x 2048, say)."""
+    lib, out = _lib.load(), ctypes.c_int64()
+    for rows in range(1, 700):
+        for cols in (1, 31, 33, 64, 100, 512, 1000, 1537, 1568, 1569, 2048, 4096, 10000, 65536, 131072):
+            for shape in ((rows, cols), (cols, rows)):
+                assert lib.fim_orthogonalize_workspace(3, *shape, ctypes.byref(out)) == 0
+                m, n = (-(-x // 32) * 32 for x in sorted(shape))
+                # halves of X twice, A and P, but for matrices that stay in a workgroup and, once, in slabs' ones
+                least = 0 if min(shape) <= 64 else 3 * 4 * (2 * m * n + 2 * m * m)
+                assert least <= out.value <= 3 * 4 * (2 * m * n + 2 * m * m) + 3 * (4 << 20) + (1 << 28), shape
