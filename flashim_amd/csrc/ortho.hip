@@ -208,21 +208,41 @@ static float ortho_scale(double most) {
   return ldexpf(1.0f, e - 1);
 }
 
-// The scales of X, A and P: no entry of a matrix is larger than its largest singular value, whose path from any s <= 1 is
-// followed here. False where it leaves the halves little room (or does not end at all).
+// The scales of X, A and P: no entry of a matrix is larger than its largest singular value. These lie in [0, x] with x = 1 at first,
+// and a step's odd polynomial takes that interval onto another that holds 0: its end is the largest value at x or where the slope
+// is zero. False where the path leaves the halves little room (or does not end at all).
 static bool ortho_scales(OrthoScalars& k) {
-  double most_x = 1.0, most_p = 0.0;
-  for (int i = 0; i <= 256; ++i) {
-    double x = i / 256.0;
-    for (int it = 0; it < k.steps; ++it) {
-      const double q = x * x, p = k.a + q * (k.b + q * k.c);
-      most_p = fmax(most_p, fabs(p));
-      x *= p;
-      if (!(fabs(p) <= 48.0) || !(fabs(x) <= 6.0)) return false;
-      if (it + 1 < k.steps) most_x = fmax(most_x, fabs(x));
-    }
+  const double a = k.a, b = k.b, c = k.c;
+  double flat[2] = {-1.0, -1.0};  // squares at which a + 3 b q + 5 c q^2 is zero
+  const double root = 9.0 * b * b - 20.0 * a * c;
+  if (c == 0.0 && b != 0.0) {
+    flat[0] = -a / (3.0 * b);
+  } else if (c != 0.0 && root >= 0.0) {
+    flat[0] = (-3.0 * b - sqrt(root)) / (10.0 * c);
+    flat[1] = (-3.0 * b + sqrt(root)) / (10.0 * c);
   }
-  // (between the grid's points and by rounding a little more)
+  double most_x = 1.0, most_p = 0.0, x = 1.0;
+  for (int it = 0; it < k.steps; ++it) {
+    double next = 0.0, p = 0.0;
+    bool fine = true;
+    auto look = [&](double q) {  // at a square within the interval
+      if (!(q >= 0.0 && q <= x * x)) return;
+      const double at = fabs(a + q * (b + q * c));
+      fine = fine && at <= 48.0 && sqrt(q) * at <= 6.0;  // (not of NaN, which fmax passes over)
+      p = fmax(p, at);
+      next = fmax(next, sqrt(q) * at);
+    };
+    look(0.0);
+    look(x * x);
+    look(flat[0]);
+    look(flat[1]);
+    if (c != 0.0) look(-b / (2.0 * c));
+    if (!fine) return false;
+    most_p = fmax(most_p, p);
+    x = next;
+    if (it + 1 < k.steps) most_x = fmax(most_x, x);
+  }
+  // (by rounding a little more)
   k.sx = ortho_scale(1.1 * most_x);
   k.sa = ortho_scale(1.25 * most_x * most_x);
   k.sp = ortho_scale(1.05 * most_p);

@@ -380,3 +380,23 @@ def test_workspaces_of_every_shape_are_found():
                 # halves of X twice, A and P, but for matrices that stay in a workgroup and, once, in slabs' ones
                 least = 0 if min(shape) <= 64 else 3 * 4 * (2 * m * n + 2 * m * m)
                 assert least <= out.value <= 3 * 4 * (2 * m * n + 2 * m * m) + 3 * (4 << 20) + (1 << 28), shape
+
+
+def test_coefficients_that_diverge_between_common_points_are_refused():
+    """Singular values in a window of 1e-4 pass 6 in ten steps of this polynomial; its neighbour keeps all of them below 2."""
+    lib, fake = _lib.load(), 1 << 20
+
+    def call(a, b, c, steps):
+        return lib.fim_orthogonalize(fake, 0, 1, 0, 300, steps, a, b, c, 1e-7, fake, 0, None, 0, None)  # (no rows: nothing is launched)
+
+    x = torch.linspace(0, 1, 2_000_001, dtype=torch.float64)
+    for (a, b, c), refused in (((2.3763397567, -4.95683002527, 1.579664002893), True), ((2.3763397567, -4.5, 1.579664002893), False)):
+        v, most = x, 0.0
+        for _ in range(10):
+            v = v * (a + b * v**2 + c * v**4)
+            most = max(most, v.abs().max().item())
+        assert (most > 6) == refused
+        assert call(a, b, c, 10) == (_lib.FIM_ERR_UNSUPPORTED if refused else 0)
+    for coefficients, steps in ((ref.NEWTON_SCHULZ, 5), (ref.NEWTON_SCHULZ, 100), ((1.5, -0.5, 0.0), 12), ((0.0, 0.0, 1.0), 3),
+                                ((1.0, 0.0, 0.0), 1), ((-1.5, 0.5, 0.0), 4)):
+        assert call(*coefficients, steps) == 0
