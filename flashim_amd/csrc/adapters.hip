@@ -29,7 +29,8 @@ static int adapter_check(const AdapterSizes& s, int dtype, int wide) {
 }
 
 // Forms by size. One row a workgroup where entries are single rows and few: their adapters differ, and a tile of rows would go
-// through them one after the other. Else tiles, four wavefronts each until rows fill the CUs, and beyond that where all four have
+// through them one after the other (512 rows of 512 -> 2048, each with one of 64 adapters: 12 us, 513 on tiles 50; of one adapter
+// 11 either way). Else tiles, four wavefronts each until rows fill the CUs, and beyond that where all four have
 // a part of either product (40000 x 512 -> 2048 at rank 16: 115 -> 92 us); narrow maps a wavefront a tile, which exchange nothing
 // (320000 x 64 -> 256 77 us, 106 with four). A tile of two sets of 16 rows halves the reads of A_j and B_j from the caches, once
 // there are enough: 512 -> 2048, 16384 rows of ranks 32, 64, 128: 30, 40 and 64 us, of one set 45, 52 and 113; 4096 rows 15, 21,

@@ -5,7 +5,7 @@
 // B_j^T lie in LDS, and so do 64 rows of x and d_out at a time, read once from memory and used three times: each wavefront
 // multiplies 16 of them into h and t and its rows of dx; then t and h (hi and lo) meet all 64 rows, read transposed, in
 // accumulators that stay in registers for the chunk. Passes of their own (adapters_rows.h, adapters_grad.h) read d_out twice and
-// write and read t and h in FP32: 320000 x 64 -> 256 at rank 8 took 77 + 55 us and 22 to join, this one 61 and 5 to join:
+// write and read t and h in FP32: 320000 x 64 -> 256 at rank 8 took 77 + 55 us and 22 to join, this one 62 and 6 to join:
 // 246 MB at 4.0 TB/s, of the 5.1 of a large copy; the rest is the turns' barriers, with two workgroups a CU to cover them.
 #pragma once
 

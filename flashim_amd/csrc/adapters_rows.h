@@ -5,11 +5,13 @@
 // go straight into registers: a tile's rows are read once, and A_j and B_j come from the caches. h stays in the accumulators'
 // layout: a lane holds 4 ranks of its row a block, and the second product's contraction is ordered by what lanes hold, hi of the 4
 // and then lo of the 4 beside the same 4 of B_j twice; so h keeps 16 bits or more and nothing is exchanged. Rows of several
-// adapters in a tile: once for each adapter that occurs, rows of others computed and not stored.
+// adapters in a tile: once for each adapter that occurs, rows of others computed and not stored. (Indices in random order cost that
+// many passes: 16384 rows of 512 -> 2048 at rank 16 and 64 adapters 330 us, sorted 47, of one adapter 31.)
 //
 // Bound by memory at low ranks: 40000 x 512 -> 2048 at rank 16, 369 MB in 92 us, 4.0 TB/s of the 5.1 of a large copy; 320000 x 64
-// -> 256 at rank 8 as many in 84. By the caches' reads of A_j and B_j at high ones: rank 32 104 us, 64 155, 128 202 (171, 278 and
-// 434 with 8-byte loads of B_j and 16 rows). 64 rows of adapters of their own, 1024 -> 4096 at rank 16: 12 MB in 7 us, latency.
+// -> 256 at rank 8 as many in 84. By the caches' reads of A_j and B_j at high ones: rank 32 106 us, 64 152, 128 213 (171, 278 and
+// 434 with 8-byte loads of B_j and 16 rows): every tile of 32 rows reads all of B_j. 64 rows of adapters of their own, 1024 -> 4096
+// at rank 16: 12 MB in 7 us, latency.
 #pragma once
 
 #include "adapters.h"

@@ -6,8 +6,9 @@
 // blocks, those above the diagonal from the ones below, read across; P X is split over the columns too, and each wavefront replaces
 // the columns it has read.
 //
-// Bound by the chain of dependent products, each of LDS latencies and two or three barriers: 64 x 256 32 us, about 6 a step; 64
-// matrices of 16 x 512 beside each other 16.
+// Bound by the chain of dependent products, each of LDS latencies and two or three barriers, and at four blocks of rows by X X^T on
+// four of the sixteen wavefronts, ten pairs of blocks each: 64 x 256 32 us, about 6 a step; 64 matrices of 16 x 512 beside each
+// other 16.
 #pragma once
 
 #include "ortho.h"
@@ -15,7 +16,7 @@
 namespace fim {
 
 // SUMS: wavefronts that X X^T is split over, and whose sums lie in LDS at once (64 matrices of 16 x 512 15.8 us; by 8 16.0, by 16
-// 16.9). SMALL_FEW: stacks that travel in kernel arguments
+// 16.9; not measured by more at four blocks of rows). SMALL_FEW: stacks that travel in kernel arguments
 constexpr int SMALL_WAVES = 16, SMALL_SUMS = 4, SMALL_FEW = 6, SMALL_ROWS = 64, SMALL_LDS = 160 * 1024;
 
 // (Three blocks of 16 rows spill some 30 registers, and are still ahead: 48 x 600 49 us, 62 in slabs, which four would need.)

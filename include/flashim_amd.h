@@ -306,7 +306,7 @@ int fim_muon_step_workspace(int64_t count, const int64_t* batch, const int64_t* 
 
 /* An optimizer step of `count` stacks of packed matrices (host arrays of device pointers, dtype codes and sizes):
  * m = momentum m + g (FP32, in place), u = g + momentum m (nesterov) or m, O as above of each u, p = keep p - factors[i] O
- * (in place). No parameter or momentum overlaps another array of the call. */
+ * (in place). No parameter or momentum overlaps another array of the call (not checked here). */
 int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, const void* const* grads, const int* grad_dtypes,
                   float* const* momenta, const int64_t* batch, const int64_t* rows, const int64_t* cols, const float* factors,
                   float momentum, int nesterov, float keep, int steps, float a, float b, float c, double eps, void* workspace,
@@ -320,7 +320,7 @@ int fim_muon_step(int64_t count, void* const* params, const int* param_dtypes, c
  * s_j = scale * scales[j] (scales FP32 [J], or NULL: 1). Sums and x A^T in FP32 (split in two 16-bit operands for the second
  * product), rounded once. out packed [M, N]; h, if not NULL (16-byte aligned), FP32 [M, columns of
  * fim_low_rank_adapters_saved], s_j x A_j^T for the backward pass (rows without an adapter are not written, and nothing where
- * there are 0 columns). M below 2^28 (else 99). No counterpart in the reference, as the next three. */
+ * there are 0 columns). M below 2^28 (else 99). out apart from the inputs. No counterpart in the reference, as the next three. */
 int fim_low_rank_adapters(const void* base, int64_t base_stride, const void* x, int64_t x_stride, int dtype, int64_t M, int64_t K,
                           int64_t N, const void* a, const void* b, int64_t J, int64_t R, const void* index, int index_wide,
                           int64_t entries, const float* scales, float scale, void* out, float* h, hipStream_t stream);

@@ -327,7 +327,7 @@ def test_tensors_that_overlap_are_refused():
 
 @pytest.mark.parametrize("shape", [(4, 4), (24, 40), (40, 24), (7, 3696), (130, 200), (200, 130)])
 def test_norms_whose_scale_fp32_does_not_hold(shape):
-    """2^13 / |g| is past FP32's largest number, or near its smallest; an eps beside which only a zero matrix counts."""
+    """2^15 / |g| is past FP32's largest number, or near its smallest; an eps beside which only a zero matrix counts."""
     for scale in (1e-34, 1e-41, 1e38):
         g = (_gradient(*shape, seed=41).double() * scale).float()
         assert g.count_nonzero() > 0
